@@ -399,6 +399,59 @@ int hsa_cross_entropy_bwd_inplace(void *logits, long long row_stride, const long
                                   long long ignore_index, float *col_sums, float *partial, void *stream);
 
 /*
+ * Dense attention of the rows of one sequence over the rows of another (cross attention): the path that
+ * HierarchicalAttention.forward takes when it is given no parents or when the lengths differ
+ * (hierarchical_attention/modules/attention.py:237-270, which builds the [B, H, Lq, Lk] weights).
+ *   Q, Out : [B, Lq, H, D];  K, V : [B, Lk, Hkv, D], H a multiple of Hkv; query head h reads key/value head h / (H / Hkv).
+ *   Out[b, i, h] = sum_j p_ij V[b, j],  p_i = softmax of scale * Q[b, i, h] . K[b, j] over the keys j that i may look at:
+ *   j < key_lengths[b] (NULL: all Lk; values outside [0, Lk] mean the nearer end) and, with a mask, its entry (i, j) set.
+ *   A query without keys gives rows of `empty_value` and LSE = -inf.  What K and V hold behind a length, or in keys that no
+ *   query of a mask's plane may look at, reaches no result (it may be NaN); keys that some queries see and others do not
+ *   must be finite, as must Q and dOut in the backward.
+ *   LSE, if not NULL, receives the log-sum-exp [B, Lq, H] float32 that the backward needs.
+ *   scale > 0.  D <= 256.  `algo`: 0 = automatic, 1 = CUDA cores, 2 = tensor cores (bf16 / f16, D a multiple of 8 up to 128,
+ *   16-byte aligned rows; HSA_ERR_ARG otherwise).
+ * Masks come packed (hsa_dense_mask_pack): `mask` points to bytes (0 = may not look), four strides in bytes, of a tensor
+ *   [batches, heads, rows, Lk] with batches 1 or B, heads 1 or H, rows 1 or Lq; `packed` receives
+ *   hsa_dense_mask_bytes(...) bytes, 256-byte aligned.
+ * Backward: dQ, dK, dV of the inputs' shapes, every row written (zeros where nothing arrives), float32 accumulation, one
+ *   writer per row: deterministic.  dK and dV of a shared head are summed over its query heads.  `workspace`:
+ *   hsa_dense_attn_bwd_workspace_bytes(...) bytes, 256-byte aligned.
+ */
+size_t hsa_dense_mask_bytes(int batches, int heads, int rows, int Lk);
+int hsa_dense_mask_pack(const void *mask, int64_t stride_b, int64_t stride_h, int64_t stride_q, int64_t stride_k, int batches,
+                        int heads, int rows, int Lk, void *packed, size_t packed_bytes, void *stream);
+size_t hsa_dense_attn_fwd_workspace_bytes(int B, int Lq, int Lk, int H, int Hkv, int D, int dtype, int algo);
+int hsa_dense_attn_fwd(hsa_view Q, hsa_view K, hsa_view V, hsa_view Out, float *LSE, const int *key_lengths,
+                       const void *packed_mask, int mask_batches, int mask_heads, int mask_rows, void *workspace,
+                       size_t workspace_bytes, int B, int Lq, int Lk, int H, int Hkv, int D, float scale, float empty_value,
+                       int dtype, int algo, void *stream);
+size_t hsa_dense_attn_bwd_workspace_bytes(int B, int Lq, int H);
+int hsa_dense_attn_bwd(hsa_view Q, hsa_view K, hsa_view V, hsa_view Out, const float *LSE, hsa_view dOut, hsa_view dQ,
+                       hsa_view dK, hsa_view dV, const int *key_lengths, const void *packed_mask, int mask_batches,
+                       int mask_heads, int mask_rows, void *workspace, size_t workspace_bytes, int B, int Lq, int Lk, int H,
+                       int Hkv, int D, float scale, int dtype, int algo, void *stream);
+
+/*
+ * Attention of one new token per sequence over a key/value cache that lives in pages: the dense counterpart of
+ * hsa_span_attn_decode.
+ *   q, out : [B, H, D] (batch_stride; row stride unused);  k_pages, v_pages : [num_pages, page_size, Hkv, D], batch_stride =
+ *   elements between pages, row_stride = between the slots of a page;  page_table [B, max_pages] int32 with `table_stride`
+ *   entries between rows;  lengths [B] int32.  Key j of sequence b is slot j % page_size of page page_table[b, j / page_size].
+ *   A sequence of length 0 gives zeros.  A page number outside [0, num_pages) among those that the length reaches, or a
+ *   length outside [0, max_pages * page_size], is not followed and makes that sequence's output NaN.
+ *   The keys are cut into `splits` ranges per sequence (hsa_paged_attn_choose_splits suggests how many) that are joined by a
+ *   second kernel; `workspace` holds hsa_paged_attn_workspace_bytes(...) bytes (0 for one split), 256-byte aligned.
+ *   D <= 256; `algo`: 0 = automatic, 1 = CUDA cores, 2 = tensor cores (bf16 / f16, D a multiple of 8, 16-byte aligned rows).
+ */
+int hsa_paged_attn_choose_splits(int B, int H, int Hkv, int page_size, int max_pages);
+size_t hsa_paged_attn_workspace_bytes(int B, int H, int D, int splits);
+int hsa_paged_attn_decode(hsa_view q, hsa_view k_pages, hsa_view v_pages, hsa_view out, const int *page_table,
+                          int64_t table_stride, const int *lengths, void *workspace, size_t workspace_bytes, int B, int H,
+                          int Hkv, int D, int page_size, int num_pages, int max_pages, float scale, int dtype, int splits,
+                          int algo, void *stream);
+
+/*
  * Span attention backward without any workspace argument.  No counterpart in the reference
  * project: it exists for hosts that cannot allocate device memory around the call (a plugin
  * execute hook that only receives pre-bound buffers; a server whose GPU memory is fully

@@ -92,6 +92,18 @@ SIGNATURES = {
                                               c_float, ctypes.c_longlong, c_void_p, c_void_p, c_void_p]),
     "hsa_dropout_apply": (c_int, [V, c_int, V, c_int, c_int, c_int, c_int, ctypes.c_longlong, ctypes.c_longlong,
                                   ctypes.c_longlong, ctypes.c_longlong, c_void_p, ctypes.c_uint, ctypes.c_uint, ctypes.c_uint, c_float, c_void_p]),
+    "hsa_dense_mask_bytes": (c_size_t, [c_int] * 4),
+    "hsa_dense_mask_pack": (c_int, [c_void_p] + [c_int64] * 4 + [c_int] * 4 + [c_void_p, c_size_t, c_void_p]),
+    "hsa_dense_attn_fwd_workspace_bytes": (c_size_t, [c_int] * 8),
+    "hsa_dense_attn_fwd": (c_int, [V, V, V, V, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_size_t]
+                           + [c_int] * 6 + [c_float, c_float, c_int, c_int, c_void_p]),
+    "hsa_dense_attn_bwd_workspace_bytes": (c_size_t, [c_int] * 3),
+    "hsa_dense_attn_bwd": (c_int, [V, V, V, V, c_void_p, V, V, V, V, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_size_t]
+                           + [c_int] * 6 + [c_float, c_int, c_int, c_void_p]),
+    "hsa_paged_attn_choose_splits": (c_int, [c_int] * 5),
+    "hsa_paged_attn_workspace_bytes": (c_size_t, [c_int] * 4),
+    "hsa_paged_attn_decode": (c_int, [V, V, V, V, c_void_p, c_int64, c_void_p, c_void_p, c_size_t] + [c_int] * 7
+                              + [c_float, c_int, c_int, c_int, c_void_p]),
     "hsa_copy_rows_async": (c_int, [c_void_p, c_size_t, c_void_p, c_size_t, c_size_t, c_size_t, c_int, c_void_p]),
     "hsa_span_attn_bwd_static": (c_int, [V, V, V, V, c_void_p, V, V, V, V] + [c_int] * 7 + [c_void_p]),
 }

@@ -1,0 +1,205 @@
+// Entry points of dense attention, the packing of its masks, and the row sums its backward starts from.
+#include "dense_attn.cuh"
+
+namespace hsa {
+
+int dense_simt(const DenseArgs &a, int what, int dtype, cudaStream_t st);
+
+// ------------------------------------------------------------------------------------------------------------ mask
+// One block per 128 x 128 cell of a plane, a warp per 32 x 32 piece: 32 coalesced row reads turn into words by ballot, 32 more
+// ballots transpose them.  The whole mask is read once (a byte per entry) and comes out at an eighth (two eighths with the
+// transposed copy) of its size; the attention kernels then read 16 bytes per query row and 128 keys.
+__global__ void __launch_bounds__(512)
+dense_mask_pack_kernel(const uint8_t *__restrict__ mask, int64_t sb, int64_t sh, int64_t sq, int64_t sk, int Hm, int rows, int Lk,
+                       uint32_t *__restrict__ bits, uint32_t *__restrict__ bits_t, uint32_t *__restrict__ seen,
+                       uint8_t *__restrict__ tiles, int wk, int wq, int tq, int tk) {
+    const long long cell = blockIdx.x;
+    const int ct = (int)(cell % tk), rt = (int)(cell / tk % tq);
+    const long long plane = cell / tk / tq;
+    const uint8_t *M = mask + (plane / Hm) * sb + (plane % Hm) * sh;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int r0 = rt * kDenseTile + (warp >> 2) * 32, c0 = ct * kDenseTile + (warp & 3) * 32;
+    const int key = c0 + lane;
+    const int nrows = max(0, min(32, rows - r0)), ncols = max(0, min(32, Lk - c0));
+    uint32_t mine = 0, any = 0, all = 0xffffffffu;
+    const uint32_t full = ncols == 32 ? 0xffffffffu : (1u << ncols) - 1u;
+#pragma unroll 8
+    for (int r = 0; r < nrows; ++r) {
+        const bool on = key < Lk && M[(int64_t)(r0 + r) * sq + (int64_t)key * sk] != 0;
+        const uint32_t w = __ballot_sync(0xffffffffu, on);
+        if (r == lane) mine = w;
+        any |= w;
+        all &= w;
+    }
+    const int word = c0 >> 5;
+    if (lane < nrows) bits[((int64_t)plane * rows + r0 + lane) * wk + word] = mine;
+    if (bits_t != nullptr) {
+        uint32_t col = 0;
+#pragma unroll 8
+        for (int j = 0; j < 32; ++j) {
+            const uint32_t w = __ballot_sync(0xffffffffu, (mine >> j) & 1u);
+            if (j == lane) col = w;
+        }
+        if (lane < ncols) bits_t[((int64_t)plane * Lk + key) * wq + (r0 >> 5)] = col;
+        if (lane == 0 && any != 0) atomicOr(seen + (int64_t)plane * wk + word, any);
+    }
+    const int some = __syncthreads_or(any != 0);
+    const int every = __syncthreads_and(nrows == 0 || (all & full) == full);
+    if (threadIdx.x == 0) tiles[((int64_t)plane * tq + rt) * tk + ct] = every ? 2 : some ? 1 : 0;
+}
+
+// ------------------------------------------------------------------------------------------------ backward's row sums
+// delta[b, h, i] = sum_d dout * out and the row's log-sum-exp in base 2, padded with rows that give weight zero.  A query
+// without keys gets +inf and 0 whatever its output row holds.
+template <typename T, int VEC, int LPR, int CPL>
+__global__ void __launch_bounds__(256) dense_delta_kernel(const DenseArgs a, float *__restrict__ lse2, float *__restrict__ delta) {
+    const long long row = (long long)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
+    const int g = threadIdx.x % LPR;
+    const int h = (int)(row % a.H), i = (int)(row / a.H % a.lq_pad);
+    const long long b = row / a.H / a.lq_pad;
+    if (b >= a.B) return;
+    const int64_t at = (b * a.H + h) * a.lq_pad + i;
+    if (i >= a.Lq) {
+        if (g == 0) { lse2[at] = INFINITY; delta[at] = 0.f; }
+        return;
+    }
+    RowFrag<T, VEC, LPR, CPL> x, y;
+    x.load((const T *)a.out.ptr + b * a.out.batch_stride + (int64_t)i * a.out.row_stride + (int64_t)h * a.D, g, a.D / VEC);
+    y.load((const T *)a.dout.ptr + b * a.dout.batch_stride + (int64_t)i * a.dout.row_stride + (int64_t)h * a.D, g, a.D / VEC);
+    const float s = group_sum<LPR>(x.dot_partial(y));
+    if (g == 0) {
+        const float l = a.lse[(b * a.Lq + i) * a.H + h];
+        const bool none = l == -INFINITY;
+        lse2[at] = none ? INFINITY : l * 1.4426950408889634f;
+        delta[at] = none ? 0.f : s;
+    }
+}
+
+static int dense_delta(const DenseArgs &a, float *lse2, float *delta, int dtype, bool vec, cudaStream_t st) {
+    return dispatch_dtype(dtype, [&]<typename T>() -> int {
+        int rc = 0;
+        const bool ok = dispatch_row_shape<T>(a.D, vec, [&]<typename T2, int VEC, int LPR, int CPL>() {
+            const long long rows = (long long)a.B * a.lq_pad * a.H, blocks = (rows + 256 / LPR - 1) / (256 / LPR);
+            if (blocks > 0x7fffffffLL) { rc = fail(HSA_ERR_ARG, "hsa_dense_attn_bwd: too many rows"); return; }
+            dense_delta_kernel<T2, VEC, LPR, CPL><<<(unsigned)blocks, 256, 0, st>>>(a, lse2, delta);
+            rc = launch_status("hsa_dense_attn_bwd(row sums)");
+        });
+        return ok ? rc : fail(HSA_ERR_ARG, "hsa_dense_attn_bwd: head dim %d not supported", a.D);
+    });
+}
+
+static bool rows_in_fours(const hsa_view &v, int esize) {
+    return (reinterpret_cast<uintptr_t>(v.ptr) % (4 * esize)) == 0 && v.batch_stride % 4 == 0 && v.row_stride % 4 == 0;
+}
+
+static int check_shape(const char *who, int B, int Lq, int Lk, int H, int Hkv, int D, float scale, int dtype, int algo) {
+    HSA_CHECK_ARG(B >= 1 && Lq >= 1 && Lk >= 1 && H >= 1 && Hkv >= 1, "%s: bad shape B=%d Lq=%d Lk=%d H=%d Hkv=%d", who, B, Lq, Lk, H, Hkv);
+    HSA_CHECK_ARG(H % Hkv == 0, "%s: %d query heads are not a multiple of %d key/value heads", who, H, Hkv);
+    HSA_CHECK_ARG(D >= 1 && D <= 256, "%s: head dim %d outside 1..256", who, D);
+    HSA_CHECK_ARG(Lq <= (1 << 30) && Lk <= (1 << 30), "%s: more than 2^30 rows", who);
+    HSA_CHECK_ARG(scale > 0.f && scale < INFINITY, "%s: the scale must be positive and finite", who);
+    HSA_CHECK_ARG(algo >= 0 && algo <= 2, "%s: unknown algo %d", who, algo);
+    if (dtype != HSA_F32 && dtype != HSA_BF16 && dtype != HSA_F16) return fail(HSA_ERR_DTYPE, "unknown dtype code %d", dtype);
+    return 0;
+}
+
+static int check_mask(const char *who, const void *packed, int mb, int mh, int mr, int B, int H, int Lq) {
+    if (packed == nullptr) return 0;
+    HSA_CHECK_ARG((mb == 1 || mb == B) && (mh == 1 || mh == H) && (mr == 1 || mr == Lq),
+                  "%s: the mask's sizes (%d, %d, %d) do not broadcast to (%d, %d, %d)", who, mb, mh, mr, B, H, Lq);
+    return 0;
+}
+
+}  // namespace hsa
+
+using namespace hsa;
+
+extern "C" size_t hsa_dense_mask_bytes(int batches, int heads, int rows, int Lk) {
+    if (batches < 1 || heads < 1 || rows < 1 || Lk < 1) return 0;
+    return dense_mask_layout((long long)batches * heads, rows, Lk).total;
+}
+
+extern "C" int hsa_dense_mask_pack(const void *mask, int64_t stride_b, int64_t stride_h, int64_t stride_q, int64_t stride_k,
+                                   int batches, int heads, int rows, int Lk, void *packed, size_t packed_bytes, void *stream) {
+    HSA_CHECK_ARG(mask && packed, "hsa_dense_mask_pack: null pointer");
+    HSA_CHECK_ARG(batches >= 1 && heads >= 1 && rows >= 1 && Lk >= 1 && rows <= (1 << 30) && Lk <= (1 << 30),
+                  "hsa_dense_mask_pack: bad shape (%d, %d, %d, %d)", batches, heads, rows, Lk);
+    const long long planes = (long long)batches * heads;
+    const DenseMaskLayout l = dense_mask_layout(planes, rows, Lk);
+    if (packed_bytes < l.total) return fail(HSA_ERR_WORKSPACE, "hsa_dense_mask_pack: %zu bytes needed, %zu given", l.total, packed_bytes);
+    if (reinterpret_cast<uintptr_t>(packed) & 255u) return fail(HSA_ERR_ALIGN, "hsa_dense_mask_pack: the packed mask must be 256-byte aligned");
+    const long long cells = planes * l.tq * l.tk;
+    HSA_CHECK_ARG(cells <= 0x7fffffffLL, "hsa_dense_mask_pack: too many cells");
+    char *p = (char *)packed;
+    if (rows > 1) {
+        const cudaError_t e = cudaMemsetAsync(p + l.seen, 0, (size_t)planes * l.wk * 4, (cudaStream_t)stream);
+        if (e != cudaSuccess) return fail((int)e, "hsa_dense_mask_pack: %s", cudaGetErrorString(e));
+    }
+    dense_mask_pack_kernel<<<(unsigned)cells, 512, 0, (cudaStream_t)stream>>>(
+        (const uint8_t *)mask, stride_b, stride_h, stride_q, stride_k, heads, rows, Lk, (uint32_t *)(p + l.bits),
+        rows > 1 ? (uint32_t *)(p + l.bits_t) : nullptr, (uint32_t *)(p + l.seen), (uint8_t *)(p + l.tiles), l.wk, l.wq, l.tq, l.tk);
+    return launch_status("hsa_dense_mask_pack");
+}
+
+extern "C" size_t hsa_dense_attn_fwd_workspace_bytes(int B, int Lq, int Lk, int H, int Hkv, int D, int dtype, int algo) {
+    (void)B; (void)Lq; (void)Lk; (void)H; (void)Hkv; (void)D; (void)dtype; (void)algo;
+    return 0;
+}
+
+extern "C" int hsa_dense_attn_fwd(hsa_view Q, hsa_view K, hsa_view V, hsa_view Out, float *LSE, const int *key_lengths,
+                                  const void *packed_mask, int mask_batches, int mask_heads, int mask_rows, void *workspace,
+                                  size_t workspace_bytes, int B, int Lq, int Lk, int H, int Hkv, int D, float scale,
+                                  float empty_value, int dtype, int algo, void *stream) {
+    (void)workspace; (void)workspace_bytes;
+    HSA_CHECK_ARG(Q.ptr && K.ptr && V.ptr && Out.ptr, "hsa_dense_attn_fwd: null pointer");
+    if (int rc = check_shape("hsa_dense_attn_fwd", B, Lq, Lk, H, Hkv, D, scale, dtype, algo)) return rc;
+    if (int rc = check_mask("hsa_dense_attn_fwd", packed_mask, mask_batches, mask_heads, mask_rows, B, H, Lq)) return rc;
+    DenseArgs a{};
+    a.q = Q; a.k = K; a.v = V; a.out = Out; a.lse = LSE;
+    a.key_lengths = key_lengths;
+    a.mask = dense_mask_view(packed_mask, mask_batches, mask_heads, mask_rows, Lk);
+    a.B = B; a.Lq = Lq; a.Lk = Lk; a.H = H; a.Hkv = Hkv; a.D = D; a.group = H / Hkv;
+    a.lq_pad = (Lq + 127) / 128 * 128;
+    a.scale = scale; a.scale_log2 = scale * 1.4426950408889634f; a.empty_value = empty_value;
+    const int es = dtype_size(dtype);
+    a.vec = D % 4 == 0;
+    for (const hsa_view &v : {Q, K, V, Out}) a.vec = a.vec && rows_in_fours(v, es);
+    HSA_CHECK_ARG(algo != 2, "hsa_dense_attn_fwd: no tensor-core kernel for these inputs");
+    return dense_simt(a, 0, dtype, (cudaStream_t)stream);
+}
+
+extern "C" size_t hsa_dense_attn_bwd_workspace_bytes(int B, int Lq, int H) {
+    if (B < 1 || Lq < 1 || H < 1) return 0;
+    return (size_t)2 * B * H * ((Lq + 127) / 128 * 128) * sizeof(float);
+}
+
+extern "C" int hsa_dense_attn_bwd(hsa_view Q, hsa_view K, hsa_view V, hsa_view Out, const float *LSE, hsa_view dOut, hsa_view dQ,
+                                  hsa_view dK, hsa_view dV, const int *key_lengths, const void *packed_mask, int mask_batches,
+                                  int mask_heads, int mask_rows, void *workspace, size_t workspace_bytes, int B, int Lq, int Lk,
+                                  int H, int Hkv, int D, float scale, int dtype, int algo, void *stream) {
+    HSA_CHECK_ARG(Q.ptr && K.ptr && V.ptr && Out.ptr && LSE && dOut.ptr && dQ.ptr && dK.ptr && dV.ptr, "hsa_dense_attn_bwd: null pointer");
+    if (int rc = check_shape("hsa_dense_attn_bwd", B, Lq, Lk, H, Hkv, D, scale, dtype, algo)) return rc;
+    if (int rc = check_mask("hsa_dense_attn_bwd", packed_mask, mask_batches, mask_heads, mask_rows, B, H, Lq)) return rc;
+    const size_t need = hsa_dense_attn_bwd_workspace_bytes(B, Lq, H);
+    if (workspace == nullptr || workspace_bytes < need)
+        return fail(HSA_ERR_WORKSPACE, "hsa_dense_attn_bwd: workspace of %zu bytes needed, %zu given", need, workspace_bytes);
+    if (reinterpret_cast<uintptr_t>(workspace) & 255u) return fail(HSA_ERR_ALIGN, "hsa_dense_attn_bwd: workspace must be 256-byte aligned");
+    DenseArgs a{};
+    a.q = Q; a.k = K; a.v = V; a.out = Out; a.dout = dOut; a.dq = dQ; a.dk = dK; a.dv = dV;
+    a.lse = const_cast<float *>(LSE);
+    a.key_lengths = key_lengths;
+    a.mask = dense_mask_view(packed_mask, mask_batches, mask_heads, mask_rows, Lk);
+    a.B = B; a.Lq = Lq; a.Lk = Lk; a.H = H; a.Hkv = Hkv; a.D = D; a.group = H / Hkv;
+    a.lq_pad = (Lq + 127) / 128 * 128;
+    a.scale = scale; a.scale_log2 = scale * 1.4426950408889634f;
+    float *lse2 = (float *)workspace, *delta = lse2 + (size_t)B * H * a.lq_pad;
+    a.lse2 = lse2; a.delta = delta;
+    const int es = dtype_size(dtype);
+    a.vec = D % 4 == 0;
+    for (const hsa_view &v : {Q, K, V, dOut, dQ, dK, dV}) a.vec = a.vec && rows_in_fours(v, es);
+    HSA_CHECK_ARG(algo != 2, "hsa_dense_attn_bwd: no tensor-core kernel for these inputs");
+    cudaStream_t st = (cudaStream_t)stream;
+    if (int rc = dense_delta(a, lse2, delta, dtype, D % (16 / es) == 0 && view_vec_ok(Out, es) && view_vec_ok(dOut, es), st)) return rc;
+    if (int rc = dense_simt(a, 1, dtype, st)) return rc;
+    return dense_simt(a, 2, dtype, st);
+}

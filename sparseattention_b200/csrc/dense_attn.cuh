@@ -1,0 +1,83 @@
+// Shared pieces of the dense attention kernels (queries of one sequence over the rows of another): launch arguments, the
+// packed form of a mask, and which keys a batch entry has.
+#pragma once
+
+#include <math.h>
+
+#include "hsa_common.cuh"
+
+namespace hsa {
+
+constexpr int kDenseTile = 128;          // keys and query rows per cell of the mask's tile table
+
+// A mask [planes, rows, Lk] in bits.  One plane per (batch entry, head) that the mask tells apart, one row per query or one
+// for all.  hsa_dense_mask_pack fills the arrays; their sizes follow from the mask's own sizes (dense_mask_layout).
+struct DenseMask {
+    const uint32_t *bits;                // [planes][rows][wk]: bit k of a row = the query may look at key k; bits >= Lk are 0
+    const uint32_t *bits_t;              // [planes][Lk][wq]: the same, keys as rows (null when the mask has one row)
+    const uint32_t *seen;                // [planes][wk]: keys that at least one query may look at
+    const uint8_t *tiles;                // [planes][tq][tk] of 128 x 128 cells: 0 nothing allowed, 1 some, 2 everything
+    int plane_b, plane_h;                // plane of (b, h) = b * plane_b + h * plane_h
+    int rows;                            // 1 or Lq
+    int wk, wq, tq, tk;
+};
+
+struct DenseMaskLayout {
+    size_t bits, bits_t, seen, tiles, total;      // byte offsets
+    int wk, wq, tq, tk;
+};
+inline DenseMaskLayout dense_mask_layout(long long planes, int rows, int Lk) {
+    DenseMaskLayout l{};
+    l.tk = (Lk + kDenseTile - 1) / kDenseTile;
+    l.tq = (rows + kDenseTile - 1) / kDenseTile;
+    l.wk = l.tk * 4;
+    l.wq = rows > 1 ? l.tq * 4 : 0;
+    auto up = [](size_t v) { return (v + 255) / 256 * 256; };
+    size_t at = 0;
+    l.bits = at;
+    at = up(at + (size_t)planes * rows * l.wk * 4);
+    l.bits_t = at;
+    if (rows > 1) at = up(at + (size_t)planes * Lk * l.wq * 4);
+    l.seen = at;
+    if (rows > 1) at = up(at + (size_t)planes * l.wk * 4); else l.seen = l.bits;
+    l.tiles = at;
+    at = up(at + (size_t)planes * l.tq * l.tk);
+    l.total = at;
+    return l;
+}
+
+inline DenseMask dense_mask_view(const void *packed, int Bm, int Hm, int rows, int Lk) {
+    DenseMask m{};
+    if (packed == nullptr) return m;
+    const DenseMaskLayout l = dense_mask_layout((long long)Bm * Hm, rows, Lk);
+    const char *p = (const char *)packed;
+    m.bits = (const uint32_t *)(p + l.bits);
+    m.bits_t = rows > 1 ? (const uint32_t *)(p + l.bits_t) : nullptr;
+    m.seen = (const uint32_t *)(p + l.seen);
+    m.tiles = (const uint8_t *)(p + l.tiles);
+    m.plane_b = Bm > 1 ? Hm : 0;
+    m.plane_h = Hm > 1 ? 1 : 0;
+    m.rows = rows;
+    m.wk = l.wk; m.wq = l.wq; m.tq = l.tq; m.tk = l.tk;
+    return m;
+}
+
+struct DenseArgs {
+    hsa_view q, k, v, out, dout, dq, dk, dv;
+    float *lse;                          // forward: [B, Lq, H] natural log-sum-exp, or null
+    const float *lse2, *delta;           // backward: [B, H, lq_pad] log-sum-exp in base 2 (+inf: no key) and row sums of dout * out
+    const int *key_lengths;              // [B] or null
+    DenseMask mask;
+    int B, Lq, Lk, H, Hkv, D, group;     // group = H / Hkv
+    int lq_pad;                          // Lq rounded up to 128
+    float scale, scale_log2;             // scale_log2 = scale * log2(e)
+    float empty_value;                   // what the output row of a query without keys holds
+    bool vec;                            // rows may be read four elements at a time
+};
+
+__device__ __forceinline__ int dense_keys(const DenseArgs &a, int b) {
+    if (a.key_lengths == nullptr) return a.Lk;
+    return max(0, min(a.Lk, __ldg(a.key_lengths + b)));      // lengths outside [0, Lk] mean the nearer end
+}
+
+}  // namespace hsa

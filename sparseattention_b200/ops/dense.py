@@ -1,0 +1,249 @@
+"""Dense attention: queries of one sequence over the rows of another, and one new token over a paged cache.
+
+`cross_attention` is the operator behind `HierarchicalAttention.forward` when it is given no parents or when the lengths of
+query and key differ (hierarchical_attention/modules/attention.py:237-270 of the reference, which builds the
+[B, H, Lq, Lk] weight matrix); `paged_attention_decode` is the dense counterpart of `span_attention_decode` for serving.
+Softmax statistics and sums are float32; the backward is deterministic (one writer per gradient row).
+"""
+from __future__ import annotations
+
+import math
+from ctypes import c_void_p
+from typing import Optional
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from .. import _lib
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """`t` [B, rows, heads, D] itself when its rows are packed, separate and aligned for vector loads, else a copy."""
+    B, rows, heads, D = t.shape
+    packed = _lib.inner_contiguous(t) and (rows == 1 or t.stride(1) >= heads * D) and (
+        B == 1 or t.stride(0) >= (rows - 1) * t.stride(1) + heads * D)
+    vec = 16 // t.element_size()
+    if packed and D % vec == 0:
+        packed = t.data_ptr() % 16 == 0 and (rows == 1 or t.stride(1) % vec == 0) and (B == 1 or t.stride(0) % vec == 0)
+    return t if packed else t.clone(memory_format=torch.contiguous_format)
+
+
+def _view(t: torch.Tensor) -> _lib.HsaView:
+    """View of a [B, rows, heads, D] tensor; strides of dimensions of one entry are what a packed tensor would have."""
+    B, rows, heads, D = t.shape
+    rs = t.stride(1) if rows > 1 else heads * D
+    return _lib.HsaView(t.data_ptr(), t.stride(0) if B > 1 else rows * rs, rs)
+
+
+class _PackedMask:
+    """A mask in the bit form of hsa_dense_mask_pack."""
+    __slots__ = ("data", "sizes")
+
+    def __init__(self, mask: torch.Tensor, B: int, H: int, Lq: int, Lk: int, dev: torch.device):
+        if mask.dtype.is_floating_point or mask.dtype.is_complex:
+            raise _lib.HsaError(f"the mask is boolean or integer (nonzero = attend), not {mask.dtype}; additive masks are not taken")
+        _lib.require_cuda(mask)
+        if mask.device != dev:
+            raise _lib.HsaError("all tensors of one call must live on the same device")
+        assert mask.dim() in (2, 4), "the mask is [Lq, Lk] or [B, H, Lq, Lk] (dimensions of size 1 are broadcast)"
+        if mask.dim() == 2:
+            mask = mask.view(1, 1, *mask.shape) if mask.is_contiguous() else mask.unsqueeze(0).unsqueeze(0)
+        want = (B, H, Lq, Lk)
+        assert all(m in (1, w) for m, w in zip(mask.shape, want)), \
+            f"mask shape {tuple(mask.shape)} does not broadcast to {want}"
+        if mask.dtype == torch.bool:
+            mask = mask.view(torch.uint8)
+        elif mask.dtype not in (torch.uint8, torch.int8):
+            mask = (mask != 0).view(torch.uint8)
+        # a dimension that is expanded (stride 0) is packed once
+        sizes = [1 if st == 0 else sz for sz, st in zip(mask.shape[:3], mask.stride()[:3])]
+        strides = [0 if sz == 1 else st for sz, st in zip(mask.shape, mask.stride())]
+        lib = _lib.load()
+        nbytes = int(lib.hsa_dense_mask_bytes(*sizes, Lk))
+        self.data = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        self.sizes = tuple(sizes)
+        rc = lib.hsa_dense_mask_pack(c_void_p(mask.data_ptr()), *strides, *sizes, Lk, c_void_p(self.data.data_ptr()), nbytes,
+                                     _lib.stream_ptr(dev))
+        _lib.check(rc, "hsa_dense_mask_pack")
+
+
+def _check_inputs(q, k, v):
+    dev = _lib.require_cuda(q, k, v)
+    _lib.dtype_code(q)
+    assert q.dim() == 4 and k.dim() == 4 and v.dim() == 4, "q is [B, Lq, H, D]; k and v are [B, Lk, Hkv, D]"
+    assert k.shape == v.shape and k.size(0) == q.size(0) and k.size(3) == q.size(3), \
+        f"shapes disagree: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}"
+    assert k.dtype == q.dtype and v.dtype == q.dtype, "dtype mismatch"
+    H, Hkv, D = q.size(2), k.size(2), q.size(3)
+    assert Hkv >= 1 and H >= 1 and H % Hkv == 0, f"{H} query heads are not a multiple of {Hkv} key/value heads"
+    assert 1 <= D <= 256, f"head dim {D} outside 1..256"
+    return dev
+
+
+def _lengths32(lengths, B: int, top: int, dev, name: str):
+    if lengths.dtype not in (torch.int32, torch.int64):
+        raise _lib.HsaError(f"{name} must be int32 or int64")
+    if lengths.device != dev:
+        raise _lib.HsaError("all tensors of one call must live on the same device")
+    assert lengths.shape == (B,), f"{name} must have shape ({B},)"
+    if lengths.dtype == torch.int64:
+        lengths = lengths.clamp(-1, top + 1).to(torch.int32)
+    return lengths if lengths.is_contiguous() else lengths.contiguous()
+
+
+def _ptr(t: Optional[torch.Tensor]):
+    return None if t is None else c_void_p(t.data_ptr())
+
+
+def dense_attention_forward(q, k, v, key_lengths=None, packed_mask=None, scale: float = 1.0, empty_value: float = 0.0,
+                            need_lse: bool = True, algo: int = _lib.ALGO_AUTO):
+    """Raw forward on checked inputs: returns (out, lse or None).  No autograd."""
+    lib = _lib.load()
+    dev = q.device
+    B, Lq, H, D = q.shape
+    Lk, Hkv = k.size(1), k.size(2)
+    out = torch.empty((B, Lq, H, D), dtype=q.dtype, device=dev)
+    lse = torch.empty((B, Lq, H), dtype=torch.float32, device=dev) if need_lse else None
+    dt = _lib.dtype_code(q)
+    with _lib.on_device(dev):
+        need = int(lib.hsa_dense_attn_fwd_workspace_bytes(B, Lq, Lk, H, Hkv, D, dt, algo))
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        rc = lib.hsa_dense_attn_fwd(_view(q), _view(k), _view(v), _view(out), _ptr(lse), _ptr(key_lengths),
+                                    _ptr(packed_mask.data) if packed_mask is not None else None,
+                                    *(packed_mask.sizes if packed_mask is not None else (0, 0, 0)), _ptr(ws), need,
+                                    B, Lq, Lk, H, Hkv, D, scale, empty_value, dt, algo, _lib.stream_ptr(dev))
+    _lib.check(rc, "hsa_dense_attn_fwd")
+    return out, lse
+
+
+def dense_attention_backward(q, k, v, out, lse, dout, key_lengths=None, packed_mask=None, scale: float = 1.0,
+                             algo: int = _lib.ALGO_AUTO):
+    """Raw backward: returns (dq, dk, dv)."""
+    lib = _lib.load()
+    dev = q.device
+    B, Lq, H, D = q.shape
+    Lk, Hkv = k.size(1), k.size(2)
+    dq = torch.empty((B, Lq, H, D), dtype=q.dtype, device=dev)
+    dk = torch.empty((B, Lk, Hkv, D), dtype=q.dtype, device=dev)
+    dv = torch.empty_like(dk)
+    need = int(lib.hsa_dense_attn_bwd_workspace_bytes(B, Lq, H))
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    with _lib.on_device(dev):
+        rc = lib.hsa_dense_attn_bwd(_view(q), _view(k), _view(v), _view(out), _ptr(lse), _view(dout), _view(dq), _view(dk),
+                                    _view(dv), _ptr(key_lengths), _ptr(packed_mask.data) if packed_mask is not None else None,
+                                    *(packed_mask.sizes if packed_mask is not None else (0, 0, 0)), _ptr(ws), need,
+                                    B, Lq, Lk, H, Hkv, D, scale, _lib.dtype_code(q), algo, _lib.stream_ptr(dev))
+    _lib.check(rc, "hsa_dense_attn_bwd")
+    return dq, dk, dv
+
+
+class _CrossAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, key_lengths, packed_mask, scale, empty_value, algo):
+        need = any(ctx.needs_input_grad[:3])
+        ctx.empty = q.size(0) * q.size(1) * k.size(1) == 0
+        if ctx.empty:                                # no query, or no key for any of them: nothing to launch
+            ctx.save_for_backward(q, k, v)
+            return torch.full(q.shape, empty_value, dtype=q.dtype, device=q.device)
+        q, k, v = _rows(q), _rows(k), _rows(v)
+        out, lse = dense_attention_forward(q, k, v, key_lengths, packed_mask, scale, empty_value, need, algo)
+        if need:
+            ctx.save_for_backward(q, k, v, out, lse, key_lengths, None if packed_mask is None else packed_mask.data)
+            ctx.meta = (packed_mask, scale, algo)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        if ctx.empty:
+            return (*(torch.zeros_like(t) for t in ctx.saved_tensors), None, None, None, None, None)
+        q, k, v, out, lse, key_lengths, _ = ctx.saved_tensors
+        packed_mask, scale, algo = ctx.meta
+        dout = _rows(dout if dout.dtype == q.dtype else dout.to(q.dtype))
+        dq, dk, dv = dense_attention_backward(q, k, v, out, lse, dout, key_lengths, packed_mask, scale, algo)
+        return dq, dk, dv, None, None, None, None, None
+
+
+def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, key_lengths: Optional[torch.Tensor] = None,
+                    mask: Optional[torch.Tensor] = None, scale: Optional[float] = None, empty_value: float = 0.0,
+                    algo: int = _lib.ALGO_AUTO) -> torch.Tensor:
+    """softmax(scale q k^T) v of every query over another sequence's rows.
+
+    q [B, Lq, H, D]; k, v [B, Lk, Hkv, D] with H a multiple of Hkv (query head h reads key/value head h // (H // Hkv));
+    float32, bfloat16 or float16, head dim up to 256; returns [B, Lq, H, D] of q's type.  Strided rows are read in place when
+    they are packed and aligned, and copied first otherwise.
+    key_lengths [B] (int32 or int64, on the device): only keys below a batch entry's length are there; values outside [0, Lk]
+        mean the nearer end.
+    mask: boolean or integer, nonzero = may attend, [Lq, Lk] or [B, H, Lq, Lk] with dimensions of size 1 broadcast.
+    scale: positive; 1 / sqrt(D) if not given.
+    A query that may look at no key gives a row of `empty_value` and passes no gradient on.  What k and v hold behind a
+    length, or in keys that a mask hides from all queries, may be anything; everything else has to be finite.
+    Differentiable once with respect to q, k and v.
+    """
+    dev = _check_inputs(q, k, v)
+    B, Lq, H, D = q.shape
+    Lk = k.size(1)
+    scale = D ** -0.5 if scale is None else float(scale)
+    if not (scale > 0.0 and math.isfinite(scale)):
+        raise _lib.HsaError("the scale must be positive and finite")
+    if key_lengths is not None:
+        key_lengths = _lengths32(key_lengths, B, Lk, dev, "key_lengths")
+    with _lib.on_device(dev):
+        packed = None if mask is None or B * Lq * Lk == 0 else _PackedMask(mask, B, H, Lq, Lk, dev)
+        return _CrossAttention.apply(q, k, v, key_lengths, packed, scale, float(empty_value), algo)
+
+
+def paged_attention_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
+                           lengths: torch.Tensor, scale: Optional[float] = None, splits: Optional[int] = None,
+                           algo: int = _lib.ALGO_AUTO) -> torch.Tensor:
+    """Attention of the single new token of every sequence over its cached keys and values, which live in pages.
+
+    q [B, H, D]; k_pages, v_pages [num_pages, page_size, Hkv, D] (pages and slots may be strided; a slot's [Hkv, D] is packed);
+    page_table [B, max_pages] int32 and lengths [B] int32 on the device: key j of sequence b is slot j % page_size of page
+    page_table[b, j // page_size], for j < lengths[b].  The new token's own key and value are in the cache if it is to see them.
+    Returns [B, H, D] of q's type; zeros for a length of 0.  A page number outside the pages that the length reaches, or a length the
+    table cannot hold, makes that sequence's output NaN; table entries behind the length are not read.
+    splits: ranges a sequence's keys are cut into (None: chosen from the sizes).  No autograd.
+    """
+    lib = _lib.load()
+    dev = _lib.require_cuda(q, k_pages, v_pages, page_table, lengths)
+    dt = _lib.dtype_code(q)
+    assert q.dim() == 3 and k_pages.dim() == 4, "q is [B, H, D]; the pages are [num_pages, page_size, Hkv, D]"
+    B, H, D = q.shape
+    num_pages, page_size, Hkv, Dk = k_pages.shape
+    assert v_pages.shape == k_pages.shape and Dk == D, \
+        f"shapes disagree: q {tuple(q.shape)}, k_pages {tuple(k_pages.shape)}, v_pages {tuple(v_pages.shape)}"
+    assert k_pages.dtype == q.dtype and v_pages.dtype == q.dtype, "dtype mismatch"
+    assert H >= 1 and Hkv >= 1 and H % Hkv == 0, f"{H} query heads are not a multiple of {Hkv} key/value heads"
+    assert 1 <= D <= 256, f"head dim {D} outside 1..256"
+    assert page_table.dtype == torch.int32 and lengths.dtype == torch.int32, "page_table and lengths are int32"
+    assert page_table.dim() == 2 and page_table.size(0) == B and lengths.shape == (B,), \
+        f"page_table is [{B}, max_pages] and lengths [{B}]"
+    if not (_lib.inner_contiguous(k_pages) and _lib.inner_contiguous(v_pages)):
+        raise _lib.HsaError("a slot's [Hkv, D] block must be packed (the cache is not copied)")
+    if scale is None:
+        scale = D ** -0.5
+    if not (scale > 0.0 and math.isfinite(scale)):
+        raise _lib.HsaError("the scale must be positive and finite")
+    max_pages = page_table.size(1)
+    out = torch.empty((B, H, D), dtype=q.dtype, device=dev)
+    if B == 0:
+        return out
+    if max_pages == 0 or num_pages == 0 or page_size == 0:
+        # no cache: every length has to be 0 (a table without room for a longer one gives NaN, as below)
+        return out.copy_(torch.where(lengths.view(B, 1, 1) == 0, 0.0, math.nan).expand(B, H, D))
+    q = q.contiguous()
+    if page_table.stride(1) != 1 and max_pages > 1:
+        page_table = page_table.contiguous()
+    lengths = lengths.contiguous()
+    with _lib.on_device(dev):
+        if splits is None:
+            splits = int(lib.hsa_paged_attn_choose_splits(B, H, Hkv, page_size, max_pages))
+        need = int(lib.hsa_paged_attn_workspace_bytes(B, H, D, splits))
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        rc = lib.hsa_paged_attn_decode(_lib.HsaView(q.data_ptr(), H * D, H * D), _lib.rows_view(k_pages), _lib.rows_view(v_pages),
+                                       _lib.HsaView(out.data_ptr(), H * D, H * D), c_void_p(page_table.data_ptr()),
+                                       page_table.stride(0), c_void_p(lengths.data_ptr()), _ptr(ws), need, B, H, Hkv, D,
+                                       page_size, num_pages, max_pages, float(scale), dt, splits, algo, _lib.stream_ptr(dev))
+    _lib.check(rc, "hsa_paged_attn_decode")
+    return out
