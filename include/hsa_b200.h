@@ -410,7 +410,8 @@ int hsa_cross_entropy_bwd_inplace(void *logits, long long row_stride, const long
  *   must be finite, as must Q and dOut in the backward.
  *   LSE, if not NULL, receives the log-sum-exp [B, Lq, H] float32 that the backward needs.
  *   scale > 0.  D <= 256.  `algo`: 0 = automatic, 1 = CUDA cores, 2 = tensor cores (bf16 / f16, D a multiple of 8 up to 128,
- *   16-byte aligned rows; HSA_ERR_ARG otherwise).
+ *   16-byte aligned rows; HSA_ERR_ARG otherwise).  `workspace`: hsa_dense_attn_fwd_workspace_bytes(...) bytes (often 0; few
+ *   queries over many keys are cut into ranges of keys that are joined afterwards), 256-byte aligned.
  * Masks come packed (hsa_dense_mask_pack): `mask` points to bytes (0 = may not look), four strides in bytes, of a tensor
  *   [batches, heads, rows, Lk] with batches 1 or B, heads 1 or H, rows 1 or Lq; `packed` receives
  *   hsa_dense_mask_bytes(...) bytes, 256-byte aligned.
@@ -431,6 +432,10 @@ int hsa_dense_attn_bwd(hsa_view Q, hsa_view K, hsa_view V, hsa_view Out, const f
                        hsa_view dK, hsa_view dV, const int *key_lengths, const void *packed_mask, int mask_batches,
                        int mask_heads, int mask_rows, void *workspace, size_t workspace_bytes, int B, int Lq, int Lk, int H,
                        int Hkv, int D, float scale, int dtype, int algo, void *stream);
+
+/* Thread blocks of the tensor-core kernels that gave up a bounded wait on an mbarrier since the library was loaded (current
+ * device); their rows hold NaN.  0 in a healthy run; synchronises. */
+int hsa_dense_attn_aborts(unsigned int *count);
 
 /*
  * Attention of one new token per sequence over a key/value cache that lives in pages: the dense counterpart of

@@ -75,6 +75,15 @@ struct DenseArgs {
     bool vec;                            // rows may be read four elements at a time
 };
 
+inline int dense_sm_count() {
+    int dev = 0, v = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || v <= 0) {
+        (void)cudaGetLastError();
+        return 148;
+    }
+    return v;
+}
+
 __device__ __forceinline__ int dense_keys(const DenseArgs &a, int b) {
     if (a.key_lengths == nullptr) return a.Lk;
     return max(0, min(a.Lk, __ldg(a.key_lengths + b)));      // lengths outside [0, Lk] mean the nearer end

@@ -1,0 +1,498 @@
+// Dense attention forward on the 5th-generation tensor cores (bf16 / f16, head dims up to 128).
+//
+//   out_i = sum_j exp2(c s_ij - m_i) v_j / sum_j exp2(c s_ij - m_i),   s_ij = q_i.k_j,  c = scale log2(e)
+//
+// One pass over the keys with a running maximum and sum.  A block owns 256 query rows of one (batch entry, head) as two tiles
+// of 128 and walks over tiles of 128 keys, 10 warps with fixed roles:
+//   warp 8     copies K and V tiles into a ring (TMA boxes of [128 rows][128 bytes], 128-byte swizzle)
+//   warp 9     issues S = Q K^T (both operands in shared memory) and O += P V (P in tensor memory, V as an MN-major operand)
+//   warps 0-3  and 4-7: the softmax of the first and of the second query tile, a thread per row
+// While one tile's softmax runs, the tensor cores work for the other.  Tensor memory (512 columns): S of both tiles (128 each),
+// O of both tiles (DP each); P replaces S in place as 16-bit numbers, so it never passes through shared memory.
+// The output is rescaled only when a row's maximum has grown by more than 2^8 since the last time (the weights then lie below
+// 2^8, which changes nothing in their relative precision), so almost every tile leaves O alone.
+// Rounding: weights are rounded to the inputs' type for the second product (what the tensor cores take); their sum is taken
+// from the unrounded 32-bit values, and the division by it comes last, in 32 bits.
+// Keys behind a sequence's length and keys that no query may look at: the scores are replaced, and their V rows are zeroed in
+// shared memory, so that NaN there cannot come back as 0 * NaN.
+#include "dense_attn.cuh"
+#include "rng_common.cuh"
+#include "tc5_common.cuh"
+#include "tc_common.cuh"
+#include "tma_common.cuh"
+
+namespace hsa {
+
+constexpr int kFwdThreads = 320;
+constexpr int kFlagTiles = 1024;                 // key tiles whose mask state fits the block's table
+
+__device__ unsigned int g_dense_aborts = 0;
+
+struct DenseSplit {
+    float *part_o, *part_ml;                     // [splits, B, Lq, H, D] and [splits, B, Lq, H, 2] when splits > 1
+    int splits;
+    long long wait_limit;
+};
+
+template <int DP>
+struct FwdShape {
+    static constexpr int kTile = 128 * DP * 2;                       // bytes of a tile of 128 rows
+    static constexpr int kSlots = DP == 128 ? 5 : 8;                 // K and V tiles in flight
+    static constexpr int kSmem = 1024 + 2 * kTile + kSlots * kTile + kFlagTiles + 256;
+};
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kFwdThreads, 1)
+dense_fwd_tc5_kernel(const DenseArgs a, const DenseSplit sp, const __grid_constant__ CUtensorMap map_q,
+                     const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                     const __grid_constant__ CUtensorMap map_o) {
+    using namespace tc5;
+    using Shape = FwdShape<DP>;
+    constexpr int TILE = Shape::kTile, SLOTS = Shape::kSlots, PLANES = DP / 64, PLANE = 128 * 128;
+    constexpr bool BF = std::is_same<T, __nv_bfloat16>::value;
+    constexpr uint32_t IDESC_S = instr_desc(128, 128, BF, false, false), IDESC_O = instr_desc(128, DP, BF, false, true);
+    constexpr uint32_t COL_S = 0, COL_O = 256;
+
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    unsigned char *smem = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
+    unsigned char *q_s = smem, *ring = smem + 2 * TILE;
+    uint8_t *flags = ring + (size_t)SLOTS * TILE;
+    unsigned long long *bars = reinterpret_cast<unsigned long long *>(flags + kFlagTiles);
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 8 + 2 * SLOTS);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+    const uint32_t bar0 = smem_addr(bars);
+    auto q_full = [&](int w) { return bar0 + 8u * w; };
+    auto s_full = [&](int w) { return bar0 + 8u * (2 + w); };
+    auto p_full = [&](int w) { return bar0 + 8u * (4 + w); };
+    auto o_full = [&](int w) { return bar0 + 8u * (6 + w); };
+    auto kv_full = [&](int s) { return bar0 + 8u * (8 + s); };
+    auto kv_empty = [&](int s) { return bar0 + 8u * (8 + SLOTS + s); };
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int qblocks = (a.Lq + 255) / 256;
+    int blk = blockIdx.x;
+    const int q0 = blk % qblocks * 256; blk /= qblocks;
+    const int h = blk % a.H; blk /= a.H;
+    const int b = blk % a.B, split = blk / a.B;
+    const int hk = h / a.group;
+    const int nw = a.Lq - q0 > 128 ? 2 : 1;              // query tiles of this block
+    const int n = dense_keys(a, b);
+    const int tiles_all = (n + 127) / 128, per = (tiles_all + sp.splits - 1) / sp.splits;
+    const int kt0 = min(tiles_all, split * per), kt1 = min(tiles_all, kt0 + per);
+    const int64_t plane = (int64_t)b * a.mask.plane_b + (int64_t)h * a.mask.plane_h;
+    const bool masked = a.mask.bits != nullptr;
+
+    if (threadIdx.x == 0) {
+        for (int w = 0; w < 2; ++w) { mbar_init(q_full(w), 1); mbar_init(s_full(w), 1); mbar_init(p_full(w), 4); mbar_init(o_full(w), 1); }
+        for (int s = 0; s < SLOTS; ++s) { mbar_init(kv_full(s), 1); mbar_init(kv_empty(s), 1); }
+        *abort_flag = 0;
+        mbar_fence_init();
+        prefetch_map(&map_q); prefetch_map(&map_k); prefetch_map(&map_v); prefetch_map(&map_o);
+    }
+    if (masked) {
+        // mask state of this block's key tiles: two bits per query tile
+        for (int t = kt0 + threadIdx.x; t < kt1; t += kFwdThreads) {
+            uint8_t f = 0;
+            for (int w = 0; w < nw; ++w) {
+                const int row = a.mask.rows > 1 ? q0 / kDenseTile + w : 0;
+                f |= a.mask.tiles[(plane * a.mask.tq + row) * a.mask.tk + t] << (2 * w);
+            }
+            flags[t - kt0] = f;
+        }
+    }
+    if (warp == 9) tmem_alloc(smem_addr(tmem_slot), 512);
+    fence_before_sync();
+    __syncthreads();
+    fence_after_sync();
+    const uint32_t tmem = *tmem_slot;
+    // a whole warp waits, and goes on or gives up as one
+    auto wait = [&](uint32_t bar, uint32_t parity) { return (bool)__all_sync(0xffffffffu, mbar_wait(bar, parity, sp.wait_limit, abort_flag)); };
+    auto skip = [&](int t) { return masked && flags[t - kt0] == 0; };
+
+    if (warp == 8) {
+        // ------------------------------------------------------------------------------------------------- copies
+        if (lane == 0) {
+            bool ok = true;
+            int slot = 0; uint32_t ph = 0;
+            bool first = true;
+            auto push = [&](const CUtensorMap *map, int row) {
+                if (!(ok = mbar_wait(kv_empty(slot), ph ^ 1, sp.wait_limit, abort_flag))) return;
+                mbar_expect_tx(kv_full(slot), TILE);
+                const uint32_t dst = smem_addr(ring + (size_t)slot * TILE);
+#pragma unroll
+                for (int p = 0; p < PLANES; ++p) tma_load_4d(dst + p * PLANE, map, p * 64, hk, row, b, kv_full(slot));
+                if (++slot == SLOTS) { slot = 0; ph ^= 1; }
+            };
+            for (int t = kt0; t < kt1 && ok; ++t) {
+                if (skip(t)) continue;
+                if (first) {
+                    for (int w = 0; w < nw; ++w) {
+                        mbar_expect_tx(q_full(w), TILE);
+#pragma unroll
+                        for (int p = 0; p < PLANES; ++p)
+                            tma_load_4d(smem_addr(q_s + w * TILE + p * PLANE), &map_q, p * 64, h, q0 + 128 * w, b, q_full(w));
+                        if (w == 0) push(&map_k, t * 128);
+                    }
+                    first = false;
+                } else {
+                    push(&map_k, t * 128);
+                }
+                if (ok) push(&map_v, t * 128);
+            }
+            if (!ok) {                                   // let copies already issued land before the block goes
+                const long long start = clock64();
+                while (clock64() - start < 200000) {}
+            }
+        }
+    } else if (warp == 9) {
+        // -------------------------------------------------------------------------------------------- matrix products
+        bool ok = true;
+        int slot = 0; uint32_t ph = 0;
+        auto next_slot = [&]() { if (++slot == SLOTS) { slot = 0; ph ^= 1; } };
+        auto issue_s = [&](int w, uint32_t k_addr) {
+            if (lane == 0) {
+                const uint32_t qa = smem_addr(q_s + w * TILE);
+#pragma unroll
+                for (int k = 0; k < DP / 16; ++k) {
+                    const uint32_t off = (k >> 2) * PLANE + (k & 3) * 32;
+                    mma_f16(tmem + COL_S + w * 128, smem_desc(qa + off, 16, 1024), smem_desc(k_addr + off, 16, 1024), IDESC_S, k > 0);
+                }
+                mma_commit(s_full(w));
+            }
+            __syncwarp();
+        };
+        int t = kt0;
+        while (t < kt1 && skip(t)) ++t;
+        if (t < kt1) {
+            int cur = slot;
+            ok = wait(kv_full(cur), ph);
+            for (int w = 0; w < nw && ok; ++w) {
+                if (!(ok = wait(q_full(w), 0))) break;
+                fence_after_sync();
+                issue_s(w, smem_addr(ring + (size_t)cur * TILE));
+            }
+            if (lane == 0) mma_commit(kv_empty(cur));
+            next_slot();
+        }
+        uint32_t par = 0;
+        bool fresh = true;
+        while (t < kt1 && ok) {
+            int tn = t + 1;
+            while (tn < kt1 && skip(tn)) ++tn;
+            const int vs = slot;
+            if (!(ok = wait(kv_full(vs), ph))) break;
+            next_slot();
+            const uint32_t v_addr = smem_addr(ring + (size_t)vs * TILE);
+            // rows of keys that are not there
+            const int left = n - t * 128;
+            if (left < 128 || masked) {
+                uint32_t word[4];
+                bool any = false;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int c = left - 32 * i;
+                    uint32_t keep = c >= 32 ? 0xffffffffu : c <= 0 ? 0u : (1u << c) - 1u;
+                    if (masked) keep &= __ldg(a.mask.seen + plane * a.mask.wk + t * 4 + i);
+                    word[i] = keep;
+                    any |= keep != 0xffffffffu;
+                }
+                if (any) {
+#pragma unroll 4
+                    for (int g = 0; g < 32; ++g) {
+                        const int r = g * 4 + (lane >> 3);
+                        if (!((word[g >> 3] >> (r & 31)) & 1u)) {
+#pragma unroll
+                            for (int p = 0; p < PLANES; ++p)
+                                *reinterpret_cast<uint4 *>(ring + (size_t)vs * TILE + p * PLANE + r * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+                        }
+                    }
+                    fence_async_smem();
+                    __syncwarp();
+                }
+            }
+            const int ks = slot;
+            bool k_ready = false;
+            for (int w = 0; w < nw && ok; ++w) {
+                if (!(ok = wait(p_full(w), par))) break;
+                fence_after_sync();
+                if (lane == 0) {
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        mma_f16_ta(tmem + COL_O + w * DP, tmem + COL_S + w * 128 + k * 8, smem_desc(v_addr + k * 2048, PLANE, 1024), IDESC_O,
+                                   (!fresh || k > 0) ? 1u : 0u);
+                    if (w == nw - 1) mma_commit(kv_empty(vs));       // before the barrier that lets the block end
+                    mma_commit(o_full(w));
+                }
+                __syncwarp();
+                if (tn < kt1) {
+                    if (!k_ready) {
+                        if (!(ok = wait(kv_full(ks), ph))) break;
+                        fence_after_sync();
+                        k_ready = true;
+                    }
+                    issue_s(w, smem_addr(ring + (size_t)ks * TILE));
+                    if (w == nw - 1 && lane == 0) mma_commit(kv_empty(ks));
+                }
+            }
+            if (tn < kt1) next_slot();
+            fresh = false;
+            par ^= 1;
+            t = tn;
+        }
+    } else {
+        // -------------------------------------------------------------------------------------------------- softmax
+        const int w = warp >> 2, quarter = warp & 3;
+        const int row = quarter * 32 + lane, qi = q0 + 128 * w + row;
+        if (w < nw) {
+            bool ok = true;
+            const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+            const uint32_t ts = tmem + COL_S + w * 128 + lanes, to = tmem + COL_O + w * DP + lanes;
+            const uint32_t *bits = masked ? a.mask.bits + (plane * a.mask.rows + (a.mask.rows > 1 ? min(qi, a.Lq - 1) : 0)) * a.mask.wk : nullptr;
+            float m = -INFINITY, l = 0.f;
+            int i = 0;                                       // tiles done
+            for (int t = kt0; t < kt1; ++t) {
+                if (skip(t)) continue;
+                const int left = n - t * 128;
+                const bool partial = left < 128 || (masked && ((flags[t - kt0] >> (2 * w)) & 3) != 2);
+                uint4 words = make_uint4(~0u, ~0u, ~0u, ~0u);
+                if (partial && masked) words = __ldg(reinterpret_cast<const uint4 *>(bits + t * 4));
+                if (!(ok = wait(s_full(w), i & 1))) break;
+                fence_after_sync();
+                uint32_t r[4][32];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) tmem_ld32(ts + 32 * c, r[c]);
+                tmem_ld_wait();
+                float top = -INFINITY;
+                if (partial) {
+                    const uint32_t wd[4] = {words.x, words.y, words.z, words.w};
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        const int k = left - 32 * c;
+                        const uint32_t keep = wd[c] & (k >= 32 ? 0xffffffffu : k <= 0 ? 0u : (1u << k) - 1u);
+#pragma unroll
+                        for (int j = 0; j < 32; ++j)
+                            if (!((keep >> j) & 1u)) r[c][j] = 0xff800000u;
+                    }
+                }
+                float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) tops[c] = fmaxf(tops[c], __uint_as_float(r[c][j]));
+                top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * a.scale_log2;
+                const bool grow = top > m + 8.f;             // also the first finite maximum (m = -inf)
+                if (__any_sync(0xffffffffu, grow)) {
+                    const float m_new = grow ? top : m;
+                    const float corr = grow ? fast_exp2(m - m_new) : 1.f;
+                    if (i > 0) {
+                        if (!(ok = wait(o_full(w), (i - 1) & 1))) break;
+                        fence_after_sync();
+#pragma unroll
+                        for (int c = 0; c < DP / 32; ++c) {
+                            uint32_t o[32];
+                            tmem_ld32(to + 32 * c, o);
+                            tmem_ld_wait();
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * corr);
+                            tmem_st32(to + 32 * c, o);
+                        }
+                        l *= corr;
+                    }
+                    m = m_new;
+                }
+                const float ref = m == -INFINITY ? 0.f : m;
+                float sum[2] = {0.f, 0.f};
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    uint32_t pk[32];
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) {
+                        const int e = 64 * c + 2 * j;
+                        const float p0 = fast_exp2(fmaf(__uint_as_float(r[e >> 5][e & 31]), a.scale_log2, -ref));
+                        const float p1 = fast_exp2(fmaf(__uint_as_float(r[(e + 1) >> 5][(e + 1) & 31]), a.scale_log2, -ref));
+                        sum[0] += p0; sum[1] += p1;
+                        pk[j] = pack2<T>(p0, p1);
+                    }
+                    tmem_st32(ts + 32 * c, pk);
+                }
+                l += sum[0] + sum[1];
+                tmem_st_wait();
+                fence_before_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_full(w));
+                ++i;
+            }
+            // ---------------------------------------------------------------------------------------------- results
+            if (ok && i > 0) ok = wait(o_full(w), (i - 1) & 1);
+            fence_after_sync();
+            if (!ok) { l = __int_as_float(0x7fffffff); m = 0.f; }
+            const bool none = l == 0.f;
+            if (sp.splits > 1) {
+                const int64_t at = (((int64_t)split * a.B + b) * a.Lq + qi) * a.H + h;
+#pragma unroll 1
+                for (int c = 0; c < DP / 32; ++c) {
+                    uint32_t o[32];
+                    if (i > 0) { tmem_ld32(to + 32 * c, o); tmem_ld_wait(); }
+                    if (qi < a.Lq) {
+#pragma unroll
+                        for (int j = 0; j < 32; j += 4)
+                            if (32 * c + j < a.D)
+                                *reinterpret_cast<float4 *>(sp.part_o + at * a.D + 32 * c + j) = i > 0
+                                    ? make_float4(__uint_as_float(o[j]), __uint_as_float(o[j + 1]), __uint_as_float(o[j + 2]), __uint_as_float(o[j + 3]))
+                                    : make_float4(0.f, 0.f, 0.f, 0.f);
+                    }
+                }
+                if (qi < a.Lq) *reinterpret_cast<float2 *>(sp.part_ml + 2 * at) = make_float2(m, l);
+            } else {
+                const float inv = 1.f / l;
+                unsigned char *stg = q_s + w * TILE;             // the queries are not needed any more
+#pragma unroll 1
+                for (int c = 0; c < DP / 32; ++c) {
+                    uint32_t o[32];
+                    if (i > 0) { tmem_ld32(to + 32 * c, o); tmem_ld_wait(); }
+                    unsigned char *line = stg + (c >> 1) * PLANE + row * 128;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        uint32_t v[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int k = 8 * j + 2 * e;
+                            v[e] = none ? pack2<T>(a.empty_value, a.empty_value)
+                                        : pack2<T>(__uint_as_float(o[k]) * inv, __uint_as_float(o[k + 1]) * inv);
+                        }
+                        *reinterpret_cast<uint4 *>(line + ((((c & 1) * 4 + j) ^ (row & 7)) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
+                    }
+                }
+                if (a.lse != nullptr && qi < a.Lq)
+                    a.lse[((int64_t)b * a.Lq + qi) * a.H + h] = none ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+                fence_async_smem();
+                asm volatile("bar.sync %0, 128;\n" ::"r"(1 + w) : "memory");
+                if (row == 0) {
+#pragma unroll
+                    for (int p = 0; p < PLANES; ++p)
+                        if (p * 64 < a.D) tma_store_4d(&map_o, smem_addr(stg + p * PLANE), p * 64, h, q0 + 128 * w, b);
+                    asm volatile("cp.async.bulk.commit_group;\n" ::: "memory");
+                    asm volatile("cp.async.bulk.wait_group 0;\n" ::: "memory");
+                }
+            }
+        }
+    }
+    fence_before_sync();
+    __syncthreads();
+    fence_after_sync();
+    if (warp == 9) tmem_dealloc(tmem, 512);
+    if (threadIdx.x == 0 && *abort_flag) atomicAdd(&g_dense_aborts, 1u);
+}
+
+// Join the ranges of a query row: out = sum 2^(m_s - M) o_s / sum 2^(m_s - M) l_s.
+template <typename T>
+__global__ void __launch_bounds__(128) dense_join_kernel(const DenseArgs a, const DenseSplit sp) {
+    const int64_t rows = (int64_t)a.B * a.Lq * a.H, row = blockIdx.x * 4LL + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    if (row >= rows) return;
+    float M = -INFINITY;
+    for (int s = 0; s < sp.splits; ++s) M = fmaxf(M, sp.part_ml[2 * (s * rows + row)]);
+    const float ref = M == -INFINITY ? 0.f : M;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float L = 0.f;
+    for (int s = 0; s < sp.splits; ++s) {
+        const int64_t at = s * rows + row;
+        const float w = exp2f(sp.part_ml[2 * at] - ref);
+        L = fmaf(w, sp.part_ml[2 * at + 1], L);
+        if (lane * 4 < a.D) {
+            const float4 o = *reinterpret_cast<const float4 *>(sp.part_o + at * a.D + lane * 4);
+            acc.x = fmaf(w, o.x, acc.x); acc.y = fmaf(w, o.y, acc.y); acc.z = fmaf(w, o.z, acc.z); acc.w = fmaf(w, o.w, acc.w);
+        }
+    }
+    const int h = (int)(row % a.H), i = (int)(row / a.H % a.Lq);
+    const int64_t b = row / a.H / a.Lq;
+    const bool none = L == 0.f;
+    const float inv = 1.f / L;
+    if (lane * 4 < a.D) {
+        uint2 v;
+        v.x = none ? pack2<T>(a.empty_value, a.empty_value) : pack2<T>(acc.x * inv, acc.y * inv);
+        v.y = none ? pack2<T>(a.empty_value, a.empty_value) : pack2<T>(acc.z * inv, acc.w * inv);
+        *reinterpret_cast<uint2 *>((T *)a.out.ptr + b * a.out.batch_stride + (int64_t)i * a.out.row_stride + (int64_t)h * a.D + lane * 4) = v;
+    }
+    if (a.lse != nullptr && lane == 0) a.lse[row] = none ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
+}
+
+// Ranges of keys per query block: with few blocks and many key tiles, the count that makes the slowest SM finish first.  A block
+// costs its tiles plus about four tiles' time of set-up and result (twice that when the result is a partial one that is joined).
+int dense_fwd_splits(int B, int Lq, int Lk, int H) {
+    const long long blocks = (long long)B * H * ((Lq + 255) / 256);
+    const int tiles = (Lk + 127) / 128, sms = dense_sm_count();
+    if (blocks * 2 > sms) return 1;
+    double best = 1e30;
+    int best_s = 1;
+    for (int s = 1; s <= 64 && s <= tiles; ++s) {
+        const double waves = (double)((blocks * s + sms - 1) / sms);
+        const double t = waves * ((tiles + s - 1) / s + (s > 1 ? 8.0 : 4.0)) + (s > 1 ? 4.0 : 0.0);
+        if (t < 0.95 * best) { best = t; best_s = s; }
+    }
+    const int per = (tiles + best_s - 1) / best_s;
+    return (tiles + per - 1) / per;
+}
+
+size_t dense_fwd_tc_workspace(int B, int Lq, int Lk, int H, int D) {
+    const int s = dense_fwd_splits(B, Lq, Lk, H);
+    return s > 1 ? (size_t)s * B * Lq * H * (D + 2) * sizeof(float) : 0;
+}
+
+static bool tc_view(const hsa_view &v, int B, int rows, int H, int D) { return view_vec_ok(v, 2) && map_ok(v, B, rows, H, D); }
+
+// bf16 / f16 with head dims in whole 16-byte pieces up to 128, rows a tensor map can describe, and a mask whose tile states
+// fit the block's table.
+bool dense_tc_ok(const DenseArgs &a, int dtype, bool backward) {
+    if ((dtype != HSA_BF16 && dtype != HSA_F16) || a.D % 8 != 0 || a.D > 128) return false;
+    if (a.mask.bits != nullptr && a.mask.tk > kFlagTiles) return false;
+    if (!tc_view(a.q, a.B, a.Lq, a.H, a.D) || !tc_view(a.k, a.B, a.Lk, a.Hkv, a.D) || !tc_view(a.v, a.B, a.Lk, a.Hkv, a.D)) return false;
+    if (!backward) return tc_view(a.out, a.B, a.Lq, a.H, a.D);
+    return tc_view(a.dout, a.B, a.Lq, a.H, a.D) && tc_view(a.dq, a.B, a.Lq, a.H, a.D) && tc_view(a.dk, a.B, a.Lk, a.Hkv, a.D) &&
+           tc_view(a.dv, a.B, a.Lk, a.Hkv, a.D);
+}
+
+template <typename T, int DP>
+static int fwd_launch(const DenseArgs &a, DenseSplit sp, cudaStream_t st) {
+    CUtensorMap mq, mk, mv, mo;
+    if (!make_map(&mq, a.q, a.B, a.Lq, a.H, a.D, 1, 128) || !make_map(&mk, a.k, a.B, a.Lk, a.Hkv, a.D, 1, 128) ||
+        !make_map(&mv, a.v, a.B, a.Lk, a.Hkv, a.D, 1, 128) || !make_map(&mo, a.out, a.B, a.Lq, a.H, a.D, 1, 128))
+        return fail(HSA_ERR_ARG, "hsa_dense_attn_fwd: the driver refused a tensor map");
+    const long long blocks = (long long)a.B * a.H * ((a.Lq + 255) / 256) * sp.splits;
+    if (blocks > 0x7fffffffLL) return fail(HSA_ERR_ARG, "hsa_dense_attn_fwd: too many tiles");
+    auto kernel = dense_fwd_tc5_kernel<T, DP>;
+    constexpr int smem = FwdShape<DP>::kSmem;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return fail((int)e, "hsa_dense_attn_fwd: shared memory %d: %s", smem, cudaGetErrorString(e));
+    kernel<<<(unsigned)blocks, kFwdThreads, smem, st>>>(a, sp, mq, mk, mv, mo);
+    if (int rc = launch_status("hsa_dense_attn_fwd")) return rc;
+    if (sp.splits == 1) return 0;
+    const long long rows = (long long)a.B * a.Lq * a.H;
+    dense_join_kernel<T><<<(unsigned)((rows + 3) / 4), 128, 0, st>>>(a, sp);
+    return launch_status("hsa_dense_attn_fwd(join)");
+}
+
+int dense_fwd_tc(const DenseArgs &a, void *workspace, size_t workspace_bytes, int dtype, cudaStream_t st) {
+    DenseSplit sp{};
+    sp.splits = dense_fwd_splits(a.B, a.Lq, a.Lk, a.H);
+    sp.wait_limit = wait_limit_cycles();
+    if (sp.splits > 1) {
+        const size_t need = dense_fwd_tc_workspace(a.B, a.Lq, a.Lk, a.H, a.D);
+        if (workspace == nullptr || workspace_bytes < need)
+            return fail(HSA_ERR_WORKSPACE, "hsa_dense_attn_fwd: workspace of %zu bytes needed, %zu given", need, workspace_bytes);
+        if (reinterpret_cast<uintptr_t>(workspace) & 255u) return fail(HSA_ERR_ALIGN, "hsa_dense_attn_fwd: workspace must be 256-byte aligned");
+        sp.part_o = (float *)workspace;
+        sp.part_ml = sp.part_o + (size_t)sp.splits * a.B * a.Lq * a.H * a.D;
+    }
+    if (dtype == HSA_BF16)
+        return a.D <= 64 ? fwd_launch<__nv_bfloat16, 64>(a, sp, st) : fwd_launch<__nv_bfloat16, 128>(a, sp, st);
+    return a.D <= 64 ? fwd_launch<__half, 64>(a, sp, st) : fwd_launch<__half, 128>(a, sp, st);
+}
+
+}  // namespace hsa
+
+extern "C" int hsa_dense_attn_aborts(unsigned int *count) {
+    if (count == nullptr) return hsa::fail(HSA_ERR_ARG, "hsa_dense_attn_aborts: null pointer");
+    cudaError_t e = cudaMemcpyFromSymbol(count, hsa::g_dense_aborts, sizeof(unsigned int));
+    return e == cudaSuccess ? 0 : hsa::fail((int)e, "hsa_dense_attn_aborts: %s", cudaGetErrorString(e));
+}

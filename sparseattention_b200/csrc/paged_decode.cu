@@ -230,15 +230,6 @@ static int paged_simt(const PagedArgs &a, cudaStream_t st) {
     return heads.template operator()<32, 2>();
 }
 
-static int sm_count_here() {
-    int dev = 0, v = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || v <= 0) {
-        (void)cudaGetLastError();
-        return 148;
-    }
-    return v;
-}
-
 }  // namespace hsa
 
 using namespace hsa;
@@ -247,7 +238,7 @@ using namespace hsa;
 extern "C" int hsa_paged_attn_choose_splits(int B, int H, int Hkv, int page_size, int max_pages) {
     if (B < 1 || H < 1 || Hkv < 1 || page_size < 1 || max_pages < 1) return 1;
     const long long units = (long long)B * Hkv, room = (long long)max_pages * page_size;
-    const long long want = (4LL * sm_count_here() + units - 1) / units, most = (room + 255) / 256;
+    const long long want = (4LL * dense_sm_count() + units - 1) / units, most = (room + 255) / 256;
     const long long s = want < most ? want : most;
     return (int)(s < 1 ? 1 : s > 128 ? 128 : s);
 }

@@ -7,6 +7,7 @@ Softmax statistics and sums are float32; the backward is deterministic (one writ
 """
 from __future__ import annotations
 
+import ctypes
 import math
 from ctypes import c_void_p
 from typing import Optional
@@ -91,6 +92,18 @@ def _lengths32(lengths, B: int, top: int, dev, name: str):
     return lengths if lengths.is_contiguous() else lengths.contiguous()
 
 
+def dense_aborts() -> int:
+    """Thread blocks of the tensor-core kernels that gave up a bounded wait (0 in a healthy run); synchronises."""
+    count = ctypes.c_uint(0)
+    _lib.check(_lib.load().hsa_dense_attn_aborts(ctypes.byref(count)), "hsa_dense_attn_aborts")
+    return int(count.value)
+
+
+def _debug_check(what: str) -> None:
+    if _lib.DEBUG and not torch.cuda.is_current_stream_capturing() and dense_aborts():
+        raise _lib.HsaError(f"{what}: a thread block gave up waiting; its rows hold NaN")
+
+
 def _ptr(t: Optional[torch.Tensor]):
     return None if t is None else c_void_p(t.data_ptr())
 
@@ -113,6 +126,7 @@ def dense_attention_forward(q, k, v, key_lengths=None, packed_mask=None, scale: 
                                     *(packed_mask.sizes if packed_mask is not None else (0, 0, 0)), _ptr(ws), need,
                                     B, Lq, Lk, H, Hkv, D, scale, empty_value, dt, algo, _lib.stream_ptr(dev))
     _lib.check(rc, "hsa_dense_attn_fwd")
+    _debug_check("hsa_dense_attn_fwd")
     return out, lse
 
 
@@ -134,6 +148,7 @@ def dense_attention_backward(q, k, v, out, lse, dout, key_lengths=None, packed_m
                                     *(packed_mask.sizes if packed_mask is not None else (0, 0, 0)), _ptr(ws), need,
                                     B, Lq, Lk, H, Hkv, D, scale, _lib.dtype_code(q), algo, _lib.stream_ptr(dev))
     _lib.check(rc, "hsa_dense_attn_bwd")
+    _debug_check("hsa_dense_attn_bwd")
     return dq, dk, dv
 
 
