@@ -6,6 +6,8 @@ namespace hsa {
 int dense_simt(const DenseArgs &a, int what, int dtype, cudaStream_t st);
 bool dense_tc_ok(const DenseArgs &a, int dtype, bool backward);
 size_t dense_fwd_tc_workspace(int B, int Lq, int Lk, int H, int D);
+bool dense_bwd_tables_ok(const DenseArgs &a);
+int dense_bwd_tc(const DenseArgs &a, int dtype, cudaStream_t st);
 int dense_fwd_tc(const DenseArgs &a, void *workspace, size_t workspace_bytes, int dtype, cudaStream_t st);
 
 // ------------------------------------------------------------------------------------------------------------ mask
@@ -202,9 +204,11 @@ extern "C" int hsa_dense_attn_bwd(hsa_view Q, hsa_view K, hsa_view V, hsa_view O
     const int es = dtype_size(dtype);
     a.vec = D % 4 == 0;
     for (const hsa_view &v : {Q, K, V, dOut, dQ, dK, dV}) a.vec = a.vec && rows_in_fours(v, es);
-    HSA_CHECK_ARG(algo != 2, "hsa_dense_attn_bwd: no tensor-core kernel for these inputs");
+    const bool tc = algo != 1 && dense_tc_ok(a, dtype, true) && dense_bwd_tables_ok(a);
+    HSA_CHECK_ARG(algo != 2 || tc, "hsa_dense_attn_bwd: no tensor-core kernel for these inputs");
     cudaStream_t st = (cudaStream_t)stream;
     if (int rc = dense_delta(a, lse2, delta, dtype, D % (16 / es) == 0 && view_vec_ok(Out, es) && view_vec_ok(dOut, es), st)) return rc;
+    if (tc) return dense_bwd_tc(a, dtype, st);
     if (int rc = dense_simt(a, 1, dtype, st)) return rc;
     return dense_simt(a, 2, dtype, st);
 }

@@ -15,16 +15,9 @@
 // from the unrounded 32-bit values, and the division by it comes last, in 32 bits.
 // Keys behind a sequence's length and keys that no query may look at: the scores are replaced, and their V rows are zeroed in
 // shared memory, so that NaN there cannot come back as 0 * NaN.
-#include "dense_attn.cuh"
-#include "rng_common.cuh"
-#include "tc5_common.cuh"
-#include "tc_common.cuh"
-#include "tma_common.cuh"
+#include "dense_attn_tc.cuh"
 
 namespace hsa {
-
-constexpr int kFwdThreads = 320;
-constexpr int kFlagTiles = 1024;                 // key tiles whose mask state fits the block's table
 
 __device__ unsigned int g_dense_aborts = 0;
 
@@ -42,7 +35,7 @@ struct FwdShape {
 };
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(kFwdThreads, 1)
+__global__ void __launch_bounds__(kTcThreads, 1)
 dense_fwd_tc5_kernel(const DenseArgs a, const DenseSplit sp, const __grid_constant__ CUtensorMap map_q,
                      const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                      const __grid_constant__ CUtensorMap map_o) {
@@ -91,7 +84,7 @@ dense_fwd_tc5_kernel(const DenseArgs a, const DenseSplit sp, const __grid_consta
     }
     if (masked) {
         // mask state of this block's key tiles: two bits per query tile
-        for (int t = kt0 + threadIdx.x; t < kt1; t += kFwdThreads) {
+        for (int t = kt0 + threadIdx.x; t < kt1; t += kTcThreads) {
             uint8_t f = 0;
             for (int w = 0; w < nw; ++w) {
                 const int row = a.mask.rows > 1 ? q0 / kDenseTile + w : 0;
@@ -185,31 +178,8 @@ dense_fwd_tc5_kernel(const DenseArgs a, const DenseSplit sp, const __grid_consta
             const uint32_t v_addr = smem_addr(ring + (size_t)vs * TILE);
             // rows of keys that are not there
             const int left = n - t * 128;
-            if (left < 128 || masked) {
-                uint32_t word[4];
-                bool any = false;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int c = left - 32 * i;
-                    uint32_t keep = c >= 32 ? 0xffffffffu : c <= 0 ? 0u : (1u << c) - 1u;
-                    if (masked) keep &= __ldg(a.mask.seen + plane * a.mask.wk + t * 4 + i);
-                    word[i] = keep;
-                    any |= keep != 0xffffffffu;
-                }
-                if (any) {
-#pragma unroll 4
-                    for (int g = 0; g < 32; ++g) {
-                        const int r = g * 4 + (lane >> 3);
-                        if (!((word[g >> 3] >> (r & 31)) & 1u)) {
-#pragma unroll
-                            for (int p = 0; p < PLANES; ++p)
-                                *reinterpret_cast<uint4 *>(ring + (size_t)vs * TILE + p * PLANE + r * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
-                        }
-                    }
-                    fence_async_smem();
-                    __syncwarp();
-                }
-            }
+            if (left < 128 || masked)
+                zero_hidden_rows<PLANES>(ring + (size_t)vs * TILE, left, masked ? a.mask.seen + plane * a.mask.wk + t * 4 : nullptr, lane);
             const int ks = slot;
             bool k_ready = false;
             for (int w = 0; w < nw && ok; ++w) {
@@ -267,8 +237,7 @@ dense_fwd_tc5_kernel(const DenseArgs a, const DenseSplit sp, const __grid_consta
                     const uint32_t wd[4] = {words.x, words.y, words.z, words.w};
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
-                        const int k = left - 32 * c;
-                        const uint32_t keep = wd[c] & (k >= 32 ? 0xffffffffu : k <= 0 ? 0u : (1u << k) - 1u);
+                        const uint32_t keep = wd[c] & tail_word(left, c);
 #pragma unroll
                         for (int j = 0; j < 32; ++j)
                             if (!((keep >> j) & 1u)) r[c][j] = 0xff800000u;
@@ -371,8 +340,7 @@ dense_fwd_tc5_kernel(const DenseArgs a, const DenseSplit sp, const __grid_consta
 #pragma unroll
                     for (int p = 0; p < PLANES; ++p)
                         if (p * 64 < a.D) tma_store_4d(&map_o, smem_addr(stg + p * PLANE), p * 64, h, q0 + 128 * w, b);
-                    asm volatile("cp.async.bulk.commit_group;\n" ::: "memory");
-                    asm volatile("cp.async.bulk.wait_group 0;\n" ::: "memory");
+                    bulk_store_done();
                 }
             }
         }
@@ -464,7 +432,7 @@ static int fwd_launch(const DenseArgs &a, DenseSplit sp, cudaStream_t st) {
     constexpr int smem = FwdShape<DP>::kSmem;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return fail((int)e, "hsa_dense_attn_fwd: shared memory %d: %s", smem, cudaGetErrorString(e));
-    kernel<<<(unsigned)blocks, kFwdThreads, smem, st>>>(a, sp, mq, mk, mv, mo);
+    kernel<<<(unsigned)blocks, kTcThreads, smem, st>>>(a, sp, mq, mk, mv, mo);
     if (int rc = launch_status("hsa_dense_attn_fwd")) return rc;
     if (sp.splits == 1) return 0;
     const long long rows = (long long)a.B * a.Lq * a.H;
@@ -491,8 +459,13 @@ int dense_fwd_tc(const DenseArgs &a, void *workspace, size_t workspace_bytes, in
 
 }  // namespace hsa
 
+namespace hsa { cudaError_t dense_bwd_aborts(unsigned int *count); }
+
 extern "C" int hsa_dense_attn_aborts(unsigned int *count) {
     if (count == nullptr) return hsa::fail(HSA_ERR_ARG, "hsa_dense_attn_aborts: null pointer");
+    unsigned int bwd = 0;
     cudaError_t e = cudaMemcpyFromSymbol(count, hsa::g_dense_aborts, sizeof(unsigned int));
+    if (e == cudaSuccess) e = hsa::dense_bwd_aborts(&bwd);
+    if (e == cudaSuccess) *count += bwd;
     return e == cudaSuccess ? 0 : hsa::fail((int)e, "hsa_dense_attn_aborts: %s", cudaGetErrorString(e));
 }
