@@ -188,27 +188,250 @@ __global__ void __launch_bounds__(kPagedWarps * 32) paged_decode_simt_kernel(con
     }
 }
 
-// ------------------------------------------------------------------------------------------------------------ join
-template <typename T>
-__global__ void __launch_bounds__(128) paged_join_kernel(const PagedArgs a) {
-    asm volatile("griddepcontrol.wait;\n" ::: "memory");       // launched while the ranges still run: their sums come first
-    const int64_t bh = blockIdx.x;
-    const int b = (int)(bh / a.H), h = (int)(bh % a.H);
-    const int64_t rows = (int64_t)a.B * a.H;
-    float M = -INFINITY;
-    for (int s = 0; s < a.splits; ++s) M = fmaxf(M, a.part_ml[2 * (s * rows + bh)]);
-    const float ref = M == -INFINITY ? 0.f : M;
-    for (int c = threadIdx.x; c < a.D; c += 128) {
-        float L = 0.f, acc = 0.f;
-        for (int s = 0; s < a.splits; ++s) {
-            const int64_t row = s * rows + bh;
-            const float w = exp2f(a.part_ml[2 * row] - ref);    // 0 for a range without keys
-            L = fmaf(w, a.part_ml[2 * row + 1], L);
-            acc = fmaf(w, a.part_o[row * a.D + c], acc);
+// ------------------------------------------------------------------------------- bf16 / f16, 16 query heads at a time
+// A warp takes 16 keys at a time through its own ring of cp.async stages (no barrier in the loop): scores and weighted sums are
+// m16n8k16 products whose 16 rows are the query heads that share the key head (rows behind them are zeros).  Half-empty tiles
+// cost nothing here: a 4 KB step of K takes 16 products, far less than HBM needs to deliver it.  Rows are 16-byte pieces
+// swizzled by the row number, which keeps ldmatrix free of bank conflicts.  The running maximum is raised, and the sums
+// rescaled, only when a score exceeds it by 2^8.  Weights are rounded to the type for the second product; their sum is not.
+template <int DP> struct PagedShape {
+    static constexpr int kStages = DP == 64 ? 6 : 3;
+    static constexpr int kStage = 2 * 16 * DP * 2;                               // 16 rows of K and of V
+    static constexpr int kSmem = kPagedWarps * kStages * kStage + 2 * kPagedWarps * 16 * 4;
+};
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kPagedWarps * 32) paged_decode_mma_kernel(const PagedArgs a) {
+    using Shape = PagedShape<DP>;
+    constexpr int ST = Shape::kStages, CPR = DP / 8, PIECES = 16 * CPR / 32;
+    extern __shared__ __align__(128) unsigned char smem[];
+    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+    const int chunks = (a.group + 15) / 16;
+    const int split = blockIdx.x % a.splits, gc = blockIdx.x / a.splits % chunks;
+    const int hk = blockIdx.x / a.splits / chunks % a.Hkv, b = blockIdx.x / a.splits / chunks / a.Hkv;
+    const int h0 = hk * a.group + gc * 16, heads = min(16, a.group - gc * 16);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quad = lane & 3, grow = lane >> 2;
+    unsigned char *ring = smem + warp * ST * Shape::kStage;
+    float *ml = reinterpret_cast<float *>(smem + kPagedWarps * ST * Shape::kStage);       // [warps][2][16]
+    int k0, k1;
+    bool bad = !split_range(a, b, split, k0, k1);
+    const int steps = (k1 - k0 + 63) / 64;                       // of 16 keys per warp
+
+    // where the row that this lane looks up (lane & 15) of step t lies; page < 0: no such key
+    auto look_up = [&](int t, int &page, int &slot) {
+        const int key = k0 + (t * kPagedWarps + warp) * 16 + (lane & 15);
+        page = -1; slot = 0;
+        if (t < steps && key < k1) {
+            int index;
+            split_page(a, key, index, slot);
+            page = __ldg(a.table + b * a.table_stride + index);
+            if (page < 0 || page >= a.num_pages) { bad = true; page = -1; }
         }
-        T *out = (T *)a.out.ptr + b * a.out.batch_stride + (int64_t)h * a.D;
-        out[c] = Traits<T>::from_f(L == 0.f ? 0.f : acc / L);
+    };
+    const T *kb = (const T *)a.k.ptr + (int64_t)hk * a.D, *vb = (const T *)a.v.ptr + (int64_t)hk * a.D;
+    auto stage_in = [&](int st, int page, int slot) {
+        const uint32_t dst = smem_u32(ring + st * Shape::kStage);
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+            const int c = i * 32 + lane, r = c / CPR, ch = c % CPR;
+            const int pg = __shfl_sync(0xffffffffu, page, r), sl = __shfl_sync(0xffffffffu, slot, r);
+            const bool there = pg >= 0 && ch * 8 < a.D;
+            const int64_t ko = there ? (int64_t)pg * a.k.batch_stride + (int64_t)sl * a.k.row_stride + ch * 8 : 0;
+            const int64_t vo = there ? (int64_t)pg * a.v.batch_stride + (int64_t)sl * a.v.row_stride + ch * 8 : 0;
+            const uint32_t at = dst + r * (DP * 2) + ((ch ^ (r & 7)) << 4);
+            cp_async16(at, kb + ko, there);
+            cp_async16(at + 16 * DP * 2, vb + vo, there);
+        }
+    };
+    int page, slot;
+#pragma unroll
+    for (int t = 0; t < ST - 1; ++t) {
+        look_up(t, page, slot);
+        stage_in(t, page, slot);
+        cp_async_commit();
     }
+    look_up(ST - 1, page, slot);                                 // one step ahead of its copies: the table's latency is hidden
+
+    uint32_t q[DP / 16][4];
+    {
+        const T *Q = (const T *)a.q.ptr + b * a.q.batch_stride + (int64_t)h0 * a.D;
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int row = grow + (e & 1) * 8, col = k * 16 + (e >> 1) * 8 + quad * 2;
+                q[k][e] = row < heads && col < a.D ? ldg32(Q + (int64_t)row * a.D + col) : 0u;
+            }
+    }
+    float o[DP / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < DP / 8; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
+
+    int st = 0, st_in = ST - 1;
+    for (int t = 0; t < steps; ++t) {
+        cp_async_wait<ST - 2>();
+        __syncwarp();                                            // everybody's pieces of this step, and nobody reads the next target any more
+        stage_in(st_in, page, slot);
+        cp_async_commit();
+        look_up(t + ST, page, slot);
+        const uint32_t kt = smem_u32(ring + st * Shape::kStage), vt = kt + 16 * DP * 2;
+        if (++st == ST) st = 0;
+        if (++st_in == ST) st_in = 0;
+        const int base = k0 + (t * kPagedWarps + warp) * 16;
+        if (base >= k1) continue;                                // the last step has keys for some of the warps only
+        float s[2][4] = {};
+        const int mi = lane >> 3, mr = lane & 7;
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k) {
+            uint32_t f[4];
+            ldmatrix_x4(f, kt + ((mi >> 1) * 8 + mr) * (DP * 2) + (((k * 2 + (mi & 1)) ^ mr) << 4));
+            mma16816<T>(s[0], q[k], f[0], f[1]);
+            mma16816<T>(s[1], q[k], f[2], f[3]);
+        }
+        float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int key = base + n * 8 + quad * 2 + (e & 1);
+                s[n][e] = key < k1 ? s[n][e] * a.scale_log2 : -INFINITY;
+                top[e >> 1] = fmaxf(top[e >> 1], s[n][e]);
+            }
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
+            top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
+        }
+        if (__any_sync(0xffffffffu, top[0] > m[0] + 8.f || top[1] > m[1] + 8.f)) {
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const float up = fmaxf(m[r], top[r]), corr = up == -INFINITY ? 1.f : fast_exp2(m[r] - up);
+                m[r] = up;
+                l[r] *= corr;
+#pragma unroll
+                for (int i = 0; i < DP / 8; ++i) { o[i][2 * r] *= corr; o[i][2 * r + 1] *= corr; }
+            }
+        }
+        const float ref[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                s[n][e] = fast_exp2(s[n][e] - ref[e >> 1]);
+                l[e >> 1] += s[n][e];
+            }
+        const uint32_t p[4] = {pack2<T>(s[0][0], s[0][1]), pack2<T>(s[0][2], s[0][3]), pack2<T>(s[1][0], s[1][1]), pack2<T>(s[1][2], s[1][3])};
+#pragma unroll
+        for (int d = 0; d < DP / 16; ++d) {
+            uint32_t f[4];
+            ldmatrix_x4_trans(f, vt + ((mi & 1) * 8 + mr) * (DP * 2) + (((d * 2 + (mi >> 1)) ^ mr) << 4));
+            mma16816<T>(o[2 * d], p, f[0], f[1]);
+            mma16816<T>(o[2 * d + 1], p, f[2], f[3]);
+        }
+    }
+    cp_async_wait<0>();
+    __syncwarp();
+    // the warps' sums meet in the room of their rings
+    float *mine = reinterpret_cast<float *>(ring);
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+        if (quad == 0) { ml[warp * 32 + grow + 8 * r] = m[r]; ml[warp * 32 + 16 + grow + 8 * r] = l[r]; }
+#pragma unroll
+        for (int i = 0; i < DP / 8; ++i)
+            *reinterpret_cast<float2 *>(mine + (grow + 8 * r) * DP + i * 8 + quad * 2) = make_float2(o[i][2 * r], o[i][2 * r + 1]);
+    }
+    const bool any_bad = __syncthreads_or(bad);
+    const int fours = a.D / 4;
+    for (int idx = threadIdx.x; idx < heads * fours; idx += kPagedWarps * 32) {
+        const int i = idx / fours, c = idx % fours * 4;
+        float M = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kPagedWarps; ++w) M = fmaxf(M, ml[w * 32 + i]);
+        const float ref = M == -INFINITY ? 0.f : M;
+        float L = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < kPagedWarps; ++w) {
+            const float f = fast_exp2(ml[w * 32 + i] - ref);
+            const float4 x = *reinterpret_cast<const float4 *>(reinterpret_cast<float *>(smem + w * ST * Shape::kStage) + i * DP + c);
+            L = fmaf(f, ml[w * 32 + 16 + i], L);
+            acc.x = fmaf(f, x.x, acc.x); acc.y = fmaf(f, x.y, acc.y); acc.z = fmaf(f, x.z, acc.z); acc.w = fmaf(f, x.w, acc.w);
+        }
+        if (any_bad) { L = NAN; M = 0.f; acc = make_float4(NAN, NAN, NAN, NAN); }
+        if (a.splits == 1) {
+            const float inv = L == 0.f ? 0.f : 1.f / L;
+            *reinterpret_cast<uint2 *>((T *)a.out.ptr + b * a.out.batch_stride + (int64_t)(h0 + i) * a.D + c) =
+                make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
+        } else {
+            const int64_t row = ((int64_t)split * a.B + b) * a.H + h0 + i;
+            *reinterpret_cast<float4 *>(a.part_o + row * a.D + c) = acc;
+            if (c == 0) *reinterpret_cast<float2 *>(a.part_ml + 2 * row) = make_float2(M, L);
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------------ join
+// A block per output row; its eight warps take every eighth range and meet in shared memory.
+constexpr int kJoinWarps = 8;
+template <typename T>
+__global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const PagedArgs a) {
+    __shared__ float so[kJoinWarps][256], sm[kJoinWarps], sl[kJoinWarps];
+    asm volatile("griddepcontrol.wait;\n" ::: "memory");       // launched while the ranges still run: their sums come first
+    const int64_t bh = blockIdx.x, rows = (int64_t)a.B * a.H;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    float M = -INFINITY;
+    for (int s = warp + lane * kJoinWarps; s < a.splits; s += 32 * kJoinWarps) M = fmaxf(M, a.part_ml[2 * (s * rows + bh)]);
+#pragma unroll
+    for (int w = 16; w > 0; w >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, w));
+    const float ref = M == -INFINITY ? 0.f : M;
+    float L = 0.f, acc[8] = {};
+#pragma unroll 4
+    for (int s = warp; s < a.splits; s += kJoinWarps) {
+        const int64_t row = s * rows + bh;
+        const float w = exp2f(a.part_ml[2 * row] - ref);        // 0 for a range without keys
+        L = fmaf(w, a.part_ml[2 * row + 1], L);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (j * 32 + lane < a.D) acc[j] = fmaf(w, a.part_o[row * a.D + j * 32 + lane], acc[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) so[warp][j * 32 + lane] = acc[j];
+    if (lane == 0) { sm[warp] = M; sl[warp] = L; }
+    __syncthreads();
+    M = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) M = fmaxf(M, sm[w]);
+    const float base = M == -INFINITY ? 0.f : M;
+    for (int c = threadIdx.x; c < a.D; c += kJoinWarps * 32) {
+        float total = 0.f, x = 0.f;
+#pragma unroll
+        for (int w = 0; w < kJoinWarps; ++w) {
+            const float f = exp2f(sm[w] - base);
+            total = fmaf(f, sl[w], total);
+            x = fmaf(f, so[w][c], x);
+        }
+        T *out = (T *)a.out.ptr + (bh / a.H) * a.out.batch_stride + (bh % a.H) * a.D;
+        out[c] = Traits<T>::from_f(total == 0.f ? 0.f : x / total);
+    }
+}
+
+template <typename T>
+static int paged_mma(const PagedArgs &a, cudaStream_t st) {
+    const long long blocks = (long long)a.B * a.Hkv * ((a.group + 15) / 16) * a.splits;
+    if (blocks > 0x7fffffffLL) return fail(HSA_ERR_ARG, "hsa_paged_attn_decode: too many blocks");
+    auto go = [&](auto kernel, int smem) -> int {
+        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e != cudaSuccess) return fail((int)e, "hsa_paged_attn_decode: shared memory %d: %s", smem, cudaGetErrorString(e));
+        kernel<<<(unsigned)blocks, kPagedWarps * 32, smem, st>>>(a);
+        return launch_status("hsa_paged_attn_decode");
+    };
+    if (a.D <= 64) return go(paged_decode_mma_kernel<T, 64>, PagedShape<64>::kSmem);
+    if (a.D <= 128) return go(paged_decode_mma_kernel<T, 128>, PagedShape<128>::kSmem);
+    return go(paged_decode_mma_kernel<T, 256>, PagedShape<256>::kSmem);
 }
 
 template <typename T>
@@ -276,14 +499,29 @@ extern "C" int hsa_paged_attn_decode(hsa_view q, hsa_view k_pages, hsa_view v_pa
     a.page = page_size; a.page_shift = (page_size & (page_size - 1)) == 0 ? ilog2((unsigned)page_size) : -1;
     a.num_pages = num_pages; a.max_pages = max_pages; a.splits = splits;
     a.scale_log2 = scale * 1.4426950408889634f;
-    HSA_CHECK_ARG(algo != 2, "hsa_paged_attn_decode: no tensor-core kernel for these inputs");
+    // Whole 16-byte pieces everywhere: the tensor-core kernel
+    const bool mma = algo != 1 && dtype != HSA_F32 && D % 8 == 0 && view_vec_ok(k_pages, 2) && view_vec_ok(v_pages, 2) &&
+                     view_vec_ok(hsa_view{q.ptr, q.batch_stride, 0}, 2) && view_vec_ok(hsa_view{out.ptr, out.batch_stride, 0}, 2);
+    HSA_CHECK_ARG(algo != 2 || mma, "hsa_paged_attn_decode: no tensor-core kernel for these inputs");
     cudaStream_t st = (cudaStream_t)stream;
-    const int rc = dispatch_dtype(dtype, [&]<typename T>() -> int { return paged_simt<T>(a, st); });
+    int rc;
+    if (mma) rc = dtype == HSA_BF16 ? paged_mma<__nv_bfloat16>(a, st) : paged_mma<__half>(a, st);
+    else rc = dispatch_dtype(dtype, [&]<typename T>() -> int { return paged_simt<T>(a, st); });
     if (rc != 0 || splits == 1) return rc;
     const long long rows = (long long)B * H;
     HSA_CHECK_ARG(rows <= 0x7fffffffLL, "hsa_paged_attn_decode: too many rows");
     return dispatch_dtype(dtype, [&]<typename T>() -> int {
-        paged_join_kernel<T><<<(unsigned)rows, 128, 0, st>>>(a);
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3((unsigned)rows);
+        cfg.blockDim = dim3(kJoinWarps * 32);
+        cfg.stream = st;
+        cudaLaunchAttribute attr;
+        attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr.val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = &attr;
+        cfg.numAttrs = 1;
+        const cudaError_t e = cudaLaunchKernelEx(&cfg, paged_join_kernel<T>, a);
+        if (e != cudaSuccess) return fail((int)e, "hsa_paged_attn_decode(join): %s", cudaGetErrorString(e));
         return launch_status("hsa_paged_attn_decode(join)");
     });
 }
