@@ -225,4 +225,5 @@ def on_device(dev: torch.device):
 
 
 def stream_ptr(dev: torch.device) -> c_void_p:
-    return c_void_p(torch.cuda.current_stream(dev).cuda_stream)
+    idx = dev.index
+    return c_void_p(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if idx is None else idx))

@@ -159,6 +159,8 @@ extern "C" int hsa_dense_attn_fwd(hsa_view Q, hsa_view K, hsa_view V, hsa_view O
     if (int rc = check_shape("hsa_dense_attn_fwd", B, Lq, Lk, H, Hkv, D, scale, dtype, algo)) return rc;
     if (int rc = check_mask("hsa_dense_attn_fwd", packed_mask, mask_batches, mask_heads, mask_rows, B, H, Lq)) return rc;
     DenseArgs a{};
+    Q = dense_view(Q, B, Lq, H, D); Out = dense_view(Out, B, Lq, H, D);
+    K = dense_view(K, B, Lk, Hkv, D); V = dense_view(V, B, Lk, Hkv, D);
     a.q = Q; a.k = K; a.v = V; a.out = Out; a.lse = LSE;
     a.key_lengths = key_lengths;
     a.mask = dense_mask_view(packed_mask, mask_batches, mask_heads, mask_rows, Lk);
@@ -192,6 +194,8 @@ extern "C" int hsa_dense_attn_bwd(hsa_view Q, hsa_view K, hsa_view V, hsa_view O
         return fail(HSA_ERR_WORKSPACE, "hsa_dense_attn_bwd: workspace of %zu bytes needed, %zu given", need, workspace_bytes);
     if (reinterpret_cast<uintptr_t>(workspace) & 255u) return fail(HSA_ERR_ALIGN, "hsa_dense_attn_bwd: workspace must be 256-byte aligned");
     DenseArgs a{};
+    for (hsa_view *v : {&Q, &Out, &dOut, &dQ}) *v = dense_view(*v, B, Lq, H, D);
+    for (hsa_view *v : {&K, &V, &dK, &dV}) *v = dense_view(*v, B, Lk, Hkv, D);
     a.q = Q; a.k = K; a.v = V; a.out = Out; a.dout = dOut; a.dq = dQ; a.dk = dK; a.dv = dV;
     a.lse = const_cast<float *>(LSE);
     a.key_lengths = key_lengths;

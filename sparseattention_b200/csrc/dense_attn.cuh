@@ -75,6 +75,13 @@ struct DenseArgs {
     bool vec;                            // rows may be read four elements at a time
 };
 
+// Strides of dimensions of one entry as a packed tensor would have them (nothing is addressed through them)
+inline hsa_view dense_view(hsa_view v, int B, int rows, int H, int D) {
+    if (rows == 1) v.row_stride = (int64_t)H * D;
+    if (B == 1) v.batch_stride = (int64_t)rows * v.row_stride;
+    return v;
+}
+
 inline int dense_sm_count() {
     int dev = 0, v = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || v <= 0) {

@@ -10,7 +10,7 @@ from __future__ import annotations
 import ctypes
 import math
 from ctypes import c_void_p
-from typing import Optional
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -21,61 +21,69 @@ from .. import _lib
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """`t` [B, rows, heads, D] itself when its rows are packed, separate and aligned for vector loads, else a copy."""
     B, rows, heads, D = t.shape
-    packed = _lib.inner_contiguous(t) and (rows == 1 or t.stride(1) >= heads * D) and (
-        B == 1 or t.stride(0) >= (rows - 1) * t.stride(1) + heads * D)
     vec = 16 // t.element_size()
-    if packed and D % vec == 0:
-        packed = t.data_ptr() % 16 == 0 and (rows == 1 or t.stride(1) % vec == 0) and (B == 1 or t.stride(0) % vec == 0)
-    return t if packed else t.clone(memory_format=torch.contiguous_format)
+    if t.is_contiguous():
+        ok = t.data_ptr() % 16 == 0 or D % vec != 0
+    else:
+        bs, rs = t.stride()[:2]
+        ok = _lib.inner_contiguous(t) and (rows == 1 or rs >= heads * D) and (B == 1 or bs >= (rows - 1) * rs + heads * D)
+        if ok and D % vec == 0:
+            ok = t.data_ptr() % 16 == 0 and (rows == 1 or rs % vec == 0) and (B == 1 or bs % vec == 0)
+    return t if ok else t.clone(memory_format=torch.contiguous_format)
 
 
 def _view(t: torch.Tensor) -> _lib.HsaView:
-    """View of a [B, rows, heads, D] tensor; strides of dimensions of one entry are what a packed tensor would have."""
-    B, rows, heads, D = t.shape
-    rs = t.stride(1) if rows > 1 else heads * D
-    return _lib.HsaView(t.data_ptr(), t.stride(0) if B > 1 else rows * rs, rs)
+    strides = t.stride()
+    return _lib.HsaView(t.data_ptr(), strides[0], strides[1])
 
 
-class _PackedMask:
-    """A mask in the bit form of hsa_dense_mask_pack."""
-    __slots__ = ("data", "sizes")
+class _Packed(NamedTuple):
+    """A mask in the bit form of hsa_dense_mask_pack: the bytes, and how many batches, heads and rows it tells apart."""
+    data: torch.Tensor
+    sizes: Tuple[int, int, int]
 
-    def __init__(self, mask: torch.Tensor, B: int, H: int, Lq: int, Lk: int, dev: torch.device):
-        if mask.dtype.is_floating_point or mask.dtype.is_complex:
-            raise _lib.HsaError(f"the mask is boolean or integer (nonzero = attend), not {mask.dtype}; additive masks are not taken")
-        _lib.require_cuda(mask)
-        if mask.device != dev:
-            raise _lib.HsaError("all tensors of one call must live on the same device")
-        assert mask.dim() in (2, 4), "the mask is [Lq, Lk] or [B, H, Lq, Lk] (dimensions of size 1 are broadcast)"
-        if mask.dim() == 2:
-            mask = mask.view(1, 1, *mask.shape) if mask.is_contiguous() else mask.unsqueeze(0).unsqueeze(0)
-        want = (B, H, Lq, Lk)
-        assert all(m in (1, w) for m, w in zip(mask.shape, want)), \
-            f"mask shape {tuple(mask.shape)} does not broadcast to {want}"
-        if mask.dtype == torch.bool:
-            mask = mask.view(torch.uint8)
-        elif mask.dtype not in (torch.uint8, torch.int8):
-            mask = (mask != 0).view(torch.uint8)
-        # a dimension that is expanded (stride 0) is packed once
-        sizes = [1 if st == 0 else sz for sz, st in zip(mask.shape[:3], mask.stride()[:3])]
-        strides = [0 if sz == 1 else st for sz, st in zip(mask.shape, mask.stride())]
-        lib = _lib.load()
-        nbytes = int(lib.hsa_dense_mask_bytes(*sizes, Lk))
-        self.data = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        self.sizes = tuple(sizes)
-        rc = lib.hsa_dense_mask_pack(c_void_p(mask.data_ptr()), *strides, *sizes, Lk, c_void_p(self.data.data_ptr()), nbytes,
-                                     _lib.stream_ptr(dev))
-        _lib.check(rc, "hsa_dense_mask_pack")
+
+def _mask_bytes(mask: torch.Tensor, B: int, H: int, Lq: int, Lk: int, dev: torch.device) -> torch.Tensor:
+    """The checked mask as a [B or 1, H or 1, Lq or 1, Lk or 1] tensor of bytes, nonzero = attend."""
+    if mask.dtype.is_floating_point or mask.dtype.is_complex:
+        raise _lib.HsaError(f"the mask is boolean or integer (nonzero = attend), not {mask.dtype}; additive masks are not taken")
+    if mask.device != dev:
+        raise _lib.HsaError("all tensors of one call must live on the same device")
+    assert mask.dim() in (2, 4), "the mask is [Lq, Lk] or [B, H, Lq, Lk] (dimensions of size 1 are broadcast)"
+    if mask.dim() == 2:
+        mask = mask.unsqueeze(0).unsqueeze(0)
+    assert all(m in (1, w) for m, w in zip(mask.shape, (B, H, Lq, Lk))), \
+        f"mask shape {tuple(mask.shape)} does not broadcast to {(B, H, Lq, Lk)}"
+    if mask.element_size() > 1:
+        mask = mask != 0
+    return mask.view(torch.uint8)
+
+
+def _pack_mask(mask: torch.Tensor, dev: torch.device, Lk: int) -> _Packed:
+    lib = _lib.load()
+    shape, strides = mask.shape, mask.stride()
+    sizes = tuple(1 if st == 0 else sz for sz, st in zip(shape[:3], strides[:3]))       # an expanded dimension is packed once
+    strides = [0 if sz == 1 else st for sz, st in zip(shape, strides)]
+    nbytes = lib.hsa_dense_mask_bytes(*sizes, Lk)
+    data = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    rc = lib.hsa_dense_mask_pack(c_void_p(mask.data_ptr()), *strides, *sizes, Lk, c_void_p(data.data_ptr()), nbytes, _lib.stream_ptr(dev))
+    _lib.check(rc, "hsa_dense_mask_pack")
+    return _Packed(data, sizes)
+
+
+def _mask_args(packed: Optional[_Packed]):
+    return (None, 0, 0, 0) if packed is None else (c_void_p(packed.data.data_ptr()), *packed.sizes)
 
 
 def _check_inputs(q, k, v):
     dev = _lib.require_cuda(q, k, v)
     _lib.dtype_code(q)
     assert q.dim() == 4 and k.dim() == 4 and v.dim() == 4, "q is [B, Lq, H, D]; k and v are [B, Lk, Hkv, D]"
-    assert k.shape == v.shape and k.size(0) == q.size(0) and k.size(3) == q.size(3), \
+    B, _, H, D = q.shape
+    Bk, _, Hkv, Dk = k.shape
+    assert k.shape == v.shape and Bk == B and Dk == D, \
         f"shapes disagree: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}"
     assert k.dtype == q.dtype and v.dtype == q.dtype, "dtype mismatch"
-    H, Hkv, D = q.size(2), k.size(2), q.size(3)
     assert Hkv >= 1 and H >= 1 and H % Hkv == 0, f"{H} query heads are not a multiple of {Hkv} key/value heads"
     assert 1 <= D <= 256, f"head dim {D} outside 1..256"
     return dev
@@ -100,7 +108,7 @@ def dense_aborts() -> int:
 
 
 def _debug_check(what: str) -> None:
-    if _lib.DEBUG and not torch.cuda.is_current_stream_capturing() and dense_aborts():
+    if not torch.cuda.is_current_stream_capturing() and dense_aborts():
         raise _lib.HsaError(f"{what}: a thread block gave up waiting; its rows hold NaN")
 
 
@@ -110,73 +118,85 @@ def _ptr(t: Optional[torch.Tensor]):
 
 def dense_attention_forward(q, k, v, key_lengths=None, packed_mask=None, scale: float = 1.0, empty_value: float = 0.0,
                             need_lse: bool = True, algo: int = _lib.ALGO_AUTO):
-    """Raw forward on checked inputs: returns (out, lse or None).  No autograd."""
+    """Raw forward on checked inputs with the device current: returns (out, lse or None).  No autograd."""
     lib = _lib.load()
     dev = q.device
     B, Lq, H, D = q.shape
-    Lk, Hkv = k.size(1), k.size(2)
+    Lk, Hkv = k.shape[1:3]
     out = torch.empty((B, Lq, H, D), dtype=q.dtype, device=dev)
     lse = torch.empty((B, Lq, H), dtype=torch.float32, device=dev) if need_lse else None
     dt = _lib.dtype_code(q)
-    with _lib.on_device(dev):
-        need = int(lib.hsa_dense_attn_fwd_workspace_bytes(B, Lq, Lk, H, Hkv, D, dt, algo))
-        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-        rc = lib.hsa_dense_attn_fwd(_view(q), _view(k), _view(v), _view(out), _ptr(lse), _ptr(key_lengths),
-                                    _ptr(packed_mask.data) if packed_mask is not None else None,
-                                    *(packed_mask.sizes if packed_mask is not None else (0, 0, 0)), _ptr(ws), need,
-                                    B, Lq, Lk, H, Hkv, D, scale, empty_value, dt, algo, _lib.stream_ptr(dev))
-    _lib.check(rc, "hsa_dense_attn_fwd")
-    _debug_check("hsa_dense_attn_fwd")
+    need = lib.hsa_dense_attn_fwd_workspace_bytes(B, Lq, Lk, H, Hkv, D, dt, algo)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    rs = H * D
+    rc = lib.hsa_dense_attn_fwd(_view(q), _view(k), _view(v), _lib.HsaView(out.data_ptr(), Lq * rs, rs), _ptr(lse), _ptr(key_lengths),
+                                *_mask_args(packed_mask), _ptr(ws), need, B, Lq, Lk, H, Hkv, D, scale, empty_value, dt, algo,
+                                _lib.stream_ptr(dev))
+    if rc:
+        _lib.check(rc, "hsa_dense_attn_fwd")
+    if _lib.DEBUG:
+        _debug_check("hsa_dense_attn_fwd")
     return out, lse
 
 
 def dense_attention_backward(q, k, v, out, lse, dout, key_lengths=None, packed_mask=None, scale: float = 1.0,
                              algo: int = _lib.ALGO_AUTO):
-    """Raw backward: returns (dq, dk, dv)."""
+    """Raw backward with the device current: returns (dq, dk, dv)."""
     lib = _lib.load()
     dev = q.device
     B, Lq, H, D = q.shape
-    Lk, Hkv = k.size(1), k.size(2)
+    Lk, Hkv = k.shape[1:3]
     dq = torch.empty((B, Lq, H, D), dtype=q.dtype, device=dev)
     dk = torch.empty((B, Lk, Hkv, D), dtype=q.dtype, device=dev)
-    dv = torch.empty_like(dk)
-    need = int(lib.hsa_dense_attn_bwd_workspace_bytes(B, Lq, H))
+    dv = torch.empty((B, Lk, Hkv, D), dtype=q.dtype, device=dev)
+    need = lib.hsa_dense_attn_bwd_workspace_bytes(B, Lq, H)
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    with _lib.on_device(dev):
-        rc = lib.hsa_dense_attn_bwd(_view(q), _view(k), _view(v), _view(out), _ptr(lse), _view(dout), _view(dq), _view(dk),
-                                    _view(dv), _ptr(key_lengths), _ptr(packed_mask.data) if packed_mask is not None else None,
-                                    *(packed_mask.sizes if packed_mask is not None else (0, 0, 0)), _ptr(ws), need,
-                                    B, Lq, Lk, H, Hkv, D, scale, _lib.dtype_code(q), algo, _lib.stream_ptr(dev))
-    _lib.check(rc, "hsa_dense_attn_bwd")
-    _debug_check("hsa_dense_attn_bwd")
+    rs, ks = H * D, Hkv * D
+    view = _lib.HsaView
+    rc = lib.hsa_dense_attn_bwd(_view(q), _view(k), _view(v), view(out.data_ptr(), Lq * rs, rs), _ptr(lse), _view(dout),
+                                view(dq.data_ptr(), Lq * rs, rs), view(dk.data_ptr(), Lk * ks, ks), view(dv.data_ptr(), Lk * ks, ks),
+                                _ptr(key_lengths), *_mask_args(packed_mask), _ptr(ws), need, B, Lq, Lk, H, Hkv, D, scale,
+                                _lib.dtype_code(q), algo, _lib.stream_ptr(dev))
+    if rc:
+        _lib.check(rc, "hsa_dense_attn_bwd")
+    if _lib.DEBUG:
+        _debug_check("hsa_dense_attn_bwd")
     return dq, dk, dv
 
 
 class _CrossAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, key_lengths, packed_mask, scale, empty_value, algo):
-        need = any(ctx.needs_input_grad[:3])
-        ctx.empty = q.size(0) * q.size(1) * k.size(1) == 0
-        if ctx.empty:                                # no query, or no key for any of them: nothing to launch
-            ctx.save_for_backward(q, k, v)
-            return torch.full(q.shape, empty_value, dtype=q.dtype, device=q.device)
         q, k, v = _rows(q), _rows(k), _rows(v)
-        out, lse = dense_attention_forward(q, k, v, key_lengths, packed_mask, scale, empty_value, need, algo)
-        if need:
-            ctx.save_for_backward(q, k, v, out, lse, key_lengths, None if packed_mask is None else packed_mask.data)
-            ctx.meta = (packed_mask, scale, algo)
+        out, lse = dense_attention_forward(q, k, v, key_lengths, packed_mask, scale, empty_value, True, algo)
+        ctx.save_for_backward(q, k, v, out, lse, key_lengths, None if packed_mask is None else packed_mask.data)
+        ctx.meta = (None if packed_mask is None else packed_mask.sizes, scale, algo)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        if ctx.empty:
-            return (*(torch.zeros_like(t) for t in ctx.saved_tensors), None, None, None, None, None)
-        q, k, v, out, lse, key_lengths, _ = ctx.saved_tensors
-        packed_mask, scale, algo = ctx.meta
-        dout = _rows(dout if dout.dtype == q.dtype else dout.to(q.dtype))
-        dq, dk, dv = dense_attention_backward(q, k, v, out, lse, dout, key_lengths, packed_mask, scale, algo)
-        return dq, dk, dv, None, None, None, None, None
+        q, k, v, out, lse, key_lengths, packed = ctx.saved_tensors
+        sizes, scale, algo = ctx.meta
+        with _lib.on_device(q.device):
+            dout = _rows(dout if dout.dtype == q.dtype else dout.to(q.dtype))
+            grads = dense_attention_backward(q, k, v, out, lse, dout, key_lengths, None if packed is None else _Packed(packed, sizes),
+                                             scale, algo)
+        return (*grads, None, None, None, None, None)
+
+
+class _NoRows(torch.autograd.Function):
+    """No query, or no key for any of them: nothing to launch, and gradients of zero."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, empty_value):
+        ctx.save_for_backward(q, k, v)
+        return torch.full(q.shape, empty_value, dtype=q.dtype, device=q.device)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        return (*(torch.zeros_like(t) for t in ctx.saved_tensors), None)
 
 
 def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, key_lengths: Optional[torch.Tensor] = None,
@@ -199,13 +219,19 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, key_lengt
     B, Lq, H, D = q.shape
     Lk = k.size(1)
     scale = D ** -0.5 if scale is None else float(scale)
-    if not (scale > 0.0 and math.isfinite(scale)):
+    if not 0.0 < scale < math.inf:
         raise _lib.HsaError("the scale must be positive and finite")
     if key_lengths is not None:
         key_lengths = _lengths32(key_lengths, B, Lk, dev, "key_lengths")
+    if mask is not None:
+        mask = _mask_bytes(mask, B, H, Lq, Lk, dev)
+    if B * Lq * Lk == 0:
+        return _NoRows.apply(q, k, v, float(empty_value))
     with _lib.on_device(dev):
-        packed = None if mask is None or B * Lq * Lk == 0 else _PackedMask(mask, B, H, Lq, Lk, dev)
-        return _CrossAttention.apply(q, k, v, key_lengths, packed, scale, float(empty_value), algo)
+        packed = None if mask is None else _pack_mask(mask, dev, Lk)
+        if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+            return _CrossAttention.apply(q, k, v, key_lengths, packed, scale, float(empty_value), algo)
+        return dense_attention_forward(_rows(q), _rows(k), _rows(v), key_lengths, packed, scale, float(empty_value), False, algo)[0]
 
 
 def paged_attention_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
@@ -238,7 +264,7 @@ def paged_attention_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
         raise _lib.HsaError("a slot's [Hkv, D] block must be packed (the cache is not copied)")
     if scale is None:
         scale = D ** -0.5
-    if not (scale > 0.0 and math.isfinite(scale)):
+    if not 0.0 < scale < math.inf:
         raise _lib.HsaError("the scale must be positive and finite")
     max_pages = page_table.size(1)
     out = torch.empty((B, H, D), dtype=q.dtype, device=dev)
@@ -253,8 +279,8 @@ def paged_attention_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     lengths = lengths.contiguous()
     with _lib.on_device(dev):
         if splits is None:
-            splits = int(lib.hsa_paged_attn_choose_splits(B, H, Hkv, page_size, max_pages))
-        need = int(lib.hsa_paged_attn_workspace_bytes(B, H, D, splits))
+            splits = lib.hsa_paged_attn_choose_splits(B, H, Hkv, page_size, max_pages)
+        need = lib.hsa_paged_attn_workspace_bytes(B, H, D, splits)
         ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
         rc = lib.hsa_paged_attn_decode(_lib.HsaView(q.data_ptr(), H * D, H * D), _lib.rows_view(k_pages), _lib.rows_view(v_pages),
                                        _lib.HsaView(out.data_ptr(), H * D, H * D), c_void_p(page_table.data_ptr()),
