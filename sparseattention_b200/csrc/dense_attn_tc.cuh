@@ -8,8 +8,13 @@
 
 namespace hsa {
 
-constexpr int kFlagTiles = 1024;                 // tiles whose mask state fits a block's table
-constexpr int kTcThreads = 320;                  // eight warps for the element-wise part, one for copies, one for products
+constexpr int kFlagTiles = 768;                  // tiles whose mask state fits one of a block's two tables
+// Eight warps for the element-wise part, one for copies, one for products; two more stand idle so that the last four form a
+// warpgroup, whose registers go to the others: 2 x 128 x 208 + 128 x 88 = 384 x 168, what the block is launched with.
+constexpr int kTcThreads = 384;
+
+__device__ __forceinline__ void give_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 88;\n"); }
+__device__ __forceinline__ void take_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 208;\n"); }
 
 // Bit words of the keys [32 w, 32 w + 32) of a tile: those before `left` (keys of the sequence that remain)
 __device__ __forceinline__ uint32_t tail_word(int left, int w) {
@@ -44,27 +49,63 @@ __device__ __forceinline__ void zero_hidden_rows(unsigned char *tile, int left, 
     __syncwarp();
 }
 
-// Four 16-byte pieces (32 columns) of a row of a staged output tile ([planes][128 rows][128 bytes], 128-byte swizzle).
+// 32 consecutive columns of an output row, as far as the head dim goes (a multiple of 8).
 template <typename T>
-__device__ __forceinline__ void stage_row32(unsigned char *tile, int row, int c32, const uint32_t (&v)[32], float scale) {
-    unsigned char *line = tile + (c32 >> 1) * 16384 + row * 128;
+__device__ __forceinline__ void store_row32(T *row, int col, int D, const uint32_t (&v)[32], float scale) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         uint32_t o[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e)
             o[e] = pack2<T>(__uint_as_float(v[8 * j + 2 * e]) * scale, __uint_as_float(v[8 * j + 2 * e + 1]) * scale);
-        *reinterpret_cast<uint4 *>(line + ((((c32 & 1) * 4 + j) ^ (row & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+        if (col + 8 * j < D) *reinterpret_cast<uint4 *>(row + col + 8 * j) = make_uint4(o[0], o[1], o[2], o[3]);
     }
+}
+template <typename T>
+__device__ __forceinline__ void fill_row(T *row, int D, float value) {
+    const uint32_t w = pack2<T>(value, value);
+    for (int c = 0; c < D; c += 8) *reinterpret_cast<uint4 *>(row + c) = make_uint4(w, w, w, w);
 }
 
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t mb) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n"
                  ::"r"(dst), "l"(src), "r"(bytes), "r"(mb) : "memory");
 }
-__device__ __forceinline__ void bulk_store_done() {
-    asm volatile("cp.async.bulk.commit_group;\n" ::: "memory");
-    asm volatile("cp.async.bulk.wait_group 0;\n" ::: "memory");
+
+// ------------------------------------------------------------------------------------------------------- work items
+// The kernels are launched with one block per work item, but a running block takes over items whose block has not started
+// (clusterlaunchcontrol.try_cancel): set-up is paid once per SM, copies and first products of the next item overlap the last
+// softmax and the output of the current one, and items of unequal length balance themselves.  Only the copy warp asks; it
+// hands the item's number (and the mask states of its tiles) to the other warps through two slots in shared memory.
+__device__ __forceinline__ void take_over(uint32_t response, uint32_t mb) {
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];\n" ::"r"(response), "r"(mb) : "memory");
 }
+// The block number that was taken over, or -1
+__device__ __forceinline__ int taken_over(uint32_t response) {
+    int item;
+    asm volatile("{\n.reg .pred p;\n.reg .b128 r;\nld.shared.b128 r, [%1];\n"
+                 "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\nmov.b32 %0, -1;\n"
+                 "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %0, r;\n}\n"
+                 : "=r"(item) : "r"(response) : "memory");
+    tc5::fence_async_smem();                          // read before the next answer lands
+    return item;
+}
+
+// A short wait of its own, for a block that has given up and looks whether more items were handed to it
+__device__ __forceinline__ bool mbar_wait_limited(uint32_t mb, uint32_t parity, long long limit) {
+    const long long start = clock64();
+    while (!tc5::mbar_try(mb, parity))
+        if (clock64() - start > limit) return false;
+    return true;
+}
+
+// Shared-memory side of it; barriers: info_full[2], info_empty[2], answer.
+struct ItemSlots {
+    int item[2];
+    int pad[2];
+    uint4 answer;
+    uint8_t flags[2][kFlagTiles];
+};
+constexpr int kItemBars = 5;
 
 }  // namespace hsa

@@ -12,7 +12,7 @@
 //          transposed (S^T = K Q^T), so that P^T and dS^T can stay in tensor memory, over the scores they came from, as the
 //          first operands of dv += P^T do and dk += dS^T q.  Two buffers of S^T and dP^T (64 columns each) alternate, one per
 //          element-wise warpgroup; with dv and dk all 512 columns are in use at DP = 128.
-// Ten warps per block: eight element-wise (a thread per row and column half, or per row), one for copies, one for products.
+// Eight element-wise warps per block (a thread per row and column half, or per row), one for copies, one for products.
 // Rounding: p and ds are rounded to the inputs' type once, as operands; all sums are 32-bit.
 #include "dense_attn_tc.cuh"
 
@@ -24,14 +24,30 @@ __device__ unsigned int g_dense_bwd_aborts = 0;
 template <int DP>
 struct DqShape {
     static constexpr int kTile = 128 * DP * 2, kKSlots = 3, kVSlots = 2;
-    static constexpr int kSmem = 1024 + (2 + kKSlots + kVSlots) * kTile + kFlagTiles + 256;
+    static constexpr int kBars = 9 + 2 * (kKSlots + kVSlots) + kItemBars;
+    static constexpr int kSmem = 1024 + (2 + kKSlots + kVSlots) * kTile + (int)sizeof(ItemSlots) + kBars * 8 + 8;
+    static_assert(kSmem <= 227 * 1024, "shared memory");
+};
+
+// A work item: 128 query rows of a (batch entry, head)
+struct DqItem {
+    int q0, h, hk, b, n, tiles;
+    int64_t plane;
+    __device__ __forceinline__ DqItem(const DenseArgs &a, int item) {
+        const int qblocks = (a.Lq + 127) / 128;
+        q0 = item % qblocks * 128; item /= qblocks;
+        h = item % a.H; b = item / a.H; hk = h / a.group;
+        n = dense_keys(a, b);
+        tiles = (n + 127) / 128;
+        plane = (int64_t)b * a.mask.plane_b + (int64_t)h * a.mask.plane_h;
+    }
 };
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(kTcThreads, 1)
-dense_dq_tc5_kernel(const DenseArgs a, const long long wait_limit, const __grid_constant__ CUtensorMap map_q,
+dense_dq_tc5_kernel(const DenseArgs a, const long long wait_limit, const unsigned int extra_tx, const __grid_constant__ CUtensorMap map_q,
                     const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-                    const __grid_constant__ CUtensorMap map_g, const __grid_constant__ CUtensorMap map_dq) {
+                    const __grid_constant__ CUtensorMap map_g) {
     using namespace tc5;
     using Shape = DqShape<DP>;
     constexpr int TILE = Shape::kTile, KS = Shape::kKSlots, VS = Shape::kVSlots, PLANES = DP / 64, PLANE = 16384;
@@ -42,39 +58,31 @@ dense_dq_tc5_kernel(const DenseArgs a, const long long wait_limit, const __grid_
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char *smem = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
     unsigned char *q_s = smem, *g_s = q_s + TILE, *k_s = g_s + TILE, *v_s = k_s + KS * TILE;
-    uint8_t *flags = v_s + VS * TILE;
-    unsigned long long *bars = reinterpret_cast<unsigned long long *>(flags + kFlagTiles);
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 8 + 2 * (KS + VS));
+    ItemSlots &items = *reinterpret_cast<ItemSlots *>(v_s + VS * TILE);
+    unsigned long long *bars = reinterpret_cast<unsigned long long *>(&items + 1);
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + Shape::kBars);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
     const uint32_t bar0 = smem_addr(bars);
     const uint32_t qg_full = bar0, s_full = bar0 + 8, s_free = bar0 + 16, p_full = bar0 + 24, p_free = bar0 + 32, d_full = bar0 + 40,
-                   d_free = bar0 + 48;
-    auto k_full = [&](int s) { return bar0 + 8u * (8 + s); };
-    auto k_empty = [&](int s) { return bar0 + 8u * (8 + KS + s); };
-    auto v_full = [&](int s) { return bar0 + 8u * (8 + 2 * KS + s); };
-    auto v_empty = [&](int s) { return bar0 + 8u * (8 + 2 * KS + VS + s); };
+                   d_free = bar0 + 48, qg_empty = bar0 + 56, answer = bar0 + 64;
+    auto k_full = [&](int s) { return bar0 + 8u * (9 + s); };
+    auto k_empty = [&](int s) { return bar0 + 8u * (9 + KS + s); };
+    auto v_full = [&](int s) { return bar0 + 8u * (9 + 2 * KS + s); };
+    auto v_empty = [&](int s) { return bar0 + 8u * (9 + 2 * KS + VS + s); };
+    auto info_full = [&](int s) { return bar0 + 8u * (9 + 2 * KS + 2 * VS + s); };
+    auto info_empty = [&](int s) { return bar0 + 8u * (11 + 2 * KS + 2 * VS + s); };
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int qblocks = (a.Lq + 127) / 128;
-    int blk = blockIdx.x;
-    const int q0 = blk % qblocks * 128; blk /= qblocks;
-    const int h = blk % a.H, b = blk / a.H, hk = h / a.group;
-    const int n = dense_keys(a, b), tiles = (n + 127) / 128;
-    const int64_t plane = (int64_t)b * a.mask.plane_b + (int64_t)h * a.mask.plane_h;
     const bool masked = a.mask.bits != nullptr;
-
     if (threadIdx.x == 0) {
         mbar_init(qg_full, 1); mbar_init(s_full, 1); mbar_init(s_free, 8); mbar_init(p_full, 1); mbar_init(p_free, 8);
-        mbar_init(d_full, 8); mbar_init(d_free, 1);
+        mbar_init(d_full, 8); mbar_init(d_free, 1); mbar_init(qg_empty, 1); mbar_init(answer, 1);
         for (int s = 0; s < KS; ++s) { mbar_init(k_full(s), 1); mbar_init(k_empty(s), 1); }
         for (int s = 0; s < VS; ++s) { mbar_init(v_full(s), 1); mbar_init(v_empty(s), 1); }
+        for (int s = 0; s < 2; ++s) { mbar_init(info_full(s), 1); mbar_init(info_empty(s), 9); }
         *abort_flag = 0;
         mbar_fence_init();
-        prefetch_map(&map_q); prefetch_map(&map_k); prefetch_map(&map_v); prefetch_map(&map_g); prefetch_map(&map_dq);
-    }
-    if (masked) {
-        const int cell = a.mask.rows > 1 ? q0 / kDenseTile : 0;
-        for (int t = threadIdx.x; t < tiles; t += kTcThreads) flags[t] = a.mask.tiles[(plane * a.mask.tq + cell) * a.mask.tk + t];
+        prefetch_map(&map_q); prefetch_map(&map_k); prefetch_map(&map_v); prefetch_map(&map_g);
     }
     if (warp == 9) tmem_alloc(smem_addr(tmem_slot), 512);
     fence_before_sync();
@@ -82,181 +90,257 @@ dense_dq_tc5_kernel(const DenseArgs a, const long long wait_limit, const __grid_
     fence_after_sync();
     const uint32_t tmem = *tmem_slot;
     auto wait = [&](uint32_t bar, uint32_t parity) { return (bool)__all_sync(0xffffffffu, mbar_wait(bar, parity, wait_limit, abort_flag)); };
-    auto next_tile = [&](int t) { while (t < tiles && masked && flags[t] == 0) ++t; return t; };
 
     if (warp == 8) {
-        if (lane == 0) {
-            bool ok = true;
-            int ks = 0, vs = 0; uint32_t kp = 0, vp = 0;
-            int t = next_tile(0);
-            if (t < tiles) {
-                mbar_expect_tx(qg_full, 2 * TILE);
+        bool ok = true;
+        int ks = 0, vs = 0; uint32_t kp = 0, vp = 0, qc = 0;
+        auto load = [&](uint32_t bar, const CUtensorMap *map, unsigned char *dst, int head, int row, int b) {
 #pragma unroll
-                for (int p = 0; p < PLANES; ++p) {
-                    tma_load_4d(smem_addr(q_s + p * PLANE), &map_q, p * 64, h, q0, b, qg_full);
-                    tma_load_4d(smem_addr(g_s + p * PLANE), &map_g, p * 64, h, q0, b, qg_full);
-                }
+            for (int p = 0; p < PLANES; ++p) tma_load_4d(smem_addr(dst + p * PLANE), map, p * 64, head, row, b, bar);
+        };
+        int item = blockIdx.x;
+        for (int k = 0; ok; ++k) {
+            const int is = k & 1;
+            if (!(ok = wait(info_empty(is), ((k >> 1) & 1) ^ 1))) break;
+            if (item >= 0 && masked) {
+                const DqItem it(a, item);
+                const int cell = a.mask.rows > 1 ? it.q0 / kDenseTile : 0;
+                for (int t = lane; t < it.tiles; t += 32) items.flags[is][t] = a.mask.tiles[(it.plane * a.mask.tq + cell) * a.mask.tk + t];
             }
-            for (; t < tiles; t = next_tile(t + 1)) {
-                if (!(ok = mbar_wait(k_empty(ks), kp ^ 1, wait_limit, abort_flag))) break;
-                mbar_expect_tx(k_full(ks), TILE);
-#pragma unroll
-                for (int p = 0; p < PLANES; ++p) tma_load_4d(smem_addr(k_s + ks * TILE + p * PLANE), &map_k, p * 64, hk, t * 128, b, k_full(ks));
+            if (lane == 0) items.item[is] = item;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(info_full(is));
+            if (item < 0) break;
+            const DqItem it(a, item);
+            bool first = true;
+            for (int t = 0; t < it.tiles && ok; ++t) {
+                if (masked && items.flags[is][t] == 0) continue;
+                if (!(ok = wait(k_empty(ks), kp ^ 1))) break;
+                if (lane == 0) {
+                    mbar_expect_tx(k_full(ks), TILE);
+                    load(k_full(ks), &map_k, k_s + ks * TILE, it.hk, t * 128, it.b);
+                }
+                __syncwarp();
                 if (++ks == KS) { ks = 0; kp ^= 1; }
-                if (!(ok = mbar_wait(v_empty(vs), vp ^ 1, wait_limit, abort_flag))) break;
-                mbar_expect_tx(v_full(vs), TILE);
-#pragma unroll
-                for (int p = 0; p < PLANES; ++p) tma_load_4d(smem_addr(v_s + vs * TILE + p * PLANE), &map_v, p * 64, hk, t * 128, b, v_full(vs));
+                if (first) {
+                    if (!(ok = wait(qg_empty, (qc & 1) ^ 1))) break;
+                    ++qc;
+                    if (lane == 0) {
+                        mbar_expect_tx(qg_full, 2 * TILE + extra_tx);
+                        load(qg_full, &map_q, q_s, it.h, it.q0, it.b);
+                        load(qg_full, &map_g, g_s, it.h, it.q0, it.b);
+                    }
+                    __syncwarp();
+                    first = false;
+                }
+                if (!(ok = wait(v_empty(vs), vp ^ 1))) break;
+                if (lane == 0) {
+                    mbar_expect_tx(v_full(vs), TILE);
+                    load(v_full(vs), &map_v, v_s + vs * TILE, it.hk, t * 128, it.b);
+                }
+                __syncwarp();
                 if (++vs == VS) { vs = 0; vp ^= 1; }
             }
-            if (!ok) {
-                const long long start = clock64();
-                while (clock64() - start < 200000) {}
+            if (!ok) break;
+            if (lane == 0) {                             // not earlier: an item that is taken over early waits here while other SMs run dry
+                mbar_expect_tx(answer, 16);
+                take_over(smem_addr(&items.answer), answer);
             }
+            __syncwarp();
+            if (!(ok = wait(answer, k & 1))) break;
+            item = taken_over(smem_addr(&items.answer));
+        }
+        if (!ok) {
+            const long long start = clock64();
+            while (clock64() - start < 200000) {}
         }
     } else if (warp == 9) {
         bool ok = true;
-        int ks = 0, vs = 0; uint32_t kp = 0, vp = 0;
-        // S and dP of tile t; the K tile stays until dq has read it
-        auto scores = [&](int t, int i) -> bool {
-            if (!wait(k_full(ks), kp)) return false;
-            if (i > 0 && !wait(s_free, (i - 1) & 1)) return false;
-            unsigned char *kt = k_s + ks * TILE;
-            if (n - t * 128 < 128 || masked)
-                zero_hidden_rows<PLANES>(kt, n - t * 128, masked ? a.mask.seen + plane * a.mask.wk + t * 4 : nullptr, lane);
-            fence_after_sync();
-            if (lane == 0) {
+        int ks = 0, vs = 0, kd = 0; uint32_t kp = 0, vp = 0, qc = 0;
+        uint32_t issued = 0, done = 0;                       // tiles whose scores, and whose dq, have been issued
+        for (int k = 0; ok; ++k) {
+            const int is = k & 1;
+            if (!(ok = wait(info_full(is), (k >> 1) & 1))) break;
+            const int item = items.item[is];
+            if (item < 0) break;
+            const DqItem it(a, item);
+            auto next_tile = [&](int t) { while (t < it.tiles && masked && items.flags[is][t] == 0) ++t; return t; };
+            // S and dP of tile t; the K tile stays until dq has read it
+            auto scores = [&](int t, bool last) -> bool {
+                if (!wait(k_full(ks), kp)) return false;
+                if (issued > 0 && !wait(s_free, (issued - 1) & 1)) return false;
+                unsigned char *kt = k_s + ks * TILE;
+                if (it.n - t * 128 < 128 || masked)
+                    zero_hidden_rows<PLANES>(kt, it.n - t * 128, masked ? a.mask.seen + it.plane * a.mask.wk + t * 4 : nullptr, lane);
+                fence_after_sync();
+                if (lane == 0) {
+                    const uint64_t qd = smem_desc(smem_addr(q_s), 16, 1024), kdsc = smem_desc(smem_addr(kt), 16, 1024);
 #pragma unroll
-                for (int k = 0; k < DP / 16; ++k) {
-                    const uint32_t off = (k >> 2) * PLANE + (k & 3) * 32;
-                    mma_f16(tmem + COL_S, smem_desc(smem_addr(q_s) + off, 16, 1024), smem_desc(smem_addr(kt) + off, 16, 1024), IDESC_S, k > 0);
+                    for (int j = 0; j < DP / 16; ++j) {
+                        const uint32_t off = (j >> 2) * (PLANE >> 4) + (j & 3) * 2;
+                        mma_f16(tmem + COL_S, qd + off, kdsc + off, IDESC_S, j > 0);
+                    }
+                    mma_commit(s_full);
                 }
-                mma_commit(s_full);
-            }
-            __syncwarp();
-            if (++ks == KS) { ks = 0; kp ^= 1; }
-            if (!wait(v_full(vs), vp)) return false;
-            if (i > 0 && !wait(p_free, (i - 1) & 1)) return false;
-            fence_after_sync();
-            if (lane == 0) {
+                __syncwarp();
+                if (++ks == KS) { ks = 0; kp ^= 1; }
+                if (!wait(v_full(vs), vp)) return false;
+                if (issued > 0 && !wait(p_free, (issued - 1) & 1)) return false;
+                fence_after_sync();
+                if (lane == 0) {
+                    const uint64_t gd = smem_desc(smem_addr(g_s), 16, 1024), vd = smem_desc(smem_addr(v_s + vs * TILE), 16, 1024);
 #pragma unroll
-                for (int k = 0; k < DP / 16; ++k) {
-                    const uint32_t off = (k >> 2) * PLANE + (k & 3) * 32;
-                    mma_f16(tmem + COL_P, smem_desc(smem_addr(g_s) + off, 16, 1024), smem_desc(smem_addr(v_s + vs * TILE) + off, 16, 1024), IDESC_S, k > 0);
+                    for (int j = 0; j < DP / 16; ++j) {
+                        const uint32_t off = (j >> 2) * (PLANE >> 4) + (j & 3) * 2;
+                        mma_f16(tmem + COL_P, gd + off, vd + off, IDESC_S, j > 0);
+                    }
+                    mma_commit(v_empty(vs));
+                    if (last) mma_commit(qg_empty);
+                    mma_commit(p_full);
                 }
-                mma_commit(v_empty(vs));
-                mma_commit(p_full);
+                __syncwarp();
+                if (++vs == VS) { vs = 0; vp ^= 1; }
+                ++issued;
+                return true;
+            };
+            int t = next_tile(0);
+            bool fresh = true;
+            if (t < it.tiles) {
+                ok = wait(qg_full, qc & 1) && scores(t, next_tile(t + 1) >= it.tiles);
+                ++qc;
             }
-            __syncwarp();
-            if (++vs == VS) { vs = 0; vp ^= 1; }
-            return true;
-        };
-        int t = next_tile(0), i = 0, kd = 0;                 // kd: slot of the K tile that dq reads next
-        if (t < tiles) ok = wait(qg_full, 0) && scores(t, 0);
-        while (ok && t < tiles) {
-            const int tn = next_tile(t + 1);
-            if (tn < tiles && !(ok = scores(tn, i + 1))) break;
-            if (!(ok = wait(d_full, i & 1))) break;
-            fence_after_sync();
-            if (lane == 0) {
-                const uint32_t kt = smem_addr(k_s + kd * TILE);
+            while (ok && t < it.tiles) {
+                const int tn = next_tile(t + 1);
+                if (tn < it.tiles && !(ok = scores(tn, next_tile(tn + 1) >= it.tiles))) break;
+                if (!(ok = wait(d_full, done & 1))) break;
+                ++done;
+                fence_after_sync();
+                if (lane == 0) {
+                    const uint64_t kdsc = smem_desc(smem_addr(k_s + kd * TILE), PLANE, 1024);
 #pragma unroll
-                for (int k = 0; k < 8; ++k)
-                    mma_f16_ta(tmem + COL_Q, tmem + COL_D + k * 8, smem_desc(kt + k * 2048, PLANE, 1024), IDESC_O, (i > 0 || k > 0) ? 1u : 0u);
-                mma_commit(k_empty(kd));
-                mma_commit(d_free);
+                    for (int j = 0; j < 8; ++j)
+                        mma_f16_ta(tmem + COL_Q, tmem + COL_D + j * 8, kdsc + j * 128, IDESC_O, (!fresh || j > 0) ? 1u : 0u);
+                    mma_commit(k_empty(kd));
+                    mma_commit(d_free);
+                }
+                __syncwarp();
+                if (++kd == KS) kd = 0;
+                fresh = false;
+                t = tn;
             }
+            if (ok && lane == 0) mbar_arrive(info_empty(is));
             __syncwarp();
-            if (++kd == KS) kd = 0;
-            t = tn;
-            ++i;
         }
-    } else {
-        const int half = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane, qi = q0 + row;
+    } else if (warp < 8) {
+        const int half = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane;
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-        const int64_t at = ((int64_t)b * a.H + h) * a.lq_pad + qi;
-        const float lse2 = a.lse2[at], delta = a.delta[at];
-        const uint32_t *bits = masked ? a.mask.bits + (plane * a.mask.rows + (a.mask.rows > 1 ? min(qi, a.Lq - 1) : 0)) * a.mask.wk : nullptr;
         bool ok = true;
-        int i = 0;
-        for (int t = next_tile(0); t < tiles; t = next_tile(t + 1), ++i) {
-            const int left = n - t * 128;
-            const bool partial = left < 128 || (masked && flags[t] != 2);
-            uint32_t keep[2] = {0xffffffffu, 0xffffffffu};
-            if (partial) {
-                uint2 w = make_uint2(~0u, ~0u);
-                if (masked) w = __ldg(reinterpret_cast<const uint2 *>(bits + t * 4 + 2 * half));
-                keep[0] = w.x & tail_word(left, 2 * half);
-                keep[1] = w.y & tail_word(left, 2 * half + 1);
-            }
-            if (!(ok = wait(s_full, i & 1))) break;
-            fence_after_sync();
-            uint32_t s[2][32], g[2][32], d[32];
-            tmem_ld32(tmem + COL_S + lanes + 64 * half, s[0]);
-            tmem_ld32(tmem + COL_S + lanes + 64 * half + 32, s[1]);
-            tmem_ld_wait();
-            fence_before_sync();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(s_free);
-#pragma unroll
-            for (int c = 0; c < 2; ++c)
-#pragma unroll
-                for (int j = 0; j < 32; ++j) s[c][j] = __float_as_uint(fast_exp2(fmaf(__uint_as_float(s[c][j]), a.scale_log2, -lse2)));
-            if (!(ok = wait(p_full, i & 1))) break;
-            fence_after_sync();
-            tmem_ld32(tmem + COL_P + lanes + 64 * half, g[0]);
-            tmem_ld32(tmem + COL_P + lanes + 64 * half + 32, g[1]);
-            tmem_ld_wait();
-            fence_before_sync();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(p_free);
-#pragma unroll
-            for (int c = 0; c < 2; ++c)
-#pragma unroll
-                for (int j = 0; j < 32; ++j) {
-                    float x = __uint_as_float(s[c][j]) * (__uint_as_float(g[c][j]) - delta);
-                    g[c][j] = __float_as_uint(x);
+        uint32_t i = 0;                                      // tiles done so far
+        int k = 0, item = -1;
+        for (; ok; ++k) {
+            const int is = k & 1;
+            item = -1;
+            if (!(ok = wait(info_full(is), (k >> 1) & 1))) break;
+            item = items.item[is];
+            if (item < 0) break;
+            const DqItem it(a, item);
+            const int qi = it.q0 + row;
+            const int64_t at = ((int64_t)it.b * a.H + it.h) * a.lq_pad + qi;
+            const float lse2 = a.lse2[at], delta = a.delta[at];
+            const uint32_t *bits = masked ? a.mask.bits + (it.plane * a.mask.rows + (a.mask.rows > 1 ? min(qi, a.Lq - 1) : 0)) * a.mask.wk : nullptr;
+            bool any = false;
+            for (int t = 0; t < it.tiles; ++t) {
+                const uint32_t flag = masked ? items.flags[is][t] : 2u;
+                if (flag == 0) continue;
+                const int left = it.n - t * 128;
+                const bool partial = left < 128 || flag != 2;
+                uint32_t keep[2] = {0xffffffffu, 0xffffffffu};
+                if (partial) {
+                    uint2 w = make_uint2(~0u, ~0u);
+                    if (masked) w = __ldg(reinterpret_cast<const uint2 *>(bits + t * 4 + 2 * half));
+                    keep[0] = w.x & tail_word(left, 2 * half);
+                    keep[1] = w.y & tail_word(left, 2 * half + 1);
                 }
-            if (partial) {
+                if (!(ok = wait(s_full, i & 1))) break;
+                fence_after_sync();
+                uint32_t s[2][32], g[2][32], d[32];
+                tmem_ld32(tmem + COL_S + lanes + 64 * half, s[0]);
+                tmem_ld32(tmem + COL_S + lanes + 64 * half + 32, s[1]);
+                tmem_ld_wait();
+                fence_before_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(s_free);
+#pragma unroll
+                for (int c = 0; c < 2; ++c)
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) s[c][j] = __float_as_uint(fast_exp2(fmaf(__uint_as_float(s[c][j]), a.scale_log2, -lse2)));
+                if (!(ok = wait(p_full, i & 1))) break;
+                fence_after_sync();
+                tmem_ld32(tmem + COL_P + lanes + 64 * half, g[0]);
+                tmem_ld32(tmem + COL_P + lanes + 64 * half + 32, g[1]);
+                tmem_ld_wait();
+                fence_before_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_free);
 #pragma unroll
                 for (int c = 0; c < 2; ++c)
 #pragma unroll
                     for (int j = 0; j < 32; ++j)
-                        if (!((keep[c] >> j) & 1u)) g[c][j] = 0u;
-            }
+                        g[c][j] = __float_as_uint(__uint_as_float(s[c][j]) * (__uint_as_float(g[c][j]) - delta));
+                if (partial) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
-                d[j] = pack2<T>(__uint_as_float(g[j >> 4][(2 * j) & 31]), __uint_as_float(g[j >> 4][(2 * j + 1) & 31]));
-            if (i > 0 && !(ok = wait(d_free, (i - 1) & 1))) break;
+                    for (int c = 0; c < 2; ++c)
+#pragma unroll
+                        for (int j = 0; j < 32; ++j)
+                            if (!((keep[c] >> j) & 1u)) g[c][j] = 0u;
+                }
+#pragma unroll
+                for (int j = 0; j < 32; ++j)
+                    d[j] = pack2<T>(__uint_as_float(g[j >> 4][(2 * j) & 31]), __uint_as_float(g[j >> 4][(2 * j + 1) & 31]));
+                if (i > 0 && !(ok = wait(d_free, (i - 1) & 1))) break;
+                fence_after_sync();
+                tmem_st32(tmem + COL_D + lanes + 32 * half, d);
+                tmem_st_wait();
+                fence_before_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(d_full);
+                ++i;
+                any = true;
+            }
+            if (ok && any) ok = wait(d_free, (i - 1) & 1);
+            if (!ok) break;                                  // with k and item of the unfinished one
             fence_after_sync();
-            tmem_st32(tmem + COL_D + lanes + 32 * half, d);
-            tmem_st_wait();
-            fence_before_sync();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(d_full);
-        }
-        if (ok && i > 0) ok = wait(d_free, (i - 1) & 1);
-        fence_after_sync();
-        const float scale = ok ? a.scale : __int_as_float(0x7fffffff);
+            T *out = (T *)a.dq.ptr + it.b * a.dq.batch_stride + (int64_t)qi * a.dq.row_stride + (int64_t)it.h * a.D;
 #pragma unroll 1
-        for (int c = half * (DP / 64); c < (half + 1) * (DP / 64); ++c) {        // 32 columns at a time
-            uint32_t o[32];
-            if (i > 0) {
-                tmem_ld32(tmem + COL_Q + lanes + 32 * c, o);
-                tmem_ld_wait();
-            } else {
+            for (int c = half * (DP / 64); c < (half + 1) * (DP / 64); ++c) {        // 32 columns at a time
+                uint32_t o[32];
+                if (any) {
+                    tmem_ld32(tmem + COL_Q + lanes + 32 * c, o);
+                    tmem_ld_wait();
+                } else {
 #pragma unroll
-                for (int j = 0; j < 32; ++j) o[j] = 0u;
+                    for (int j = 0; j < 32; ++j) o[j] = 0u;
+                }
+                if (qi < a.Lq) store_row32<T>(out, 32 * c, a.D, o, a.scale);
             }
-            stage_row32<T>(q_s, row, c, o, scale);           // the queries are not needed any more
+            fence_before_sync();                             // the accumulator may be written again
+            __syncwarp();
+            if (lane == 0) mbar_arrive(info_empty(is));
         }
-        fence_async_smem();
-        asm volatile("bar.sync 1, 256;\n" ::: "memory");
-        if (threadIdx.x == 0) {
-#pragma unroll
-            for (int p = 0; p < PLANES; ++p)
-                if (p * 64 < a.D) tma_store_4d(&map_dq, smem_addr(q_s + p * PLANE), p * 64, h, q0, b);
-            bulk_store_done();
+        if (!ok) {
+            // gave up: this item, and any that the block has already taken over, read NaN
+            for (;; ++k) {
+                if (item < 0) {
+                    if (!__all_sync(0xffffffffu, mbar_wait_limited(info_full(k & 1), (k >> 1) & 1, 400000))) break;
+                    item = items.item[k & 1];
+                    if (item < 0) break;
+                }
+                const DqItem it(a, item);
+                if (it.q0 + row < a.Lq)
+                    fill_row<T>((T *)a.dq.ptr + it.b * a.dq.batch_stride + (int64_t)(it.q0 + row) * a.dq.row_stride + (int64_t)it.h * a.D, a.D,
+                                __int_as_float(0x7fffffff));
+                item = -1;
+            }
         }
     }
     fence_before_sync();
@@ -271,15 +355,28 @@ template <int DP>
 struct DkvShape {
     static constexpr int kTile = 128 * DP * 2, kHalf = 64 * DP * 2, kStages = 4;
     static constexpr int kStage = 2 * kHalf;                                      // a query tile and its output gradients
-    static constexpr int kSmem = 1024 + 2 * kTile + kStages * (kStage + 512) + kFlagTiles + 256;
+    static constexpr int kBars = 9 + 2 * kStages + kItemBars;
+    static constexpr int kSmem = 1024 + 2 * kTile + kStages * (kStage + 512) + (int)sizeof(ItemSlots) + kBars * 8 + 8;
+    static_assert(kSmem <= 227 * 1024, "shared memory");
+};
+
+// A work item: 128 keys of a (batch entry, key/value head) against (query head of the group, tile of 64 queries), in this order
+struct DkvItem {
+    int kt, k0, hk, b, n, total;
+    __device__ __forceinline__ DkvItem(const DenseArgs &a, int item, int qtiles) {
+        const int ktiles = (a.Lk + 127) / 128;
+        kt = item % ktiles; k0 = kt * 128; item /= ktiles;
+        hk = item % a.Hkv; b = item / a.Hkv;
+        n = dense_keys(a, b);
+        total = k0 < n ? a.group * qtiles : 0;
+    }
 };
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(kTcThreads, 1)
-dense_dkdv_tc5_kernel(const DenseArgs a, const long long wait_limit, const __grid_constant__ CUtensorMap map_q,
+dense_dkdv_tc5_kernel(const DenseArgs a, const long long wait_limit, const unsigned int extra_tx, const __grid_constant__ CUtensorMap map_q,
                       const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-                      const __grid_constant__ CUtensorMap map_g, const __grid_constant__ CUtensorMap map_dk,
-                      const __grid_constant__ CUtensorMap map_dv) {
+                      const __grid_constant__ CUtensorMap map_g) {
     using namespace tc5;
     using Shape = DkvShape<DP>;
     constexpr int TILE = Shape::kTile, HALF = Shape::kHalf, ST = Shape::kStages, PLANES = DP / 64, PLANE = 16384, HPLANE = 8192;
@@ -291,234 +388,300 @@ dense_dkdv_tc5_kernel(const DenseArgs a, const long long wait_limit, const __gri
     unsigned char *smem = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
     unsigned char *k_s = smem, *v_s = k_s + TILE, *ring = v_s + TILE;
     float *stats = reinterpret_cast<float *>(ring + ST * Shape::kStage);          // per stage: 64 log-sum-exps, 64 row sums
-    uint8_t *flags = reinterpret_cast<uint8_t *>(stats + ST * 128);
-    unsigned long long *bars = reinterpret_cast<unsigned long long *>(flags + kFlagTiles);
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 6 + 2 * ST);
+    ItemSlots &items = *reinterpret_cast<ItemSlots *>(stats + ST * 128);
+    unsigned long long *bars = reinterpret_cast<unsigned long long *>(&items + 1);
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + Shape::kBars);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
     const uint32_t bar0 = smem_addr(bars);
-    const uint32_t kv_full = bar0, done = bar0 + 8;
-    auto s_full = [&](int x) { return bar0 + 8u * (2 + x); };
-    auto d_full = [&](int x) { return bar0 + 8u * (4 + x); };
-    auto full = [&](int s) { return bar0 + 8u * (6 + s); };
-    auto empty = [&](int s) { return bar0 + 8u * (6 + ST + s); };
+    const uint32_t kv_full = bar0, kv_empty = bar0 + 8, done = bar0 + 16, acc_free = bar0 + 24, answer = bar0 + 32;
+    auto s_full = [&](int x) { return bar0 + 8u * (5 + x); };
+    auto d_full = [&](int x) { return bar0 + 8u * (7 + x); };
+    auto full = [&](int s) { return bar0 + 8u * (9 + s); };
+    auto empty = [&](int s) { return bar0 + 8u * (9 + ST + s); };
+    auto info_full = [&](int s) { return bar0 + 8u * (9 + 2 * ST + s); };
+    auto info_empty = [&](int s) { return bar0 + 8u * (11 + 2 * ST + s); };
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int ktiles = (a.Lk + 127) / 128;
-    int blk = blockIdx.x;
-    const int kt = blk % ktiles, k0 = kt * 128; blk /= ktiles;
-    const int hk = blk % a.Hkv, b = blk / a.Hkv;
-    const int n = dense_keys(a, b);
     const int qtiles = (a.Lq + 63) / 64;
-    const int total = k0 < n ? a.group * qtiles : 0;          // (query head of the group, tile of 64 queries), in this order
     const bool masked = a.mask.bits != nullptr;
     const int cells = masked ? a.mask.tq : 0;
-    auto plane_of = [&](int g) { return (int64_t)b * a.mask.plane_b + (int64_t)(hk * a.group + g) * a.mask.plane_h; };
 
     if (threadIdx.x == 0) {
-        mbar_init(kv_full, 1); mbar_init(done, 1);
-        for (int x = 0; x < 2; ++x) { mbar_init(s_full(x), 1); mbar_init(d_full(x), 4); }
+        mbar_init(kv_full, 1); mbar_init(kv_empty, 1); mbar_init(done, 1); mbar_init(acc_free, 8); mbar_init(answer, 1);
+        for (int x = 0; x < 2; ++x) { mbar_init(s_full(x), 1); mbar_init(d_full(x), 4); mbar_init(info_full(x), 1); mbar_init(info_empty(x), 9); }
         for (int s = 0; s < ST; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
         *abort_flag = 0;
         mbar_fence_init();
-        prefetch_map(&map_q); prefetch_map(&map_k); prefetch_map(&map_v); prefetch_map(&map_g); prefetch_map(&map_dk); prefetch_map(&map_dv);
+        prefetch_map(&map_q); prefetch_map(&map_k); prefetch_map(&map_v); prefetch_map(&map_g);
     }
-    if (masked && total > 0)
-        for (int c = threadIdx.x; c < a.group * cells; c += kTcThreads)
-            flags[c] = a.mask.tiles[(plane_of(c / cells) * cells + c % cells) * a.mask.tk + kt];
     if (warp == 9) tmem_alloc(smem_addr(tmem_slot), 512);
     fence_before_sync();
     __syncthreads();
     fence_after_sync();
     const uint32_t tmem = *tmem_slot;
     auto wait = [&](uint32_t bar, uint32_t parity) { return (bool)__all_sync(0xffffffffu, mbar_wait(bar, parity, wait_limit, abort_flag)); };
-    auto flag_of = [&](int u) { return flags[u / qtiles * cells + (a.mask.rows > 1 ? (u % qtiles) >> 1 : 0)]; };
-    auto next_unit = [&](int u) { while (u < total && masked && flag_of(u) == 0) ++u; return u; };
+    auto plane_of = [&](int b, int h) { return (int64_t)b * a.mask.plane_b + (int64_t)h * a.mask.plane_h; };
+    auto flag_of = [&](int is, int u) { return items.flags[is][u / qtiles * cells + (a.mask.rows > 1 ? (u % qtiles) >> 1 : 0)]; };
+    auto next_unit = [&](int is, int u, int total) { while (u < total && masked && flag_of(is, u) == 0) ++u; return u; };
 
     if (warp == 8) {
-        if (lane == 0) {
-            bool ok = true;
-            int s = 0; uint32_t ph = 0;
-            int u = next_unit(0);
-            if (u < total) {
-                mbar_expect_tx(kv_full, 2 * TILE);
-#pragma unroll
-                for (int p = 0; p < PLANES; ++p) {
-                    tma_load_4d(smem_addr(k_s + p * PLANE), &map_k, p * 64, hk, k0, b, kv_full);
-                    tma_load_4d(smem_addr(v_s + p * PLANE), &map_v, p * 64, hk, k0, b, kv_full);
-                }
+        bool ok = true;
+        int s = 0; uint32_t ph = 0, kc = 0;
+        int item = blockIdx.x;
+        for (int k = 0; ok; ++k) {
+            const int is = k & 1;
+            if (!(ok = wait(info_empty(is), ((k >> 1) & 1) ^ 1))) break;
+            if (item >= 0 && masked) {
+                const DkvItem it(a, item, qtiles);
+                if (it.total > 0)
+                    for (int c = lane; c < a.group * cells; c += 32)
+                        items.flags[is][c] = a.mask.tiles[(plane_of(it.b, it.hk * a.group + c / cells) * cells + c % cells) * a.mask.tk + it.kt];
             }
-            for (; u < total; u = next_unit(u + 1)) {
-                const int h = hk * a.group + u / qtiles, q0 = u % qtiles * 64;
-                if (!(ok = mbar_wait(empty(s), ph ^ 1, wait_limit, abort_flag))) break;
-                mbar_expect_tx(full(s), 2 * HALF + 512);
-                const uint32_t qs = smem_addr(ring + s * Shape::kStage), gs = qs + HALF, fs = smem_addr(stats + s * 128);
-                const int64_t at = ((int64_t)b * a.H + h) * a.lq_pad + q0;
+            if (lane == 0) items.item[is] = item;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(info_full(is));
+            if (item < 0) break;
+            const DkvItem it(a, item, qtiles);
+            int u = next_unit(is, 0, it.total);
+            if (u < it.total) {
+                if (!(ok = wait(kv_empty, (kc & 1) ^ 1))) break;
+                ++kc;
+                if (lane == 0) {
+                    mbar_expect_tx(kv_full, 2 * TILE + extra_tx);
 #pragma unroll
-                for (int p = 0; p < PLANES; ++p) tma_load_4d(qs + p * HPLANE, &map_q, p * 64, h, q0, b, full(s));
-                bulk_load(fs, a.lse2 + at, 256, full(s));
+                    for (int p = 0; p < PLANES; ++p) {
+                        tma_load_4d(smem_addr(k_s + p * PLANE), &map_k, p * 64, it.hk, it.k0, it.b, kv_full);
+                        tma_load_4d(smem_addr(v_s + p * PLANE), &map_v, p * 64, it.hk, it.k0, it.b, kv_full);
+                    }
+                }
+                __syncwarp();
+            }
+            for (; u < it.total; u = next_unit(is, u + 1, it.total)) {
+                const int h = it.hk * a.group + u / qtiles, q0 = u % qtiles * 64;
+                if (!(ok = wait(empty(s), ph ^ 1))) break;
+                if (lane == 0) {
+                    mbar_expect_tx(full(s), 2 * HALF + 512);
+                    const uint32_t qs = smem_addr(ring + s * Shape::kStage), gs = qs + HALF, fs = smem_addr(stats + s * 128);
+                    const int64_t at = ((int64_t)it.b * a.H + h) * a.lq_pad + q0;
 #pragma unroll
-                for (int p = 0; p < PLANES; ++p) tma_load_4d(gs + p * HPLANE, &map_g, p * 64, h, q0, b, full(s));
-                bulk_load(fs + 256, a.delta + at, 256, full(s));
+                    for (int p = 0; p < PLANES; ++p) tma_load_4d(qs + p * HPLANE, &map_q, p * 64, h, q0, it.b, full(s));
+                    bulk_load(fs, a.lse2 + at, 256, full(s));
+#pragma unroll
+                    for (int p = 0; p < PLANES; ++p) tma_load_4d(gs + p * HPLANE, &map_g, p * 64, h, q0, it.b, full(s));
+                    bulk_load(fs + 256, a.delta + at, 256, full(s));
+                }
+                __syncwarp();
                 if (++s == ST) { s = 0; ph ^= 1; }
             }
-            if (!ok) {
-                const long long start = clock64();
-                while (clock64() - start < 200000) {}
+            if (!ok) break;
+            if (lane == 0) {                             // not earlier: an item that is taken over early waits here while other SMs run dry
+                mbar_expect_tx(answer, 16);
+                take_over(smem_addr(&items.answer), answer);
             }
+            __syncwarp();
+            if (!(ok = wait(answer, k & 1))) break;
+            item = taken_over(smem_addr(&items.answer));
+        }
+        if (!ok) {
+            const long long start = clock64();
+            while (clock64() - start < 200000) {}
         }
     } else if (warp == 9) {
         bool ok = true;
-        int s = 0; uint32_t ph = 0;
-        auto scores = [&](int i) -> bool {                    // S^T and dP^T of the i-th tile into buffer i & 1
+        int s = 0, sd = 0; uint32_t ph = 0, kc = 0;
+        uint32_t issued = 0, i = 0;                          // tiles whose scores, and whose products, have been issued
+        auto scores = [&](bool last) -> bool {                // S^T and dP^T of the next tile into buffer issued & 1
             if (!wait(full(s), ph)) return false;
             fence_after_sync();
             if (lane == 0) {
-                const uint32_t qs = smem_addr(ring + s * Shape::kStage), gs = qs + HALF, col = tmem + (i & 1) * 128;
+                const uint32_t qs = smem_addr(ring + s * Shape::kStage), col = tmem + (issued & 1) * 128;
+                const uint64_t kd = smem_desc(smem_addr(k_s), 16, 1024), vd = smem_desc(smem_addr(v_s), 16, 1024);
+                const uint64_t qd = smem_desc(qs, 16, 1024), gd = smem_desc(qs + HALF, 16, 1024);
 #pragma unroll
-                for (int k = 0; k < DP / 16; ++k) {
-                    const uint32_t ao = (k >> 2) * PLANE + (k & 3) * 32, bo = (k >> 2) * HPLANE + (k & 3) * 32;
-                    mma_f16(col, smem_desc(smem_addr(k_s) + ao, 16, 1024), smem_desc(qs + bo, 16, 1024), IDESC_S, k > 0);
-                }
+                for (int j = 0; j < DP / 16; ++j)
+                    mma_f16(col, kd + (j >> 2) * (PLANE >> 4) + (j & 3) * 2, qd + (j >> 2) * (HPLANE >> 4) + (j & 3) * 2, IDESC_S, j > 0);
 #pragma unroll
-                for (int k = 0; k < DP / 16; ++k) {
-                    const uint32_t ao = (k >> 2) * PLANE + (k & 3) * 32, bo = (k >> 2) * HPLANE + (k & 3) * 32;
-                    mma_f16(col + 64, smem_desc(smem_addr(v_s) + ao, 16, 1024), smem_desc(gs + bo, 16, 1024), IDESC_S, k > 0);
-                }
-                mma_commit(s_full(i & 1));
+                for (int j = 0; j < DP / 16; ++j)
+                    mma_f16(col + 64, vd + (j >> 2) * (PLANE >> 4) + (j & 3) * 2, gd + (j >> 2) * (HPLANE >> 4) + (j & 3) * 2, IDESC_S, j > 0);
+                if (last) mma_commit(kv_empty);
+                mma_commit(s_full(issued & 1));
             }
             __syncwarp();
             if (++s == ST) { s = 0; ph ^= 1; }
+            ++issued;
             return true;
         };
-        int u = next_unit(0), i = 0, sd = 0;
-        if (u < total) ok = wait(kv_full, 0) && scores(0);
-        while (ok && u < total) {
-            const int un = next_unit(u + 1);
-            if (un < total && !(ok = scores(i + 1))) break;
-            if (!(ok = wait(d_full(i & 1), (i >> 1) & 1))) break;
-            fence_after_sync();
-            if (lane == 0) {
-                const uint32_t qs = smem_addr(ring + sd * Shape::kStage), gs = qs + HALF, col = tmem + (i & 1) * 128;
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    mma_f16_ta(tmem + COL_V, col + k * 8, smem_desc(gs + k * 2048, HPLANE, 1024), IDESC_O, (i > 0 || k > 0) ? 1u : 0u);
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    mma_f16_ta(tmem + COL_K, col + 64 + k * 8, smem_desc(qs + k * 2048, HPLANE, 1024), IDESC_O, (i > 0 || k > 0) ? 1u : 0u);
-                mma_commit(empty(sd));
-                if (un >= total) mma_commit(done);
+        for (int k = 0; ok; ++k) {
+            const int is = k & 1;
+            if (!(ok = wait(info_full(is), (k >> 1) & 1))) break;
+            const int item = items.item[is];
+            if (item < 0) break;
+            const DkvItem it(a, item, qtiles);
+            int u = next_unit(is, 0, it.total);
+            bool fresh = true;
+            if (u < it.total) {
+                ok = wait(kv_full, kc & 1) && scores(next_unit(is, u + 1, it.total) >= it.total);
+                ++kc;
             }
+            while (ok && u < it.total) {
+                const int un = next_unit(is, u + 1, it.total);
+                if (un < it.total && !(ok = scores(next_unit(is, un + 1, it.total) >= it.total))) break;
+                if (!(ok = wait(d_full(i & 1), (i >> 1) & 1))) break;
+                // the first product of an item overwrites both accumulators: the other warpgroup may still read the last item's
+                if (fresh && kc > 1 && !(ok = wait(acc_free, kc & 1))) break;
+                fence_after_sync();
+                if (lane == 0) {
+                    const uint32_t qs = smem_addr(ring + sd * Shape::kStage), col = tmem + (i & 1) * 128;
+                    const uint64_t qd = smem_desc(qs, HPLANE, 1024), gd = smem_desc(qs + HALF, HPLANE, 1024);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) mma_f16_ta(tmem + COL_V, col + j * 8, gd + j * 128, IDESC_O, (!fresh || j > 0) ? 1u : 0u);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) mma_f16_ta(tmem + COL_K, col + 64 + j * 8, qd + j * 128, IDESC_O, (!fresh || j > 0) ? 1u : 0u);
+                    mma_commit(empty(sd));
+                    if (un >= it.total) mma_commit(done);
+                }
+                __syncwarp();
+                if (++sd == ST) sd = 0;
+                fresh = false;
+                u = un;
+                ++i;
+            }
+            if (ok && lane == 0) mbar_arrive(info_empty(is));
             __syncwarp();
-            if (++sd == ST) sd = 0;
-            u = un;
-            ++i;
         }
-    } else {
-        const int x = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane, key = k0 + row;
+    } else if (warp < 8) {
+        const int x = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane;
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16, ts = tmem + lanes + x * 128;
-        const bool tail = n - k0 < 128;
         bool ok = true;
-        int i = 0, s = 0; uint32_t ph = 0;
-        for (int u = next_unit(0); u < total; u = next_unit(u + 1), ++i) {
-            const int mine = s; const uint32_t mph = ph;
-            if (++s == ST) { s = 0; ph ^= 1; }
-            if ((i & 1) != x) continue;
-            uint32_t keep[2] = {0xffffffffu, 0xffffffffu};
-            bool partial = tail;
-            if (masked && flag_of(u) != 2) {
-                partial = true;
-                const int64_t plane = plane_of(u / qtiles);
-                if (key < a.Lk) {
-                    if (a.mask.rows > 1) {
-                        const uint2 w = __ldg(reinterpret_cast<const uint2 *>(a.mask.bits_t + (plane * a.Lk + key) * a.mask.wq + u % qtiles * 2));
-                        keep[0] = w.x; keep[1] = w.y;
-                    } else if (!((__ldg(a.mask.bits + plane * a.mask.wk + (key >> 5)) >> (key & 31)) & 1u)) {
-                        keep[0] = keep[1] = 0u;
+        uint32_t i = 0, kc = 0;                              // tiles, and items that had any
+        int s = 0, k = 0, item = -1; uint32_t ph = 0;
+        for (; ok; ++k) {
+            const int is = k & 1;
+            item = -1;
+            if (!(ok = wait(info_full(is), (k >> 1) & 1))) break;
+            item = items.item[is];
+            if (item < 0) break;
+            const DkvItem it(a, item, qtiles);
+            const int key = it.k0 + row;
+            const bool tail = it.n - it.k0 < 128;
+            bool any = false;
+            for (int u = next_unit(is, 0, it.total); u < it.total; u = next_unit(is, u + 1, it.total), ++i) {
+                const int mine = s; const uint32_t mph = ph;
+                if (++s == ST) { s = 0; ph ^= 1; }
+                any = true;
+                if ((i & 1) != x) continue;
+                uint32_t keep[2] = {0xffffffffu, 0xffffffffu};
+                bool partial = tail;
+                if (masked && flag_of(is, u) != 2) {
+                    partial = true;
+                    const int64_t plane = plane_of(it.b, it.hk * a.group + u / qtiles);
+                    if (key < a.Lk) {
+                        if (a.mask.rows > 1) {
+                            const uint2 w = __ldg(reinterpret_cast<const uint2 *>(a.mask.bits_t + (plane * a.Lk + key) * a.mask.wq + u % qtiles * 2));
+                            keep[0] = w.x; keep[1] = w.y;
+                        } else if (!((__ldg(a.mask.bits + plane * a.mask.wk + (key >> 5)) >> (key & 31)) & 1u)) {
+                            keep[0] = keep[1] = 0u;
+                        }
                     }
                 }
+                if (key >= it.n) keep[0] = keep[1] = 0u;
+                if (!(ok = wait(full(mine), mph) && wait(s_full(x), (i >> 1) & 1))) break;
+                fence_after_sync();
+                const float *st = stats + mine * 128;
+                uint32_t r[2][32], p[2][32], pk[32];
+                tmem_ld32(ts, r[0]);
+                tmem_ld32(ts + 32, r[1]);
+                tmem_ld_wait();
+#pragma unroll
+                for (int c = 0; c < 2; ++c)
+#pragma unroll
+                    for (int j = 0; j < 32; j += 4) {
+                        const float4 lse = *reinterpret_cast<const float4 *>(st + 32 * c + j);
+                        p[c][j] = __float_as_uint(fast_exp2(fmaf(__uint_as_float(r[c][j]), a.scale_log2, -lse.x)));
+                        p[c][j + 1] = __float_as_uint(fast_exp2(fmaf(__uint_as_float(r[c][j + 1]), a.scale_log2, -lse.y)));
+                        p[c][j + 2] = __float_as_uint(fast_exp2(fmaf(__uint_as_float(r[c][j + 2]), a.scale_log2, -lse.z)));
+                        p[c][j + 3] = __float_as_uint(fast_exp2(fmaf(__uint_as_float(r[c][j + 3]), a.scale_log2, -lse.w)));
+                    }
+                if (partial) {
+#pragma unroll
+                    for (int c = 0; c < 2; ++c)
+#pragma unroll
+                        for (int j = 0; j < 32; ++j)
+                            if (!((keep[c] >> j) & 1u)) p[c][j] = 0u;
+                }
+#pragma unroll
+                for (int j = 0; j < 32; ++j)
+                    pk[j] = pack2<T>(__uint_as_float(p[j >> 4][(2 * j) & 31]), __uint_as_float(p[j >> 4][(2 * j + 1) & 31]));
+                tmem_st32(ts, pk);
+                tmem_ld32(ts + 64, r[0]);
+                tmem_ld32(ts + 96, r[1]);
+                tmem_ld_wait();
+#pragma unroll
+                for (int c = 0; c < 2; ++c)
+#pragma unroll
+                    for (int j = 0; j < 32; j += 4) {
+                        const float4 dl = *reinterpret_cast<const float4 *>(st + 64 + 32 * c + j);
+                        r[c][j] = __float_as_uint(__uint_as_float(p[c][j]) * (__uint_as_float(r[c][j]) - dl.x));
+                        r[c][j + 1] = __float_as_uint(__uint_as_float(p[c][j + 1]) * (__uint_as_float(r[c][j + 1]) - dl.y));
+                        r[c][j + 2] = __float_as_uint(__uint_as_float(p[c][j + 2]) * (__uint_as_float(r[c][j + 2]) - dl.z));
+                        r[c][j + 3] = __float_as_uint(__uint_as_float(p[c][j + 3]) * (__uint_as_float(r[c][j + 3]) - dl.w));
+                    }
+                if (partial) {                                   // not through p = 0: what a hidden row holds may be NaN
+#pragma unroll
+                    for (int c = 0; c < 2; ++c)
+#pragma unroll
+                        for (int j = 0; j < 32; ++j)
+                            if (!((keep[c] >> j) & 1u)) r[c][j] = 0u;
+                }
+#pragma unroll
+                for (int j = 0; j < 32; ++j)
+                    pk[j] = pack2<T>(__uint_as_float(r[j >> 4][(2 * j) & 31]), __uint_as_float(r[j >> 4][(2 * j + 1) & 31]));
+                tmem_st32(ts + 64, pk);
+                tmem_st_wait();
+                fence_before_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(d_full(x));
             }
-            if (key >= n) keep[0] = keep[1] = 0u;
-            if (!(ok = wait(full(mine), mph) && wait(s_full(x), (i >> 1) & 1))) break;
+            if (ok && any) { ok = wait(done, kc & 1); ++kc; }
+            if (!ok) break;                                      // with k and item of the unfinished one
             fence_after_sync();
-            const float *st = stats + mine * 128;
-            uint32_t r[2][32], p[2][32], pk[32];
-            tmem_ld32(ts, r[0]);
-            tmem_ld32(ts + 32, r[1]);
-            tmem_ld_wait();
+            // dv by the first warpgroup, dk by the second
+            const hsa_view &g = x == 0 ? a.dv : a.dk;
+            T *out = (T *)g.ptr + it.b * g.batch_stride + (int64_t)key * g.row_stride + (int64_t)it.hk * a.D;
+#pragma unroll 1
+            for (int c = 0; c < DP / 32; ++c) {
+                uint32_t o[32];
+                if (any) {
+                    tmem_ld32(tmem + lanes + (x == 0 ? COL_V : COL_K) + 32 * c, o);
+                    tmem_ld_wait();
+                } else {
 #pragma unroll
-            for (int c = 0; c < 2; ++c)
-#pragma unroll
-                for (int j = 0; j < 32; j += 4) {
-                    const float4 lse = *reinterpret_cast<const float4 *>(st + 32 * c + j);
-                    p[c][j] = __float_as_uint(fast_exp2(fmaf(__uint_as_float(r[c][j]), a.scale_log2, -lse.x)));
-                    p[c][j + 1] = __float_as_uint(fast_exp2(fmaf(__uint_as_float(r[c][j + 1]), a.scale_log2, -lse.y)));
-                    p[c][j + 2] = __float_as_uint(fast_exp2(fmaf(__uint_as_float(r[c][j + 2]), a.scale_log2, -lse.z)));
-                    p[c][j + 3] = __float_as_uint(fast_exp2(fmaf(__uint_as_float(r[c][j + 3]), a.scale_log2, -lse.w)));
+                    for (int j = 0; j < 32; ++j) o[j] = 0u;
                 }
-            if (partial) {
-#pragma unroll
-                for (int c = 0; c < 2; ++c)
-#pragma unroll
-                    for (int j = 0; j < 32; ++j)
-                        if (!((keep[c] >> j) & 1u)) p[c][j] = 0u;
+                if (key < a.Lk) store_row32<T>(out, 32 * c, a.D, o, x == 0 ? 1.f : a.scale);
             }
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-                pk[j] = pack2<T>(__uint_as_float(p[j >> 4][(2 * j) & 31]), __uint_as_float(p[j >> 4][(2 * j + 1) & 31]));
-            tmem_st32(ts, pk);
-            tmem_ld32(ts + 64, r[0]);
-            tmem_ld32(ts + 96, r[1]);
-            tmem_ld_wait();
-#pragma unroll
-            for (int c = 0; c < 2; ++c)
-#pragma unroll
-                for (int j = 0; j < 32; j += 4) {
-                    const float4 dl = *reinterpret_cast<const float4 *>(st + 64 + 32 * c + j);
-                    r[c][j] = __float_as_uint(__uint_as_float(p[c][j]) * (__uint_as_float(r[c][j]) - dl.x));
-                    r[c][j + 1] = __float_as_uint(__uint_as_float(p[c][j + 1]) * (__uint_as_float(r[c][j + 1]) - dl.y));
-                    r[c][j + 2] = __float_as_uint(__uint_as_float(p[c][j + 2]) * (__uint_as_float(r[c][j + 2]) - dl.z));
-                    r[c][j + 3] = __float_as_uint(__uint_as_float(p[c][j + 3]) * (__uint_as_float(r[c][j + 3]) - dl.w));
-                }
-            if (partial) {                                       // not through p = 0: what a hidden row holds may be NaN
-#pragma unroll
-                for (int c = 0; c < 2; ++c)
-#pragma unroll
-                    for (int j = 0; j < 32; ++j)
-                        if (!((keep[c] >> j) & 1u)) r[c][j] = 0u;
-            }
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-                pk[j] = pack2<T>(__uint_as_float(r[j >> 4][(2 * j) & 31]), __uint_as_float(r[j >> 4][(2 * j + 1) & 31]));
-            tmem_st32(ts + 64, pk);
-            tmem_st_wait();
             fence_before_sync();
             __syncwarp();
-            if (lane == 0) mbar_arrive(d_full(x));
-        }
-        if (ok && i > 0) ok = wait(done, 0);
-        fence_after_sync();
-        // dv by the first warpgroup through V's room, dk by the second through K's
-        unsigned char *stg = x == 0 ? v_s : k_s;
-        const float scale = !ok ? __int_as_float(0x7fffffff) : x == 0 ? 1.f : a.scale;
-#pragma unroll 1
-        for (int c = 0; c < DP / 32; ++c) {
-            uint32_t o[32];
-            if (i > 0) {
-                tmem_ld32(tmem + lanes + (x == 0 ? COL_V : COL_K) + 32 * c, o);
-                tmem_ld_wait();
-            } else {
-#pragma unroll
-                for (int j = 0; j < 32; ++j) o[j] = 0u;
+            if (lane == 0) {
+                if (any) mbar_arrive(acc_free);
+                mbar_arrive(info_empty(is));
             }
-            stage_row32<T>(stg, row, c, o, scale);
         }
-        fence_async_smem();
-        asm volatile("bar.sync %0, 128;\n" ::"r"(1 + x) : "memory");
-        if (row == 0) {
-#pragma unroll
-            for (int p = 0; p < PLANES; ++p)
-                if (p * 64 < a.D) tma_store_4d(x == 0 ? &map_dv : &map_dk, smem_addr(stg + p * PLANE), p * 64, hk, k0, b);
-            bulk_store_done();
+        if (!ok) {
+            // gave up: this item, and any that the block has already taken over, read NaN
+            const hsa_view &g = x == 0 ? a.dv : a.dk;
+            for (;; ++k) {
+                if (item < 0) {
+                    if (!__all_sync(0xffffffffu, mbar_wait_limited(info_full(k & 1), (k >> 1) & 1, 400000))) break;
+                    item = items.item[k & 1];
+                    if (item < 0) break;
+                }
+                const DkvItem it(a, item, qtiles);
+                if (it.k0 + row < a.Lk)
+                    fill_row<T>((T *)g.ptr + it.b * g.batch_stride + (int64_t)(it.k0 + row) * g.row_stride + (int64_t)it.hk * a.D, a.D,
+                                __int_as_float(0x7fffffff));
+                item = -1;
+            }
         }
     }
     fence_before_sync();
@@ -530,25 +693,24 @@ dense_dkdv_tc5_kernel(const DenseArgs a, const long long wait_limit, const __gri
 
 template <typename T, int DP>
 static int bwd_launch(const DenseArgs &a, cudaStream_t st) {
-    CUtensorMap mq, mq64, mk, mv, mg, mg64, mdq, mdk, mdv;
+    CUtensorMap mq, mq64, mk, mv, mg, mg64;
     if (!make_map(&mq, a.q, a.B, a.Lq, a.H, a.D, 1, 128) || !make_map(&mq64, a.q, a.B, a.Lq, a.H, a.D, 1, 64) ||
         !make_map(&mk, a.k, a.B, a.Lk, a.Hkv, a.D, 1, 128) || !make_map(&mv, a.v, a.B, a.Lk, a.Hkv, a.D, 1, 128) ||
-        !make_map(&mg, a.dout, a.B, a.Lq, a.H, a.D, 1, 128) || !make_map(&mg64, a.dout, a.B, a.Lq, a.H, a.D, 1, 64) ||
-        !make_map(&mdq, a.dq, a.B, a.Lq, a.H, a.D, 1, 128) || !make_map(&mdk, a.dk, a.B, a.Lk, a.Hkv, a.D, 1, 128) ||
-        !make_map(&mdv, a.dv, a.B, a.Lk, a.Hkv, a.D, 1, 128))
+        !make_map(&mg, a.dout, a.B, a.Lq, a.H, a.D, 1, 128) || !make_map(&mg64, a.dout, a.B, a.Lq, a.H, a.D, 1, 64))
         return fail(HSA_ERR_ARG, "hsa_dense_attn_bwd: the driver refused a tensor map");
     const long long dq_blocks = (long long)a.B * a.H * ((a.Lq + 127) / 128), kv_blocks = (long long)a.B * a.Hkv * ((a.Lk + 127) / 128);
     if (dq_blocks > 0x7fffffffLL || kv_blocks > 0x7fffffffLL) return fail(HSA_ERR_ARG, "hsa_dense_attn_bwd: too many tiles");
     const long long limit = wait_limit_cycles();
+    const unsigned int extra = wait_extra_tx();
     auto kdq = dense_dq_tc5_kernel<T, DP>;
     auto kkv = dense_dkdv_tc5_kernel<T, DP>;
     constexpr int smem_dq = DqShape<DP>::kSmem, smem_kv = DkvShape<DP>::kSmem;
     cudaError_t e = cudaFuncSetAttribute(kdq, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_dq);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(kkv, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_kv);
     if (e != cudaSuccess) return fail((int)e, "hsa_dense_attn_bwd: shared memory %d / %d: %s", smem_dq, smem_kv, cudaGetErrorString(e));
-    kkv<<<(unsigned)kv_blocks, kTcThreads, smem_kv, st>>>(a, limit, mq64, mk, mv, mg64, mdk, mdv);
+    kkv<<<(unsigned)kv_blocks, kTcThreads, smem_kv, st>>>(a, limit, extra, mq64, mk, mv, mg64);
     if (int rc = launch_status("hsa_dense_attn_bwd(dk, dv)")) return rc;
-    kdq<<<(unsigned)dq_blocks, kTcThreads, smem_dq, st>>>(a, limit, mq, mk, mv, mg, mdq);
+    kdq<<<(unsigned)dq_blocks, kTcThreads, smem_dq, st>>>(a, limit, extra, mq, mk, mv, mg);
     return launch_status("hsa_dense_attn_bwd(dq)");
 }
 

@@ -24,6 +24,7 @@ __device__ unsigned int g_dense_aborts = 0;
 struct DenseSplit {
     float *part_o, *part_ml;                     // [splits, B, Lq, H, D] and [splits, B, Lq, H, 2] when splits > 1
     int splits;
+    unsigned int extra_tx;                       // test hook: bytes that the first copy is announced with and never brings
     long long wait_limit;
 };
 
@@ -31,14 +32,33 @@ template <int DP>
 struct FwdShape {
     static constexpr int kTile = 128 * DP * 2;                       // bytes of a tile of 128 rows
     static constexpr int kSlots = DP == 128 ? 5 : 8;                 // K and V tiles in flight
-    static constexpr int kSmem = 1024 + 2 * kTile + kSlots * kTile + kFlagTiles + 256;
+    static constexpr int kSmem = 1024 + 2 * kTile + kSlots * kTile + (int)sizeof(ItemSlots) + (10 + 2 * kSlots + kItemBars) * 8 + 8;
+    static_assert(kSmem <= 227 * 1024, "shared memory");
+};
+
+// A work item: 256 query rows of a (batch entry, head) against one range of its keys
+struct FwdItem {
+    int q0, h, b, split, hk, nw, n, kt0, kt1;
+    int64_t plane;
+    __device__ __forceinline__ FwdItem(const DenseArgs &a, int splits, int item) {
+        const int qblocks = (a.Lq + 255) / 256;
+        q0 = item % qblocks * 256; item /= qblocks;
+        h = item % a.H; item /= a.H;
+        b = item % a.B; split = item / a.B;
+        hk = h / a.group;
+        nw = a.Lq - q0 > 128 ? 2 : 1;                    // query tiles
+        n = dense_keys(a, b);
+        const int tiles = (n + 127) / 128, per = (tiles + splits - 1) / splits;
+        kt0 = min(tiles, split * per);
+        kt1 = min(tiles, kt0 + per);
+        plane = (int64_t)b * a.mask.plane_b + (int64_t)h * a.mask.plane_h;
+    }
 };
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(kTcThreads, 1)
 dense_fwd_tc5_kernel(const DenseArgs a, const DenseSplit sp, const __grid_constant__ CUtensorMap map_q,
-                     const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-                     const __grid_constant__ CUtensorMap map_o) {
+                     const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
     using namespace tc5;
     using Shape = FwdShape<DP>;
     constexpr int TILE = Shape::kTile, SLOTS = Shape::kSlots, PLANES = DP / 64, PLANE = 128 * 128;
@@ -49,49 +69,34 @@ dense_fwd_tc5_kernel(const DenseArgs a, const DenseSplit sp, const __grid_consta
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char *smem = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
     unsigned char *q_s = smem, *ring = smem + 2 * TILE;
-    uint8_t *flags = ring + (size_t)SLOTS * TILE;
-    unsigned long long *bars = reinterpret_cast<unsigned long long *>(flags + kFlagTiles);
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 8 + 2 * SLOTS);
+    ItemSlots &items = *reinterpret_cast<ItemSlots *>(ring + (size_t)SLOTS * TILE);
+    unsigned long long *bars = reinterpret_cast<unsigned long long *>(&items + 1);
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 10 + 2 * SLOTS + kItemBars);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
     const uint32_t bar0 = smem_addr(bars);
     auto q_full = [&](int w) { return bar0 + 8u * w; };
-    auto s_full = [&](int w) { return bar0 + 8u * (2 + w); };
-    auto p_full = [&](int w) { return bar0 + 8u * (4 + w); };
-    auto o_full = [&](int w) { return bar0 + 8u * (6 + w); };
-    auto kv_full = [&](int s) { return bar0 + 8u * (8 + s); };
-    auto kv_empty = [&](int s) { return bar0 + 8u * (8 + SLOTS + s); };
+    auto q_empty = [&](int w) { return bar0 + 8u * (2 + w); };
+    auto s_full = [&](int w) { return bar0 + 8u * (4 + w); };
+    auto p_full = [&](int w) { return bar0 + 8u * (6 + w); };
+    auto o_full = [&](int w) { return bar0 + 8u * (8 + w); };
+    auto kv_full = [&](int s) { return bar0 + 8u * (10 + s); };
+    auto kv_empty = [&](int s) { return bar0 + 8u * (10 + SLOTS + s); };
+    auto info_full = [&](int s) { return bar0 + 8u * (10 + 2 * SLOTS + s); };
+    auto info_empty = [&](int s) { return bar0 + 8u * (12 + 2 * SLOTS + s); };
+    const uint32_t answer = bar0 + 8u * (14 + 2 * SLOTS);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int qblocks = (a.Lq + 255) / 256;
-    int blk = blockIdx.x;
-    const int q0 = blk % qblocks * 256; blk /= qblocks;
-    const int h = blk % a.H; blk /= a.H;
-    const int b = blk % a.B, split = blk / a.B;
-    const int hk = h / a.group;
-    const int nw = a.Lq - q0 > 128 ? 2 : 1;              // query tiles of this block
-    const int n = dense_keys(a, b);
-    const int tiles_all = (n + 127) / 128, per = (tiles_all + sp.splits - 1) / sp.splits;
-    const int kt0 = min(tiles_all, split * per), kt1 = min(tiles_all, kt0 + per);
-    const int64_t plane = (int64_t)b * a.mask.plane_b + (int64_t)h * a.mask.plane_h;
     const bool masked = a.mask.bits != nullptr;
-
     if (threadIdx.x == 0) {
-        for (int w = 0; w < 2; ++w) { mbar_init(q_full(w), 1); mbar_init(s_full(w), 1); mbar_init(p_full(w), 4); mbar_init(o_full(w), 1); }
+        for (int w = 0; w < 2; ++w) {
+            mbar_init(q_full(w), 1); mbar_init(q_empty(w), 1); mbar_init(s_full(w), 1); mbar_init(p_full(w), 4); mbar_init(o_full(w), 1);
+            mbar_init(info_full(w), 1); mbar_init(info_empty(w), 9);
+        }
         for (int s = 0; s < SLOTS; ++s) { mbar_init(kv_full(s), 1); mbar_init(kv_empty(s), 1); }
+        mbar_init(answer, 1);
         *abort_flag = 0;
         mbar_fence_init();
-        prefetch_map(&map_q); prefetch_map(&map_k); prefetch_map(&map_v); prefetch_map(&map_o);
-    }
-    if (masked) {
-        // mask state of this block's key tiles: two bits per query tile
-        for (int t = kt0 + threadIdx.x; t < kt1; t += kTcThreads) {
-            uint8_t f = 0;
-            for (int w = 0; w < nw; ++w) {
-                const int row = a.mask.rows > 1 ? q0 / kDenseTile + w : 0;
-                f |= a.mask.tiles[(plane * a.mask.tq + row) * a.mask.tk + t] << (2 * w);
-            }
-            flags[t - kt0] = f;
-        }
+        prefetch_map(&map_q); prefetch_map(&map_k); prefetch_map(&map_v);
     }
     if (warp == 9) tmem_alloc(smem_addr(tmem_slot), 512);
     fence_before_sync();
@@ -100,248 +105,325 @@ dense_fwd_tc5_kernel(const DenseArgs a, const DenseSplit sp, const __grid_consta
     const uint32_t tmem = *tmem_slot;
     // a whole warp waits, and goes on or gives up as one
     auto wait = [&](uint32_t bar, uint32_t parity) { return (bool)__all_sync(0xffffffffu, mbar_wait(bar, parity, sp.wait_limit, abort_flag)); };
-    auto skip = [&](int t) { return masked && flags[t - kt0] == 0; };
 
     if (warp == 8) {
+        give_registers();
         // ------------------------------------------------------------------------------------------------- copies
-        if (lane == 0) {
-            bool ok = true;
-            int slot = 0; uint32_t ph = 0;
-            bool first = true;
-            auto push = [&](const CUtensorMap *map, int row) {
-                if (!(ok = mbar_wait(kv_empty(slot), ph ^ 1, sp.wait_limit, abort_flag))) return;
+        bool ok = true;
+        int slot = 0; uint32_t ph = 0, qc[2] = {0, 0};
+        auto push = [&](const CUtensorMap *map, int hk, int row, int b) {
+            if (!(ok = wait(kv_empty(slot), ph ^ 1))) return;
+            if (lane == 0) {
                 mbar_expect_tx(kv_full(slot), TILE);
                 const uint32_t dst = smem_addr(ring + (size_t)slot * TILE);
 #pragma unroll
                 for (int p = 0; p < PLANES; ++p) tma_load_4d(dst + p * PLANE, map, p * 64, hk, row, b, kv_full(slot));
-                if (++slot == SLOTS) { slot = 0; ph ^= 1; }
-            };
-            for (int t = kt0; t < kt1 && ok; ++t) {
-                if (skip(t)) continue;
+            }
+            __syncwarp();
+            if (++slot == SLOTS) { slot = 0; ph ^= 1; }
+        };
+        int item = blockIdx.x;
+        for (int k = 0; ok; ++k) {
+            const int is = k & 1;
+            if (!(ok = wait(info_empty(is), ((k >> 1) & 1) ^ 1))) break;
+            if (item >= 0 && masked) {
+                // mask states of the item's key tiles: two bits per query tile
+                const FwdItem it(a, sp.splits, item);
+                for (int t = it.kt0 + lane; t < it.kt1; t += 32) {
+                    uint8_t f = 0;
+                    for (int w = 0; w < it.nw; ++w) {
+                        const int row = a.mask.rows > 1 ? it.q0 / kDenseTile + w : 0;
+                        f |= a.mask.tiles[(it.plane * a.mask.tq + row) * a.mask.tk + t] << (2 * w);
+                    }
+                    items.flags[is][t - it.kt0] = f;
+                }
+            }
+            if (lane == 0) items.item[is] = item;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(info_full(is));
+            if (item < 0) break;
+            const FwdItem it(a, sp.splits, item);
+            bool first = true;
+            for (int t = it.kt0; t < it.kt1 && ok; ++t) {
+                if (masked && items.flags[is][t - it.kt0] == 0) continue;
+                push(&map_k, it.hk, t * 128, it.b);
                 if (first) {
-                    for (int w = 0; w < nw; ++w) {
-                        mbar_expect_tx(q_full(w), TILE);
+                    for (int w = 0; w < it.nw && ok; ++w) {
+                        if (!(ok = wait(q_empty(w), (qc[w] & 1) ^ 1))) break;
+                        ++qc[w];
+                        if (lane == 0) {
+                            mbar_expect_tx(q_full(w), TILE + sp.extra_tx);
 #pragma unroll
-                        for (int p = 0; p < PLANES; ++p)
-                            tma_load_4d(smem_addr(q_s + w * TILE + p * PLANE), &map_q, p * 64, h, q0 + 128 * w, b, q_full(w));
-                        if (w == 0) push(&map_k, t * 128);
+                            for (int p = 0; p < PLANES; ++p)
+                                tma_load_4d(smem_addr(q_s + w * TILE + p * PLANE), &map_q, p * 64, it.h, it.q0 + 128 * w, it.b, q_full(w));
+                        }
+                        __syncwarp();
                     }
                     first = false;
-                } else {
-                    push(&map_k, t * 128);
                 }
-                if (ok) push(&map_v, t * 128);
+                if (ok) push(&map_v, it.hk, t * 128, it.b);
             }
-            if (!ok) {                                   // let copies already issued land before the block goes
-                const long long start = clock64();
-                while (clock64() - start < 200000) {}
+            if (!ok) break;
+            if (lane == 0) {                             // not earlier: an item that is taken over early waits here while other SMs run dry
+                mbar_expect_tx(answer, 16);
+                take_over(smem_addr(&items.answer), answer);
             }
+            __syncwarp();
+            if (!(ok = wait(answer, k & 1))) break;
+            item = taken_over(smem_addr(&items.answer));
+        }
+        if (!ok) {                                       // let copies already issued land before the block goes
+            const long long start = clock64();
+            while (clock64() - start < 200000) {}
         }
     } else if (warp == 9) {
+        give_registers();
         // -------------------------------------------------------------------------------------------- matrix products
         bool ok = true;
-        int slot = 0; uint32_t ph = 0;
+        int slot = 0; uint32_t ph = 0, qc[2] = {0, 0}, pc[2] = {0, 0};
         auto next_slot = [&]() { if (++slot == SLOTS) { slot = 0; ph ^= 1; } };
-        auto issue_s = [&](int w, uint32_t k_addr) {
+        auto issue_s = [&](int w, uint32_t k_addr, bool last) {
             if (lane == 0) {
-                const uint32_t qa = smem_addr(q_s + w * TILE);
+                // a descriptor's start address counts in 16 bytes, and no sum of these leaves its field
+                const uint64_t qd = smem_desc(smem_addr(q_s + w * TILE), 16, 1024), kd = smem_desc(k_addr, 16, 1024);
 #pragma unroll
                 for (int k = 0; k < DP / 16; ++k) {
-                    const uint32_t off = (k >> 2) * PLANE + (k & 3) * 32;
-                    mma_f16(tmem + COL_S + w * 128, smem_desc(qa + off, 16, 1024), smem_desc(k_addr + off, 16, 1024), IDESC_S, k > 0);
+                    constexpr uint32_t kStep = 32 >> 4;
+                    const uint32_t off = (k >> 2) * (PLANE >> 4) + (k & 3) * kStep;
+                    mma_f16(tmem + COL_S + w * 128, qd + off, kd + off, IDESC_S, k > 0);
                 }
+                if (last) mma_commit(q_empty(w));
                 mma_commit(s_full(w));
             }
             __syncwarp();
         };
-        int t = kt0;
-        while (t < kt1 && skip(t)) ++t;
-        if (t < kt1) {
-            int cur = slot;
-            ok = wait(kv_full(cur), ph);
-            for (int w = 0; w < nw && ok; ++w) {
-                if (!(ok = wait(q_full(w), 0))) break;
-                fence_after_sync();
-                issue_s(w, smem_addr(ring + (size_t)cur * TILE));
-            }
-            if (lane == 0) mma_commit(kv_empty(cur));
-            next_slot();
-        }
-        uint32_t par = 0;
-        bool fresh = true;
-        while (t < kt1 && ok) {
-            int tn = t + 1;
-            while (tn < kt1 && skip(tn)) ++tn;
-            const int vs = slot;
-            if (!(ok = wait(kv_full(vs), ph))) break;
-            next_slot();
-            const uint32_t v_addr = smem_addr(ring + (size_t)vs * TILE);
-            // rows of keys that are not there
-            const int left = n - t * 128;
-            if (left < 128 || masked)
-                zero_hidden_rows<PLANES>(ring + (size_t)vs * TILE, left, masked ? a.mask.seen + plane * a.mask.wk + t * 4 : nullptr, lane);
-            const int ks = slot;
-            bool k_ready = false;
-            for (int w = 0; w < nw && ok; ++w) {
-                if (!(ok = wait(p_full(w), par))) break;
-                fence_after_sync();
-                if (lane == 0) {
-#pragma unroll
-                    for (int k = 0; k < 8; ++k)
-                        mma_f16_ta(tmem + COL_O + w * DP, tmem + COL_S + w * 128 + k * 8, smem_desc(v_addr + k * 2048, PLANE, 1024), IDESC_O,
-                                   (!fresh || k > 0) ? 1u : 0u);
-                    if (w == nw - 1) mma_commit(kv_empty(vs));       // before the barrier that lets the block end
-                    mma_commit(o_full(w));
+        for (int k = 0; ok; ++k) {
+            const int is = k & 1;
+            if (!(ok = wait(info_full(is), (k >> 1) & 1))) break;
+            const int item = items.item[is];
+            if (item < 0) break;
+            const FwdItem it(a, sp.splits, item);
+            auto next_tile = [&](int t) { while (t < it.kt1 && masked && items.flags[is][t - it.kt0] == 0) ++t; return t; };
+            int t = next_tile(it.kt0);
+            if (t < it.kt1) {
+                const int cur = slot;
+                const bool last = next_tile(t + 1) >= it.kt1;
+                if (!(ok = wait(kv_full(cur), ph))) break;
+                for (int w = 0; w < it.nw && ok; ++w) {
+                    if (!(ok = wait(q_full(w), qc[w] & 1))) break;
+                    ++qc[w];
+                    fence_after_sync();
+                    issue_s(w, smem_addr(ring + (size_t)cur * TILE), last);
                 }
+                if (lane == 0) mma_commit(kv_empty(cur));
                 __syncwarp();
-                if (tn < kt1) {
-                    if (!k_ready) {
-                        if (!(ok = wait(kv_full(ks), ph))) break;
-                        fence_after_sync();
-                        k_ready = true;
-                    }
-                    issue_s(w, smem_addr(ring + (size_t)ks * TILE));
-                    if (w == nw - 1 && lane == 0) mma_commit(kv_empty(ks));
-                }
+                next_slot();
             }
-            if (tn < kt1) next_slot();
-            fresh = false;
-            par ^= 1;
-            t = tn;
+            bool fresh = true;
+            while (t < it.kt1 && ok) {
+                const int tn = next_tile(t + 1);
+                const bool last = tn >= it.kt1 || next_tile(tn + 1) >= it.kt1;           // tn is the item's last tile
+                const int vs = slot;
+                if (!(ok = wait(kv_full(vs), ph))) break;
+                next_slot();
+                const uint32_t v_addr = smem_addr(ring + (size_t)vs * TILE);
+                if (it.n - t * 128 < 128 || masked)
+                    zero_hidden_rows<PLANES>(ring + (size_t)vs * TILE, it.n - t * 128,
+                                             masked ? a.mask.seen + it.plane * a.mask.wk + t * 4 : nullptr, lane);
+                const int ks = slot;
+                bool k_ready = false;
+                for (int w = 0; w < it.nw && ok; ++w) {
+                    if (!(ok = wait(p_full(w), pc[w] & 1))) break;
+                    ++pc[w];
+                    fence_after_sync();
+                    if (lane == 0) {
+                        const uint64_t vd = smem_desc(v_addr, PLANE, 1024);
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            mma_f16_ta(tmem + COL_O + w * DP, tmem + COL_S + w * 128 + j * 8, vd + j * (2048 >> 4), IDESC_O, (!fresh || j > 0) ? 1u : 0u);
+                        if (w == it.nw - 1) mma_commit(kv_empty(vs));       // before the barrier that lets the block end
+                        mma_commit(o_full(w));
+                    }
+                    __syncwarp();
+                    if (tn < it.kt1) {
+                        if (!k_ready) {
+                            if (!(ok = wait(kv_full(ks), ph))) break;
+                            fence_after_sync();
+                            k_ready = true;
+                        }
+                        if (w == it.nw - 1) {
+                            issue_s(w, smem_addr(ring + (size_t)ks * TILE), last);
+                            if (lane == 0) mma_commit(kv_empty(ks));
+                            __syncwarp();
+                        } else {
+                            issue_s(w, smem_addr(ring + (size_t)ks * TILE), last);
+                        }
+                    }
+                }
+                if (tn < it.kt1) next_slot();
+                fresh = false;
+                t = tn;
+            }
+            if (ok && lane == 0) mbar_arrive(info_empty(is));
+            __syncwarp();
         }
+    } else if (warp > 9) {
+        give_registers();
     } else {
+        take_registers();
         // -------------------------------------------------------------------------------------------------- softmax
         const int w = warp >> 2, quarter = warp & 3;
-        const int row = quarter * 32 + lane, qi = q0 + 128 * w + row;
-        if (w < nw) {
-            bool ok = true;
-            const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-            const uint32_t ts = tmem + COL_S + w * 128 + lanes, to = tmem + COL_O + w * DP + lanes;
-            const uint32_t *bits = masked ? a.mask.bits + (plane * a.mask.rows + (a.mask.rows > 1 ? min(qi, a.Lq - 1) : 0)) * a.mask.wk : nullptr;
-            float m = -INFINITY, l = 0.f;
-            int i = 0;                                       // tiles done
-            for (int t = kt0; t < kt1; ++t) {
-                if (skip(t)) continue;
-                const int left = n - t * 128;
-                const bool partial = left < 128 || (masked && ((flags[t - kt0] >> (2 * w)) & 3) != 2);
-                uint4 words = make_uint4(~0u, ~0u, ~0u, ~0u);
-                if (partial && masked) words = __ldg(reinterpret_cast<const uint4 *>(bits + t * 4));
-                if (!(ok = wait(s_full(w), i & 1))) break;
-                fence_after_sync();
-                uint32_t r[4][32];
-#pragma unroll
-                for (int c = 0; c < 4; ++c) tmem_ld32(ts + 32 * c, r[c]);
-                tmem_ld_wait();
-                float top = -INFINITY;
-                if (partial) {
-                    const uint32_t wd[4] = {words.x, words.y, words.z, words.w};
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        const uint32_t keep = wd[c] & tail_word(left, c);
-#pragma unroll
-                        for (int j = 0; j < 32; ++j)
-                            if (!((keep >> j) & 1u)) r[c][j] = 0xff800000u;
+        const int row = quarter * 32 + lane;
+        const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+        const uint32_t ts = tmem + COL_S + w * 128 + lanes, to = tmem + COL_O + w * DP + lanes;
+        bool ok = true;
+        uint32_t sc = 0;                                     // tiles done so far
+        int k = 0, item = -1;
+        for (; ok; ++k) {
+            const int is = k & 1;
+            item = -1;
+            if (!(ok = wait(info_full(is), (k >> 1) & 1))) break;
+            item = items.item[is];
+            if (item < 0) break;
+            const FwdItem it(a, sp.splits, item);
+            const int qi = it.q0 + 128 * w + row;
+            if (w < it.nw) {
+                const uint32_t *bits = masked ? a.mask.bits + (it.plane * a.mask.rows + (a.mask.rows > 1 ? min(qi, a.Lq - 1) : 0)) * a.mask.wk : nullptr;
+                float m = -INFINITY, l = 0.f;
+                bool any = false;
+                for (int t = it.kt0; t < it.kt1; ++t) {
+                    uint32_t flag = 2;
+                    if (masked) {
+                        flag = items.flags[is][t - it.kt0];
+                        if (flag == 0) continue;
+                        flag = (flag >> (2 * w)) & 3;
                     }
-                }
-                float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                    const int left = it.n - t * 128;
+                    const bool partial = left < 128 || flag != 2;
+                    uint4 words = make_uint4(~0u, ~0u, ~0u, ~0u);
+                    if (partial && masked) words = __ldg(reinterpret_cast<const uint4 *>(bits + t * 4));
+                    if (!(ok = wait(s_full(w), sc & 1))) break;
+                    fence_after_sync();
+                    uint32_t r[4][32];
 #pragma unroll
-                for (int c = 0; c < 4; ++c)
+                    for (int c = 0; c < 4; ++c) tmem_ld32(ts + 32 * c, r[c]);
+                    tmem_ld_wait();
+                    if (partial) {
+                        const uint32_t wd[4] = {words.x, words.y, words.z, words.w};
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) tops[c] = fmaxf(tops[c], __uint_as_float(r[c][j]));
-                top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * a.scale_log2;
-                const bool grow = top > m + 8.f;             // also the first finite maximum (m = -inf)
-                if (__any_sync(0xffffffffu, grow)) {
-                    const float m_new = grow ? top : m;
-                    const float corr = grow ? fast_exp2(m - m_new) : 1.f;
-                    if (i > 0) {
-                        if (!(ok = wait(o_full(w), (i - 1) & 1))) break;
-                        fence_after_sync();
+                        for (int c = 0; c < 4; ++c) {
+                            const uint32_t keep = wd[c] & tail_word(left, c);
 #pragma unroll
-                        for (int c = 0; c < DP / 32; ++c) {
-                            uint32_t o[32];
-                            tmem_ld32(to + 32 * c, o);
-                            tmem_ld_wait();
-#pragma unroll
-                            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * corr);
-                            tmem_st32(to + 32 * c, o);
+                            for (int j = 0; j < 32; ++j)
+                                if (!((keep >> j) & 1u)) r[c][j] = 0xff800000u;
                         }
-                        l *= corr;
                     }
-                    m = m_new;
-                }
-                const float ref = m == -INFINITY ? 0.f : m;
-                float sum[2] = {0.f, 0.f};
+                    float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    uint32_t pk[32];
+                    for (int c = 0; c < 4; ++c)
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) {
-                        const int e = 64 * c + 2 * j;
-                        const float p0 = fast_exp2(fmaf(__uint_as_float(r[e >> 5][e & 31]), a.scale_log2, -ref));
-                        const float p1 = fast_exp2(fmaf(__uint_as_float(r[(e + 1) >> 5][(e + 1) & 31]), a.scale_log2, -ref));
-                        sum[0] += p0; sum[1] += p1;
-                        pk[j] = pack2<T>(p0, p1);
+                        for (int j = 0; j < 32; ++j) tops[c] = fmaxf(tops[c], __uint_as_float(r[c][j]));
+                    const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * a.scale_log2;
+                    const bool grow = top > m + 8.f;             // also the first finite maximum (m = -inf)
+                    if (__any_sync(0xffffffffu, grow)) {
+                        const float m_new = grow ? top : m;
+                        const float corr = grow ? fast_exp2(m - m_new) : 1.f;
+                        if (any) {
+                            if (!(ok = wait(o_full(w), (sc - 1) & 1))) break;
+                            fence_after_sync();
+#pragma unroll
+                            for (int c = 0; c < DP / 32; ++c) {
+                                uint32_t o[32];
+                                tmem_ld32(to + 32 * c, o);
+                                tmem_ld_wait();
+#pragma unroll
+                                for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * corr);
+                                tmem_st32(to + 32 * c, o);
+                            }
+                            l *= corr;
+                        }
+                        m = m_new;
                     }
-                    tmem_st32(ts + 32 * c, pk);
+                    const float ref = m == -INFINITY ? 0.f : m;
+                    float sum[2] = {0.f, 0.f};
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        uint32_t pk[32];
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) {
+                            const int e = 64 * c + 2 * j;
+                            const float p0 = fast_exp2(fmaf(__uint_as_float(r[e >> 5][e & 31]), a.scale_log2, -ref));
+                            const float p1 = fast_exp2(fmaf(__uint_as_float(r[(e + 1) >> 5][(e + 1) & 31]), a.scale_log2, -ref));
+                            sum[0] += p0; sum[1] += p1;
+                            pk[j] = pack2<T>(p0, p1);
+                        }
+                        tmem_st32(ts + 32 * c, pk);
+                    }
+                    l += sum[0] + sum[1];
+                    tmem_st_wait();
+                    fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(p_full(w));
+                    ++sc;
+                    any = true;
                 }
-                l += sum[0] + sum[1];
-                tmem_st_wait();
-                fence_before_sync();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(p_full(w));
-                ++i;
-            }
-            // ---------------------------------------------------------------------------------------------- results
-            if (ok && i > 0) ok = wait(o_full(w), (i - 1) & 1);
-            fence_after_sync();
-            if (!ok) { l = __int_as_float(0x7fffffff); m = 0.f; }
-            const bool none = l == 0.f;
-            if (sp.splits > 1) {
-                const int64_t at = (((int64_t)split * a.B + b) * a.Lq + qi) * a.H + h;
+                // ------------------------------------------------------------------------------------------ results
+                if (ok && any) ok = wait(o_full(w), (sc - 1) & 1);
+                if (!ok) break;                                  // with k and item of the unfinished one
+                fence_after_sync();
+                const bool none = l == 0.f;
+                const float inv = 1.f / l;
+                const int64_t at = (((int64_t)it.split * a.B + it.b) * a.Lq + qi) * a.H + it.h;
+                T *orow = (T *)a.out.ptr + it.b * a.out.batch_stride + (int64_t)qi * a.out.row_stride + (int64_t)it.h * a.D;
 #pragma unroll 1
                 for (int c = 0; c < DP / 32; ++c) {
                     uint32_t o[32];
-                    if (i > 0) { tmem_ld32(to + 32 * c, o); tmem_ld_wait(); }
-                    if (qi < a.Lq) {
+                    if (any) {
+                        tmem_ld32(to + 32 * c, o);
+                        tmem_ld_wait();
+                    }
+                    if (none) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) o[j] = 0u;
+                    }
+                    if (qi >= a.Lq) continue;
+                    if (sp.splits > 1) {
 #pragma unroll
                         for (int j = 0; j < 32; j += 4)
                             if (32 * c + j < a.D)
-                                *reinterpret_cast<float4 *>(sp.part_o + at * a.D + 32 * c + j) = i > 0
-                                    ? make_float4(__uint_as_float(o[j]), __uint_as_float(o[j + 1]), __uint_as_float(o[j + 2]), __uint_as_float(o[j + 3]))
-                                    : make_float4(0.f, 0.f, 0.f, 0.f);
+                                *reinterpret_cast<uint4 *>(sp.part_o + at * a.D + 32 * c + j) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+                    } else if (!none) {
+                        store_row32<T>(orow, 32 * c, a.D, o, inv);
                     }
                 }
-                if (qi < a.Lq) *reinterpret_cast<float2 *>(sp.part_ml + 2 * at) = make_float2(m, l);
-            } else {
-                const float inv = 1.f / l;
-                unsigned char *stg = q_s + w * TILE;             // the queries are not needed any more
-#pragma unroll 1
-                for (int c = 0; c < DP / 32; ++c) {
-                    uint32_t o[32];
-                    if (i > 0) { tmem_ld32(to + 32 * c, o); tmem_ld_wait(); }
-                    unsigned char *line = stg + (c >> 1) * PLANE + row * 128;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        uint32_t v[4];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int k = 8 * j + 2 * e;
-                            v[e] = none ? pack2<T>(a.empty_value, a.empty_value)
-                                        : pack2<T>(__uint_as_float(o[k]) * inv, __uint_as_float(o[k + 1]) * inv);
-                        }
-                        *reinterpret_cast<uint4 *>(line + ((((c & 1) * 4 + j) ^ (row & 7)) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
-                    }
+                if (qi < a.Lq) {
+                    if (sp.splits > 1) *reinterpret_cast<float2 *>(sp.part_ml + 2 * at) = make_float2(m, l);
+                    else if (none) fill_row<T>(orow, a.D, a.empty_value);
+                    if (sp.splits == 1 && a.lse != nullptr) a.lse[at] = none ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
                 }
-                if (a.lse != nullptr && qi < a.Lq)
-                    a.lse[((int64_t)b * a.Lq + qi) * a.H + h] = none ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
-                fence_async_smem();
-                asm volatile("bar.sync %0, 128;\n" ::"r"(1 + w) : "memory");
-                if (row == 0) {
-#pragma unroll
-                    for (int p = 0; p < PLANES; ++p)
-                        if (p * 64 < a.D) tma_store_4d(&map_o, smem_addr(stg + p * PLANE), p * 64, h, q0 + 128 * w, b);
-                    bulk_store_done();
+                fence_before_sync();                             // the accumulator may be written again
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(info_empty(is));
+        }
+        if (!ok) {
+            // gave up: this item, and any that the block has already taken over, read NaN
+            const float nan = __int_as_float(0x7fffffff);
+            for (;; ++k) {
+                if (item < 0) {
+                    if (!__all_sync(0xffffffffu, mbar_wait_limited(info_full(k & 1), (k >> 1) & 1, 400000))) break;
+                    item = items.item[k & 1];
+                    if (item < 0) break;
                 }
+                const FwdItem it(a, sp.splits, item);
+                const int qi = it.q0 + 128 * w + row;
+                if (qi < a.Lq) {
+                    const int64_t at = (((int64_t)it.split * a.B + it.b) * a.Lq + qi) * a.H + it.h;
+                    if (sp.splits > 1) *reinterpret_cast<float2 *>(sp.part_ml + 2 * at) = make_float2(0.f, nan);
+                    else fill_row<T>((T *)a.out.ptr + it.b * a.out.batch_stride + (int64_t)qi * a.out.row_stride + (int64_t)it.h * a.D, a.D, nan);
+                    if (sp.splits == 1 && a.lse != nullptr) a.lse[at] = nan;
+                }
+                item = -1;
             }
         }
     }
@@ -422,9 +504,9 @@ bool dense_tc_ok(const DenseArgs &a, int dtype, bool backward) {
 
 template <typename T, int DP>
 static int fwd_launch(const DenseArgs &a, DenseSplit sp, cudaStream_t st) {
-    CUtensorMap mq, mk, mv, mo;
+    CUtensorMap mq, mk, mv;
     if (!make_map(&mq, a.q, a.B, a.Lq, a.H, a.D, 1, 128) || !make_map(&mk, a.k, a.B, a.Lk, a.Hkv, a.D, 1, 128) ||
-        !make_map(&mv, a.v, a.B, a.Lk, a.Hkv, a.D, 1, 128) || !make_map(&mo, a.out, a.B, a.Lq, a.H, a.D, 1, 128))
+        !make_map(&mv, a.v, a.B, a.Lk, a.Hkv, a.D, 1, 128))
         return fail(HSA_ERR_ARG, "hsa_dense_attn_fwd: the driver refused a tensor map");
     const long long blocks = (long long)a.B * a.H * ((a.Lq + 255) / 256) * sp.splits;
     if (blocks > 0x7fffffffLL) return fail(HSA_ERR_ARG, "hsa_dense_attn_fwd: too many tiles");
@@ -432,7 +514,7 @@ static int fwd_launch(const DenseArgs &a, DenseSplit sp, cudaStream_t st) {
     constexpr int smem = FwdShape<DP>::kSmem;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return fail((int)e, "hsa_dense_attn_fwd: shared memory %d: %s", smem, cudaGetErrorString(e));
-    kernel<<<(unsigned)blocks, kTcThreads, smem, st>>>(a, sp, mq, mk, mv, mo);
+    kernel<<<(unsigned)blocks, kTcThreads, smem, st>>>(a, sp, mq, mk, mv);
     if (int rc = launch_status("hsa_dense_attn_fwd")) return rc;
     if (sp.splits == 1) return 0;
     const long long rows = (long long)a.B * a.Lq * a.H;
@@ -444,6 +526,7 @@ int dense_fwd_tc(const DenseArgs &a, void *workspace, size_t workspace_bytes, in
     DenseSplit sp{};
     sp.splits = dense_fwd_splits(a.B, a.Lq, a.Lk, a.H);
     sp.wait_limit = wait_limit_cycles();
+    sp.extra_tx = wait_extra_tx();
     if (sp.splits > 1) {
         const size_t need = dense_fwd_tc_workspace(a.B, a.Lq, a.Lk, a.H, a.D);
         if (workspace == nullptr || workspace_bytes < need)
