@@ -54,10 +54,10 @@ dense_mask_pack_kernel(const uint8_t *__restrict__ mask, int64_t sb, int64_t sh,
 }
 
 // ------------------------------------------------------------------------------------------------ backward's row sums
-// delta[b, h, i] = sum_d dout * out and the row's log-sum-exp in base 2, padded with rows that give weight zero.  A query
-// without keys gets +inf and 0 whatever its output row holds.
+// -sum_d dout * out and minus the row's log-sum-exp in base 2 (the kernels add both), padded with rows that give weight zero.  A
+// query without keys gets -inf and 0 whatever its output row holds.
 template <typename T, int VEC, int LPR, int CPL>
-__global__ void __launch_bounds__(256) dense_delta_kernel(const DenseArgs a, float *__restrict__ lse2, float *__restrict__ delta) {
+__global__ void __launch_bounds__(256) dense_delta_kernel(const DenseArgs a, float *__restrict__ neg_lse2, float *__restrict__ neg_delta) {
     const long long row = (long long)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
     const int g = threadIdx.x % LPR;
     const int h = (int)(row % a.H), i = (int)(row / a.H % a.lq_pad);
@@ -65,7 +65,7 @@ __global__ void __launch_bounds__(256) dense_delta_kernel(const DenseArgs a, flo
     if (b >= a.B) return;
     const int64_t at = (b * a.H + h) * a.lq_pad + i;
     if (i >= a.Lq) {
-        if (g == 0) { lse2[at] = INFINITY; delta[at] = 0.f; }
+        if (g == 0) { neg_lse2[at] = -INFINITY; neg_delta[at] = 0.f; }
         return;
     }
     RowFrag<T, VEC, LPR, CPL> x, y;
@@ -75,18 +75,18 @@ __global__ void __launch_bounds__(256) dense_delta_kernel(const DenseArgs a, flo
     if (g == 0) {
         const float l = a.lse[(b * a.Lq + i) * a.H + h];
         const bool none = l == -INFINITY;
-        lse2[at] = none ? INFINITY : l * 1.4426950408889634f;
-        delta[at] = none ? 0.f : s;
+        neg_lse2[at] = none ? -INFINITY : l * -1.4426950408889634f;
+        neg_delta[at] = none ? 0.f : -s;
     }
 }
 
-static int dense_delta(const DenseArgs &a, float *lse2, float *delta, int dtype, bool vec, cudaStream_t st) {
+static int dense_delta(const DenseArgs &a, float *neg_lse2, float *neg_delta, int dtype, bool vec, cudaStream_t st) {
     return dispatch_dtype(dtype, [&]<typename T>() -> int {
         int rc = 0;
         const bool ok = dispatch_row_shape<T>(a.D, vec, [&]<typename T2, int VEC, int LPR, int CPL>() {
             const long long rows = (long long)a.B * a.lq_pad * a.H, blocks = (rows + 256 / LPR - 1) / (256 / LPR);
             if (blocks > 0x7fffffffLL) { rc = fail(HSA_ERR_ARG, "hsa_dense_attn_bwd: too many rows"); return; }
-            dense_delta_kernel<T2, VEC, LPR, CPL><<<(unsigned)blocks, 256, 0, st>>>(a, lse2, delta);
+            dense_delta_kernel<T2, VEC, LPR, CPL><<<(unsigned)blocks, 256, 0, st>>>(a, neg_lse2, neg_delta);
             rc = launch_status("hsa_dense_attn_bwd(row sums)");
         });
         return ok ? rc : fail(HSA_ERR_ARG, "hsa_dense_attn_bwd: head dim %d not supported", a.D);
@@ -203,15 +203,15 @@ extern "C" int hsa_dense_attn_bwd(hsa_view Q, hsa_view K, hsa_view V, hsa_view O
     a.B = B; a.Lq = Lq; a.Lk = Lk; a.H = H; a.Hkv = Hkv; a.D = D; a.group = H / Hkv;
     a.lq_pad = (Lq + 127) / 128 * 128;
     a.scale = scale; a.scale_log2 = scale * 1.4426950408889634f;
-    float *lse2 = (float *)workspace, *delta = lse2 + (size_t)B * H * a.lq_pad;
-    a.lse2 = lse2; a.delta = delta;
+    float *neg_lse2 = (float *)workspace, *neg_delta = neg_lse2 + (size_t)B * H * a.lq_pad;
+    a.neg_lse2 = neg_lse2; a.neg_delta = neg_delta;
     const int es = dtype_size(dtype);
     a.vec = D % 4 == 0;
     for (const hsa_view &v : {Q, K, V, dOut, dQ, dK, dV}) a.vec = a.vec && rows_in_fours(v, es);
     const bool tc = algo != 1 && dense_tc_ok(a, dtype, true) && dense_bwd_tables_ok(a);
     HSA_CHECK_ARG(algo != 2 || tc, "hsa_dense_attn_bwd: no tensor-core kernel for these inputs");
     cudaStream_t st = (cudaStream_t)stream;
-    if (int rc = dense_delta(a, lse2, delta, dtype, D % (16 / es) == 0 && view_vec_ok(Out, es) && view_vec_ok(dOut, es), st)) return rc;
+    if (int rc = dense_delta(a, neg_lse2, neg_delta, dtype, D % (16 / es) == 0 && view_vec_ok(Out, es) && view_vec_ok(dOut, es), st)) return rc;
     if (tc) return dense_bwd_tc(a, dtype, st);
     if (int rc = dense_simt(a, 1, dtype, st)) return rc;
     return dense_simt(a, 2, dtype, st);

@@ -235,12 +235,12 @@ __global__ void __launch_bounds__(kSimtThreads) dense_dq_simt_kernel(const Dense
     load_rows<T, BT, DP>(Qs, Q, a.q.row_stride, q0, a.Lq, a.D, a.vec, nullptr);
     load_rows<T, BT, DP>(Gs, G, a.dout.row_stride, q0, a.Lq, a.D, a.vec, nullptr);
     float4 o[R][NC];
-    float lse2[R], delta[R];
+    float lse2[R], delta[R];                                // both negated
 #pragma unroll
     for (int i = 0; i < R; ++i) {
         const int64_t at = ((int64_t)b * a.H + h) * a.lq_pad + q0 + ty + 16 * i;      // lq_pad covers whole tiles
-        lse2[i] = a.lse2[at];
-        delta[i] = a.delta[at];
+        lse2[i] = a.neg_lse2[at];
+        delta[i] = a.neg_delta[at];
 #pragma unroll
         for (int c = 0; c < NC; ++c) o[i][c] = make_float4(0.f, 0.f, 0.f, 0.f);
     }
@@ -262,8 +262,8 @@ __global__ void __launch_bounds__(kSimtThreads) dense_dq_simt_kernel(const Dense
 #pragma unroll
             for (int j = 0; j < R; ++j) {
                 const int kj = k0 + tx + 16 * j;
-                const bool ok = kj < n && lse2[i] != INFINITY && (bits == nullptr || mask_allows(a.mask, bits, qi, kj));
-                Ds[(ty + 16 * i) * (BT + 4) + tx + 16 * j] = ok ? exp2f(s[i][j] * a.scale_log2 - lse2[i]) * (dp[i][j] - delta[i]) : 0.f;
+                const bool ok = kj < n && lse2[i] != -INFINITY && (bits == nullptr || mask_allows(a.mask, bits, qi, kj));
+                Ds[(ty + 16 * i) * (BT + 4) + tx + 16 * j] = ok ? exp2f(fmaf(s[i][j], a.scale_log2, lse2[i])) * (dp[i][j] + delta[i]) : 0.f;
             }
         }
         __syncwarp();
@@ -327,14 +327,14 @@ __global__ void __launch_bounds__(kSimtThreads) dense_dkdv_simt_kernel(const Den
                 for (int j = 0; j < R; ++j) {
                     const int qj = q0 + tx + 16 * j;
                     const int64_t at = ((int64_t)b * a.H + h) * a.lq_pad + qj;
-                    const float lse2 = a.lse2[at], delta = a.delta[at];
+                    const float lse2 = a.neg_lse2[at], delta = a.neg_delta[at];
 #pragma unroll
                     for (int i = 0; i < R; ++i) {
                         const int ki = k0 + ty + 16 * i;
-                        const bool ok = ki < n && lse2 != INFINITY && (bits == nullptr || mask_allows(a.mask, bits, qj, ki));
-                        const float p = ok ? exp2f(s[i][j] * a.scale_log2 - lse2) : 0.f;
+                        const bool ok = ki < n && lse2 != -INFINITY && (bits == nullptr || mask_allows(a.mask, bits, qj, ki));
+                        const float p = ok ? exp2f(fmaf(s[i][j], a.scale_log2, lse2)) : 0.f;
                         Ps[(ty + 16 * i) * (BT + 4) + tx + 16 * j] = p;
-                        Ds[(ty + 16 * i) * (BT + 4) + tx + 16 * j] = ok ? p * (dp[i][j] - delta) : 0.f;
+                        Ds[(ty + 16 * i) * (BT + 4) + tx + 16 * j] = ok ? p * (dp[i][j] + delta) : 0.f;
                     }
                 }
                 __syncwarp();

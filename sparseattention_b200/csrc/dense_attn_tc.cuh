@@ -9,12 +9,40 @@
 namespace hsa {
 
 constexpr int kFlagTiles = 768;                  // tiles whose mask state fits one of a block's two tables
-// Eight warps for the element-wise part, one for copies, one for products; two more stand idle so that the last four form a
-// warpgroup, whose registers go to the others: 2 x 128 x 208 + 128 x 88 = 384 x 168, what the block is launched with.
-constexpr int kTcThreads = 384;
+constexpr int kTcThreads = 320;                  // eight warps for the element-wise part, one for copies, one for products
 
-__device__ __forceinline__ void give_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 88;\n"); }
-__device__ __forceinline__ void take_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 208;\n"); }
+// Two 32-bit numbers in a register pair: one instruction for both
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+    uint64_t v;
+    asm("mov.b64 %0, {%1, %2};\n" : "=l"(v) : "f"(lo), "f"(hi));
+    return v;
+}
+__device__ __forceinline__ float2 unpair(uint64_t v) {
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;\n" : "=f"(f.x), "=f"(f.y) : "l"(v));
+    return f;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;\n" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t pair_bits(uint32_t lo, uint32_t hi) { return pair(__uint_as_float(lo), __uint_as_float(hi)); }
+
+// The value of lane 0, which is every lane's: tells the compiler that what depends on it is the same in the whole warp.  The
+// warps that issue products need that: with descriptors and loop state in uniform registers an issue takes ISSUE_NEW cycles,
+// with per-lane ones 69 (and a commit 100), which bound all three kernels.
+__device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
 
 // Bit words of the keys [32 w, 32 w + 32) of a tile: those before `left` (keys of the sequence that remain)
 __device__ __forceinline__ uint32_t tail_word(int left, int w) {

@@ -5,14 +5,16 @@
 //
 // Two kernels, one per side, each of which recomputes the scores: seven products instead of the five that one kernel would need,
 // but every gradient row has one writer and a fixed order of summation, and no 32-bit partial gradients cross HBM.
-//   dq:    a block owns 128 queries and walks over tiles of 128 keys.  Tensor memory: S, dP (128 columns each), dS as 16-bit
-//          numbers (64), dq (DP).  S and dP of the next tile are issued as soon as the element-wise warps have this tile's in
-//          registers.
-//   dk/dv: a block owns 128 keys of a key/value head and walks over tiles of 64 queries of all its query heads, with everything
-//          transposed (S^T = K Q^T), so that P^T and dS^T can stay in tensor memory, over the scores they came from, as the
-//          first operands of dv += P^T do and dk += dS^T q.  Two buffers of S^T and dP^T (64 columns each) alternate, one per
-//          element-wise warpgroup; with dv and dk all 512 columns are in use at DP = 128.
-// Eight element-wise warps per block (a thread per row and column half, or per row), one for copies, one for products.
+//   dq:    a work item is 128 queries against tiles of 128 keys, in halves of 64.  Tensor memory: two buffers of S and dP (64
+//          columns each) and dq (DP columns).  dS replaces S in place, as the first operand of dq += dS k.
+//   dk/dv: a work item is 128 keys of a key/value head against tiles of 64 queries of all its query heads, with everything
+//          transposed (S^T = K Q^T), so that P^T and dS^T can stay in tensor memory, in place of the scores they came from, as
+//          the first operands of dv += P^T do and dk += dS^T q.  Two buffers of S^T and dP^T; with dv and dk all 512 columns are
+//          in use at DP = 128.
+// Eight element-wise warps (two per 32 rows, half of the columns each), one for copies, one for products.  While the element-wise
+// warps work on one buffer, the products fill the other.  (With a warpgroup per buffer instead of both on one, a warpgroup
+// waited half its time for its own buffer: dk/dv took 738 us at 4096 x 4096, batch 2, 16 heads of 128, where this takes DKV_US;
+// dq with 128 columns in one buffer took 436 us where this takes DQ_US.)
 // Rounding: p and ds are rounded to the inputs' type once, as operands; all sums are 32-bit.
 #include "dense_attn_tc.cuh"
 
@@ -52,8 +54,8 @@ dense_dq_tc5_kernel(const DenseArgs a, const long long wait_limit, const unsigne
     using Shape = DqShape<DP>;
     constexpr int TILE = Shape::kTile, KS = Shape::kKSlots, VS = Shape::kVSlots, PLANES = DP / 64, PLANE = 16384;
     constexpr bool BF = std::is_same<T, __nv_bfloat16>::value;
-    constexpr uint32_t IDESC_S = instr_desc(128, 128, BF, false, false), IDESC_O = instr_desc(128, DP, BF, false, true);
-    constexpr uint32_t COL_S = 0, COL_P = 128, COL_D = 256, COL_Q = 320;
+    constexpr uint32_t IDESC_S = instr_desc(128, 64, BF, false, false), IDESC_O = instr_desc(128, DP, BF, false, true);
+    constexpr uint32_t COL_Q = 256;                          // below: two buffers of S and dP, 64 columns each
 
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char *smem = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
@@ -63,8 +65,9 @@ dense_dq_tc5_kernel(const DenseArgs a, const long long wait_limit, const unsigne
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + Shape::kBars);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
     const uint32_t bar0 = smem_addr(bars);
-    const uint32_t qg_full = bar0, s_full = bar0 + 8, s_free = bar0 + 16, p_full = bar0 + 24, p_free = bar0 + 32, d_full = bar0 + 40,
-                   d_free = bar0 + 48, qg_empty = bar0 + 56, answer = bar0 + 64;
+    const uint32_t qg_full = bar0, qg_empty = bar0 + 8, q_done = bar0 + 16, answer = bar0 + 24;
+    auto s_full = [&](uint32_t x) { return bar0 + 8u * (5 + x); };
+    auto d_full = [&](uint32_t x) { return bar0 + 8u * (7 + x); };
     auto k_full = [&](int s) { return bar0 + 8u * (9 + s); };
     auto k_empty = [&](int s) { return bar0 + 8u * (9 + KS + s); };
     auto v_full = [&](int s) { return bar0 + 8u * (9 + 2 * KS + s); };
@@ -72,14 +75,13 @@ dense_dq_tc5_kernel(const DenseArgs a, const long long wait_limit, const unsigne
     auto info_full = [&](int s) { return bar0 + 8u * (9 + 2 * KS + 2 * VS + s); };
     auto info_empty = [&](int s) { return bar0 + 8u * (11 + 2 * KS + 2 * VS + s); };
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
     const bool masked = a.mask.bits != nullptr;
     if (threadIdx.x == 0) {
-        mbar_init(qg_full, 1); mbar_init(s_full, 1); mbar_init(s_free, 8); mbar_init(p_full, 1); mbar_init(p_free, 8);
-        mbar_init(d_full, 8); mbar_init(d_free, 1); mbar_init(qg_empty, 1); mbar_init(answer, 1);
+        mbar_init(qg_full, 1); mbar_init(qg_empty, 1); mbar_init(q_done, 1); mbar_init(answer, 1);
         for (int s = 0; s < KS; ++s) { mbar_init(k_full(s), 1); mbar_init(k_empty(s), 1); }
         for (int s = 0; s < VS; ++s) { mbar_init(v_full(s), 1); mbar_init(v_empty(s), 1); }
-        for (int s = 0; s < 2; ++s) { mbar_init(info_full(s), 1); mbar_init(info_empty(s), 9); }
+        for (int x = 0; x < 2; ++x) { mbar_init(s_full(x), 1); mbar_init(d_full(x), 8); mbar_init(info_full(x), 1); mbar_init(info_empty(x), 9); }
         *abort_flag = 0;
         mbar_fence_init();
         prefetch_map(&map_q); prefetch_map(&map_k); prefetch_map(&map_v); prefetch_map(&map_g);
@@ -155,87 +157,100 @@ dense_dq_tc5_kernel(const DenseArgs a, const long long wait_limit, const unsigne
             while (clock64() - start < 200000) {}
         }
     } else if (warp == 9) {
+        // S and dP of half tile j + 1 are issued before dq takes half tile j; half tile j + 2 goes where j was, after it.
         bool ok = true;
         int ks = 0, vs = 0, kd = 0; uint32_t kp = 0, vp = 0, qc = 0;
-        uint32_t issued = 0, done = 0;                       // tiles whose scores, and whose dq, have been issued
+        uint32_t issued = 0, done = 0;                       // half tiles whose scores, and whose dq, have been issued
         for (int k = 0; ok; ++k) {
             const int is = k & 1;
             if (!(ok = wait(info_full(is), (k >> 1) & 1))) break;
-            const int item = items.item[is];
+            const int item = uniform(items.item[is]);
             if (item < 0) break;
-            const DqItem it(a, item);
-            auto next_tile = [&](int t) { while (t < it.tiles && masked && items.flags[is][t] == 0) ++t; return t; };
-            // S and dP of tile t; the K tile stays until dq has read it
-            auto scores = [&](int t, bool last) -> bool {
-                if (!wait(k_full(ks), kp)) return false;
-                if (issued > 0 && !wait(s_free, (issued - 1) & 1)) return false;
+            DqItem it(a, item);
+            it.n = uniform(it.n); it.tiles = uniform(it.tiles);
+            auto next_tile = [&](int t) {
+                if (masked) { while (t < it.tiles && items.flags[is][t] == 0) ++t; t = uniform(t); }
+                return t;
+            };
+            auto halves = [&](int t) { return it.n - t * 128 > 64 ? 2 : 1; };
+            int ts = next_tile(0), hs = 0, td = ts, hd = 0;  // next half tile to score, next to sum
+            // S and dP of (ts, hs); the K tile stays until dq has read it
+            auto scores = [&]() -> bool {
                 unsigned char *kt = k_s + ks * TILE;
-                if (it.n - t * 128 < 128 || masked)
-                    zero_hidden_rows<PLANES>(kt, it.n - t * 128, masked ? a.mask.seen + it.plane * a.mask.wk + t * 4 : nullptr, lane);
+                if (hs == 0) {
+                    if (!wait(k_full(ks), kp)) return false;
+                    if (it.n - ts * 128 < 128 || masked)
+                        zero_hidden_rows<PLANES>(kt, it.n - ts * 128, masked ? a.mask.seen + it.plane * a.mask.wk + ts * 4 : nullptr, lane);
+                    if (!wait(v_full(vs), vp)) return false;
+                }
                 fence_after_sync();
-                if (lane == 0) {
-                    const uint64_t qd = smem_desc(smem_addr(q_s), 16, 1024), kdsc = smem_desc(smem_addr(kt), 16, 1024);
+                const bool half_last = hs + 1 == halves(ts);
+                const int tn = half_last ? next_tile(ts + 1) : ts;
+                if (elect_one()) {
+                    const uint32_t d = tmem + (issued & 1) * 128;
+                    const uint64_t qd = smem_desc(smem_addr(q_s), 16, 1024), kdsc = smem_desc(smem_addr(kt) + hs * 8192, 16, 1024);
+                    const uint64_t gd = smem_desc(smem_addr(g_s), 16, 1024), vd = smem_desc(smem_addr(v_s + vs * TILE) + hs * 8192, 16, 1024);
 #pragma unroll
                     for (int j = 0; j < DP / 16; ++j) {
                         const uint32_t off = (j >> 2) * (PLANE >> 4) + (j & 3) * 2;
-                        mma_f16(tmem + COL_S, qd + off, kdsc + off, IDESC_S, j > 0);
+                        mma_f16(d, qd + off, kdsc + off, IDESC_S, j > 0);
                     }
-                    mma_commit(s_full);
-                }
-                __syncwarp();
-                if (++ks == KS) { ks = 0; kp ^= 1; }
-                if (!wait(v_full(vs), vp)) return false;
-                if (issued > 0 && !wait(p_free, (issued - 1) & 1)) return false;
-                fence_after_sync();
-                if (lane == 0) {
-                    const uint64_t gd = smem_desc(smem_addr(g_s), 16, 1024), vd = smem_desc(smem_addr(v_s + vs * TILE), 16, 1024);
 #pragma unroll
                     for (int j = 0; j < DP / 16; ++j) {
                         const uint32_t off = (j >> 2) * (PLANE >> 4) + (j & 3) * 2;
-                        mma_f16(tmem + COL_P, gd + off, vd + off, IDESC_S, j > 0);
+                        mma_f16(d + 64, gd + off, vd + off, IDESC_S, j > 0);
                     }
-                    mma_commit(v_empty(vs));
-                    if (last) mma_commit(qg_empty);
-                    mma_commit(p_full);
+                    if (half_last) mma_commit(v_empty(vs));
+                    if (tn >= it.tiles) mma_commit(qg_empty);
+                    mma_commit(s_full(issued & 1));
                 }
                 __syncwarp();
-                if (++vs == VS) { vs = 0; vp ^= 1; }
+                if (half_last) {
+                    if (++ks == KS) { ks = 0; kp ^= 1; }
+                    if (++vs == VS) { vs = 0; vp ^= 1; }
+                    hs = 0;
+                } else {
+                    hs = 1;
+                }
+                ts = tn;
                 ++issued;
                 return true;
             };
-            int t = next_tile(0);
             bool fresh = true;
-            if (t < it.tiles) {
-                ok = wait(qg_full, qc & 1) && scores(t, next_tile(t + 1) >= it.tiles);
+            if (ts < it.tiles) {
+                ok = wait(qg_full, qc & 1) && scores();
                 ++qc;
             }
-            while (ok && t < it.tiles) {
-                const int tn = next_tile(t + 1);
-                if (tn < it.tiles && !(ok = scores(tn, next_tile(tn + 1) >= it.tiles))) break;
-                if (!(ok = wait(d_full, done & 1))) break;
-                ++done;
+            while (ok && td < it.tiles) {
+                if (ts < it.tiles && !(ok = scores())) break;
+                if (!(ok = wait(d_full(done & 1), done >> 1 & 1))) break;
                 fence_after_sync();
-                if (lane == 0) {
-                    const uint64_t kdsc = smem_desc(smem_addr(k_s + kd * TILE), PLANE, 1024);
+                const bool half_last = hd + 1 == halves(td);
+                const int tn = half_last ? next_tile(td + 1) : td;
+                if (elect_one()) {
+                    const uint64_t kdsc = smem_desc(smem_addr(k_s + kd * TILE) + hd * 8192, PLANE, 1024);
+                    const uint32_t d = tmem + (done & 1) * 128;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        mma_f16_ta(tmem + COL_Q, tmem + COL_D + j * 8, kdsc + j * 128, IDESC_O, (!fresh || j > 0) ? 1u : 0u);
-                    mma_commit(k_empty(kd));
-                    mma_commit(d_free);
+                    for (int j = 0; j < 4; ++j)              // either warpgroup's 32 keys lie where its scores were
+                        mma_f16_ta(tmem + COL_Q, d + (j >> 1) * 32 + (j & 1) * 8, kdsc + j * 128, IDESC_O, (!fresh || j > 0) ? 1u : 0u);
+                    if (half_last) mma_commit(k_empty(kd));
+                    if (tn >= it.tiles) mma_commit(q_done);
                 }
                 __syncwarp();
-                if (++kd == KS) kd = 0;
+                if (half_last && ++kd == KS) kd = 0;
+                hd = half_last ? 0 : 1;
+                td = tn;
                 fresh = false;
-                t = tn;
+                ++done;
             }
             if (ok && lane == 0) mbar_arrive(info_empty(is));
             __syncwarp();
         }
-    } else if (warp < 8) {
-        const int half = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane;
+    } else {
+        const int x = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane;      // warpgroup x: keys [32 x, 32 x + 32) of a half tile
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
         bool ok = true;
-        uint32_t i = 0;                                      // tiles done so far
+        uint32_t i = 0, qc = 0;                              // half tiles, and items that had any
         int k = 0, item = -1;
         for (; ok; ++k) {
             const int is = k & 1;
@@ -246,73 +261,54 @@ dense_dq_tc5_kernel(const DenseArgs a, const long long wait_limit, const unsigne
             const DqItem it(a, item);
             const int qi = it.q0 + row;
             const int64_t at = ((int64_t)it.b * a.H + it.h) * a.lq_pad + qi;
-            const float lse2 = a.lse2[at], delta = a.delta[at];
+            const float neg_lse2 = a.neg_lse2[at], neg_delta = a.neg_delta[at];
+            const uint64_t c2 = pair(a.scale_log2, a.scale_log2), lse22 = pair(neg_lse2, neg_lse2), delta2 = pair(neg_delta, neg_delta);
             const uint32_t *bits = masked ? a.mask.bits + (it.plane * a.mask.rows + (a.mask.rows > 1 ? min(qi, a.Lq - 1) : 0)) * a.mask.wk : nullptr;
             bool any = false;
-            for (int t = 0; t < it.tiles; ++t) {
+            for (int t = 0; t < it.tiles && ok; ++t) {
                 const uint32_t flag = masked ? items.flags[is][t] : 2u;
                 if (flag == 0) continue;
                 const int left = it.n - t * 128;
                 const bool partial = left < 128 || flag != 2;
-                uint32_t keep[2] = {0xffffffffu, 0xffffffffu};
-                if (partial) {
-                    uint2 w = make_uint2(~0u, ~0u);
-                    if (masked) w = __ldg(reinterpret_cast<const uint2 *>(bits + t * 4 + 2 * half));
-                    keep[0] = w.x & tail_word(left, 2 * half);
-                    keep[1] = w.y & tail_word(left, 2 * half + 1);
+                for (int half = 0; half < (left > 64 ? 2 : 1); ++half) {
+                    uint32_t keep = 0xffffffffu;
+                    if (partial) {
+                        keep = tail_word(left, 2 * half + x);
+                        if (masked) keep &= __ldg(bits + t * 4 + 2 * half + x);
+                    }
+                    if (!(ok = wait(s_full(i & 1), i >> 1 & 1))) break;
+                    fence_after_sync();
+                    const uint32_t ts = tmem + lanes + (i & 1) * 128 + 32 * x;
+                    uint32_t r[32], g[32], d[16];
+                    tmem_ld32(ts, r);
+                    tmem_ld32(ts + 64, g);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        const float2 e = unpair(fma2(pair_bits(r[2 * j], r[2 * j + 1]), c2, lse22));
+                        const uint64_t p = pair(fast_exp2(e.x), fast_exp2(e.y));
+                        float2 y = unpair(mul2(p, add2(pair_bits(g[2 * j], g[2 * j + 1]), delta2)));
+                        if (partial) {                       // not through p = 0: what a hidden row holds may be NaN
+                            if (!((keep >> (2 * j)) & 1u)) y.x = 0.f;
+                            if (!((keep >> (2 * j + 1)) & 1u)) y.y = 0.f;
+                        }
+                        d[j] = pack2<T>(y.x, y.y);
+                    }
+                    tmem_st16(ts, d);
+                    tmem_st_wait();
+                    fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(d_full(i & 1));
+                    ++i;
+                    any = true;
                 }
-                if (!(ok = wait(s_full, i & 1))) break;
-                fence_after_sync();
-                uint32_t s[2][32], g[2][32], d[32];
-                tmem_ld32(tmem + COL_S + lanes + 64 * half, s[0]);
-                tmem_ld32(tmem + COL_S + lanes + 64 * half + 32, s[1]);
-                tmem_ld_wait();
-                fence_before_sync();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(s_free);
-#pragma unroll
-                for (int c = 0; c < 2; ++c)
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) s[c][j] = __float_as_uint(fast_exp2(fmaf(__uint_as_float(s[c][j]), a.scale_log2, -lse2)));
-                if (!(ok = wait(p_full, i & 1))) break;
-                fence_after_sync();
-                tmem_ld32(tmem + COL_P + lanes + 64 * half, g[0]);
-                tmem_ld32(tmem + COL_P + lanes + 64 * half + 32, g[1]);
-                tmem_ld_wait();
-                fence_before_sync();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(p_free);
-#pragma unroll
-                for (int c = 0; c < 2; ++c)
-#pragma unroll
-                    for (int j = 0; j < 32; ++j)
-                        g[c][j] = __float_as_uint(__uint_as_float(s[c][j]) * (__uint_as_float(g[c][j]) - delta));
-                if (partial) {
-#pragma unroll
-                    for (int c = 0; c < 2; ++c)
-#pragma unroll
-                        for (int j = 0; j < 32; ++j)
-                            if (!((keep[c] >> j) & 1u)) g[c][j] = 0u;
-                }
-#pragma unroll
-                for (int j = 0; j < 32; ++j)
-                    d[j] = pack2<T>(__uint_as_float(g[j >> 4][(2 * j) & 31]), __uint_as_float(g[j >> 4][(2 * j + 1) & 31]));
-                if (i > 0 && !(ok = wait(d_free, (i - 1) & 1))) break;
-                fence_after_sync();
-                tmem_st32(tmem + COL_D + lanes + 32 * half, d);
-                tmem_st_wait();
-                fence_before_sync();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(d_full);
-                ++i;
-                any = true;
             }
-            if (ok && any) ok = wait(d_free, (i - 1) & 1);
+            if (ok && any) { ok = wait(q_done, qc & 1); ++qc; }
             if (!ok) break;                                  // with k and item of the unfinished one
             fence_after_sync();
             T *out = (T *)a.dq.ptr + it.b * a.dq.batch_stride + (int64_t)qi * a.dq.row_stride + (int64_t)it.h * a.D;
 #pragma unroll 1
-            for (int c = half * (DP / 64); c < (half + 1) * (DP / 64); ++c) {        // 32 columns at a time
+            for (int c = x * (DP / 64); c < (x + 1) * (DP / 64); ++c) {        // 32 columns at a time
                 uint32_t o[32];
                 if (any) {
                     tmem_ld32(tmem + COL_Q + lanes + 32 * c, o);
@@ -387,13 +383,13 @@ dense_dkdv_tc5_kernel(const DenseArgs a, const long long wait_limit, const unsig
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char *smem = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
     unsigned char *k_s = smem, *v_s = k_s + TILE, *ring = v_s + TILE;
-    float *stats = reinterpret_cast<float *>(ring + ST * Shape::kStage);          // per stage: 64 log-sum-exps, 64 row sums
+    float *stats = reinterpret_cast<float *>(ring + ST * Shape::kStage);          // per stage: 64 log-sum-exps, 64 row sums, both negated
     ItemSlots &items = *reinterpret_cast<ItemSlots *>(stats + ST * 128);
     unsigned long long *bars = reinterpret_cast<unsigned long long *>(&items + 1);
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + Shape::kBars);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
     const uint32_t bar0 = smem_addr(bars);
-    const uint32_t kv_full = bar0, kv_empty = bar0 + 8, done = bar0 + 16, acc_free = bar0 + 24, answer = bar0 + 32;
+    const uint32_t kv_full = bar0, kv_empty = bar0 + 8, done = bar0 + 16, answer = bar0 + 24;
     auto s_full = [&](int x) { return bar0 + 8u * (5 + x); };
     auto d_full = [&](int x) { return bar0 + 8u * (7 + x); };
     auto full = [&](int s) { return bar0 + 8u * (9 + s); };
@@ -401,14 +397,14 @@ dense_dkdv_tc5_kernel(const DenseArgs a, const long long wait_limit, const unsig
     auto info_full = [&](int s) { return bar0 + 8u * (9 + 2 * ST + s); };
     auto info_empty = [&](int s) { return bar0 + 8u * (11 + 2 * ST + s); };
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
     const int qtiles = (a.Lq + 63) / 64;
     const bool masked = a.mask.bits != nullptr;
     const int cells = masked ? a.mask.tq : 0;
 
     if (threadIdx.x == 0) {
-        mbar_init(kv_full, 1); mbar_init(kv_empty, 1); mbar_init(done, 1); mbar_init(acc_free, 8); mbar_init(answer, 1);
-        for (int x = 0; x < 2; ++x) { mbar_init(s_full(x), 1); mbar_init(d_full(x), 4); mbar_init(info_full(x), 1); mbar_init(info_empty(x), 9); }
+        mbar_init(kv_full, 1); mbar_init(kv_empty, 1); mbar_init(done, 1); mbar_init(answer, 1);
+        for (int x = 0; x < 2; ++x) { mbar_init(s_full(x), 1); mbar_init(d_full(x), 8); mbar_init(info_full(x), 1); mbar_init(info_empty(x), 9); }
         for (int s = 0; s < ST; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
         *abort_flag = 0;
         mbar_fence_init();
@@ -422,7 +418,10 @@ dense_dkdv_tc5_kernel(const DenseArgs a, const long long wait_limit, const unsig
     auto wait = [&](uint32_t bar, uint32_t parity) { return (bool)__all_sync(0xffffffffu, mbar_wait(bar, parity, wait_limit, abort_flag)); };
     auto plane_of = [&](int b, int h) { return (int64_t)b * a.mask.plane_b + (int64_t)h * a.mask.plane_h; };
     auto flag_of = [&](int is, int u) { return items.flags[is][u / qtiles * cells + (a.mask.rows > 1 ? (u % qtiles) >> 1 : 0)]; };
-    auto next_unit = [&](int is, int u, int total) { while (u < total && masked && flag_of(is, u) == 0) ++u; return u; };
+    auto next_unit = [&](int is, int u, int total) {
+        if (masked) { while (u < total && flag_of(is, u) == 0) ++u; u = uniform(u); }
+        return u;
+    };
 
     if (warp == 8) {
         bool ok = true;
@@ -465,10 +464,10 @@ dense_dkdv_tc5_kernel(const DenseArgs a, const long long wait_limit, const unsig
                     const int64_t at = ((int64_t)it.b * a.H + h) * a.lq_pad + q0;
 #pragma unroll
                     for (int p = 0; p < PLANES; ++p) tma_load_4d(qs + p * HPLANE, &map_q, p * 64, h, q0, it.b, full(s));
-                    bulk_load(fs, a.lse2 + at, 256, full(s));
+                    bulk_load(fs, a.neg_lse2 + at, 256, full(s));
 #pragma unroll
                     for (int p = 0; p < PLANES; ++p) tma_load_4d(gs + p * HPLANE, &map_g, p * 64, h, q0, it.b, full(s));
-                    bulk_load(fs + 256, a.delta + at, 256, full(s));
+                    bulk_load(fs + 256, a.neg_delta + at, 256, full(s));
                 }
                 __syncwarp();
                 if (++s == ST) { s = 0; ph ^= 1; }
@@ -493,7 +492,7 @@ dense_dkdv_tc5_kernel(const DenseArgs a, const long long wait_limit, const unsig
         auto scores = [&](bool last) -> bool {                // S^T and dP^T of the next tile into buffer issued & 1
             if (!wait(full(s), ph)) return false;
             fence_after_sync();
-            if (lane == 0) {
+            if (elect_one()) {
                 const uint32_t qs = smem_addr(ring + s * Shape::kStage), col = tmem + (issued & 1) * 128;
                 const uint64_t kd = smem_desc(smem_addr(k_s), 16, 1024), vd = smem_desc(smem_addr(v_s), 16, 1024);
                 const uint64_t qd = smem_desc(qs, 16, 1024), gd = smem_desc(qs + HALF, 16, 1024);
@@ -514,9 +513,10 @@ dense_dkdv_tc5_kernel(const DenseArgs a, const long long wait_limit, const unsig
         for (int k = 0; ok; ++k) {
             const int is = k & 1;
             if (!(ok = wait(info_full(is), (k >> 1) & 1))) break;
-            const int item = items.item[is];
+            const int item = uniform(items.item[is]);
             if (item < 0) break;
-            const DkvItem it(a, item, qtiles);
+            DkvItem it(a, item, qtiles);
+            it.total = uniform(it.total);
             int u = next_unit(is, 0, it.total);
             bool fresh = true;
             if (u < it.total) {
@@ -527,16 +527,14 @@ dense_dkdv_tc5_kernel(const DenseArgs a, const long long wait_limit, const unsig
                 const int un = next_unit(is, u + 1, it.total);
                 if (un < it.total && !(ok = scores(next_unit(is, un + 1, it.total) >= it.total))) break;
                 if (!(ok = wait(d_full(i & 1), (i >> 1) & 1))) break;
-                // the first product of an item overwrites both accumulators: the other warpgroup may still read the last item's
-                if (fresh && kc > 1 && !(ok = wait(acc_free, kc & 1))) break;
                 fence_after_sync();
-                if (lane == 0) {
+                if (elect_one()) {
                     const uint32_t qs = smem_addr(ring + sd * Shape::kStage), col = tmem + (i & 1) * 128;
                     const uint64_t qd = smem_desc(qs, HPLANE, 1024), gd = smem_desc(qs + HALF, HPLANE, 1024);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) mma_f16_ta(tmem + COL_V, col + j * 8, gd + j * 128, IDESC_O, (!fresh || j > 0) ? 1u : 0u);
+                    for (int j = 0; j < 4; ++j) mma_f16_ta(tmem + COL_V, col + (j >> 1) * 32 + (j & 1) * 8, gd + j * 128, IDESC_O, (!fresh || j > 0) ? 1u : 0u);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) mma_f16_ta(tmem + COL_K, col + 64 + j * 8, qd + j * 128, IDESC_O, (!fresh || j > 0) ? 1u : 0u);
+                    for (int j = 0; j < 4; ++j) mma_f16_ta(tmem + COL_K, col + 64 + (j >> 1) * 32 + (j & 1) * 8, qd + j * 128, IDESC_O, (!fresh || j > 0) ? 1u : 0u);
                     mma_commit(empty(sd));
                     if (un >= it.total) mma_commit(done);
                 }
@@ -549,9 +547,10 @@ dense_dkdv_tc5_kernel(const DenseArgs a, const long long wait_limit, const unsig
             if (ok && lane == 0) mbar_arrive(info_empty(is));
             __syncwarp();
         }
-    } else if (warp < 8) {
-        const int x = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane;
-        const uint32_t lanes = (uint32_t)(quarter * 32) << 16, ts = tmem + lanes + x * 128;
+    } else {
+        const int x = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane;      // warpgroup x: queries [32 x, 32 x + 32) of a tile
+        const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+        const uint64_t c2 = pair(a.scale_log2, a.scale_log2);
         bool ok = true;
         uint32_t i = 0, kc = 0;                              // tiles, and items that had any
         int s = 0, k = 0, item = -1; uint32_t ph = 0;
@@ -565,82 +564,52 @@ dense_dkdv_tc5_kernel(const DenseArgs a, const long long wait_limit, const unsig
             const int key = it.k0 + row;
             const bool tail = it.n - it.k0 < 128;
             bool any = false;
-            for (int u = next_unit(is, 0, it.total); u < it.total; u = next_unit(is, u + 1, it.total), ++i) {
-                const int mine = s; const uint32_t mph = ph;
-                if (++s == ST) { s = 0; ph ^= 1; }
-                any = true;
-                if ((i & 1) != x) continue;
-                uint32_t keep[2] = {0xffffffffu, 0xffffffffu};
+            for (int u = next_unit(is, 0, it.total); u < it.total; u = next_unit(is, u + 1, it.total)) {
+                uint32_t keep = 0xffffffffu;
                 bool partial = tail;
                 if (masked && flag_of(is, u) != 2) {
                     partial = true;
                     const int64_t plane = plane_of(it.b, it.hk * a.group + u / qtiles);
                     if (key < a.Lk) {
-                        if (a.mask.rows > 1) {
-                            const uint2 w = __ldg(reinterpret_cast<const uint2 *>(a.mask.bits_t + (plane * a.Lk + key) * a.mask.wq + u % qtiles * 2));
-                            keep[0] = w.x; keep[1] = w.y;
-                        } else if (!((__ldg(a.mask.bits + plane * a.mask.wk + (key >> 5)) >> (key & 31)) & 1u)) {
-                            keep[0] = keep[1] = 0u;
-                        }
+                        if (a.mask.rows > 1) keep = __ldg(a.mask.bits_t + (plane * a.Lk + key) * a.mask.wq + u % qtiles * 2 + x);
+                        else if (!((__ldg(a.mask.bits + plane * a.mask.wk + (key >> 5)) >> (key & 31)) & 1u)) keep = 0u;
                     }
                 }
-                if (key >= it.n) keep[0] = keep[1] = 0u;
-                if (!(ok = wait(full(mine), mph) && wait(s_full(x), (i >> 1) & 1))) break;
+                if (key >= it.n) keep = 0u;
+                if (!(ok = wait(full(s), ph) && wait(s_full(i & 1), i >> 1 & 1))) break;
                 fence_after_sync();
-                const float *st = stats + mine * 128;
-                uint32_t r[2][32], p[2][32], pk[32];
-                tmem_ld32(ts, r[0]);
-                tmem_ld32(ts + 32, r[1]);
+                const float *st = stats + s * 128 + 32 * x;
+                const uint32_t ts = tmem + lanes + (i & 1) * 128 + 32 * x;
+                uint32_t r[32], g[32], pk[16], dk[16];
+                tmem_ld32(ts, r);
+                tmem_ld32(ts + 64, g);
                 tmem_ld_wait();
 #pragma unroll
-                for (int c = 0; c < 2; ++c)
+                for (int j = 0; j < 16; j += 2) {
+                    const float4 lse = *reinterpret_cast<const float4 *>(st + 2 * j), dl = *reinterpret_cast<const float4 *>(st + 64 + 2 * j);
 #pragma unroll
-                    for (int j = 0; j < 32; j += 4) {
-                        const float4 lse = *reinterpret_cast<const float4 *>(st + 32 * c + j);
-                        p[c][j] = __float_as_uint(fast_exp2(fmaf(__uint_as_float(r[c][j]), a.scale_log2, -lse.x)));
-                        p[c][j + 1] = __float_as_uint(fast_exp2(fmaf(__uint_as_float(r[c][j + 1]), a.scale_log2, -lse.y)));
-                        p[c][j + 2] = __float_as_uint(fast_exp2(fmaf(__uint_as_float(r[c][j + 2]), a.scale_log2, -lse.z)));
-                        p[c][j + 3] = __float_as_uint(fast_exp2(fmaf(__uint_as_float(r[c][j + 3]), a.scale_log2, -lse.w)));
+                    for (int e = 0; e < 2; ++e) {
+                        const int c = j + e;
+                        const float2 z = unpair(fma2(pair_bits(r[2 * c], r[2 * c + 1]), c2, e == 0 ? pair(lse.x, lse.y) : pair(lse.z, lse.w)));
+                        float2 p = make_float2(fast_exp2(z.x), fast_exp2(z.y));
+                        float2 y = unpair(mul2(pair(p.x, p.y), add2(pair_bits(g[2 * c], g[2 * c + 1]), e == 0 ? pair(dl.x, dl.y) : pair(dl.z, dl.w))));
+                        if (partial) {                           // not through p = 0: what a hidden row holds may be NaN
+                            if (!((keep >> (2 * c)) & 1u)) p.x = y.x = 0.f;
+                            if (!((keep >> (2 * c + 1)) & 1u)) p.y = y.y = 0.f;
+                        }
+                        pk[c] = pack2<T>(p.x, p.y);
+                        dk[c] = pack2<T>(y.x, y.y);
                     }
-                if (partial) {
-#pragma unroll
-                    for (int c = 0; c < 2; ++c)
-#pragma unroll
-                        for (int j = 0; j < 32; ++j)
-                            if (!((keep[c] >> j) & 1u)) p[c][j] = 0u;
                 }
-#pragma unroll
-                for (int j = 0; j < 32; ++j)
-                    pk[j] = pack2<T>(__uint_as_float(p[j >> 4][(2 * j) & 31]), __uint_as_float(p[j >> 4][(2 * j + 1) & 31]));
-                tmem_st32(ts, pk);
-                tmem_ld32(ts + 64, r[0]);
-                tmem_ld32(ts + 96, r[1]);
-                tmem_ld_wait();
-#pragma unroll
-                for (int c = 0; c < 2; ++c)
-#pragma unroll
-                    for (int j = 0; j < 32; j += 4) {
-                        const float4 dl = *reinterpret_cast<const float4 *>(st + 64 + 32 * c + j);
-                        r[c][j] = __float_as_uint(__uint_as_float(p[c][j]) * (__uint_as_float(r[c][j]) - dl.x));
-                        r[c][j + 1] = __float_as_uint(__uint_as_float(p[c][j + 1]) * (__uint_as_float(r[c][j + 1]) - dl.y));
-                        r[c][j + 2] = __float_as_uint(__uint_as_float(p[c][j + 2]) * (__uint_as_float(r[c][j + 2]) - dl.z));
-                        r[c][j + 3] = __float_as_uint(__uint_as_float(p[c][j + 3]) * (__uint_as_float(r[c][j + 3]) - dl.w));
-                    }
-                if (partial) {                                   // not through p = 0: what a hidden row holds may be NaN
-#pragma unroll
-                    for (int c = 0; c < 2; ++c)
-#pragma unroll
-                        for (int j = 0; j < 32; ++j)
-                            if (!((keep[c] >> j) & 1u)) r[c][j] = 0u;
-                }
-#pragma unroll
-                for (int j = 0; j < 32; ++j)
-                    pk[j] = pack2<T>(__uint_as_float(r[j >> 4][(2 * j) & 31]), __uint_as_float(r[j >> 4][(2 * j + 1) & 31]));
-                tmem_st32(ts + 64, pk);
+                tmem_st16(ts, pk);
+                tmem_st16(ts + 64, dk);
                 tmem_st_wait();
                 fence_before_sync();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(d_full(x));
+                if (lane == 0) mbar_arrive(d_full(i & 1));
+                if (++s == ST) { s = 0; ph ^= 1; }
+                ++i;
+                any = true;
             }
             if (ok && any) { ok = wait(done, kc & 1); ++kc; }
             if (!ok) break;                                      // with k and item of the unfinished one
@@ -662,10 +631,7 @@ dense_dkdv_tc5_kernel(const DenseArgs a, const long long wait_limit, const unsig
             }
             fence_before_sync();
             __syncwarp();
-            if (lane == 0) {
-                if (any) mbar_arrive(acc_free);
-                mbar_arrive(info_empty(is));
-            }
+            if (lane == 0) mbar_arrive(info_empty(is));
         }
         if (!ok) {
             // gave up: this item, and any that the block has already taken over, read NaN

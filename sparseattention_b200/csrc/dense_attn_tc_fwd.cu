@@ -2,13 +2,15 @@
 //
 //   out_i = sum_j exp2(c s_ij - m_i) v_j / sum_j exp2(c s_ij - m_i),   s_ij = q_i.k_j,  c = scale log2(e)
 //
-// One pass over the keys with a running maximum and sum.  A block owns 256 query rows of one (batch entry, head) as two tiles
-// of 128 and walks over tiles of 128 keys, 10 warps with fixed roles:
+// One pass over the keys with a running maximum and sum.  A work item is 256 query rows of one (batch entry, head), two tiles of
+// 128, against tiles of 128 keys in halves of 64; 10 warps with fixed roles:
 //   warp 8     copies K and V tiles into a ring (TMA boxes of [128 rows][128 bytes], 128-byte swizzle)
 //   warp 9     issues S = Q K^T (both operands in shared memory) and O += P V (P in tensor memory, V as an MN-major operand)
 //   warps 0-3  and 4-7: the softmax of the first and of the second query tile, a thread per row
-// While one tile's softmax runs, the tensor cores work for the other.  Tensor memory (512 columns): S of both tiles (128 each),
-// O of both tiles (DP each); P replaces S in place as 16-bit numbers, so it never passes through shared memory.
+// Tensor memory (512 columns): two half tiles of S for either query tile (64 columns each), O of both (DP each).  P replaces the
+// S it came from as 16-bit numbers, so it never passes through shared memory, and the other half tile's scores are computed
+// meanwhile.  (Scores in one piece of 128 columns, which had to wait for the product that consumes P, left a softmax warp
+// waiting a third of its time: 594 us where this takes FWD_US at 4096 x 4096, batch 4, 16 heads of 128.)
 // The output is rescaled only when a row's maximum has grown by more than 2^8 since the last time (the weights then lie below
 // 2^8, which changes nothing in their relative precision), so almost every tile leaves O alone.
 // Rounding: weights are rounded to the inputs' type for the second product (what the tensor cores take); their sum is taken
@@ -32,7 +34,7 @@ template <int DP>
 struct FwdShape {
     static constexpr int kTile = 128 * DP * 2;                       // bytes of a tile of 128 rows
     static constexpr int kSlots = DP == 128 ? 5 : 8;                 // K and V tiles in flight
-    static constexpr int kSmem = 1024 + 2 * kTile + kSlots * kTile + (int)sizeof(ItemSlots) + (10 + 2 * kSlots + kItemBars) * 8 + 8;
+    static constexpr int kSmem = 1024 + 2 * kTile + kSlots * kTile + (int)sizeof(ItemSlots) + (16 + 2 * kSlots + kItemBars) * 8 + 8;
     static_assert(kSmem <= 227 * 1024, "shared memory");
 };
 
@@ -63,7 +65,7 @@ dense_fwd_tc5_kernel(const DenseArgs a, const DenseSplit sp, const __grid_consta
     using Shape = FwdShape<DP>;
     constexpr int TILE = Shape::kTile, SLOTS = Shape::kSlots, PLANES = DP / 64, PLANE = 128 * 128;
     constexpr bool BF = std::is_same<T, __nv_bfloat16>::value;
-    constexpr uint32_t IDESC_S = instr_desc(128, 128, BF, false, false), IDESC_O = instr_desc(128, DP, BF, false, true);
+    constexpr uint32_t IDESC_S = instr_desc(128, 64, BF, false, false), IDESC_O = instr_desc(128, DP, BF, false, true);
     constexpr uint32_t COL_S = 0, COL_O = 256;
 
     extern __shared__ __align__(1024) unsigned char smem_raw[];
@@ -71,25 +73,27 @@ dense_fwd_tc5_kernel(const DenseArgs a, const DenseSplit sp, const __grid_consta
     unsigned char *q_s = smem, *ring = smem + 2 * TILE;
     ItemSlots &items = *reinterpret_cast<ItemSlots *>(ring + (size_t)SLOTS * TILE);
     unsigned long long *bars = reinterpret_cast<unsigned long long *>(&items + 1);
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 10 + 2 * SLOTS + kItemBars);
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 16 + 2 * SLOTS + kItemBars);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
     const uint32_t bar0 = smem_addr(bars);
     auto q_full = [&](int w) { return bar0 + 8u * w; };
     auto q_empty = [&](int w) { return bar0 + 8u * (2 + w); };
-    auto s_full = [&](int w) { return bar0 + 8u * (4 + w); };
-    auto p_full = [&](int w) { return bar0 + 8u * (6 + w); };
-    auto o_full = [&](int w) { return bar0 + 8u * (8 + w); };
-    auto kv_full = [&](int s) { return bar0 + 8u * (10 + s); };
-    auto kv_empty = [&](int s) { return bar0 + 8u * (10 + SLOTS + s); };
-    auto info_full = [&](int s) { return bar0 + 8u * (10 + 2 * SLOTS + s); };
-    auto info_empty = [&](int s) { return bar0 + 8u * (12 + 2 * SLOTS + s); };
-    const uint32_t answer = bar0 + 8u * (14 + 2 * SLOTS);
+    auto o_full = [&](int w) { return bar0 + 8u * (4 + w); };
+    auto s_full = [&](int w, uint32_t x) { return bar0 + 8u * (6 + 2 * w + x); };
+    auto p_full = [&](int w, uint32_t x) { return bar0 + 8u * (10 + 2 * w + x); };
+    auto o_done = [&](int w) { return bar0 + 8u * (14 + w); };
+    auto kv_full = [&](int s) { return bar0 + 8u * (16 + s); };
+    auto kv_empty = [&](int s) { return bar0 + 8u * (16 + SLOTS + s); };
+    auto info_full = [&](int s) { return bar0 + 8u * (16 + 2 * SLOTS + s); };
+    auto info_empty = [&](int s) { return bar0 + 8u * (18 + 2 * SLOTS + s); };
+    const uint32_t answer = bar0 + 8u * (20 + 2 * SLOTS);
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
     const bool masked = a.mask.bits != nullptr;
     if (threadIdx.x == 0) {
         for (int w = 0; w < 2; ++w) {
-            mbar_init(q_full(w), 1); mbar_init(q_empty(w), 1); mbar_init(s_full(w), 1); mbar_init(p_full(w), 4); mbar_init(o_full(w), 1);
+            mbar_init(q_full(w), 1); mbar_init(q_empty(w), 1); mbar_init(o_full(w), 1); mbar_init(o_done(w), 1);
+            for (int x = 0; x < 2; ++x) { mbar_init(s_full(w, x), 1); mbar_init(p_full(w, x), 4); }
             mbar_init(info_full(w), 1); mbar_init(info_empty(w), 9);
         }
         for (int s = 0; s < SLOTS; ++s) { mbar_init(kv_full(s), 1); mbar_init(kv_empty(s), 1); }
@@ -107,7 +111,6 @@ dense_fwd_tc5_kernel(const DenseArgs a, const DenseSplit sp, const __grid_consta
     auto wait = [&](uint32_t bar, uint32_t parity) { return (bool)__all_sync(0xffffffffu, mbar_wait(bar, parity, sp.wait_limit, abort_flag)); };
 
     if (warp == 8) {
-        give_registers();
         // ------------------------------------------------------------------------------------------------- copies
         bool ok = true;
         int slot = 0; uint32_t ph = 0, qc[2] = {0, 0};
@@ -177,107 +180,101 @@ dense_fwd_tc5_kernel(const DenseArgs a, const DenseSplit sp, const __grid_consta
             while (clock64() - start < 200000) {}
         }
     } else if (warp == 9) {
-        give_registers();
         // -------------------------------------------------------------------------------------------- matrix products
+        // Half tiles of 64 keys: S of half tile j + 2 follows the product that has consumed the weights of half tile j, whose
+        // columns it takes, so that the softmax always finds the next scores ready.
         bool ok = true;
-        int slot = 0; uint32_t ph = 0, qc[2] = {0, 0}, pc[2] = {0, 0};
-        auto next_slot = [&]() { if (++slot == SLOTS) { slot = 0; ph ^= 1; } };
-        auto issue_s = [&](int w, uint32_t k_addr, bool last) {
-            if (lane == 0) {
-                // a descriptor's start address counts in 16 bytes, and no sum of these leaves its field
-                const uint64_t qd = smem_desc(smem_addr(q_s + w * TILE), 16, 1024), kd = smem_desc(k_addr, 16, 1024);
-#pragma unroll
-                for (int k = 0; k < DP / 16; ++k) {
-                    constexpr uint32_t kStep = 32 >> 4;
-                    const uint32_t off = (k >> 2) * (PLANE >> 4) + (k & 3) * kStep;
-                    mma_f16(tmem + COL_S + w * 128, qd + off, kd + off, IDESC_S, k > 0);
-                }
-                if (last) mma_commit(q_empty(w));
-                mma_commit(s_full(w));
-            }
-            __syncwarp();
-        };
+        uint32_t qc[2] = {0, 0}, sn[2] = {0, 0}, pn[2] = {0, 0};       // per query tile: items, half tiles scored, half tiles summed
+        uint32_t ks_tile = 0, pv_tile = 0;                             // tiles so far on either side; tile m: ring places 2 m (K), 2 m + 1 (V)
         for (int k = 0; ok; ++k) {
             const int is = k & 1;
             if (!(ok = wait(info_full(is), (k >> 1) & 1))) break;
-            const int item = items.item[is];
+            const int item = uniform(items.item[is]);
             if (item < 0) break;
-            const FwdItem it(a, sp.splits, item);
-            auto next_tile = [&](int t) { while (t < it.kt1 && masked && items.flags[is][t - it.kt0] == 0) ++t; return t; };
-            int t = next_tile(it.kt0);
-            if (t < it.kt1) {
-                const int cur = slot;
-                const bool last = next_tile(t + 1) >= it.kt1;
-                if (!(ok = wait(kv_full(cur), ph))) break;
-                for (int w = 0; w < it.nw && ok; ++w) {
-                    if (!(ok = wait(q_full(w), qc[w] & 1))) break;
-                    ++qc[w];
-                    fence_after_sync();
-                    issue_s(w, smem_addr(ring + (size_t)cur * TILE), last);
+            FwdItem it(a, sp.splits, item);
+            it.n = uniform(it.n); it.kt0 = uniform(it.kt0); it.kt1 = uniform(it.kt1);
+            auto next_tile = [&](int t) {
+                if (masked) { while (t < it.kt1 && items.flags[is][t - it.kt0] == 0) ++t; t = uniform(t); }
+                return t;
+            };
+            auto halves = [&](int t) { return it.n - t * 128 > 64 ? 2 : 1; };
+            int ts = next_tile(it.kt0), hs = 0, tp = ts, hp = 0;        // next half tile to score, next to sum
+            bool fresh_q = true;
+            auto score = [&](int w) -> bool {                           // S of (ts, hs) for query tile w
+                const uint32_t place = 2 * ks_tile, slot = place % SLOTS;
+                if (w == 0 && hs == 0 && !wait(kv_full(slot), place / SLOTS & 1)) return false;
+                if (fresh_q && !wait(q_full(w), qc[w] & 1)) return false;
+                fence_after_sync();
+                const bool half_last = hs + 1 == halves(ts), last = half_last && next_tile(ts + 1) >= it.kt1;
+                if (elect_one()) {
+                    // a descriptor's start address counts in 16 bytes, and no sum of these leaves its field
+                    const uint64_t qd = smem_desc(smem_addr(q_s + w * TILE), 16, 1024),
+                                   kd = smem_desc(smem_addr(ring + slot * TILE) + hs * 8192, 16, 1024);
+                    const uint32_t d = tmem + COL_S + w * 128 + (sn[w] & 1) * 64;
+#pragma unroll
+                    for (int j = 0; j < DP / 16; ++j) {
+                        const uint32_t off = (j >> 2) * (PLANE >> 4) + (j & 3) * 2;
+                        mma_f16(d, qd + off, kd + off, IDESC_S, j > 0);
+                    }
+                    if (half_last && w == it.nw - 1) mma_commit(kv_empty(slot));
+                    if (last) mma_commit(q_empty(w));
+                    mma_commit(s_full(w, sn[w] & 1));
                 }
-                if (lane == 0) mma_commit(kv_empty(cur));
                 __syncwarp();
-                next_slot();
+                ++sn[w];
+                return true;
+            };
+            auto scored = [&]() {                                       // both query tiles have (ts, hs)
+                if (++hs == halves(ts)) { hs = 0; ts = next_tile(ts + 1); ++ks_tile; }
+            };
+            for (int ahead = 0; ahead < 2 && ok && ts < it.kt1; ++ahead) {
+                for (int w = 0; w < it.nw && ok; ++w) ok = score(w);
+                if (fresh_q) { ++qc[0]; if (it.nw == 2) ++qc[1]; }
+                fresh_q = false;
+                scored();
             }
             bool fresh = true;
-            while (t < it.kt1 && ok) {
-                const int tn = next_tile(t + 1);
-                const bool last = tn >= it.kt1 || next_tile(tn + 1) >= it.kt1;           // tn is the item's last tile
-                const int vs = slot;
-                if (!(ok = wait(kv_full(vs), ph))) break;
-                next_slot();
-                const uint32_t v_addr = smem_addr(ring + (size_t)vs * TILE);
-                if (it.n - t * 128 < 128 || masked)
-                    zero_hidden_rows<PLANES>(ring + (size_t)vs * TILE, it.n - t * 128,
-                                             masked ? a.mask.seen + it.plane * a.mask.wk + t * 4 : nullptr, lane);
-                const int ks = slot;
-                bool k_ready = false;
+            while (ok && tp < it.kt1) {
+                const uint32_t place = 2 * pv_tile + 1, slot = place % SLOTS;
+                if (hp == 0) {
+                    if (!(ok = wait(kv_full(slot), place / SLOTS & 1))) break;
+                    if (it.n - tp * 128 < 128 || masked)
+                        zero_hidden_rows<PLANES>(ring + slot * TILE, it.n - tp * 128,
+                                                 masked ? a.mask.seen + it.plane * a.mask.wk + tp * 4 : nullptr, lane);
+                }
+                const bool half_last = hp + 1 == halves(tp), more = ts < it.kt1, last = half_last && next_tile(tp + 1) >= it.kt1;
                 for (int w = 0; w < it.nw && ok; ++w) {
-                    if (!(ok = wait(p_full(w), pc[w] & 1))) break;
-                    ++pc[w];
+                    if (!(ok = wait(p_full(w, pn[w] & 1), pn[w] >> 1 & 1))) break;
                     fence_after_sync();
-                    if (lane == 0) {
-                        const uint64_t vd = smem_desc(v_addr, PLANE, 1024);
+                    if (elect_one()) {
+                        const uint64_t vd = smem_desc(smem_addr(ring + slot * TILE) + hp * 8192, PLANE, 1024);
+                        const uint32_t p = tmem + COL_S + w * 128 + (pn[w] & 1) * 64;
 #pragma unroll
-                        for (int j = 0; j < 8; ++j)
-                            mma_f16_ta(tmem + COL_O + w * DP, tmem + COL_S + w * 128 + j * 8, vd + j * (2048 >> 4), IDESC_O, (!fresh || j > 0) ? 1u : 0u);
-                        if (w == it.nw - 1) mma_commit(kv_empty(vs));       // before the barrier that lets the block end
+                        for (int j = 0; j < 4; ++j)
+                            mma_f16_ta(tmem + COL_O + w * DP, p + j * 8, vd + j * 128, IDESC_O, (!fresh || j > 0) ? 1u : 0u);
+                        if (half_last && w == it.nw - 1) mma_commit(kv_empty(slot));       // before the barrier that lets the block end
                         mma_commit(o_full(w));
+                        if (last) mma_commit(o_done(w));
                     }
                     __syncwarp();
-                    if (tn < it.kt1) {
-                        if (!k_ready) {
-                            if (!(ok = wait(kv_full(ks), ph))) break;
-                            fence_after_sync();
-                            k_ready = true;
-                        }
-                        if (w == it.nw - 1) {
-                            issue_s(w, smem_addr(ring + (size_t)ks * TILE), last);
-                            if (lane == 0) mma_commit(kv_empty(ks));
-                            __syncwarp();
-                        } else {
-                            issue_s(w, smem_addr(ring + (size_t)ks * TILE), last);
-                        }
-                    }
+                    ++pn[w];
+                    if (more) ok = score(w);
                 }
-                if (tn < it.kt1) next_slot();
+                if (ok && more) scored();
                 fresh = false;
-                t = tn;
+                if (half_last) { hp = 0; tp = next_tile(tp + 1); ++pv_tile; } else { hp = 1; }
             }
             if (ok && lane == 0) mbar_arrive(info_empty(is));
             __syncwarp();
         }
-    } else if (warp > 9) {
-        give_registers();
     } else {
-        take_registers();
         // -------------------------------------------------------------------------------------------------- softmax
         const int w = warp >> 2, quarter = warp & 3;
         const int row = quarter * 32 + lane;
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
         const uint32_t ts = tmem + COL_S + w * 128 + lanes, to = tmem + COL_O + w * DP + lanes;
         bool ok = true;
-        uint32_t sc = 0;                                     // tiles done so far
+        uint32_t sc = 0, oc = 0;                             // half tiles, and items with any, done so far
         int k = 0, item = -1;
         for (; ok; ++k) {
             const int is = k & 1;
@@ -291,7 +288,7 @@ dense_fwd_tc5_kernel(const DenseArgs a, const DenseSplit sp, const __grid_consta
                 const uint32_t *bits = masked ? a.mask.bits + (it.plane * a.mask.rows + (a.mask.rows > 1 ? min(qi, a.Lq - 1) : 0)) * a.mask.wk : nullptr;
                 float m = -INFINITY, l = 0.f;
                 bool any = false;
-                for (int t = it.kt0; t < it.kt1; ++t) {
+                for (int t = it.kt0; t < it.kt1 && ok; ++t) {
                     uint32_t flag = 2;
                     if (masked) {
                         flag = items.flags[is][t - it.kt0];
@@ -300,75 +297,80 @@ dense_fwd_tc5_kernel(const DenseArgs a, const DenseSplit sp, const __grid_consta
                     }
                     const int left = it.n - t * 128;
                     const bool partial = left < 128 || flag != 2;
-                    uint4 words = make_uint4(~0u, ~0u, ~0u, ~0u);
-                    if (partial && masked) words = __ldg(reinterpret_cast<const uint4 *>(bits + t * 4));
-                    if (!(ok = wait(s_full(w), sc & 1))) break;
-                    fence_after_sync();
-                    uint32_t r[4][32];
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) tmem_ld32(ts + 32 * c, r[c]);
-                    tmem_ld_wait();
+                    uint32_t words[4] = {~0u, ~0u, ~0u, ~0u};
                     if (partial) {
-                        const uint32_t wd[4] = {words.x, words.y, words.z, words.w};
-#pragma unroll
-                        for (int c = 0; c < 4; ++c) {
-                            const uint32_t keep = wd[c] & tail_word(left, c);
-#pragma unroll
-                            for (int j = 0; j < 32; ++j)
-                                if (!((keep >> j) & 1u)) r[c][j] = 0xff800000u;
+                        if (masked) {
+                            const uint4 m4 = __ldg(reinterpret_cast<const uint4 *>(bits + t * 4));
+                            words[0] = m4.x; words[1] = m4.y; words[2] = m4.z; words[3] = m4.w;
                         }
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) words[c] &= tail_word(left, c);
                     }
-                    float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                    for (int half = 0; half < (left > 64 ? 2 : 1); ++half) {
+                        const uint32_t x = sc & 1, tsx = ts + x * 64;
+                        if (!(ok = wait(s_full(w, x), sc >> 1 & 1))) break;
+                        fence_after_sync();
+                        uint32_t r[2][32];
+                        tmem_ld32(tsx, r[0]);
+                        tmem_ld32(tsx + 32, r[1]);
+                        tmem_ld_wait();
+                        if (partial) {
 #pragma unroll
-                    for (int c = 0; c < 4; ++c)
+                            for (int c = 0; c < 2; ++c) {
+                                const uint32_t keep = half == 0 ? words[c] : words[2 + c];
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) tops[c] = fmaxf(tops[c], __uint_as_float(r[c][j]));
-                    const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * a.scale_log2;
-                    const bool grow = top > m + 8.f;             // also the first finite maximum (m = -inf)
-                    if (__any_sync(0xffffffffu, grow)) {
-                        const float m_new = grow ? top : m;
-                        const float corr = grow ? fast_exp2(m - m_new) : 1.f;
-                        if (any) {
-                            if (!(ok = wait(o_full(w), (sc - 1) & 1))) break;
-                            fence_after_sync();
-#pragma unroll
-                            for (int c = 0; c < DP / 32; ++c) {
-                                uint32_t o[32];
-                                tmem_ld32(to + 32 * c, o);
-                                tmem_ld_wait();
-#pragma unroll
-                                for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * corr);
-                                tmem_st32(to + 32 * c, o);
+                                for (int j = 0; j < 32; ++j)
+                                    if (!((keep >> j) & 1u)) r[c][j] = 0xff800000u;
                             }
-                            l *= corr;
                         }
-                        m = m_new;
-                    }
-                    const float ref = m == -INFINITY ? 0.f : m;
-                    float sum[2] = {0.f, 0.f};
+                        float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) {
+                        for (int j = 0; j < 64; ++j) tops[j & 3] = fmaxf(tops[j & 3], __uint_as_float(r[j >> 5][j & 31]));
+                        const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * a.scale_log2;
+                        const bool grow = top > m + 8.f;             // also the first finite maximum (m = -inf)
+                        if (__any_sync(0xffffffffu, grow)) {
+                            const float m_new = grow ? top : m;
+                            const float corr = grow ? fast_exp2(m - m_new) : 1.f;
+                            if (any) {
+                                if (!(ok = wait(o_full(w), (sc - 1) & 1))) break;      // these scores follow the product before that one
+                                fence_after_sync();
+#pragma unroll
+                                for (int c = 0; c < DP / 32; ++c) {
+                                    uint32_t o[32];
+                                    tmem_ld32(to + 32 * c, o);
+                                    tmem_ld_wait();
+#pragma unroll
+                                    for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * corr);
+                                    tmem_st32(to + 32 * c, o);
+                                }
+                                l *= corr;
+                            }
+                            m = m_new;
+                        }
+                        const float ref = m == -INFINITY ? 0.f : m;
+                        const uint64_t c2 = pair(a.scale_log2, a.scale_log2), ref2 = pair(-ref, -ref);
+                        uint64_t sum[2] = {0, 0};                    // two pairs of zeros
                         uint32_t pk[32];
 #pragma unroll
                         for (int j = 0; j < 32; ++j) {
-                            const int e = 64 * c + 2 * j;
-                            const float p0 = fast_exp2(fmaf(__uint_as_float(r[e >> 5][e & 31]), a.scale_log2, -ref));
-                            const float p1 = fast_exp2(fmaf(__uint_as_float(r[(e + 1) >> 5][(e + 1) & 31]), a.scale_log2, -ref));
-                            sum[0] += p0; sum[1] += p1;
+                            const float2 e = unpair(fma2(pair_bits(r[j >> 4][(2 * j) & 31], r[j >> 4][(2 * j + 1) & 31]), c2, ref2));
+                            const float p0 = fast_exp2(e.x), p1 = fast_exp2(e.y);
+                            sum[j & 1] = add2(sum[j & 1], pair(p0, p1));
                             pk[j] = pack2<T>(p0, p1);
                         }
-                        tmem_st32(ts + 32 * c, pk);
+                        tmem_st32(tsx, pk);
+                        const float2 total = unpair(add2(sum[0], sum[1]));
+                        l += total.x + total.y;
+                        tmem_st_wait();
+                        fence_before_sync();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(p_full(w, x));
+                        ++sc;
+                        any = true;
                     }
-                    l += sum[0] + sum[1];
-                    tmem_st_wait();
-                    fence_before_sync();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(p_full(w));
-                    ++sc;
-                    any = true;
                 }
                 // ------------------------------------------------------------------------------------------ results
-                if (ok && any) ok = wait(o_full(w), (sc - 1) & 1);
+                if (ok && any) { ok = wait(o_done(w), oc & 1); ++oc; }
                 if (!ok) break;                                  // with k and item of the unfinished one
                 fence_after_sync();
                 const bool none = l == 0.f;
