@@ -9,8 +9,6 @@
 namespace hsa {
 
 constexpr int kFlagTiles = 768;                  // tiles whose mask state fits one of a block's two tables
-constexpr int kTcThreads = 320;                  // eight warps for the element-wise part, one for copies, one for products
-
 // Two 32-bit numbers in a register pair: one instruction for both
 __device__ __forceinline__ uint64_t pair(float lo, float hi) {
     uint64_t v;

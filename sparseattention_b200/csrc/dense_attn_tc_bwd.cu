@@ -11,8 +11,8 @@
 //          transposed (S^T = K Q^T), so that P^T and dS^T can stay in tensor memory, in place of the scores they came from, as
 //          the first operands of dv += P^T do and dk += dS^T q.  Two buffers of S^T and dP^T; with dv and dk all 512 columns are
 //          in use at DP = 128.
-// Eight element-wise warps (two per 32 rows, half of the columns each), one for copies, one for products.  While the element-wise
-// warps work on one buffer, the products fill the other.  (With a warpgroup per buffer instead of both on one, a warpgroup
+// Eight element-wise warps (two per 32 rows, half of the columns each), one for copies, two for products (scores, gradients).
+// While the element-wise warps work on one buffer, the products fill the other.  (With a warpgroup per buffer instead of both on one, a warpgroup
 // waited half its time for its own buffer: dk/dv took 738 us at 4096 x 4096, batch 2, 16 heads of 128, where this takes DKV_US;
 // dq with 128 columns in one buffer took 436 us where this takes DQ_US.)
 // Rounding: p and ds are rounded to the inputs' type once, as operands; all sums are 32-bit.
@@ -20,13 +20,15 @@
 
 namespace hsa {
 
+constexpr int kBwdThreads = 352;                 // eight element-wise warps, copies, score products, gradient products
+
 __device__ unsigned int g_dense_bwd_aborts = 0;
 
 // ------------------------------------------------------------------------------------------------------------------ dq
 template <int DP>
 struct DqShape {
     static constexpr int kTile = 128 * DP * 2, kKSlots = 3, kVSlots = 2;
-    static constexpr int kBars = 9 + 2 * (kKSlots + kVSlots) + kItemBars;
+    static constexpr int kBars = 11 + 2 * (kKSlots + kVSlots) + kItemBars;
     static constexpr int kSmem = 1024 + (2 + kKSlots + kVSlots) * kTile + (int)sizeof(ItemSlots) + kBars * 8 + 8;
     static_assert(kSmem <= 227 * 1024, "shared memory");
 };
@@ -46,7 +48,7 @@ struct DqItem {
 };
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(kTcThreads, 1)
+__global__ void __launch_bounds__(kBwdThreads, 1)
 dense_dq_tc5_kernel(const DenseArgs a, const long long wait_limit, const unsigned int extra_tx, const __grid_constant__ CUtensorMap map_q,
                     const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                     const __grid_constant__ CUtensorMap map_g) {
@@ -68,12 +70,13 @@ dense_dq_tc5_kernel(const DenseArgs a, const long long wait_limit, const unsigne
     const uint32_t qg_full = bar0, qg_empty = bar0 + 8, q_done = bar0 + 16, answer = bar0 + 24;
     auto s_full = [&](uint32_t x) { return bar0 + 8u * (5 + x); };
     auto d_full = [&](uint32_t x) { return bar0 + 8u * (7 + x); };
-    auto k_full = [&](int s) { return bar0 + 8u * (9 + s); };
-    auto k_empty = [&](int s) { return bar0 + 8u * (9 + KS + s); };
-    auto v_full = [&](int s) { return bar0 + 8u * (9 + 2 * KS + s); };
-    auto v_empty = [&](int s) { return bar0 + 8u * (9 + 2 * KS + VS + s); };
-    auto info_full = [&](int s) { return bar0 + 8u * (9 + 2 * KS + 2 * VS + s); };
-    auto info_empty = [&](int s) { return bar0 + 8u * (11 + 2 * KS + 2 * VS + s); };
+    auto s_free = [&](uint32_t x) { return bar0 + 8u * (9 + x); };
+    auto k_full = [&](int s) { return bar0 + 8u * (11 + s); };
+    auto k_empty = [&](int s) { return bar0 + 8u * (11 + KS + s); };
+    auto v_full = [&](int s) { return bar0 + 8u * (11 + 2 * KS + s); };
+    auto v_empty = [&](int s) { return bar0 + 8u * (11 + 2 * KS + VS + s); };
+    auto info_full = [&](int s) { return bar0 + 8u * (11 + 2 * KS + 2 * VS + s); };
+    auto info_empty = [&](int s) { return bar0 + 8u * (13 + 2 * KS + 2 * VS + s); };
 
     const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
     const bool masked = a.mask.bits != nullptr;
@@ -81,7 +84,7 @@ dense_dq_tc5_kernel(const DenseArgs a, const long long wait_limit, const unsigne
         mbar_init(qg_full, 1); mbar_init(qg_empty, 1); mbar_init(q_done, 1); mbar_init(answer, 1);
         for (int s = 0; s < KS; ++s) { mbar_init(k_full(s), 1); mbar_init(k_empty(s), 1); }
         for (int s = 0; s < VS; ++s) { mbar_init(v_full(s), 1); mbar_init(v_empty(s), 1); }
-        for (int x = 0; x < 2; ++x) { mbar_init(s_full(x), 1); mbar_init(d_full(x), 8); mbar_init(info_full(x), 1); mbar_init(info_empty(x), 9); }
+        for (int x = 0; x < 2; ++x) { mbar_init(s_full(x), 1); mbar_init(d_full(x), 8); mbar_init(s_free(x), 1); mbar_init(info_full(x), 1); mbar_init(info_empty(x), 10); }
         *abort_flag = 0;
         mbar_fence_init();
         prefetch_map(&map_q); prefetch_map(&map_k); prefetch_map(&map_v); prefetch_map(&map_g);
@@ -157,10 +160,11 @@ dense_dq_tc5_kernel(const DenseArgs a, const long long wait_limit, const unsigne
             while (clock64() - start < 200000) {}
         }
     } else if (warp == 9) {
-        // S and dP of half tile j + 1 are issued before dq takes half tile j; half tile j + 2 goes where j was, after it.
+        // S and dP: half tile j into buffer j & 1, once dq has taken half tile j - 2 from there
         bool ok = true;
-        int ks = 0, vs = 0, kd = 0; uint32_t kp = 0, vp = 0, qc = 0;
-        uint32_t issued = 0, done = 0;                       // half tiles whose scores, and whose dq, have been issued
+        int ks = 0, vs = 0; uint32_t kp = 0, vp = 0, qc = 0, i = 0;
+        const uint64_t q_desc = smem_desc(smem_addr(q_s), 16, 1024), g_desc = smem_desc(smem_addr(g_s), 16, 1024);
+        const uint64_t k_desc = smem_desc(smem_addr(k_s), 16, 1024), v_desc = smem_desc(smem_addr(v_s), 16, 1024);
         for (int k = 0; ok; ++k) {
             const int is = k & 1;
             if (!(ok = wait(info_full(is), (k >> 1) & 1))) break;
@@ -172,76 +176,85 @@ dense_dq_tc5_kernel(const DenseArgs a, const long long wait_limit, const unsigne
                 if (masked) { while (t < it.tiles && items.flags[is][t] == 0) ++t; t = uniform(t); }
                 return t;
             };
-            auto halves = [&](int t) { return it.n - t * 128 > 64 ? 2 : 1; };
-            int ts = next_tile(0), hs = 0, td = ts, hd = 0;  // next half tile to score, next to sum
-            // S and dP of (ts, hs); the K tile stays until dq has read it
-            auto scores = [&]() -> bool {
-                unsigned char *kt = k_s + ks * TILE;
-                if (hs == 0) {
-                    if (!wait(k_full(ks), kp)) return false;
-                    if (it.n - ts * 128 < 128 || masked)
-                        zero_hidden_rows<PLANES>(kt, it.n - ts * 128, masked ? a.mask.seen + it.plane * a.mask.wk + ts * 4 : nullptr, lane);
-                    if (!wait(v_full(vs), vp)) return false;
-                }
-                fence_after_sync();
-                const bool half_last = hs + 1 == halves(ts);
-                const int tn = half_last ? next_tile(ts + 1) : ts;
-                if (elect_one()) {
-                    const uint32_t d = tmem + (issued & 1) * 128;
-                    const uint64_t qd = smem_desc(smem_addr(q_s), 16, 1024), kdsc = smem_desc(smem_addr(kt) + hs * 8192, 16, 1024);
-                    const uint64_t gd = smem_desc(smem_addr(g_s), 16, 1024), vd = smem_desc(smem_addr(v_s + vs * TILE) + hs * 8192, 16, 1024);
+            int t = next_tile(0);
+            if (t < it.tiles) { ok = wait(qg_full, qc & 1); ++qc; }
+            while (ok && t < it.tiles) {
+                if (!(ok = wait(k_full(ks), kp))) break;
+                if (it.n - t * 128 < 128 || masked)
+                    zero_hidden_rows<PLANES>(k_s + ks * TILE, it.n - t * 128, masked ? a.mask.seen + it.plane * a.mask.wk + t * 4 : nullptr, lane);
+                if (!(ok = wait(v_full(vs), vp))) break;
+                const int halves = it.n - t * 128 > 64 ? 2 : 1, tn = next_tile(t + 1);
+                for (int half = 0; half < halves; ++half, ++i) {
+                    if (!(ok = wait(s_free(i & 1), (i >> 1 & 1) ^ 1))) break;
+                    fence_after_sync();
+                    if (elect_one()) {
+                        const uint32_t d = tmem + (i & 1) * 128;
+                        const uint64_t kd = k_desc + (ks * (TILE >> 4) + half * (8192 >> 4)), vd = v_desc + (vs * (TILE >> 4) + half * (8192 >> 4));
 #pragma unroll
-                    for (int j = 0; j < DP / 16; ++j) {
-                        const uint32_t off = (j >> 2) * (PLANE >> 4) + (j & 3) * 2;
-                        mma_f16(d, qd + off, kdsc + off, IDESC_S, j > 0);
-                    }
+                        for (int j = 0; j < DP / 16; ++j) {
+                            const uint32_t off = (j >> 2) * (PLANE >> 4) + (j & 3) * 2;
+                            mma_f16(d, q_desc + off, kd + off, IDESC_S, j > 0);
+                        }
 #pragma unroll
-                    for (int j = 0; j < DP / 16; ++j) {
-                        const uint32_t off = (j >> 2) * (PLANE >> 4) + (j & 3) * 2;
-                        mma_f16(d + 64, gd + off, vd + off, IDESC_S, j > 0);
+                        for (int j = 0; j < DP / 16; ++j) {
+                            const uint32_t off = (j >> 2) * (PLANE >> 4) + (j & 3) * 2;
+                            mma_f16(d + 64, g_desc + off, vd + off, IDESC_S, j > 0);
+                        }
+                        mma_commit(s_full(i & 1));
+                        if (half + 1 == halves) {
+                            mma_commit(v_empty(vs));
+                            if (tn >= it.tiles) mma_commit(qg_empty);
+                        }
                     }
-                    if (half_last) mma_commit(v_empty(vs));
-                    if (tn >= it.tiles) mma_commit(qg_empty);
-                    mma_commit(s_full(issued & 1));
+                    __syncwarp();
                 }
-                __syncwarp();
-                if (half_last) {
-                    if (++ks == KS) { ks = 0; kp ^= 1; }
-                    if (++vs == VS) { vs = 0; vp ^= 1; }
-                    hs = 0;
-                } else {
-                    hs = 1;
-                }
-                ts = tn;
-                ++issued;
-                return true;
+                if (++ks == KS) { ks = 0; kp ^= 1; }
+                if (++vs == VS) { vs = 0; vp ^= 1; }
+                t = tn;
+            }
+            if (ok && lane == 0) mbar_arrive(info_empty(is));
+            __syncwarp();
+        }
+    } else if (warp == 10) {
+        // dq += dS K
+        bool ok = true;
+        int ks = 0; uint32_t i = 0;
+        const uint64_t k_desc = smem_desc(smem_addr(k_s), PLANE, 1024);
+        for (int k = 0; ok; ++k) {
+            const int is = k & 1;
+            if (!(ok = wait(info_full(is), (k >> 1) & 1))) break;
+            const int item = uniform(items.item[is]);
+            if (item < 0) break;
+            DqItem it(a, item);
+            it.n = uniform(it.n); it.tiles = uniform(it.tiles);
+            auto next_tile = [&](int t) {
+                if (masked) { while (t < it.tiles && items.flags[is][t] == 0) ++t; t = uniform(t); }
+                return t;
             };
             bool fresh = true;
-            if (ts < it.tiles) {
-                ok = wait(qg_full, qc & 1) && scores();
-                ++qc;
-            }
-            while (ok && td < it.tiles) {
-                if (ts < it.tiles && !(ok = scores())) break;
-                if (!(ok = wait(d_full(done & 1), done >> 1 & 1))) break;
-                fence_after_sync();
-                const bool half_last = hd + 1 == halves(td);
-                const int tn = half_last ? next_tile(td + 1) : td;
-                if (elect_one()) {
-                    const uint64_t kdsc = smem_desc(smem_addr(k_s + kd * TILE) + hd * 8192, PLANE, 1024);
-                    const uint32_t d = tmem + (done & 1) * 128;
+            int t = next_tile(0);
+            while (ok && t < it.tiles) {
+                const int halves = it.n - t * 128 > 64 ? 2 : 1, tn = next_tile(t + 1);
+                for (int half = 0; half < halves; ++half, ++i) {
+                    if (!(ok = wait(d_full(i & 1), i >> 1 & 1))) break;
+                    fence_after_sync();
+                    if (elect_one()) {
+                        const uint64_t kd = k_desc + (ks * (TILE >> 4) + half * (8192 >> 4));
+                        const uint32_t d = tmem + (i & 1) * 128;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)              // either warpgroup's 32 keys lie where its scores were
-                        mma_f16_ta(tmem + COL_Q, d + (j >> 1) * 32 + (j & 1) * 8, kdsc + j * 128, IDESC_O, (!fresh || j > 0) ? 1u : 0u);
-                    if (half_last) mma_commit(k_empty(kd));
-                    if (tn >= it.tiles) mma_commit(q_done);
+                        for (int j = 0; j < 4; ++j)          // either warpgroup's 32 keys lie where its scores were
+                            mma_f16_ta(tmem + COL_Q, d + (j >> 1) * 32 + (j & 1) * 8, kd + j * 128, IDESC_O, (!fresh || j > 0) ? 1u : 0u);
+                        mma_commit(s_free(i & 1));
+                        if (half + 1 == halves) {
+                            mma_commit(k_empty(ks));
+                            if (tn >= it.tiles) mma_commit(q_done);      // last: the block may end after it
+                        }
+                    }
+                    __syncwarp();
+                    fresh = false;
                 }
-                __syncwarp();
-                if (half_last && ++kd == KS) kd = 0;
-                hd = half_last ? 0 : 1;
-                td = tn;
-                fresh = false;
-                ++done;
+                if (++ks == KS) ks = 0;
+                t = tn;
             }
             if (ok && lane == 0) mbar_arrive(info_empty(is));
             __syncwarp();
@@ -351,7 +364,7 @@ template <int DP>
 struct DkvShape {
     static constexpr int kTile = 128 * DP * 2, kHalf = 64 * DP * 2, kStages = 4;
     static constexpr int kStage = 2 * kHalf;                                      // a query tile and its output gradients
-    static constexpr int kBars = 9 + 2 * kStages + kItemBars;
+    static constexpr int kBars = 11 + 2 * kStages + kItemBars;
     static constexpr int kSmem = 1024 + 2 * kTile + kStages * (kStage + 512) + (int)sizeof(ItemSlots) + kBars * 8 + 8;
     static_assert(kSmem <= 227 * 1024, "shared memory");
 };
@@ -369,7 +382,7 @@ struct DkvItem {
 };
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(kTcThreads, 1)
+__global__ void __launch_bounds__(kBwdThreads, 1)
 dense_dkdv_tc5_kernel(const DenseArgs a, const long long wait_limit, const unsigned int extra_tx, const __grid_constant__ CUtensorMap map_q,
                       const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                       const __grid_constant__ CUtensorMap map_g) {
@@ -390,12 +403,13 @@ dense_dkdv_tc5_kernel(const DenseArgs a, const long long wait_limit, const unsig
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
     const uint32_t bar0 = smem_addr(bars);
     const uint32_t kv_full = bar0, kv_empty = bar0 + 8, done = bar0 + 16, answer = bar0 + 24;
-    auto s_full = [&](int x) { return bar0 + 8u * (5 + x); };
-    auto d_full = [&](int x) { return bar0 + 8u * (7 + x); };
-    auto full = [&](int s) { return bar0 + 8u * (9 + s); };
-    auto empty = [&](int s) { return bar0 + 8u * (9 + ST + s); };
-    auto info_full = [&](int s) { return bar0 + 8u * (9 + 2 * ST + s); };
-    auto info_empty = [&](int s) { return bar0 + 8u * (11 + 2 * ST + s); };
+    auto s_full = [&](uint32_t x) { return bar0 + 8u * (5 + x); };
+    auto d_full = [&](uint32_t x) { return bar0 + 8u * (7 + x); };
+    auto s_free = [&](uint32_t x) { return bar0 + 8u * (9 + x); };
+    auto full = [&](int s) { return bar0 + 8u * (11 + s); };
+    auto empty = [&](int s) { return bar0 + 8u * (11 + ST + s); };
+    auto info_full = [&](int s) { return bar0 + 8u * (11 + 2 * ST + s); };
+    auto info_empty = [&](int s) { return bar0 + 8u * (13 + 2 * ST + s); };
 
     const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
     const int qtiles = (a.Lq + 63) / 64;
@@ -404,7 +418,7 @@ dense_dkdv_tc5_kernel(const DenseArgs a, const long long wait_limit, const unsig
 
     if (threadIdx.x == 0) {
         mbar_init(kv_full, 1); mbar_init(kv_empty, 1); mbar_init(done, 1); mbar_init(answer, 1);
-        for (int x = 0; x < 2; ++x) { mbar_init(s_full(x), 1); mbar_init(d_full(x), 8); mbar_init(info_full(x), 1); mbar_init(info_empty(x), 9); }
+        for (int x = 0; x < 2; ++x) { mbar_init(s_full(x), 1); mbar_init(d_full(x), 8); mbar_init(s_free(x), 1); mbar_init(info_full(x), 1); mbar_init(info_empty(x), 10); }
         for (int s = 0; s < ST; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
         *abort_flag = 0;
         mbar_fence_init();
@@ -486,63 +500,80 @@ dense_dkdv_tc5_kernel(const DenseArgs a, const long long wait_limit, const unsig
             while (clock64() - start < 200000) {}
         }
     } else if (warp == 9) {
+        // S^T and dP^T: tile j into buffer j & 1, once the gradients have taken tile j - 2 from there
         bool ok = true;
-        int s = 0, sd = 0; uint32_t ph = 0, kc = 0;
-        uint32_t issued = 0, i = 0;                          // tiles whose scores, and whose products, have been issued
-        auto scores = [&](bool last) -> bool {                // S^T and dP^T of the next tile into buffer issued & 1
-            if (!wait(full(s), ph)) return false;
-            fence_after_sync();
-            if (elect_one()) {
-                const uint32_t qs = smem_addr(ring + s * Shape::kStage), col = tmem + (issued & 1) * 128;
-                const uint64_t kd = smem_desc(smem_addr(k_s), 16, 1024), vd = smem_desc(smem_addr(v_s), 16, 1024);
-                const uint64_t qd = smem_desc(qs, 16, 1024), gd = smem_desc(qs + HALF, 16, 1024);
-#pragma unroll
-                for (int j = 0; j < DP / 16; ++j)
-                    mma_f16(col, kd + (j >> 2) * (PLANE >> 4) + (j & 3) * 2, qd + (j >> 2) * (HPLANE >> 4) + (j & 3) * 2, IDESC_S, j > 0);
-#pragma unroll
-                for (int j = 0; j < DP / 16; ++j)
-                    mma_f16(col + 64, vd + (j >> 2) * (PLANE >> 4) + (j & 3) * 2, gd + (j >> 2) * (HPLANE >> 4) + (j & 3) * 2, IDESC_S, j > 0);
-                if (last) mma_commit(kv_empty);
-                mma_commit(s_full(issued & 1));
-            }
-            __syncwarp();
-            if (++s == ST) { s = 0; ph ^= 1; }
-            ++issued;
-            return true;
-        };
+        int s = 0; uint32_t ph = 0, kc = 0, i = 0;
+        const uint64_t k_desc = smem_desc(smem_addr(k_s), 16, 1024), v_desc = smem_desc(smem_addr(v_s), 16, 1024);
+        const uint64_t ring_desc = smem_desc(smem_addr(ring), 16, 1024);
         for (int k = 0; ok; ++k) {
             const int is = k & 1;
             if (!(ok = wait(info_full(is), (k >> 1) & 1))) break;
             const int item = uniform(items.item[is]);
             if (item < 0) break;
-            DkvItem it(a, item, qtiles);
-            it.total = uniform(it.total);
-            int u = next_unit(is, 0, it.total);
-            bool fresh = true;
-            if (u < it.total) {
-                ok = wait(kv_full, kc & 1) && scores(next_unit(is, u + 1, it.total) >= it.total);
-                ++kc;
-            }
-            while (ok && u < it.total) {
-                const int un = next_unit(is, u + 1, it.total);
-                if (un < it.total && !(ok = scores(next_unit(is, un + 1, it.total) >= it.total))) break;
-                if (!(ok = wait(d_full(i & 1), (i >> 1) & 1))) break;
+            const DkvItem it(a, item, qtiles);
+            const int total = uniform(it.total);
+            int u = next_unit(is, 0, total);
+            if (u < total) { ok = wait(kv_full, kc & 1); ++kc; }
+            while (ok && u < total) {
+                const int un = next_unit(is, u + 1, total);
+                if (!(ok = wait(full(s), ph) && wait(s_free(i & 1), (i >> 1 & 1) ^ 1))) break;
                 fence_after_sync();
                 if (elect_one()) {
-                    const uint32_t qs = smem_addr(ring + sd * Shape::kStage), col = tmem + (i & 1) * 128;
-                    const uint64_t qd = smem_desc(qs, HPLANE, 1024), gd = smem_desc(qs + HALF, HPLANE, 1024);
+                    const uint32_t col = tmem + (i & 1) * 128;
+                    const uint64_t qd = ring_desc + s * (Shape::kStage >> 4), gd = qd + (HALF >> 4);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) mma_f16_ta(tmem + COL_V, col + (j >> 1) * 32 + (j & 1) * 8, gd + j * 128, IDESC_O, (!fresh || j > 0) ? 1u : 0u);
+                    for (int j = 0; j < DP / 16; ++j)
+                        mma_f16(col, k_desc + (j >> 2) * (PLANE >> 4) + (j & 3) * 2, qd + (j >> 2) * (HPLANE >> 4) + (j & 3) * 2, IDESC_S, j > 0);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) mma_f16_ta(tmem + COL_K, col + 64 + (j >> 1) * 32 + (j & 1) * 8, qd + j * 128, IDESC_O, (!fresh || j > 0) ? 1u : 0u);
-                    mma_commit(empty(sd));
-                    if (un >= it.total) mma_commit(done);
+                    for (int j = 0; j < DP / 16; ++j)
+                        mma_f16(col + 64, v_desc + (j >> 2) * (PLANE >> 4) + (j & 3) * 2, gd + (j >> 2) * (HPLANE >> 4) + (j & 3) * 2, IDESC_S, j > 0);
+                    mma_commit(s_full(i & 1));
+                    if (un >= total) mma_commit(kv_empty);
                 }
                 __syncwarp();
-                if (++sd == ST) sd = 0;
+                if (++s == ST) { s = 0; ph ^= 1; }
+                ++i;
+                u = un;
+            }
+            if (ok && lane == 0) mbar_arrive(info_empty(is));
+            __syncwarp();
+        }
+    } else if (warp == 10) {
+        // dv += P^T do, dk += dS^T q
+        bool ok = true;
+        int s = 0; uint32_t i = 0;
+        const uint64_t ring_desc = smem_desc(smem_addr(ring), HPLANE, 1024);
+        for (int k = 0; ok; ++k) {
+            const int is = k & 1;
+            if (!(ok = wait(info_full(is), (k >> 1) & 1))) break;
+            const int item = uniform(items.item[is]);
+            if (item < 0) break;
+            const DkvItem it(a, item, qtiles);
+            const int total = uniform(it.total);
+            bool fresh = true;
+            int u = next_unit(is, 0, total);
+            while (ok && u < total) {
+                const int un = next_unit(is, u + 1, total);
+                if (!(ok = wait(d_full(i & 1), i >> 1 & 1))) break;
+                fence_after_sync();
+                if (elect_one()) {
+                    const uint32_t col = tmem + (i & 1) * 128;
+                    const uint64_t qd = ring_desc + s * (Shape::kStage >> 4), gd = qd + (HALF >> 4);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)              // either warpgroup's 32 queries lie where its scores were
+                        mma_f16_ta(tmem + COL_V, col + (j >> 1) * 32 + (j & 1) * 8, gd + j * 128, IDESC_O, (!fresh || j > 0) ? 1u : 0u);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        mma_f16_ta(tmem + COL_K, col + 64 + (j >> 1) * 32 + (j & 1) * 8, qd + j * 128, IDESC_O, (!fresh || j > 0) ? 1u : 0u);
+                    mma_commit(s_free(i & 1));
+                    mma_commit(empty(s));
+                    if (un >= total) mma_commit(done);       // last: the block may end after it
+                }
+                __syncwarp();
+                if (++s == ST) s = 0;
+                ++i;
                 fresh = false;
                 u = un;
-                ++i;
             }
             if (ok && lane == 0) mbar_arrive(info_empty(is));
             __syncwarp();
@@ -674,9 +705,9 @@ static int bwd_launch(const DenseArgs &a, cudaStream_t st) {
     cudaError_t e = cudaFuncSetAttribute(kdq, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_dq);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(kkv, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_kv);
     if (e != cudaSuccess) return fail((int)e, "hsa_dense_attn_bwd: shared memory %d / %d: %s", smem_dq, smem_kv, cudaGetErrorString(e));
-    kkv<<<(unsigned)kv_blocks, kTcThreads, smem_kv, st>>>(a, limit, extra, mq64, mk, mv, mg64);
+    kkv<<<(unsigned)kv_blocks, kBwdThreads, smem_kv, st>>>(a, limit, extra, mq64, mk, mv, mg64);
     if (int rc = launch_status("hsa_dense_attn_bwd(dk, dv)")) return rc;
-    kdq<<<(unsigned)dq_blocks, kTcThreads, smem_dq, st>>>(a, limit, extra, mq, mk, mv, mg);
+    kdq<<<(unsigned)dq_blocks, kBwdThreads, smem_dq, st>>>(a, limit, extra, mq, mk, mv, mg);
     return launch_status("hsa_dense_attn_bwd(dq)");
 }
 

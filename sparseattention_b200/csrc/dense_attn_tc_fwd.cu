@@ -3,9 +3,10 @@
 //   out_i = sum_j exp2(c s_ij - m_i) v_j / sum_j exp2(c s_ij - m_i),   s_ij = q_i.k_j,  c = scale log2(e)
 //
 // One pass over the keys with a running maximum and sum.  A work item is 256 query rows of one (batch entry, head), two tiles of
-// 128, against tiles of 128 keys in halves of 64; 10 warps with fixed roles:
+// 128, against tiles of 128 keys in halves of 64; 11 warps with fixed roles:
 //   warp 8     copies K and V tiles into a ring (TMA boxes of [128 rows][128 bytes], 128-byte swizzle)
-//   warp 9     issues S = Q K^T (both operands in shared memory) and O += P V (P in tensor memory, V as an MN-major operand)
+//   warps 9, 10  issue S = Q K^T (both operands in shared memory) and O += P V (P in tensor memory, V as an MN-major operand),
+//              each for one query tile
 //   warps 0-3  and 4-7: the softmax of the first and of the second query tile, a thread per row
 // Tensor memory (512 columns): two half tiles of S for either query tile (64 columns each), O of both (DP each).  P replaces the
 // S it came from as 16-bit numbers, so it never passes through shared memory, and the other half tile's scores are computed
@@ -22,6 +23,8 @@
 namespace hsa {
 
 __device__ unsigned int g_dense_aborts = 0;
+
+constexpr int kFwdThreads = 352;                 // softmax of two query tiles, copies, and a warp of products for either tile
 
 struct DenseSplit {
     float *part_o, *part_ml;                     // [splits, B, Lq, H, D] and [splits, B, Lq, H, 2] when splits > 1
@@ -58,7 +61,7 @@ struct FwdItem {
 };
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(kTcThreads, 1)
+__global__ void __launch_bounds__(kFwdThreads, 1)
 dense_fwd_tc5_kernel(const DenseArgs a, const DenseSplit sp, const __grid_constant__ CUtensorMap map_q,
                      const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
     using namespace tc5;
@@ -94,9 +97,9 @@ dense_fwd_tc5_kernel(const DenseArgs a, const DenseSplit sp, const __grid_consta
         for (int w = 0; w < 2; ++w) {
             mbar_init(q_full(w), 1); mbar_init(q_empty(w), 1); mbar_init(o_full(w), 1); mbar_init(o_done(w), 1);
             for (int x = 0; x < 2; ++x) { mbar_init(s_full(w, x), 1); mbar_init(p_full(w, x), 4); }
-            mbar_init(info_full(w), 1); mbar_init(info_empty(w), 9);
+            mbar_init(info_full(w), 1); mbar_init(info_empty(w), 10);
         }
-        for (int s = 0; s < SLOTS; ++s) { mbar_init(kv_full(s), 1); mbar_init(kv_empty(s), 1); }
+        for (int s = 0; s < SLOTS; ++s) { mbar_init(kv_full(s), 1); mbar_init(kv_empty(s), 2); }
         mbar_init(answer, 1);
         *abort_flag = 0;
         mbar_fence_init();
@@ -179,13 +182,19 @@ dense_fwd_tc5_kernel(const DenseArgs a, const DenseSplit sp, const __grid_consta
             const long long start = clock64();
             while (clock64() - start < 200000) {}
         }
-    } else if (warp == 9) {
+    } else if (warp >= 9) {
         // -------------------------------------------------------------------------------------------- matrix products
         // Half tiles of 64 keys: S of half tile j + 2 follows the product that has consumed the weights of half tile j, whose
-        // columns it takes, so that the softmax always finds the next scores ready.
+        // columns it takes, so that the softmax always finds the next scores ready.  One warp for either query tile: with one
+        // for both, issuing took as long as the products.
+        const int w = warp - 9;
         bool ok = true;
-        uint32_t qc[2] = {0, 0}, sn[2] = {0, 0}, pn[2] = {0, 0};       // per query tile: items, half tiles scored, half tiles summed
+        uint32_t qc = 0, sn = 0, pn = 0;                               // items, half tiles scored, half tiles summed
         uint32_t ks_tile = 0, pv_tile = 0;                             // tiles so far on either side; tile m: ring places 2 m (K), 2 m + 1 (V)
+        const uint64_t q_desc = smem_desc(smem_addr(q_s + w * TILE), 16, 1024);
+        // a descriptor's start address counts in 16 bytes, and no sum of these leaves its field
+        const uint64_t k_desc = smem_desc(smem_addr(ring), 16, 1024), v_desc = smem_desc(smem_addr(ring), PLANE, 1024);
+        const uint32_t s_col = tmem + COL_S + w * 128, o_col = tmem + COL_O + w * DP;
         for (int k = 0; ok; ++k) {
             const int is = k & 1;
             if (!(ok = wait(info_full(is), (k >> 1) & 1))) break;
@@ -199,70 +208,76 @@ dense_fwd_tc5_kernel(const DenseArgs a, const DenseSplit sp, const __grid_consta
             };
             auto halves = [&](int t) { return it.n - t * 128 > 64 ? 2 : 1; };
             int ts = next_tile(it.kt0), hs = 0, tp = ts, hp = 0;        // next half tile to score, next to sum
-            bool fresh_q = true;
-            auto score = [&](int w) -> bool {                           // S of (ts, hs) for query tile w
+            if (w >= it.nw) {                                           // no such query tile: let the key tiles go
+                for (; tp < it.kt1 && ok; tp = next_tile(tp + 1), ++ks_tile, ++pv_tile)
+                    for (uint32_t place = 2 * pv_tile; place < 2 * pv_tile + 2 && ok; ++place) {
+                        ok = wait(kv_full(place % SLOTS), place / SLOTS & 1);
+                        if (ok && lane == 0) mbar_arrive(kv_empty(place % SLOTS));
+                        __syncwarp();
+                    }
+                if (ok && lane == 0) mbar_arrive(info_empty(is));
+                __syncwarp();
+                continue;
+            }
+            auto score = [&]() -> bool {                                // S of (ts, hs)
                 const uint32_t place = 2 * ks_tile, slot = place % SLOTS;
-                if (w == 0 && hs == 0 && !wait(kv_full(slot), place / SLOTS & 1)) return false;
-                if (fresh_q && !wait(q_full(w), qc[w] & 1)) return false;
+                if (hs == 0 && !wait(kv_full(slot), place / SLOTS & 1)) return false;
                 fence_after_sync();
-                const bool half_last = hs + 1 == halves(ts), last = half_last && next_tile(ts + 1) >= it.kt1;
+                const bool half_last = hs + 1 == halves(ts);
+                const int tn = half_last ? next_tile(ts + 1) : ts;
                 if (elect_one()) {
-                    // a descriptor's start address counts in 16 bytes, and no sum of these leaves its field
-                    const uint64_t qd = smem_desc(smem_addr(q_s + w * TILE), 16, 1024),
-                                   kd = smem_desc(smem_addr(ring + slot * TILE) + hs * 8192, 16, 1024);
-                    const uint32_t d = tmem + COL_S + w * 128 + (sn[w] & 1) * 64;
+                    const uint64_t kd = k_desc + (slot * (TILE >> 4) + hs * (8192 >> 4));
+                    const uint32_t d = s_col + (sn & 1) * 64;
 #pragma unroll
                     for (int j = 0; j < DP / 16; ++j) {
                         const uint32_t off = (j >> 2) * (PLANE >> 4) + (j & 3) * 2;
-                        mma_f16(d, qd + off, kd + off, IDESC_S, j > 0);
+                        mma_f16(d, q_desc + off, kd + off, IDESC_S, j > 0);
                     }
-                    if (half_last && w == it.nw - 1) mma_commit(kv_empty(slot));
-                    if (last) mma_commit(q_empty(w));
-                    mma_commit(s_full(w, sn[w] & 1));
+                    mma_commit(s_full(w, sn & 1));
+                    if (half_last) mma_commit(kv_empty(slot));
+                    if (tn >= it.kt1) mma_commit(q_empty(w));
                 }
                 __syncwarp();
-                ++sn[w];
+                ++sn;
+                if (half_last) ++ks_tile;
+                hs = half_last ? 0 : 1;
+                ts = tn;
                 return true;
             };
-            auto scored = [&]() {                                       // both query tiles have (ts, hs)
-                if (++hs == halves(ts)) { hs = 0; ts = next_tile(ts + 1); ++ks_tile; }
-            };
-            for (int ahead = 0; ahead < 2 && ok && ts < it.kt1; ++ahead) {
-                for (int w = 0; w < it.nw && ok; ++w) ok = score(w);
-                if (fresh_q) { ++qc[0]; if (it.nw == 2) ++qc[1]; }
-                fresh_q = false;
-                scored();
+            if (ts < it.kt1) {
+                ok = wait(q_full(w), qc & 1) && score();
+                ++qc;
+                if (ok && ts < it.kt1) ok = score();
             }
             bool fresh = true;
             while (ok && tp < it.kt1) {
                 const uint32_t place = 2 * pv_tile + 1, slot = place % SLOTS;
                 if (hp == 0) {
                     if (!(ok = wait(kv_full(slot), place / SLOTS & 1))) break;
-                    if (it.n - tp * 128 < 128 || masked)
+                    if (it.n - tp * 128 < 128 || masked)             // (both warps write the same zeros)
                         zero_hidden_rows<PLANES>(ring + slot * TILE, it.n - tp * 128,
                                                  masked ? a.mask.seen + it.plane * a.mask.wk + tp * 4 : nullptr, lane);
                 }
-                const bool half_last = hp + 1 == halves(tp), more = ts < it.kt1, last = half_last && next_tile(tp + 1) >= it.kt1;
-                for (int w = 0; w < it.nw && ok; ++w) {
-                    if (!(ok = wait(p_full(w, pn[w] & 1), pn[w] >> 1 & 1))) break;
-                    fence_after_sync();
-                    if (elect_one()) {
-                        const uint64_t vd = smem_desc(smem_addr(ring + slot * TILE) + hp * 8192, PLANE, 1024);
-                        const uint32_t p = tmem + COL_S + w * 128 + (pn[w] & 1) * 64;
+                const bool half_last = hp + 1 == halves(tp);
+                const int tn = half_last ? next_tile(tp + 1) : tp;
+                if (!(ok = wait(p_full(w, pn & 1), pn >> 1 & 1))) break;
+                fence_after_sync();
+                if (elect_one()) {
+                    const uint64_t vd = v_desc + (slot * (TILE >> 4) + hp * (8192 >> 4));
+                    const uint32_t p = s_col + (pn & 1) * 64;
 #pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            mma_f16_ta(tmem + COL_O + w * DP, p + j * 8, vd + j * 128, IDESC_O, (!fresh || j > 0) ? 1u : 0u);
-                        if (half_last && w == it.nw - 1) mma_commit(kv_empty(slot));       // before the barrier that lets the block end
-                        mma_commit(o_full(w));
-                        if (last) mma_commit(o_done(w));
-                    }
-                    __syncwarp();
-                    ++pn[w];
-                    if (more) ok = score(w);
+                    for (int j = 0; j < 4; ++j) mma_f16_ta(o_col, p + j * 8, vd + j * 128, IDESC_O, (!fresh || j > 0) ? 1u : 0u);
+                    mma_commit(o_full(w));
+                    if (half_last) mma_commit(kv_empty(slot));
+                    if (tn >= it.kt1) mma_commit(o_done(w));         // last: the block may end after it
                 }
-                if (ok && more) scored();
+                __syncwarp();
+                ++pn;
+                if (ts < it.kt1) ok = score();
                 fresh = false;
-                if (half_last) { hp = 0; tp = next_tile(tp + 1); ++pv_tile; } else { hp = 1; }
+                if (half_last) ++pv_tile;
+                hp = half_last ? 0 : 1;
+                tp = tn;
             }
             if (ok && lane == 0) mbar_arrive(info_empty(is));
             __syncwarp();
@@ -516,7 +531,7 @@ static int fwd_launch(const DenseArgs &a, DenseSplit sp, cudaStream_t st) {
     constexpr int smem = FwdShape<DP>::kSmem;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return fail((int)e, "hsa_dense_attn_fwd: shared memory %d: %s", smem, cudaGetErrorString(e));
-    kernel<<<(unsigned)blocks, kTcThreads, smem, st>>>(a, sp, mq, mk, mv);
+    kernel<<<(unsigned)blocks, kFwdThreads, smem, st>>>(a, sp, mq, mk, mv);
     if (int rc = launch_status("hsa_dense_attn_fwd")) return rc;
     if (sp.splits == 1) return 0;
     const long long rows = (long long)a.B * a.Lq * a.H;
