@@ -4,6 +4,8 @@
 
 #include <math.h>
 
+#include <atomic>
+
 #include "hsa_common.cuh"
 
 namespace hsa {
@@ -74,6 +76,20 @@ struct DenseArgs {
     float empty_value;                   // what the output row of a query without keys holds
     bool vec;                            // rows may be read four elements at a time
 };
+
+// Raise a kernel's shared-memory limit, once per device
+template <auto Kernel>
+cudaError_t allow_smem(int bytes) {
+    static std::atomic<unsigned long long> done{0};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const unsigned long long bit = 1ull << (dev & 63);
+    if (dev < 64 && (done.load(std::memory_order_acquire) & bit)) return cudaSuccess;
+    e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess && dev < 64) done.fetch_or(bit, std::memory_order_release);
+    return e;
+}
 
 // Strides of dimensions of one entry as a packed tensor would have them (nothing is addressed through them)
 inline hsa_view dense_view(hsa_view v, int B, int rows, int H, int D) {

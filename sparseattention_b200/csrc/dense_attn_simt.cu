@@ -364,15 +364,15 @@ static int simt_launch(const DenseArgs &a, int what, cudaStream_t st) {
     const size_t smem = what == 0 ? 3 * rows + weights : what == 1 ? 4 * rows + weights : 4 * rows + 2 * weights;
     const long long blocks = what == 2 ? (long long)a.B * a.Hkv * ((a.Lk + BT - 1) / BT) : (long long)a.B * a.H * ((a.Lq + BT - 1) / BT);
     if (blocks > 0x7fffffffLL) return fail(HSA_ERR_ARG, "hsa_dense_attn: too many tiles");
-    auto go = [&](auto kernel) -> int {
-        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    auto go = [&]<auto kernel>() -> int {
+        const cudaError_t e = allow_smem<kernel>((int)smem);
         if (e != cudaSuccess) return fail((int)e, "hsa_dense_attn: shared memory %zu: %s", smem, cudaGetErrorString(e));
         kernel<<<(unsigned)blocks, kSimtThreads, smem, st>>>(a);
         return launch_status("hsa_dense_attn");
     };
-    if (what == 0) return go(dense_fwd_simt_kernel<T, DP, BT>);
-    if (what == 1) return go(dense_dq_simt_kernel<T, DP, BT>);
-    return go(dense_dkdv_simt_kernel<T, DP, BT>);
+    if (what == 0) return go.template operator()<dense_fwd_simt_kernel<T, DP, BT>>();
+    if (what == 1) return go.template operator()<dense_dq_simt_kernel<T, DP, BT>>();
+    return go.template operator()<dense_dkdv_simt_kernel<T, DP, BT>>();
 }
 
 // Tiles of 64 x 64 up to 128 head dims (70 to 170 KB of shared memory); 32 x 32 above, where 64 would not fit.

@@ -116,9 +116,21 @@ dense_dq_tc5_kernel(const DenseArgs a, const long long wait_limit, const unsigne
             __syncwarp();
             if (lane == 0) mbar_arrive(info_full(is));
             if (item < 0) break;
+            // The next item is asked for when this one's last copies are due: an item taken over earlier would wait here while
+            // other SMs run dry.
+            bool asked = false;
+            auto ask = [&]() {
+                if (!asked && lane == 0) {
+                    mbar_expect_tx(answer, 16);
+                    take_over(smem_addr(&items.answer), answer);
+                }
+                asked = true;
+                __syncwarp();
+            };
             const DqItem it(a, item);
             bool first = true;
             for (int t = 0; t < it.tiles && ok; ++t) {
+                if (t + 2 >= it.tiles) ask();
                 if (masked && items.flags[is][t] == 0) continue;
                 if (!(ok = wait(k_empty(ks), kp ^ 1))) break;
                 if (lane == 0) {
@@ -147,11 +159,7 @@ dense_dq_tc5_kernel(const DenseArgs a, const long long wait_limit, const unsigne
                 if (++vs == VS) { vs = 0; vp ^= 1; }
             }
             if (!ok) break;
-            if (lane == 0) {                             // not earlier: an item that is taken over early waits here while other SMs run dry
-                mbar_expect_tx(answer, 16);
-                take_over(smem_addr(&items.answer), answer);
-            }
-            __syncwarp();
+            ask();
             if (!(ok = wait(answer, k & 1))) break;
             item = taken_over(smem_addr(&items.answer));
         }
@@ -454,6 +462,17 @@ dense_dkdv_tc5_kernel(const DenseArgs a, const long long wait_limit, const unsig
             __syncwarp();
             if (lane == 0) mbar_arrive(info_full(is));
             if (item < 0) break;
+            // The next item is asked for when this one's last copies are due: an item taken over earlier would wait here while
+            // other SMs run dry.
+            bool asked = false;
+            auto ask = [&]() {
+                if (!asked && lane == 0) {
+                    mbar_expect_tx(answer, 16);
+                    take_over(smem_addr(&items.answer), answer);
+                }
+                asked = true;
+                __syncwarp();
+            };
             const DkvItem it(a, item, qtiles);
             int u = next_unit(is, 0, it.total);
             if (u < it.total) {
@@ -471,6 +490,7 @@ dense_dkdv_tc5_kernel(const DenseArgs a, const long long wait_limit, const unsig
             }
             for (; u < it.total; u = next_unit(is, u + 1, it.total)) {
                 const int h = it.hk * a.group + u / qtiles, q0 = u % qtiles * 64;
+                if (u + 4 >= it.total) ask();
                 if (!(ok = wait(empty(s), ph ^ 1))) break;
                 if (lane == 0) {
                     mbar_expect_tx(full(s), 2 * HALF + 512);
@@ -487,11 +507,7 @@ dense_dkdv_tc5_kernel(const DenseArgs a, const long long wait_limit, const unsig
                 if (++s == ST) { s = 0; ph ^= 1; }
             }
             if (!ok) break;
-            if (lane == 0) {                             // not earlier: an item that is taken over early waits here while other SMs run dry
-                mbar_expect_tx(answer, 16);
-                take_over(smem_addr(&items.answer), answer);
-            }
-            __syncwarp();
+            ask();
             if (!(ok = wait(answer, k & 1))) break;
             item = taken_over(smem_addr(&items.answer));
         }
@@ -699,11 +715,11 @@ static int bwd_launch(const DenseArgs &a, cudaStream_t st) {
     if (dq_blocks > 0x7fffffffLL || kv_blocks > 0x7fffffffLL) return fail(HSA_ERR_ARG, "hsa_dense_attn_bwd: too many tiles");
     const long long limit = wait_limit_cycles();
     const unsigned int extra = wait_extra_tx();
-    auto kdq = dense_dq_tc5_kernel<T, DP>;
-    auto kkv = dense_dkdv_tc5_kernel<T, DP>;
+    constexpr auto kdq = dense_dq_tc5_kernel<T, DP>;
+    constexpr auto kkv = dense_dkdv_tc5_kernel<T, DP>;
     constexpr int smem_dq = DqShape<DP>::kSmem, smem_kv = DkvShape<DP>::kSmem;
-    cudaError_t e = cudaFuncSetAttribute(kdq, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_dq);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(kkv, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_kv);
+    cudaError_t e = allow_smem<kdq>(smem_dq);
+    if (e == cudaSuccess) e = allow_smem<kkv>(smem_kv);
     if (e != cudaSuccess) return fail((int)e, "hsa_dense_attn_bwd: shared memory %d / %d: %s", smem_dq, smem_kv, cudaGetErrorString(e));
     kkv<<<(unsigned)kv_blocks, kBwdThreads, smem_kv, st>>>(a, limit, extra, mq64, mk, mv, mg64);
     if (int rc = launch_status("hsa_dense_attn_bwd(dk, dv)")) return rc;

@@ -148,9 +148,21 @@ dense_fwd_tc5_kernel(const DenseArgs a, const DenseSplit sp, const __grid_consta
             __syncwarp();
             if (lane == 0) mbar_arrive(info_full(is));
             if (item < 0) break;
+            // The next item is asked for when this one's last copies are due: an item taken over earlier would wait here while
+            // other SMs run dry.
+            bool asked = false;
+            auto ask = [&]() {
+                if (!asked && lane == 0) {
+                    mbar_expect_tx(answer, 16);
+                    take_over(smem_addr(&items.answer), answer);
+                }
+                asked = true;
+                __syncwarp();
+            };
             const FwdItem it(a, sp.splits, item);
             bool first = true;
             for (int t = it.kt0; t < it.kt1 && ok; ++t) {
+                if (t + 2 >= it.kt1) ask();
                 if (masked && items.flags[is][t - it.kt0] == 0) continue;
                 push(&map_k, it.hk, t * 128, it.b);
                 if (first) {
@@ -170,11 +182,7 @@ dense_fwd_tc5_kernel(const DenseArgs a, const DenseSplit sp, const __grid_consta
                 if (ok) push(&map_v, it.hk, t * 128, it.b);
             }
             if (!ok) break;
-            if (lane == 0) {                             // not earlier: an item that is taken over early waits here while other SMs run dry
-                mbar_expect_tx(answer, 16);
-                take_over(smem_addr(&items.answer), answer);
-            }
-            __syncwarp();
+            ask();
             if (!(ok = wait(answer, k & 1))) break;
             item = taken_over(smem_addr(&items.answer));
         }
@@ -535,9 +543,9 @@ static int fwd_launch(const DenseArgs &a, DenseSplit sp, cudaStream_t st) {
         return fail(HSA_ERR_ARG, "hsa_dense_attn_fwd: the driver refused a tensor map");
     const long long blocks = (long long)a.B * a.H * ((a.Lq + 255) / 256) * sp.splits;
     if (blocks > 0x7fffffffLL) return fail(HSA_ERR_ARG, "hsa_dense_attn_fwd: too many tiles");
-    auto kernel = dense_fwd_tc5_kernel<T, DP>;
+    constexpr auto kernel = dense_fwd_tc5_kernel<T, DP>;
     constexpr int smem = FwdShape<DP>::kSmem;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    const cudaError_t e = allow_smem<kernel>(smem);
     if (e != cudaSuccess) return fail((int)e, "hsa_dense_attn_fwd: shared memory %d: %s", smem, cudaGetErrorString(e));
     kernel<<<(unsigned)blocks, kFwdThreads, smem, st>>>(a, sp, mq, mk, mv);
     if (int rc = launch_status("hsa_dense_attn_fwd")) return rc;

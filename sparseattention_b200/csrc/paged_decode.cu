@@ -423,15 +423,17 @@ template <typename T>
 static int paged_mma(const PagedArgs &a, cudaStream_t st) {
     const long long blocks = (long long)a.B * a.Hkv * ((a.group + 15) / 16) * a.splits;
     if (blocks > 0x7fffffffLL) return fail(HSA_ERR_ARG, "hsa_paged_attn_decode: too many blocks");
-    auto go = [&](auto kernel, int smem) -> int {
-        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    auto go = [&]<int DP>() -> int {
+        constexpr auto kernel = paged_decode_mma_kernel<T, DP>;
+        constexpr int smem = PagedShape<DP>::kSmem;
+        const cudaError_t e = allow_smem<kernel>(smem);
         if (e != cudaSuccess) return fail((int)e, "hsa_paged_attn_decode: shared memory %d: %s", smem, cudaGetErrorString(e));
         kernel<<<(unsigned)blocks, kPagedWarps * 32, smem, st>>>(a);
         return launch_status("hsa_paged_attn_decode");
     };
-    if (a.D <= 64) return go(paged_decode_mma_kernel<T, 64>, PagedShape<64>::kSmem);
-    if (a.D <= 128) return go(paged_decode_mma_kernel<T, 128>, PagedShape<128>::kSmem);
-    return go(paged_decode_mma_kernel<T, 256>, PagedShape<256>::kSmem);
+    if (a.D <= 64) return go.template operator()<64>();
+    if (a.D <= 128) return go.template operator()<128>();
+    return go.template operator()<256>();
 }
 
 template <typename T>

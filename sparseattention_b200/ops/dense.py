@@ -13,7 +13,6 @@ from ctypes import c_void_p
 from typing import NamedTuple, Optional, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import _lib
 
@@ -164,25 +163,47 @@ def dense_attention_backward(q, k, v, out, lse, dout, key_lengths=None, packed_m
     return dq, dk, dv
 
 
+class _Once(torch.autograd.Function):
+    """Gradients as they are; differentiating them again is refused."""
+
+    @staticmethod
+    def forward(ctx, *grads):
+        return tuple(t.view_as(t) for t in grads)
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError("cross_attention is differentiable once")
+
+
+def _once(grads):
+    # gradient mode is on inside a backward only when its result is to be differentiated (create_graph)
+    if not torch.is_grad_enabled():
+        return grads
+    return _Once.apply(*(t.requires_grad_(True) for t in grads))
+
+
 class _CrossAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, key_lengths, packed_mask, scale, empty_value, algo):
         q, k, v = _rows(q), _rows(k), _rows(v)
         out, lse = dense_attention_forward(q, k, v, key_lengths, packed_mask, scale, empty_value, True, algo)
-        ctx.save_for_backward(q, k, v, out, lse, key_lengths, None if packed_mask is None else packed_mask.data)
-        ctx.meta = (None if packed_mask is None else packed_mask.sizes, scale, algo)
+        if packed_mask is None:
+            ctx.save_for_backward(q, k, v, out, lse, key_lengths)
+            ctx.meta = (None, scale, algo)
+        else:
+            ctx.save_for_backward(q, k, v, out, lse, key_lengths, packed_mask.data)
+            ctx.meta = (packed_mask.sizes, scale, algo)
         return out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dout):
-        q, k, v, out, lse, key_lengths, packed = ctx.saved_tensors
+        q, k, v, out, lse, key_lengths, *packed = ctx.saved_tensors
         sizes, scale, algo = ctx.meta
         with _lib.on_device(q.device):
             dout = _rows(dout if dout.dtype == q.dtype else dout.to(q.dtype))
-            grads = dense_attention_backward(q, k, v, out, lse, dout, key_lengths, None if packed is None else _Packed(packed, sizes),
+            grads = dense_attention_backward(q, k, v, out, lse, dout, key_lengths, _Packed(packed[0], sizes) if packed else None,
                                              scale, algo)
-        return (*grads, None, None, None, None, None)
+        return (*_once(grads), None, None, None, None, None)
 
 
 class _NoRows(torch.autograd.Function):
@@ -194,9 +215,8 @@ class _NoRows(torch.autograd.Function):
         return torch.full(q.shape, empty_value, dtype=q.dtype, device=q.device)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dout):
-        return (*(torch.zeros_like(t) for t in ctx.saved_tensors), None)
+        return (*_once(tuple(torch.zeros_like(t) for t in ctx.saved_tensors)), None)
 
 
 def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, key_lengths: Optional[torch.Tensor] = None,
