@@ -6,8 +6,8 @@ Same public surface as the reference project's `hierarchical_attention` package
 __version__ = "0.1.0"
 
 from .modules import HierarchicalAttention
-from .ops import (build_hierarchical_logits, build_parent_nodes, build_tree_topology, generate_span_input_Y,
-                  hierarchical_attention)
+from .ops import (build_hierarchical_logits, build_parent_nodes, build_tree_topology, cross_attention,
+                  generate_span_input_Y, hierarchical_attention, paged_attention_decode)
 
 __all__ = [
     "HierarchicalAttention",
@@ -16,5 +16,7 @@ __all__ = [
     "build_parent_nodes",
     "hierarchical_attention",
     "build_hierarchical_logits",       # the logits op of the reference's first prototype (Hierarchical_Attention_Triton.py:456)
+    "cross_attention",                 # dense attention over another sequence's rows
+    "paged_attention_decode",          # one new token over a key/value cache in pages
     "__version__",
 ]

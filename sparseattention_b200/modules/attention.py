@@ -19,6 +19,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from ..ops.dense import cross_attention
 from ..ops.functional import build_parent_nodes, hierarchical_attention
 from ..ops.topology import build_tree_topology, generate_span_input_Y  # noqa: F401  (re-exported like the reference)
 
@@ -43,6 +44,10 @@ class HierarchicalAttention(nn.Module):
         hierarchical mode when `y` is given and the three lengths agree: leaves attend to a
         radius-`window_size` window plus one sibling node per level of the parents `y`;
         `mask is not None` selects the causal variant (its content is not read).
+        Otherwise (no parents, or key rows of another length: an encoder's states, a memory) plain multi-head
+        attention of `query` over `key` / `value`; `mask == 0` hides an entry.  On CUDA in bfloat16 or float16, with no
+        dropout active and no weights asked for, that runs as one kernel (ops.dense.cross_attention) without the
+        [B, H, L_Q, L_K] matrix; set `fused_attention = False` for the eager operations (differentiable twice).
     cross_update_Y(x, y_in)  bottom-up refresh of the parents from x.
     update_X_from_Y(x, y, mask=None)  the top-down pass used by forward.
     """
@@ -61,6 +66,7 @@ class HierarchicalAttention(nn.Module):
             setattr(self, name, nn.Linear(dim, dim, bias=False))
         self.out_proj_x = nn.Linear(dim, dim)
         self.dropout = nn.Dropout(dropout)
+        self.fused_attention = True
 
         self.cached_tables = None
         self.cached_seq_len = -1
@@ -138,6 +144,23 @@ class HierarchicalAttention(nn.Module):
         attn = self.dropout(scores.softmax(dim=-1))
         return attn @ V, attn
 
+    def _dense_mask(self, q, k, v, mask):
+        """(whether the dense kernel takes these inputs, the mask in its form)."""
+        B, L_Q, H, Dh = q.shape
+        if not (self.fused_attention and q.is_cuda and q.dtype in (torch.bfloat16, torch.float16) and k.shape == v.shape
+                and k.dtype == v.dtype == q.dtype and Dh % 8 == 0 and Dh <= 128 and k.size(1) > 0):
+            return False, None
+        if self.training and self.dropout.p > 0.0:
+            return False, None
+        if mask is None:
+            return True, None
+        if not isinstance(mask, torch.Tensor) or mask.device != q.device or mask.dim() > 4:
+            return False, None
+        shape = (1,) * (4 - mask.dim()) + tuple(mask.shape)
+        if any(m not in (1, w) for m, w in zip(shape, (B, H, L_Q, k.size(1)))):
+            return False, None
+        return True, (mask if mask.dtype == torch.bool else mask != 0).view(shape)
+
     def forward(self, query, key, value, y=None, mask=None, return_attention=False):
         B, L_Q, D = query.shape
         if y is not None and L_Q == key.size(1) == value.size(1):
@@ -145,8 +168,11 @@ class HierarchicalAttention(nn.Module):
             return (output, None) if return_attention else output
         # the reference's fallback branch (attention.py:257-270): plain multi-head attention on the X projections
         H, Dh = self.num_heads, self.head_dim
-        split = lambda t, proj: proj(t).view(B, t.size(1), H, Dh).transpose(1, 2)        # noqa: E731
-        ctx, weights = self._standard_attention(split(query, self.Wq_x), split(key, self.Wk_x),
-                                                split(value, self.Wv_x), mask)
+        split = lambda t, proj: proj(t).view(B, t.size(1), H, Dh)                        # noqa: E731
+        q, k, v = split(query, self.Wq_x), split(key, self.Wk_x), split(value, self.Wv_x)
+        fused, allowed = (False, None) if return_attention else self._dense_mask(q, k, v, mask)
+        if fused:                                        # a row that the mask leaves empty is NaN, as a softmax over nothing is
+            return self.out_proj_x(cross_attention(q, k, v, mask=allowed, empty_value=math.nan).reshape(B, L_Q, D))
+        ctx, weights = self._standard_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), mask)
         output = self.out_proj_x(ctx.transpose(1, 2).reshape(B, L_Q, D))
         return (output, weights) if return_attention else output

@@ -15,9 +15,10 @@ import math
 import pytest
 import torch
 
-from sparseattention_b200 import _lib
+from sparseattention_b200 import HierarchicalAttention, _lib
 from sparseattention_b200.ops import cross_attention, paged_attention_decode
-from sparseattention_b200.ops.dense import dense_attention_forward
+from sparseattention_b200.ops.dense import dense_aborts, dense_attention_backward, dense_attention_forward
+from tests.conftest import rel_err
 
 pytestmark = pytest.mark.gpu
 
@@ -586,3 +587,102 @@ def test_training_then_serving_the_same_rows():
     for i in range(Lq):
         step = paged_attention_decode(q[:, i].contiguous(), kp, vp, table, lengths)
         near(step, want.out[:, i], want.out_tol[:, i], f"token {i}")
+
+
+# --------------------------------------------------------------------------------------------------------------- module
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("kind", [None, "row", "keys", "square", "empty"])
+def test_module_over_another_sequence(dtype, kind):
+    """HierarchicalAttention without parents: the kernel against the module's eager operations on the same weights in 32 bits
+    (2e-2, what the suite grants 16-bit layers), outputs, input and weight gradients."""
+    B, Lq, Lk, d, H = 2, 75, 140, 256, 4
+    torch.manual_seed(5)
+    layer = HierarchicalAttention(d, H, dropout=0.1).cuda().eval()
+    exact = HierarchicalAttention(d, H, dropout=0.1).cuda().eval()
+    layer = layer.to(dtype)
+    exact.load_state_dict({n: t.float() for n, t in layer.state_dict().items()})
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    q, m, g = (torch.randn(B, n, d, generator=gen, device="cuda").to(dtype) for n in (Lq, Lk, Lq))
+    mask = {None: None, "row": torch.rand(Lk, generator=gen, device="cuda").gt(0.3),
+            "keys": torch.rand(B, 1, 1, Lk, generator=gen, device="cuda").gt(0.3).float(),
+            "square": torch.rand(Lq, Lk, generator=gen, device="cuda").gt(0.5).to(torch.int32),
+            "empty": torch.ones(Lq, Lk, dtype=torch.bool, device="cuda")}[kind]
+    if kind == "empty":
+        mask[3] = False
+    calls = []
+    hook = layer.dropout.register_forward_hook(lambda *a: calls.append(1))         # the eager path passes its weights through it
+    ql, ml = q.clone().requires_grad_(True), m.clone().requires_grad_(True)
+    out = layer(ql, ml, ml, mask=mask)
+    hook.remove()
+    assert not calls
+    qe, me = q.float().requires_grad_(True), m.float().requires_grad_(True)
+    want = exact(qe, me, me, mask=mask)
+    if kind == "empty":
+        assert out[:, 3].isnan().all() and want[:, 3].isnan().all()
+        rest = torch.arange(Lq, device="cuda") != 3
+        assert rel_err(out[:, rest].float(), want[:, rest]) < 2e-2
+        return
+    assert rel_err(out.float(), want) < 2e-2
+    got = torch.autograd.grad(out, [ql, ml, layer.Wq_x.weight, layer.Wk_x.weight, layer.Wv_x.weight, layer.out_proj_x.bias], g)
+    ref = torch.autograd.grad(want, [qe, me, exact.Wq_x.weight, exact.Wk_x.weight, exact.Wv_x.weight, exact.out_proj_x.bias], g.float())
+    for a, b in zip(got, ref):
+        assert rel_err(a.float(), b) < 2e-2
+
+
+def test_module_keeps_its_eager_path_where_the_kernel_does_not_apply():
+    layer = HierarchicalAttention(64, 2, dropout=0.5).cuda().to(torch.bfloat16)
+    q, m = torch.randn(2, 9, 64, device="cuda", dtype=torch.bfloat16), torch.randn(2, 13, 64, device="cuda", dtype=torch.bfloat16)
+    calls = []
+    layer.dropout.register_forward_hook(lambda *a: calls.append(1))
+    layer(q, m, m)                                                # dropout is active
+    assert len(calls) == 1
+    layer.eval()
+    out, weights = layer(q, m, m, return_attention=True)          # weights asked for
+    assert len(calls) == 2 and weights.shape == (2, 2, 9, 13)
+    near = layer(q, m, m)
+    assert len(calls) == 2 and rel_err(near.float(), out.float()) < 2e-2
+    layer.fused_attention = False
+    assert torch.equal(layer(q, m, m), out) and len(calls) == 3
+    layer.float()
+    layer.fused_attention = True
+    layer(q.float(), m.float(), m.float())                        # 32 bits
+    assert len(calls) == 4
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        layer(q.float(), m.float(), m.float())
+    assert len(calls) == 4
+
+
+# -------------------------------------------------------------------------------------------------------- bounded waits
+def test_a_wait_that_runs_out_shows():
+    """Every copy completes, but the first barrier of an item expects bytes that never come: the blocks give up after a short
+    limit, count themselves and leave NaN; afterwards everything is as before."""
+    lib = _lib.load()
+    q, k, v, g = make(2, 200, 300, 2, 2, 64, torch.bfloat16)
+    out, lse = dense_attention_forward(q, k, v, None, None, 0.125)
+    good = (out, *dense_attention_backward(q, k, v, out, lse, g, None, None, 0.125))
+    torch.cuda.synchronize()
+    before = dense_aborts()
+    _lib.check(lib.hsa_debug_wait_test(20_000_000, 16), "hsa_debug_wait_test")
+    try:
+        bad, bad_lse = dense_attention_forward(q, k, v, None, None, 0.125)
+        torch.cuda.synchronize()
+        mid = dense_aborts()
+        grads = dense_attention_backward(q, k, v, out, lse, g, None, None, 0.125)
+        torch.cuda.synchronize()
+    finally:
+        _lib.check(lib.hsa_debug_wait_test(2_000_000_000, 0), "hsa_debug_wait_test")
+    assert mid > before and dense_aborts() > mid
+    assert bad.isnan().all() and bad_lse.isnan().all()
+    assert all(t.isnan().all() for t in grads)
+    out, lse = dense_attention_forward(q, k, v, None, None, 0.125)
+    again = (out, *dense_attention_backward(q, k, v, out, lse, g, None, None, 0.125))
+    assert all(torch.equal(a, b) for a, b in zip(good, again))
+
+
+def test_no_wait_has_run_out():
+    """Sorts last in this file: the only blocks that ever gave up are those of the test above."""
+    q, k, v, g = make(4, 700, 900, 8, 8, 128, torch.bfloat16)
+    before = dense_aborts()
+    for _ in range(5):
+        check(q, k, v, g)
+    assert dense_aborts() == before
