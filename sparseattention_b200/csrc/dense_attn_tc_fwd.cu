@@ -24,7 +24,9 @@ namespace hsa {
 
 __device__ unsigned int g_dense_aborts = 0;
 
-constexpr int kFwdThreads = 352;                 // softmax of two query tiles, copies, and a warp of products for either tile
+// Softmax of two query tiles, copies, a warp of products for either tile, and an idle warp that completes the last warpgroup:
+// its registers go to the softmax (2 x 128 x 200 + 128 x 104 = 384 x 168, what the block is launched with).
+constexpr int kFwdThreads = 384;
 
 struct DenseSplit {
     float *part_o, *part_ml;                     // [splits, B, Lq, H, D] and [splits, B, Lq, H, 2] when splits > 1
@@ -114,6 +116,7 @@ dense_fwd_tc5_kernel(const DenseArgs a, const DenseSplit sp, const __grid_consta
     auto wait = [&](uint32_t bar, uint32_t parity) { return (bool)__all_sync(0xffffffffu, mbar_wait(bar, parity, sp.wait_limit, abort_flag)); };
 
     if (warp == 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 104;\n");
         // ------------------------------------------------------------------------------------------------- copies
         bool ok = true;
         int slot = 0; uint32_t ph = 0, qc[2] = {0, 0};
@@ -190,7 +193,8 @@ dense_fwd_tc5_kernel(const DenseArgs a, const DenseSplit sp, const __grid_consta
             const long long start = clock64();
             while (clock64() - start < 200000) {}
         }
-    } else if (warp >= 9) {
+    } else if (warp == 9 || warp == 10) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 104;\n");
         // -------------------------------------------------------------------------------------------- matrix products
         // Half tiles of 64 keys: S of half tile j + 2 follows the product that has consumed the weights of half tile j, whose
         // columns it takes, so that the softmax always finds the next scores ready.  One warp for either query tile: with one
@@ -290,7 +294,10 @@ dense_fwd_tc5_kernel(const DenseArgs a, const DenseSplit sp, const __grid_consta
             if (ok && lane == 0) mbar_arrive(info_empty(is));
             __syncwarp();
         }
+    } else if (warp == 11) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 104;\n");
     } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 200;\n");
         // -------------------------------------------------------------------------------------------------- softmax
         const int w = warp >> 2, quarter = warp & 3;
         const int row = quarter * 32 + lane;
@@ -379,15 +386,15 @@ dense_fwd_tc5_kernel(const DenseArgs a, const DenseSplit sp, const __grid_consta
                             for (int j = 0; j < 32; ++j) {
                                 const float2 e = unpair(fma2(pair_bits(r[j >> 4][(2 * j) & 31], r[j >> 4][(2 * j + 1) & 31]), c2, ref2));
                                 float2 p;
-                                if (decltype(mixed)::value && j % 4 == 0) p = exp2_poly(e);
+                                if (decltype(mixed)::value && j % 3 == 0) p = exp2_poly(e);
                                 else p = make_float2(fast_exp2(e.x), fast_exp2(e.y));
                                 sum[j & 1] = add2(sum[j & 1], pair(p.x, p.y));
                                 pk[j] = pack2<T>(p.x, p.y);
                             }
                         };
-                        // A quarter of the exponentials goes to the multiply-add units: with none the special-function unit, with
-                        // half of them those units are the busier (277 / 271 / 307 us at 8 x 2048 x 4096, 8 heads of 64).  Hidden
-                        // scores (-inf) have to give 0, which the polynomial does not.
+                        // A third of the exponentials goes to the multiply-add units: with fewer the special-function unit, with
+                        // half of them those units are the busier (none 469 us, a quarter 464, a third 459 at 4096 x 4096, batch 4,
+                        // 16 heads of 128).  Hidden scores (-inf) have to give 0, which the polynomial does not.
                         if (partial) weights(std::false_type{}); else weights(std::true_type{});
                         tmem_st32(tsx, pk);
                         const float2 total = unpair(add2(sum[0], sum[1]));
