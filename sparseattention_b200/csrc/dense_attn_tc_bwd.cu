@@ -338,7 +338,7 @@ dense_dq_tc5_kernel(const DenseArgs a, const long long wait_limit, const unsigne
 #pragma unroll
                     for (int j = 0; j < 32; ++j) o[j] = 0u;
                 }
-                if (qi < a.Lq) store_row32<T>(out, 32 * c, a.D, o, a.scale);
+                store_rows32<T>(out, a.dq.row_stride, a.Lq - qi, 32 * c, a.D, o, a.scale);
             }
             fence_before_sync();                             // the accumulator may be written again
             __syncwarp();
@@ -674,7 +674,7 @@ dense_dkdv_tc5_kernel(const DenseArgs a, const long long wait_limit, const unsig
 #pragma unroll
                     for (int j = 0; j < 32; ++j) o[j] = 0u;
                 }
-                if (key < a.Lk) store_row32<T>(out, 32 * c, a.D, o, x == 0 ? 1.f : a.scale);
+                store_rows32<T>(out, g.row_stride, a.Lk - key, 32 * c, a.D, o, x == 0 ? 1.f : a.scale);
             }
             fence_before_sync();
             __syncwarp();

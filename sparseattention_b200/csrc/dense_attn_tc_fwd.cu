@@ -412,7 +412,7 @@ dense_fwd_tc5_kernel(const DenseArgs a, const DenseSplit sp, const __grid_consta
                 if (!ok) break;                                  // with k and item of the unfinished one
                 fence_after_sync();
                 const bool none = l == 0.f;
-                const float inv = 1.f / l;
+                const float inv = none ? 0.f : 1.f / l;
                 const int64_t at = (((int64_t)it.split * a.B + it.b) * a.Lq + qi) * a.H + it.h;
                 T *orow = (T *)a.out.ptr + it.b * a.out.batch_stride + (int64_t)qi * a.out.row_stride + (int64_t)it.h * a.D;
 #pragma unroll 1
@@ -426,20 +426,31 @@ dense_fwd_tc5_kernel(const DenseArgs a, const DenseSplit sp, const __grid_consta
 #pragma unroll
                         for (int j = 0; j < 32; ++j) o[j] = 0u;
                     }
-                    if (qi >= a.Lq) continue;
                     if (sp.splits > 1) {
+                        const int quad = lane & 3;
 #pragma unroll
-                        for (int j = 0; j < 32; j += 4)
-                            if (32 * c + j < a.D)
-                                *reinterpret_cast<uint4 *>(sp.part_o + at * a.D + 32 * c + j) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
-                    } else if (!none) {
-                        store_row32<T>(orow, 32 * c, a.D, o, inv);
+                        for (int g = 0; g < 2; ++g) {                // 16 columns are four pieces of 32-bit numbers
+                            uint4 p[4];
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) p[j] = make_uint4(o[16 * g + 4 * j], o[16 * g + 4 * j + 1], o[16 * g + 4 * j + 2], o[16 * g + 4 * j + 3]);
+                            quad_pieces(p, quad);
+                            const int col = 32 * c + 16 * g + 4 * quad;
+#pragma unroll
+                            for (int j = 0; j < 4; ++j)
+                                if (qi + j - quad < a.Lq && col < a.D)
+                                    *reinterpret_cast<uint4 *>(sp.part_o + (at + (int64_t)(j - quad) * a.H) * a.D + col) = p[j];
+                        }
+                    } else {
+                        store_rows32<T>(orow, a.out.row_stride, a.Lq - qi, 32 * c, a.D, o, inv);
                     }
                 }
                 if (qi < a.Lq) {
                     if (sp.splits > 1) *reinterpret_cast<float2 *>(sp.part_ml + 2 * at) = make_float2(m, l);
-                    else if (none) fill_row<T>(orow, a.D, a.empty_value);
                     if (sp.splits == 1 && a.lse != nullptr) a.lse[at] = none ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+                }
+                if (sp.splits == 1 && a.empty_value != 0.f) {        // other lanes wrote the row's zeros: they come first
+                    __syncwarp();
+                    if (qi < a.Lq && none) fill_row<T>(orow, a.D, a.empty_value);
                 }
                 fence_before_sync();                             // the accumulator may be written again
             }
