@@ -427,7 +427,7 @@ int hsa_dense_attn_fwd(hsa_view Q, hsa_view K, hsa_view V, hsa_view Out, float *
                        const void *packed_mask, int mask_batches, int mask_heads, int mask_rows, void *workspace,
                        size_t workspace_bytes, int B, int Lq, int Lk, int H, int Hkv, int D, float scale, float empty_value,
                        int dtype, int algo, void *stream);
-size_t hsa_dense_attn_bwd_workspace_bytes(int B, int Lq, int H);
+size_t hsa_dense_attn_bwd_workspace_bytes(int B, int Lq, int Lk, int H, int Hkv, int D, int dtype, int algo);
 int hsa_dense_attn_bwd(hsa_view Q, hsa_view K, hsa_view V, hsa_view Out, const float *LSE, hsa_view dOut, hsa_view dQ,
                        hsa_view dK, hsa_view dV, const int *key_lengths, const void *packed_mask, int mask_batches,
                        int mask_heads, int mask_rows, void *workspace, size_t workspace_bytes, int B, int Lq, int Lk, int H,

@@ -7,7 +7,8 @@ int dense_simt(const DenseArgs &a, int what, int dtype, cudaStream_t st);
 bool dense_tc_ok(const DenseArgs &a, int dtype, bool backward);
 size_t dense_fwd_tc_workspace(int B, int Lq, int Lk, int H, int D);
 bool dense_bwd_tables_ok(const DenseArgs &a);
-int dense_bwd_tc(const DenseArgs &a, int dtype, cudaStream_t st);
+size_t dense_bwd_tc_workspace(int B, int Lq, int Lk, int H, int Hkv, int D);
+int dense_bwd_tc(const DenseArgs &a, void *workspace, int dtype, cudaStream_t st);
 int dense_fwd_tc(const DenseArgs &a, void *workspace, size_t workspace_bytes, int dtype, cudaStream_t st);
 
 // ------------------------------------------------------------------------------------------------------------ mask
@@ -102,6 +103,7 @@ static int check_shape(const char *who, int B, int Lq, int Lk, int H, int Hkv, i
     HSA_CHECK_ARG(H % Hkv == 0, "%s: %d query heads are not a multiple of %d key/value heads", who, H, Hkv);
     HSA_CHECK_ARG(D >= 1 && D <= 256, "%s: head dim %d outside 1..256", who, D);
     HSA_CHECK_ARG(Lq <= (1 << 30) && Lk <= (1 << 30), "%s: more than 2^30 rows", who);
+    HSA_CHECK_ARG((long long)(H / Hkv) * Lq <= (1LL << 30), "%s: more than 2^30 query rows per key/value head", who);
     HSA_CHECK_ARG(scale > 0.f && scale < INFINITY, "%s: the scale must be positive and finite", who);
     HSA_CHECK_ARG(algo >= 0 && algo <= 2, "%s: unknown algo %d", who, algo);
     if (dtype != HSA_F32 && dtype != HSA_BF16 && dtype != HSA_F16) return fail(HSA_ERR_DTYPE, "unknown dtype code %d", dtype);
@@ -177,9 +179,14 @@ extern "C" int hsa_dense_attn_fwd(hsa_view Q, hsa_view K, hsa_view V, hsa_view O
     return dense_simt(a, 0, dtype, (cudaStream_t)stream);
 }
 
-extern "C" size_t hsa_dense_attn_bwd_workspace_bytes(int B, int Lq, int H) {
-    if (B < 1 || Lq < 1 || H < 1) return 0;
-    return (size_t)2 * B * H * ((Lq + 127) / 128 * 128) * sizeof(float);
+// Row sums and log-sum-exps of the padded rows, then what the tensor-core kernels keep of partial gradients
+static size_t bwd_stats_bytes(int B, int Lq, int H) { return (size_t)2 * B * H * ((Lq + 127) / 128 * 128) * sizeof(float); }
+
+extern "C" size_t hsa_dense_attn_bwd_workspace_bytes(int B, int Lq, int Lk, int H, int Hkv, int D, int dtype, int algo) {
+    if (B < 1 || Lq < 1 || Lk < 1 || H < 1 || Hkv < 1 || H % Hkv != 0 || D < 1) return 0;
+    size_t n = bwd_stats_bytes(B, Lq, H);
+    if (D <= 128 && D % 8 == 0 && algo != 1 && dtype != HSA_F32) n += dense_bwd_tc_workspace(B, Lq, Lk, H, Hkv, D);
+    return n;
 }
 
 extern "C" int hsa_dense_attn_bwd(hsa_view Q, hsa_view K, hsa_view V, hsa_view Out, const float *LSE, hsa_view dOut, hsa_view dQ,
@@ -189,7 +196,7 @@ extern "C" int hsa_dense_attn_bwd(hsa_view Q, hsa_view K, hsa_view V, hsa_view O
     HSA_CHECK_ARG(Q.ptr && K.ptr && V.ptr && Out.ptr && LSE && dOut.ptr && dQ.ptr && dK.ptr && dV.ptr, "hsa_dense_attn_bwd: null pointer");
     if (int rc = check_shape("hsa_dense_attn_bwd", B, Lq, Lk, H, Hkv, D, scale, dtype, algo)) return rc;
     if (int rc = check_mask("hsa_dense_attn_bwd", packed_mask, mask_batches, mask_heads, mask_rows, B, H, Lq)) return rc;
-    const size_t need = hsa_dense_attn_bwd_workspace_bytes(B, Lq, H);
+    const size_t need = hsa_dense_attn_bwd_workspace_bytes(B, Lq, Lk, H, Hkv, D, dtype, algo);
     if (workspace == nullptr || workspace_bytes < need)
         return fail(HSA_ERR_WORKSPACE, "hsa_dense_attn_bwd: workspace of %zu bytes needed, %zu given", need, workspace_bytes);
     if (reinterpret_cast<uintptr_t>(workspace) & 255u) return fail(HSA_ERR_ALIGN, "hsa_dense_attn_bwd: workspace must be 256-byte aligned");
@@ -212,7 +219,7 @@ extern "C" int hsa_dense_attn_bwd(hsa_view Q, hsa_view K, hsa_view V, hsa_view O
     HSA_CHECK_ARG(algo != 2 || tc, "hsa_dense_attn_bwd: no tensor-core kernel for these inputs");
     cudaStream_t st = (cudaStream_t)stream;
     if (int rc = dense_delta(a, neg_lse2, neg_delta, dtype, D % (16 / es) == 0 && view_vec_ok(Out, es) && view_vec_ok(dOut, es), st)) return rc;
-    if (tc) return dense_bwd_tc(a, dtype, st);
+    if (tc) return dense_bwd_tc(a, (char *)workspace + bwd_stats_bytes(B, Lq, H), dtype, st);
     if (int rc = dense_simt(a, 1, dtype, st)) return rc;
     return dense_simt(a, 2, dtype, st);
 }

@@ -9,6 +9,22 @@
 namespace hsa {
 
 constexpr int kFlagTiles = 768;                  // tiles whose mask state fits one of a block's two tables
+// Ranges per work item when there are few items and each is long: the count that lets the slowest SM finish first.  `steps` tiles per
+// item; an item costs `once` tiles' time besides, `once_split` as one of several ranges, whose partial results are then joined.
+inline int range_count(long long items, int steps, double once, double once_split) {
+    const int sms = dense_sm_count();
+    if (items * 2 > sms) return 1;
+    double best = 1e30;
+    int best_s = 1;
+    for (int s = 1; s <= 64 && s <= steps; ++s) {
+        const double waves = (double)((items * s + sms - 1) / sms);
+        const double t = waves * ((steps + s - 1) / s + (s > 1 ? once_split : once)) + (s > 1 ? once : 0.0);
+        if (t < 0.95 * best) { best = t; best_s = s; }
+    }
+    const int per = (steps + best_s - 1) / best_s;
+    return (steps + per - 1) / per;
+}
+
 // Two 32-bit numbers in a register pair: one instruction for both
 __device__ __forceinline__ uint64_t pair(float lo, float hi) {
     uint64_t v;
@@ -126,6 +142,21 @@ __device__ __forceinline__ void store_rows32(T *row, int64_t row_stride, int bel
 #pragma unroll
     for (int t = 0; t < 4; ++t)
         if (t - quad < below) *reinterpret_cast<uint4 *>(row + (t - quad) * row_stride + col + 8 * quad) = p[t];
+}
+// The same for 32-bit rows.
+__device__ __forceinline__ void store_rows32_f32(float *row, int64_t row_stride, int below, int col, int D, const uint32_t (&v)[32]) {
+    const int quad = threadIdx.x & 3;
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {                                        // 16 columns are four pieces
+        uint4 p[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) p[j] = make_uint4(v[16 * g + 4 * j], v[16 * g + 4 * j + 1], v[16 * g + 4 * j + 2], v[16 * g + 4 * j + 3]);
+        quad_pieces(p, quad);
+        const int c = col + 16 * g + 4 * quad;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+            if (t - quad < below && c < D) *reinterpret_cast<uint4 *>(row + (t - quad) * row_stride + c) = p[t];
+    }
 }
 template <typename T>
 __device__ __forceinline__ void fill_row(T *row, int D, float value) {

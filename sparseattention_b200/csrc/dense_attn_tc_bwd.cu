@@ -24,6 +24,13 @@ constexpr int kBwdThreads = 352;                 // eight element-wise warps, co
 
 __device__ unsigned int g_dense_bwd_aborts = 0;
 
+struct BwdSplit {
+    float *part;                                 // partial gradients, [splits][B, rows, heads, D] 32-bit (dk before dv), when splits > 1
+    int splits;
+    unsigned int extra_tx;                       // test hook: bytes that the first copy is announced with and never brings
+    long long wait_limit;
+};
+
 // ------------------------------------------------------------------------------------------------------------------ dq
 template <int DP>
 struct DqShape {
@@ -33,23 +40,27 @@ struct DqShape {
     static_assert(kSmem <= 227 * 1024, "shared memory");
 };
 
-// A work item: 128 query rows of a (batch entry, head)
+// A work item: 128 query rows of a (batch entry, head) against one range of its keys
 struct DqItem {
-    int q0, h, hk, b, n, tiles;
+    int q0, h, hk, b, split, n, kt0, kt1;
     int64_t plane;
-    __device__ __forceinline__ DqItem(const DenseArgs &a, int item) {
+    __device__ __forceinline__ DqItem(const DenseArgs &a, int splits, int item) {
         const int qblocks = (a.Lq + 127) / 128;
         q0 = item % qblocks * 128; item /= qblocks;
-        h = item % a.H; b = item / a.H; hk = h / a.group;
+        h = item % a.H; item /= a.H;
+        b = item % a.B; split = item / a.B;
+        hk = h / a.group;
         n = dense_keys(a, b);
-        tiles = (n + 127) / 128;
+        const int tiles = (n + 127) / 128, per = (tiles + splits - 1) / splits;
+        kt0 = min(tiles, split * per);
+        kt1 = min(tiles, kt0 + per);
         plane = (int64_t)b * a.mask.plane_b + (int64_t)h * a.mask.plane_h;
     }
 };
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(kBwdThreads, 1)
-dense_dq_tc5_kernel(const DenseArgs a, const long long wait_limit, const unsigned int extra_tx, const __grid_constant__ CUtensorMap map_q,
+dense_dq_tc5_kernel(const DenseArgs a, const BwdSplit sp, const __grid_constant__ CUtensorMap map_q,
                     const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                     const __grid_constant__ CUtensorMap map_g) {
     using namespace tc5;
@@ -94,7 +105,7 @@ dense_dq_tc5_kernel(const DenseArgs a, const long long wait_limit, const unsigne
     __syncthreads();
     fence_after_sync();
     const uint32_t tmem = *tmem_slot;
-    auto wait = [&](uint32_t bar, uint32_t parity) { return (bool)__all_sync(0xffffffffu, mbar_wait(bar, parity, wait_limit, abort_flag)); };
+    auto wait = [&](uint32_t bar, uint32_t parity) { return (bool)__all_sync(0xffffffffu, mbar_wait(bar, parity, sp.wait_limit, abort_flag)); };
 
     if (warp == 8) {
         bool ok = true;
@@ -108,9 +119,9 @@ dense_dq_tc5_kernel(const DenseArgs a, const long long wait_limit, const unsigne
             const int is = k & 1;
             if (!(ok = wait(info_empty(is), ((k >> 1) & 1) ^ 1))) break;
             if (item >= 0 && masked) {
-                const DqItem it(a, item);
+                const DqItem it(a, sp.splits, item);
                 const int cell = a.mask.rows > 1 ? it.q0 / kDenseTile : 0;
-                for (int t = lane; t < it.tiles; t += 32) items.flags[is][t] = a.mask.tiles[(it.plane * a.mask.tq + cell) * a.mask.tk + t];
+                for (int t = it.kt0 + lane; t < it.kt1; t += 32) items.flags[is][t - it.kt0] = a.mask.tiles[(it.plane * a.mask.tq + cell) * a.mask.tk + t];
             }
             if (lane == 0) items.item[is] = item;
             __syncwarp();
@@ -127,11 +138,11 @@ dense_dq_tc5_kernel(const DenseArgs a, const long long wait_limit, const unsigne
                 asked = true;
                 __syncwarp();
             };
-            const DqItem it(a, item);
+            const DqItem it(a, sp.splits, item);
             bool first = true;
-            for (int t = 0; t < it.tiles && ok; ++t) {
-                if (t + 2 >= it.tiles) ask();
-                if (masked && items.flags[is][t] == 0) continue;
+            for (int t = it.kt0; t < it.kt1 && ok; ++t) {
+                if (t + 2 >= it.kt1) ask();
+                if (masked && items.flags[is][t - it.kt0] == 0) continue;
                 if (!(ok = wait(k_empty(ks), kp ^ 1))) break;
                 if (lane == 0) {
                     mbar_expect_tx(k_full(ks), TILE);
@@ -143,7 +154,7 @@ dense_dq_tc5_kernel(const DenseArgs a, const long long wait_limit, const unsigne
                     if (!(ok = wait(qg_empty, (qc & 1) ^ 1))) break;
                     ++qc;
                     if (lane == 0) {
-                        mbar_expect_tx(qg_full, 2 * TILE + extra_tx);
+                        mbar_expect_tx(qg_full, 2 * TILE + sp.extra_tx);
                         load(qg_full, &map_q, q_s, it.h, it.q0, it.b);
                         load(qg_full, &map_g, g_s, it.h, it.q0, it.b);
                     }
@@ -178,15 +189,15 @@ dense_dq_tc5_kernel(const DenseArgs a, const long long wait_limit, const unsigne
             if (!(ok = wait(info_full(is), (k >> 1) & 1))) break;
             const int item = uniform(items.item[is]);
             if (item < 0) break;
-            DqItem it(a, item);
-            it.n = uniform(it.n); it.tiles = uniform(it.tiles);
+            DqItem it(a, sp.splits, item);
+            it.n = uniform(it.n); it.kt0 = uniform(it.kt0); it.kt1 = uniform(it.kt1);
             auto next_tile = [&](int t) {
-                if (masked) { while (t < it.tiles && items.flags[is][t] == 0) ++t; t = uniform(t); }
+                if (masked) { while (t < it.kt1 && items.flags[is][t - it.kt0] == 0) ++t; t = uniform(t); }
                 return t;
             };
-            int t = next_tile(0);
-            if (t < it.tiles) { ok = wait(qg_full, qc & 1); ++qc; }
-            while (ok && t < it.tiles) {
+            int t = next_tile(it.kt0);
+            if (t < it.kt1) { ok = wait(qg_full, qc & 1); ++qc; }
+            while (ok && t < it.kt1) {
                 if (!(ok = wait(k_full(ks), kp))) break;
                 if (it.n - t * 128 < 128 || masked)
                     zero_hidden_rows<PLANES>(k_s + ks * TILE, it.n - t * 128, masked ? a.mask.seen + it.plane * a.mask.wk + t * 4 : nullptr, lane);
@@ -211,7 +222,7 @@ dense_dq_tc5_kernel(const DenseArgs a, const long long wait_limit, const unsigne
                         mma_commit(s_full(i & 1));
                         if (half + 1 == halves) {
                             mma_commit(v_empty(vs));
-                            if (tn >= it.tiles) mma_commit(qg_empty);
+                            if (tn >= it.kt1) mma_commit(qg_empty);
                         }
                     }
                     __syncwarp();
@@ -233,15 +244,15 @@ dense_dq_tc5_kernel(const DenseArgs a, const long long wait_limit, const unsigne
             if (!(ok = wait(info_full(is), (k >> 1) & 1))) break;
             const int item = uniform(items.item[is]);
             if (item < 0) break;
-            DqItem it(a, item);
-            it.n = uniform(it.n); it.tiles = uniform(it.tiles);
+            DqItem it(a, sp.splits, item);
+            it.n = uniform(it.n); it.kt0 = uniform(it.kt0); it.kt1 = uniform(it.kt1);
             auto next_tile = [&](int t) {
-                if (masked) { while (t < it.tiles && items.flags[is][t] == 0) ++t; t = uniform(t); }
+                if (masked) { while (t < it.kt1 && items.flags[is][t - it.kt0] == 0) ++t; t = uniform(t); }
                 return t;
             };
             bool fresh = true;
-            int t = next_tile(0);
-            while (ok && t < it.tiles) {
+            int t = next_tile(it.kt0);
+            while (ok && t < it.kt1) {
                 const int halves = it.n - t * 128 > 64 ? 2 : 1, tn = next_tile(t + 1);
                 for (int half = 0; half < halves; ++half, ++i) {
                     if (!(ok = wait(d_full(i & 1), i >> 1 & 1))) break;
@@ -255,7 +266,7 @@ dense_dq_tc5_kernel(const DenseArgs a, const long long wait_limit, const unsigne
                         mma_commit(s_free(i & 1));
                         if (half + 1 == halves) {
                             mma_commit(k_empty(ks));
-                            if (tn >= it.tiles) mma_commit(q_done);      // last: the block may end after it
+                            if (tn >= it.kt1) mma_commit(q_done);      // last: the block may end after it
                         }
                     }
                     __syncwarp();
@@ -279,15 +290,15 @@ dense_dq_tc5_kernel(const DenseArgs a, const long long wait_limit, const unsigne
             if (!(ok = wait(info_full(is), (k >> 1) & 1))) break;
             item = items.item[is];
             if (item < 0) break;
-            const DqItem it(a, item);
+            const DqItem it(a, sp.splits, item);
             const int qi = it.q0 + row;
             const int64_t at = ((int64_t)it.b * a.H + it.h) * a.lq_pad + qi;
             const float neg_lse2 = a.neg_lse2[at], neg_delta = a.neg_delta[at];
             const uint64_t c2 = pair(a.scale_log2, a.scale_log2), lse22 = pair(neg_lse2, neg_lse2), delta2 = pair(neg_delta, neg_delta);
             const uint32_t *bits = masked ? a.mask.bits + (it.plane * a.mask.rows + (a.mask.rows > 1 ? min(qi, a.Lq - 1) : 0)) * a.mask.wk : nullptr;
             bool any = false;
-            for (int t = 0; t < it.tiles && ok; ++t) {
-                const uint32_t flag = masked ? items.flags[is][t] : 2u;
+            for (int t = it.kt0; t < it.kt1 && ok; ++t) {
+                const uint32_t flag = masked ? items.flags[is][t - it.kt0] : 2u;
                 if (flag == 0) continue;
                 const int left = it.n - t * 128;
                 const bool partial = left < 128 || flag != 2;
@@ -338,7 +349,11 @@ dense_dq_tc5_kernel(const DenseArgs a, const long long wait_limit, const unsigne
 #pragma unroll
                     for (int j = 0; j < 32; ++j) o[j] = 0u;
                 }
-                store_rows32<T>(out, a.dq.row_stride, a.Lq - qi, 32 * c, a.D, o, a.scale);
+                if (sp.splits > 1)
+                    store_rows32_f32(sp.part + ((((int64_t)it.split * a.B + it.b) * a.Lq + qi) * a.H + it.h) * a.D, (int64_t)a.H * a.D, a.Lq - qi,
+                                     32 * c, a.D, o);
+                else
+                    store_rows32<T>(out, a.dq.row_stride, a.Lq - qi, 32 * c, a.D, o, a.scale);
             }
             fence_before_sync();                             // the accumulator may be written again
             __syncwarp();
@@ -352,10 +367,13 @@ dense_dq_tc5_kernel(const DenseArgs a, const long long wait_limit, const unsigne
                     item = items.item[k & 1];
                     if (item < 0) break;
                 }
-                const DqItem it(a, item);
-                if (it.q0 + row < a.Lq)
-                    fill_row<T>((T *)a.dq.ptr + it.b * a.dq.batch_stride + (int64_t)(it.q0 + row) * a.dq.row_stride + (int64_t)it.h * a.D, a.D,
-                                __int_as_float(0x7fffffff));
+                const DqItem it(a, sp.splits, item);
+                const float nan = __int_as_float(0x7fffffff);
+                const int qi = it.q0 + row;
+                if (qi < a.Lq && sp.splits > 1)
+                    for (int d = 0; d < a.D; ++d) sp.part[((((int64_t)it.split * a.B + it.b) * a.Lq + qi) * a.H + it.h) * a.D + d] = nan;
+                else if (qi < a.Lq)
+                    fill_row<T>((T *)a.dq.ptr + it.b * a.dq.batch_stride + (int64_t)qi * a.dq.row_stride + (int64_t)it.h * a.D, a.D, nan);
                 item = -1;
             }
         }
@@ -377,21 +395,25 @@ struct DkvShape {
     static_assert(kSmem <= 227 * 1024, "shared memory");
 };
 
-// A work item: 128 keys of a (batch entry, key/value head) against (query head of the group, tile of 64 queries), in this order
+// A work item: 128 keys of a (batch entry, key/value head) against one range of the units (query head of the group, tile of 64
+// queries), in this order
 struct DkvItem {
-    int kt, k0, hk, b, n, total;
-    __device__ __forceinline__ DkvItem(const DenseArgs &a, int item, int qtiles) {
+    int kt, k0, hk, b, split, n, u0, u1;
+    __device__ __forceinline__ DkvItem(const DenseArgs &a, int splits, int item, int qtiles) {
         const int ktiles = (a.Lk + 127) / 128;
         kt = item % ktiles; k0 = kt * 128; item /= ktiles;
-        hk = item % a.Hkv; b = item / a.Hkv;
+        hk = item % a.Hkv; item /= a.Hkv;
+        b = item % a.B; split = item / a.B;
         n = dense_keys(a, b);
-        total = k0 < n ? a.group * qtiles : 0;
+        const int total = k0 < n ? a.group * qtiles : 0, per = (total + splits - 1) / splits;
+        u0 = min(total, split * per);
+        u1 = min(total, u0 + per);
     }
 };
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(kBwdThreads, 1)
-dense_dkdv_tc5_kernel(const DenseArgs a, const long long wait_limit, const unsigned int extra_tx, const __grid_constant__ CUtensorMap map_q,
+dense_dkdv_tc5_kernel(const DenseArgs a, const BwdSplit sp, const __grid_constant__ CUtensorMap map_q,
                       const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                       const __grid_constant__ CUtensorMap map_g) {
     using namespace tc5;
@@ -437,7 +459,7 @@ dense_dkdv_tc5_kernel(const DenseArgs a, const long long wait_limit, const unsig
     __syncthreads();
     fence_after_sync();
     const uint32_t tmem = *tmem_slot;
-    auto wait = [&](uint32_t bar, uint32_t parity) { return (bool)__all_sync(0xffffffffu, mbar_wait(bar, parity, wait_limit, abort_flag)); };
+    auto wait = [&](uint32_t bar, uint32_t parity) { return (bool)__all_sync(0xffffffffu, mbar_wait(bar, parity, sp.wait_limit, abort_flag)); };
     auto plane_of = [&](int b, int h) { return (int64_t)b * a.mask.plane_b + (int64_t)h * a.mask.plane_h; };
     auto flag_of = [&](int is, int u) { return items.flags[is][u / qtiles * cells + (a.mask.rows > 1 ? (u % qtiles) >> 1 : 0)]; };
     auto next_unit = [&](int is, int u, int total) {
@@ -453,8 +475,8 @@ dense_dkdv_tc5_kernel(const DenseArgs a, const long long wait_limit, const unsig
             const int is = k & 1;
             if (!(ok = wait(info_empty(is), ((k >> 1) & 1) ^ 1))) break;
             if (item >= 0 && masked) {
-                const DkvItem it(a, item, qtiles);
-                if (it.total > 0)
+                const DkvItem it(a, sp.splits, item, qtiles);
+                if (it.u0 < it.u1)
                     for (int c = lane; c < a.group * cells; c += 32)
                         items.flags[is][c] = a.mask.tiles[(plane_of(it.b, it.hk * a.group + c / cells) * cells + c % cells) * a.mask.tk + it.kt];
             }
@@ -473,13 +495,13 @@ dense_dkdv_tc5_kernel(const DenseArgs a, const long long wait_limit, const unsig
                 asked = true;
                 __syncwarp();
             };
-            const DkvItem it(a, item, qtiles);
-            int u = next_unit(is, 0, it.total);
-            if (u < it.total) {
+            const DkvItem it(a, sp.splits, item, qtiles);
+            int u = next_unit(is, it.u0, it.u1);
+            if (u < it.u1) {
                 if (!(ok = wait(kv_empty, (kc & 1) ^ 1))) break;
                 ++kc;
                 if (lane == 0) {
-                    mbar_expect_tx(kv_full, 2 * TILE + extra_tx);
+                    mbar_expect_tx(kv_full, 2 * TILE + sp.extra_tx);
 #pragma unroll
                     for (int p = 0; p < PLANES; ++p) {
                         tma_load_4d(smem_addr(k_s + p * PLANE), &map_k, p * 64, it.hk, it.k0, it.b, kv_full);
@@ -488,9 +510,9 @@ dense_dkdv_tc5_kernel(const DenseArgs a, const long long wait_limit, const unsig
                 }
                 __syncwarp();
             }
-            for (; u < it.total; u = next_unit(is, u + 1, it.total)) {
+            for (; u < it.u1; u = next_unit(is, u + 1, it.u1)) {
                 const int h = it.hk * a.group + u / qtiles, q0 = u % qtiles * 64;
-                if (u + 4 >= it.total) ask();
+                if (u + 4 >= it.u1) ask();
                 if (!(ok = wait(empty(s), ph ^ 1))) break;
                 if (lane == 0) {
                     mbar_expect_tx(full(s), 2 * HALF + 512);
@@ -526,12 +548,12 @@ dense_dkdv_tc5_kernel(const DenseArgs a, const long long wait_limit, const unsig
             if (!(ok = wait(info_full(is), (k >> 1) & 1))) break;
             const int item = uniform(items.item[is]);
             if (item < 0) break;
-            const DkvItem it(a, item, qtiles);
-            const int total = uniform(it.total);
-            int u = next_unit(is, 0, total);
-            if (u < total) { ok = wait(kv_full, kc & 1); ++kc; }
-            while (ok && u < total) {
-                const int un = next_unit(is, u + 1, total);
+            const DkvItem it(a, sp.splits, item, qtiles);
+            const int u0 = uniform(it.u0), u1 = uniform(it.u1);
+            int u = next_unit(is, u0, u1);
+            if (u < u1) { ok = wait(kv_full, kc & 1); ++kc; }
+            while (ok && u < u1) {
+                const int un = next_unit(is, u + 1, u1);
                 if (!(ok = wait(full(s), ph) && wait(s_free(i & 1), (i >> 1 & 1) ^ 1))) break;
                 fence_after_sync();
                 if (elect_one()) {
@@ -544,7 +566,7 @@ dense_dkdv_tc5_kernel(const DenseArgs a, const long long wait_limit, const unsig
                     for (int j = 0; j < DP / 16; ++j)
                         mma_f16(col + 64, v_desc + (j >> 2) * (PLANE >> 4) + (j & 3) * 2, gd + (j >> 2) * (HPLANE >> 4) + (j & 3) * 2, IDESC_S, j > 0);
                     mma_commit(s_full(i & 1));
-                    if (un >= total) mma_commit(kv_empty);
+                    if (un >= u1) mma_commit(kv_empty);
                 }
                 __syncwarp();
                 if (++s == ST) { s = 0; ph ^= 1; }
@@ -564,12 +586,12 @@ dense_dkdv_tc5_kernel(const DenseArgs a, const long long wait_limit, const unsig
             if (!(ok = wait(info_full(is), (k >> 1) & 1))) break;
             const int item = uniform(items.item[is]);
             if (item < 0) break;
-            const DkvItem it(a, item, qtiles);
-            const int total = uniform(it.total);
+            const DkvItem it(a, sp.splits, item, qtiles);
+            const int u0 = uniform(it.u0), u1 = uniform(it.u1);
             bool fresh = true;
-            int u = next_unit(is, 0, total);
-            while (ok && u < total) {
-                const int un = next_unit(is, u + 1, total);
+            int u = next_unit(is, u0, u1);
+            while (ok && u < u1) {
+                const int un = next_unit(is, u + 1, u1);
                 if (!(ok = wait(d_full(i & 1), i >> 1 & 1))) break;
                 fence_after_sync();
                 if (elect_one()) {
@@ -583,7 +605,7 @@ dense_dkdv_tc5_kernel(const DenseArgs a, const long long wait_limit, const unsig
                         mma_f16_ta(tmem + COL_K, col + 64 + (j >> 1) * 32 + (j & 1) * 8, qd + j * 128, IDESC_O, (!fresh || j > 0) ? 1u : 0u);
                     mma_commit(s_free(i & 1));
                     mma_commit(empty(s));
-                    if (un >= total) mma_commit(done);       // last: the block may end after it
+                    if (un >= u1) mma_commit(done);       // last: the block may end after it
                 }
                 __syncwarp();
                 if (++s == ST) s = 0;
@@ -598,6 +620,9 @@ dense_dkdv_tc5_kernel(const DenseArgs a, const long long wait_limit, const unsig
         const int x = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane;      // warpgroup x: queries [32 x, 32 x + 32) of a tile
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
         const uint64_t c2 = pair(a.scale_log2, a.scale_log2);
+        auto part_row = [&](const DkvItem &it, int key) {
+            return sp.part + (((((int64_t)(x == 0 ? sp.splits : 0) + it.split) * a.B + it.b) * a.Lk + key) * a.Hkv + it.hk) * a.D;
+        };
         bool ok = true;
         uint32_t i = 0, kc = 0;                              // tiles, and items that had any
         int s = 0, k = 0, item = -1; uint32_t ph = 0;
@@ -607,11 +632,11 @@ dense_dkdv_tc5_kernel(const DenseArgs a, const long long wait_limit, const unsig
             if (!(ok = wait(info_full(is), (k >> 1) & 1))) break;
             item = items.item[is];
             if (item < 0) break;
-            const DkvItem it(a, item, qtiles);
+            const DkvItem it(a, sp.splits, item, qtiles);
             const int key = it.k0 + row;
             const bool tail = it.n - it.k0 < 128;
             bool any = false;
-            for (int u = next_unit(is, 0, it.total); u < it.total; u = next_unit(is, u + 1, it.total)) {
+            for (int u = next_unit(is, it.u0, it.u1); u < it.u1; u = next_unit(is, u + 1, it.u1)) {
                 uint32_t keep = 0xffffffffu;
                 bool partial = tail;
                 if (masked && flag_of(is, u) != 2) {
@@ -674,7 +699,10 @@ dense_dkdv_tc5_kernel(const DenseArgs a, const long long wait_limit, const unsig
 #pragma unroll
                     for (int j = 0; j < 32; ++j) o[j] = 0u;
                 }
-                store_rows32<T>(out, g.row_stride, a.Lk - key, 32 * c, a.D, o, x == 0 ? 1.f : a.scale);
+                if (sp.splits > 1)
+                    store_rows32_f32(part_row(it, key), (int64_t)a.Hkv * a.D, a.Lk - key, 32 * c, a.D, o);
+                else
+                    store_rows32<T>(out, g.row_stride, a.Lk - key, 32 * c, a.D, o, x == 0 ? 1.f : a.scale);
             }
             fence_before_sync();
             __syncwarp();
@@ -689,10 +717,13 @@ dense_dkdv_tc5_kernel(const DenseArgs a, const long long wait_limit, const unsig
                     item = items.item[k & 1];
                     if (item < 0) break;
                 }
-                const DkvItem it(a, item, qtiles);
-                if (it.k0 + row < a.Lk)
-                    fill_row<T>((T *)g.ptr + it.b * g.batch_stride + (int64_t)(it.k0 + row) * g.row_stride + (int64_t)it.hk * a.D, a.D,
-                                __int_as_float(0x7fffffff));
+                const DkvItem it(a, sp.splits, item, qtiles);
+                const float nan = __int_as_float(0x7fffffff);
+                const int key = it.k0 + row;
+                if (key < a.Lk && sp.splits > 1)
+                    for (int d = 0; d < a.D; ++d) part_row(it, key)[d] = nan;
+                else if (key < a.Lk)
+                    fill_row<T>((T *)g.ptr + it.b * g.batch_stride + (int64_t)key * g.row_stride + (int64_t)it.hk * a.D, a.D, nan);
                 item = -1;
             }
         }
@@ -704,27 +735,79 @@ dense_dkdv_tc5_kernel(const DenseArgs a, const long long wait_limit, const unsig
     if (threadIdx.x == 0 && *abort_flag) atomicAdd(&g_dense_bwd_aborts, 1u);
 }
 
+// out = scale * sum over the ranges, in their order
+template <typename T>
+__global__ void __launch_bounds__(256) dense_grad_join_kernel(const float *__restrict__ part, int splits, int64_t slab, hsa_view out,
+                                                             int rows, int row_elems, int64_t total, float scale) {
+    const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (i >= total) return;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int s = 0; s < splits; ++s) {
+        const float4 v = __ldg(reinterpret_cast<const float4 *>(part + s * slab + i));
+        acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
+    }
+    const int64_t row = i / row_elems;
+    T *o = (T *)out.ptr + (row / rows) * out.batch_stride + (row % rows) * out.row_stride + i % row_elems;
+    *reinterpret_cast<uint2 *>(o) = make_uint2(pack2<T>(acc.x * scale, acc.y * scale), pack2<T>(acc.z * scale, acc.w * scale));
+}
+
+// Few queries over many keys cut the keys of a dq item; few keys under many queries cut the queries of a dk/dv item.  A dq item costs
+// about three key tiles' time besides its own (seven as a partial one), a dk/dv item about six query tiles' (twelve).
+static int dq_splits(int B, int Lq, int Lk, int H) { return range_count((long long)B * H * ((Lq + 127) / 128), (Lk + 127) / 128, 3.0, 7.0); }
+static int dkdv_splits(int B, int Lq, int Lk, int H, int Hkv) {
+    const long long units = (long long)(H / Hkv) * ((Lq + 63) / 64);
+    return units > (1 << 30) ? 1 : range_count((long long)B * Hkv * ((Lk + 127) / 128), (int)units, 6.0, 12.0);
+}
+static size_t up256(size_t v) { return (v + 255) / 256 * 256; }
+
+size_t dense_bwd_tc_workspace(int B, int Lq, int Lk, int H, int Hkv, int D) {
+    const int sq = dq_splits(B, Lq, Lk, H), sk = dkdv_splits(B, Lq, Lk, H, Hkv);
+    size_t n = 0;
+    if (sq > 1) n += up256((size_t)sq * B * Lq * H * D * sizeof(float));
+    if (sk > 1) n += up256((size_t)2 * sk * B * Lk * Hkv * D * sizeof(float));
+    return n;
+}
+
 template <typename T, int DP>
-static int bwd_launch(const DenseArgs &a, cudaStream_t st) {
+static int bwd_launch(const DenseArgs &a, void *workspace, cudaStream_t st) {
     CUtensorMap mq, mq64, mk, mv, mg, mg64;
     if (!make_map(&mq, a.q, a.B, a.Lq, a.H, a.D, 1, 128) || !make_map(&mq64, a.q, a.B, a.Lq, a.H, a.D, 1, 64) ||
         !make_map(&mk, a.k, a.B, a.Lk, a.Hkv, a.D, 1, 128) || !make_map(&mv, a.v, a.B, a.Lk, a.Hkv, a.D, 1, 128) ||
         !make_map(&mg, a.dout, a.B, a.Lq, a.H, a.D, 1, 128) || !make_map(&mg64, a.dout, a.B, a.Lq, a.H, a.D, 1, 64))
         return fail(HSA_ERR_ARG, "hsa_dense_attn_bwd: the driver refused a tensor map");
-    const long long dq_blocks = (long long)a.B * a.H * ((a.Lq + 127) / 128), kv_blocks = (long long)a.B * a.Hkv * ((a.Lk + 127) / 128);
+    BwdSplit sq{}, sk{};
+    sq.splits = dq_splits(a.B, a.Lq, a.Lk, a.H);
+    sk.splits = dkdv_splits(a.B, a.Lq, a.Lk, a.H, a.Hkv);
+    sq.wait_limit = sk.wait_limit = wait_limit_cycles();
+    sq.extra_tx = sk.extra_tx = wait_extra_tx();
+    const int64_t q_elems = (int64_t)a.B * a.Lq * a.H * a.D, k_elems = (int64_t)a.B * a.Lk * a.Hkv * a.D;
+    sq.part = (float *)workspace;
+    sk.part = (float *)((char *)workspace + (sq.splits > 1 ? up256((size_t)sq.splits * q_elems * sizeof(float)) : 0));
+    const long long dq_blocks = (long long)a.B * a.H * ((a.Lq + 127) / 128) * sq.splits;
+    const long long kv_blocks = (long long)a.B * a.Hkv * ((a.Lk + 127) / 128) * sk.splits;
     if (dq_blocks > 0x7fffffffLL || kv_blocks > 0x7fffffffLL) return fail(HSA_ERR_ARG, "hsa_dense_attn_bwd: too many tiles");
-    const long long limit = wait_limit_cycles();
-    const unsigned int extra = wait_extra_tx();
     constexpr auto kdq = dense_dq_tc5_kernel<T, DP>;
     constexpr auto kkv = dense_dkdv_tc5_kernel<T, DP>;
     constexpr int smem_dq = DqShape<DP>::kSmem, smem_kv = DkvShape<DP>::kSmem;
     cudaError_t e = allow_smem<kdq>(smem_dq);
     if (e == cudaSuccess) e = allow_smem<kkv>(smem_kv);
     if (e != cudaSuccess) return fail((int)e, "hsa_dense_attn_bwd: shared memory %d / %d: %s", smem_dq, smem_kv, cudaGetErrorString(e));
-    kkv<<<(unsigned)kv_blocks, kBwdThreads, smem_kv, st>>>(a, limit, extra, mq64, mk, mv, mg64);
+    kkv<<<(unsigned)kv_blocks, kBwdThreads, smem_kv, st>>>(a, sk, mq64, mk, mv, mg64);
     if (int rc = launch_status("hsa_dense_attn_bwd(dk, dv)")) return rc;
-    kdq<<<(unsigned)dq_blocks, kBwdThreads, smem_dq, st>>>(a, limit, extra, mq, mk, mv, mg);
-    return launch_status("hsa_dense_attn_bwd(dq)");
+    kdq<<<(unsigned)dq_blocks, kBwdThreads, smem_dq, st>>>(a, sq, mq, mk, mv, mg);
+    if (int rc = launch_status("hsa_dense_attn_bwd(dq)")) return rc;
+    auto join = [&](const float *part, int splits, int64_t elems, const hsa_view &out, int rows, int heads, float scale) -> int {
+        dense_grad_join_kernel<T><<<(unsigned)((elems / 4 + 255) / 256), 256, 0, st>>>(part, splits, elems, out, rows, heads * a.D, elems, scale);
+        return launch_status("hsa_dense_attn_bwd(join)");
+    };
+    if (sq.splits > 1)
+        if (int rc = join(sq.part, sq.splits, q_elems, a.dq, a.Lq, a.H, a.scale)) return rc;
+    if (sk.splits > 1) {
+        if (int rc = join(sk.part, sk.splits, k_elems, a.dk, a.Lk, a.Hkv, a.scale)) return rc;
+        return join(sk.part + sk.splits * k_elems, sk.splits, k_elems, a.dv, a.Lk, a.Hkv, 1.f);
+    }
+    return 0;
 }
 
 // Whether the mask's tile states fit a block's table on both sides.
@@ -732,9 +815,9 @@ bool dense_bwd_tables_ok(const DenseArgs &a) {
     return a.mask.bits == nullptr || (a.mask.tk <= kFlagTiles && (long long)a.group * a.mask.tq <= kFlagTiles);
 }
 
-int dense_bwd_tc(const DenseArgs &a, int dtype, cudaStream_t st) {
-    if (dtype == HSA_BF16) return a.D <= 64 ? bwd_launch<__nv_bfloat16, 64>(a, st) : bwd_launch<__nv_bfloat16, 128>(a, st);
-    return a.D <= 64 ? bwd_launch<__half, 64>(a, st) : bwd_launch<__half, 128>(a, st);
+int dense_bwd_tc(const DenseArgs &a, void *workspace, int dtype, cudaStream_t st) {
+    if (dtype == HSA_BF16) return a.D <= 64 ? bwd_launch<__nv_bfloat16, 64>(a, workspace, st) : bwd_launch<__nv_bfloat16, 128>(a, workspace, st);
+    return a.D <= 64 ? bwd_launch<__half, 64>(a, workspace, st) : bwd_launch<__half, 128>(a, workspace, st);
 }
 
 cudaError_t dense_bwd_aborts(unsigned int *count) { return cudaMemcpyFromSymbol(count, g_dense_bwd_aborts, sizeof(unsigned int)); }

@@ -427,19 +427,7 @@ dense_fwd_tc5_kernel(const DenseArgs a, const DenseSplit sp, const __grid_consta
                         for (int j = 0; j < 32; ++j) o[j] = 0u;
                     }
                     if (sp.splits > 1) {
-                        const int quad = lane & 3;
-#pragma unroll
-                        for (int g = 0; g < 2; ++g) {                // 16 columns are four pieces of 32-bit numbers
-                            uint4 p[4];
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) p[j] = make_uint4(o[16 * g + 4 * j], o[16 * g + 4 * j + 1], o[16 * g + 4 * j + 2], o[16 * g + 4 * j + 3]);
-                            quad_pieces(p, quad);
-                            const int col = 32 * c + 16 * g + 4 * quad;
-#pragma unroll
-                            for (int j = 0; j < 4; ++j)
-                                if (qi + j - quad < a.Lq && col < a.D)
-                                    *reinterpret_cast<uint4 *>(sp.part_o + (at + (int64_t)(j - quad) * a.H) * a.D + col) = p[j];
-                        }
+                        store_rows32_f32(sp.part_o + at * a.D, (int64_t)a.H * a.D, a.Lq - qi, 32 * c, a.D, o);
                     } else {
                         store_rows32<T>(orow, a.out.row_stride, a.Lq - qi, 32 * c, a.D, o, inv);
                     }
@@ -518,21 +506,9 @@ __global__ void __launch_bounds__(128) dense_join_kernel(const DenseArgs a, cons
     if (a.lse != nullptr && lane == 0) a.lse[row] = none ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
 }
 
-// Ranges of keys per query block: with few blocks and many key tiles, the count that makes the slowest SM finish first.  A block
-// costs its tiles plus about four tiles' time of set-up and result (twice that when the result is a partial one that is joined).
+// A block of queries costs its key tiles plus about four tiles' time of set-up and result, twice that when the result is partial.
 int dense_fwd_splits(int B, int Lq, int Lk, int H) {
-    const long long blocks = (long long)B * H * ((Lq + 255) / 256);
-    const int tiles = (Lk + 127) / 128, sms = dense_sm_count();
-    if (blocks * 2 > sms) return 1;
-    double best = 1e30;
-    int best_s = 1;
-    for (int s = 1; s <= 64 && s <= tiles; ++s) {
-        const double waves = (double)((blocks * s + sms - 1) / sms);
-        const double t = waves * ((tiles + s - 1) / s + (s > 1 ? 8.0 : 4.0)) + (s > 1 ? 4.0 : 0.0);
-        if (t < 0.95 * best) { best = t; best_s = s; }
-    }
-    const int per = (tiles + best_s - 1) / best_s;
-    return (tiles + per - 1) / per;
+    return range_count((long long)B * H * ((Lq + 255) / 256), (Lk + 127) / 128, 4.0, 8.0);
 }
 
 size_t dense_fwd_tc_workspace(int B, int Lq, int Lk, int H, int D) {

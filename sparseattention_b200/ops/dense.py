@@ -148,14 +148,15 @@ def dense_attention_backward(q, k, v, out, lse, dout, key_lengths=None, packed_m
     dq = torch.empty((B, Lq, H, D), dtype=q.dtype, device=dev)
     dk = torch.empty((B, Lk, Hkv, D), dtype=q.dtype, device=dev)
     dv = torch.empty((B, Lk, Hkv, D), dtype=q.dtype, device=dev)
-    need = lib.hsa_dense_attn_bwd_workspace_bytes(B, Lq, H)
+    dt = _lib.dtype_code(q)
+    need = lib.hsa_dense_attn_bwd_workspace_bytes(B, Lq, Lk, H, Hkv, D, dt, algo)
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
     rs, ks = H * D, Hkv * D
     view = _lib.HsaView
     rc = lib.hsa_dense_attn_bwd(_view(q), _view(k), _view(v), view(out.data_ptr(), Lq * rs, rs), _ptr(lse), _view(dout),
                                 view(dq.data_ptr(), Lq * rs, rs), view(dk.data_ptr(), Lk * ks, ks), view(dv.data_ptr(), Lk * ks, ks),
                                 _ptr(key_lengths), *_mask_args(packed_mask), _ptr(ws), need, B, Lq, Lk, H, Hkv, D, scale,
-                                _lib.dtype_code(q), algo, _lib.stream_ptr(dev))
+                                dt, algo, _lib.stream_ptr(dev))
     if rc:
         _lib.check(rc, "hsa_dense_attn_bwd")
     if _lib.DEBUG:

@@ -132,7 +132,7 @@ def check(q, k, v, g, key_lengths=None, mask=None, scale=None, algo=0, empty_val
 
 SHAPES = [(1, 1, 1, 1, 1, 8), (2, 3, 5, 2, 1, 10), (1, 16, 77, 8, 8, 64), (2, 130, 129, 4, 2, 64), (1, 128, 128, 2, 2, 32),
           (2, 257, 300, 4, 4, 128), (3, 65, 127, 6, 2, 96), (1, 300, 1000, 2, 2, 80), (2, 33, 70, 2, 1, 256), (1, 5, 20, 3, 1, 200),
-          (2, 1, 259, 4, 4, 64), (1, 513, 1, 2, 1, 128), (1, 70, 640, 3, 3, 24), (1, 256, 385, 8, 1, 72), (2, 64, 64, 1, 1, 17)]
+          (2, 1, 259, 4, 4, 64), (1, 513, 1, 2, 1, 128), (1, 40, 6000, 2, 1, 64), (1, 5000, 70, 4, 2, 128), (1, 70, 640, 3, 3, 24), (1, 256, 385, 8, 1, 72), (2, 64, 64, 1, 1, 17)]
 
 
 @pytest.mark.parametrize("shape", SHAPES)
