@@ -409,8 +409,8 @@ int hsa_cross_entropy_bwd_inplace(void *logits, long long row_stride, const long
  *   query of a mask's plane may look at, reaches no result (it may be NaN); keys that some queries see and others do not
  *   must be finite, as must Q and dOut in the backward.
  *   LSE, if not NULL, receives the log-sum-exp [B, Lq, H] float32 that the backward needs.
- *   scale > 0.  D <= 256.  `algo`: 0 = automatic, 1 = CUDA cores, 2 = tensor cores (bf16 / f16, D a multiple of 8 up to 128,
- *   16-byte aligned rows; HSA_ERR_ARG otherwise).  `workspace`: hsa_dense_attn_fwd_workspace_bytes(...) bytes (often 0; few
+ *   scale > 0.  D <= 256.  `algo`: 0 = automatic, 1 = 32-bit kernels (any type), 2 = tcgen05 kernels (bf16 / f16, D a multiple of
+ *   8 up to 128, 16-byte aligned rows; HSA_ERR_ARG otherwise).  `workspace`: hsa_dense_attn_fwd_workspace_bytes(...) bytes (often 0; few
  *   queries over many keys are cut into ranges of keys that are joined afterwards), 256-byte aligned.
  * Masks come packed (hsa_dense_mask_pack): `mask` points to bytes (0 = may not look), four strides in bytes, of a tensor
  *   [batches, heads, rows, Lk] with batches 1 or B, heads 1 or H, rows 1 or Lq; `packed` receives

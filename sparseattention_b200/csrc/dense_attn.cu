@@ -3,13 +3,16 @@
 
 namespace hsa {
 
-int dense_simt(const DenseArgs &a, int what, int dtype, cudaStream_t st);
+int dense_fwd_f32(const DenseArgs &a, void *workspace, int dtype, cudaStream_t st);
+int dense_bwd_f32(const DenseArgs &a, void *workspace, int dtype, cudaStream_t st);
+size_t dense_fwd_f32_workspace(int B, int Lq, int Lk, int H, int D);
+size_t dense_bwd_f32_workspace(int B, int Lq, int Lk, int H, int Hkv, int D);
 bool dense_tc_ok(const DenseArgs &a, int dtype, bool backward);
 size_t dense_fwd_tc_workspace(int B, int Lq, int Lk, int H, int D);
 bool dense_bwd_tables_ok(const DenseArgs &a);
 size_t dense_bwd_tc_workspace(int B, int Lq, int Lk, int H, int Hkv, int D);
 int dense_bwd_tc(const DenseArgs &a, void *workspace, int dtype, cudaStream_t st);
-int dense_fwd_tc(const DenseArgs &a, void *workspace, size_t workspace_bytes, int dtype, cudaStream_t st);
+int dense_fwd_tc(const DenseArgs &a, void *workspace, int dtype, cudaStream_t st);
 
 // ------------------------------------------------------------------------------------------------------------ mask
 // One block per 128 x 128 cell of a plane, a warp per 32 x 32 piece: 32 coalesced row reads turn into words by ballot, 32 more
@@ -148,9 +151,14 @@ extern "C" int hsa_dense_mask_pack(const void *mask, int64_t stride_b, int64_t s
     return launch_status("hsa_dense_mask_pack");
 }
 
+// The tcgen05 kernels may turn inputs down for their alignment as well, so the room is that of whichever kernels need more.
+static bool tc_shape(int D, int dtype, int algo) { return D <= 128 && D % 8 == 0 && algo != 1 && dtype != HSA_F32; }
+
 extern "C" size_t hsa_dense_attn_fwd_workspace_bytes(int B, int Lq, int Lk, int H, int Hkv, int D, int dtype, int algo) {
-    if (B < 1 || Lq < 1 || Lk < 1 || H < 1 || Hkv < 1 || D < 1 || D > 128 || D % 8 != 0 || algo == 1 || dtype == HSA_F32) return 0;
-    return dense_fwd_tc_workspace(B, Lq, Lk, H, D);
+    if (B < 1 || Lq < 1 || Lk < 1 || H < 1 || Hkv < 1 || D < 1) return 0;
+    const size_t f32 = algo != 2 ? dense_fwd_f32_workspace(B, Lq, Lk, H, D) : 0;
+    const size_t tc = tc_shape(D, dtype, algo) ? dense_fwd_tc_workspace(B, Lq, Lk, H, D) : 0;
+    return f32 > tc ? f32 : tc;
 }
 
 extern "C" int hsa_dense_attn_fwd(hsa_view Q, hsa_view K, hsa_view V, hsa_view Out, float *LSE, const int *key_lengths,
@@ -172,11 +180,15 @@ extern "C" int hsa_dense_attn_fwd(hsa_view Q, hsa_view K, hsa_view V, hsa_view O
     const int es = dtype_size(dtype);
     a.vec = D % 4 == 0;
     for (const hsa_view &v : {Q, K, V, Out}) a.vec = a.vec && rows_in_fours(v, es);
-    // The tensor-core kernel wherever its layout rules allow it: it is ahead of the CUDA-core kernel from the smallest call on
+    // The tensor-core kernel wherever its layout rules allow it: it is ahead of the 32-bit kernel from the smallest call on
     // (16 x 77, 8 heads of 64: both are bound by the launch) and 40 times as fast at 4096 x 4096.
-    if (algo != 1 && dense_tc_ok(a, dtype, false)) return dense_fwd_tc(a, workspace, workspace_bytes, dtype, (cudaStream_t)stream);
+    const size_t need = hsa_dense_attn_fwd_workspace_bytes(B, Lq, Lk, H, Hkv, D, dtype, algo);
+    if (need && (workspace == nullptr || workspace_bytes < need))
+        return fail(HSA_ERR_WORKSPACE, "hsa_dense_attn_fwd: workspace of %zu bytes needed, %zu given", need, workspace_bytes);
+    if (reinterpret_cast<uintptr_t>(workspace) & 255u) return fail(HSA_ERR_ALIGN, "hsa_dense_attn_fwd: workspace must be 256-byte aligned");
+    if (algo != 1 && dense_tc_ok(a, dtype, false)) return dense_fwd_tc(a, workspace, dtype, (cudaStream_t)stream);
     HSA_CHECK_ARG(algo != 2, "hsa_dense_attn_fwd: no tensor-core kernel for these inputs");
-    return dense_simt(a, 0, dtype, (cudaStream_t)stream);
+    return dense_fwd_f32(a, workspace, dtype, (cudaStream_t)stream);
 }
 
 // Row sums and log-sum-exps of the padded rows, then what the tensor-core kernels keep of partial gradients
@@ -184,9 +196,9 @@ static size_t bwd_stats_bytes(int B, int Lq, int H) { return (size_t)2 * B * H *
 
 extern "C" size_t hsa_dense_attn_bwd_workspace_bytes(int B, int Lq, int Lk, int H, int Hkv, int D, int dtype, int algo) {
     if (B < 1 || Lq < 1 || Lk < 1 || H < 1 || Hkv < 1 || H % Hkv != 0 || D < 1) return 0;
-    size_t n = bwd_stats_bytes(B, Lq, H);
-    if (D <= 128 && D % 8 == 0 && algo != 1 && dtype != HSA_F32) n += dense_bwd_tc_workspace(B, Lq, Lk, H, Hkv, D);
-    return n;
+    const size_t f32 = algo != 2 ? dense_bwd_f32_workspace(B, Lq, Lk, H, Hkv, D) : 0;
+    const size_t tc = tc_shape(D, dtype, algo) ? dense_bwd_tc_workspace(B, Lq, Lk, H, Hkv, D) : 0;
+    return bwd_stats_bytes(B, Lq, H) + (f32 > tc ? f32 : tc);
 }
 
 extern "C" int hsa_dense_attn_bwd(hsa_view Q, hsa_view K, hsa_view V, hsa_view Out, const float *LSE, hsa_view dOut, hsa_view dQ,
@@ -219,7 +231,6 @@ extern "C" int hsa_dense_attn_bwd(hsa_view Q, hsa_view K, hsa_view V, hsa_view O
     HSA_CHECK_ARG(algo != 2 || tc, "hsa_dense_attn_bwd: no tensor-core kernel for these inputs");
     cudaStream_t st = (cudaStream_t)stream;
     if (int rc = dense_delta(a, neg_lse2, neg_delta, dtype, D % (16 / es) == 0 && view_vec_ok(Out, es) && view_vec_ok(dOut, es), st)) return rc;
-    if (tc) return dense_bwd_tc(a, (char *)workspace + bwd_stats_bytes(B, Lq, H), dtype, st);
-    if (int rc = dense_simt(a, 1, dtype, st)) return rc;
-    return dense_simt(a, 2, dtype, st);
+    void *rest = (char *)workspace + bwd_stats_bytes(B, Lq, H);
+    return tc ? dense_bwd_tc(a, rest, dtype, st) : dense_bwd_f32(a, rest, dtype, st);
 }

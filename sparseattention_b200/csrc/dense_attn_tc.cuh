@@ -1,30 +1,12 @@
 // Pieces shared by the tensor-core kernels of dense attention.
 #pragma once
 
-#include "dense_attn.cuh"
+#include "dense_attn_split.cuh"
 #include "tc5_common.cuh"
-#include "tc_common.cuh"
-#include "tma_common.cuh"
 
 namespace hsa {
 
 constexpr int kFlagTiles = 768;                  // tiles whose mask state fits one of a block's two tables
-// Ranges per work item when there are few items and each is long: the count that lets the slowest SM finish first.  `steps` tiles per
-// item; an item costs `once` tiles' time besides, `once_split` as one of several ranges, whose partial results are then joined.
-inline int range_count(long long items, int steps, double once, double once_split) {
-    const int sms = dense_sm_count();
-    if (items * 2 > sms) return 1;
-    double best = 1e30;
-    int best_s = 1;
-    for (int s = 1; s <= 64 && s <= steps; ++s) {
-        const double waves = (double)((items * s + sms - 1) / sms);
-        const double t = waves * ((steps + s - 1) / s + (s > 1 ? once_split : once)) + (s > 1 ? once : 0.0);
-        if (t < 0.95 * best) { best = t; best_s = s; }
-    }
-    const int per = (steps + best_s - 1) / best_s;
-    return (steps + per - 1) / per;
-}
-
 // Two 32-bit numbers in a register pair: one instruction for both
 __device__ __forceinline__ uint64_t pair(float lo, float hi) {
     uint64_t v;

@@ -24,13 +24,6 @@ constexpr int kBwdThreads = 352;                 // eight element-wise warps, co
 
 __device__ unsigned int g_dense_bwd_aborts = 0;
 
-struct BwdSplit {
-    float *part;                                 // partial gradients, [splits][B, rows, heads, D] 32-bit (dk before dv), when splits > 1
-    int splits;
-    unsigned int extra_tx;                       // test hook: bytes that the first copy is announced with and never brings
-    long long wait_limit;
-};
-
 // ------------------------------------------------------------------------------------------------------------------ dq
 template <int DP>
 struct DqShape {
@@ -735,23 +728,6 @@ dense_dkdv_tc5_kernel(const DenseArgs a, const BwdSplit sp, const __grid_constan
     if (threadIdx.x == 0 && *abort_flag) atomicAdd(&g_dense_bwd_aborts, 1u);
 }
 
-// out = scale * sum over the ranges, in their order
-template <typename T>
-__global__ void __launch_bounds__(256) dense_grad_join_kernel(const float *__restrict__ part, int splits, int64_t slab, hsa_view out,
-                                                             int rows, int row_elems, int64_t total, float scale) {
-    const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
-    if (i >= total) return;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int s = 0; s < splits; ++s) {
-        const float4 v = __ldg(reinterpret_cast<const float4 *>(part + s * slab + i));
-        acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
-    }
-    const int64_t row = i / row_elems;
-    T *o = (T *)out.ptr + (row / rows) * out.batch_stride + (row % rows) * out.row_stride + i % row_elems;
-    *reinterpret_cast<uint2 *>(o) = make_uint2(pack2<T>(acc.x * scale, acc.y * scale), pack2<T>(acc.z * scale, acc.w * scale));
-}
-
 // Few queries over many keys cut the keys of a dq item; few keys under many queries cut the queries of a dk/dv item.  A dq item costs
 // about three key tiles' time besides its own (seven as a partial one), a dk/dv item about six query tiles' (twelve).
 static int dq_splits(int B, int Lq, int Lk, int H) { return range_count((long long)B * H * ((Lq + 127) / 128), (Lk + 127) / 128, 3.0, 7.0); }
@@ -759,14 +735,9 @@ static int dkdv_splits(int B, int Lq, int Lk, int H, int Hkv) {
     const long long units = (long long)(H / Hkv) * ((Lq + 63) / 64);
     return units > (1 << 30) ? 1 : range_count((long long)B * Hkv * ((Lk + 127) / 128), (int)units, 6.0, 12.0);
 }
-static size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 
 size_t dense_bwd_tc_workspace(int B, int Lq, int Lk, int H, int Hkv, int D) {
-    const int sq = dq_splits(B, Lq, Lk, H), sk = dkdv_splits(B, Lq, Lk, H, Hkv);
-    size_t n = 0;
-    if (sq > 1) n += up256((size_t)sq * B * Lq * H * D * sizeof(float));
-    if (sk > 1) n += up256((size_t)2 * sk * B * Lk * Hkv * D * sizeof(float));
-    return n;
+    return bwd_part_bytes(dq_splits(B, Lq, Lk, H), dkdv_splits(B, Lq, Lk, H, Hkv), B, Lq, Lk, H, Hkv, D);
 }
 
 template <typename T, int DP>
@@ -776,14 +747,8 @@ static int bwd_launch(const DenseArgs &a, void *workspace, cudaStream_t st) {
         !make_map(&mk, a.k, a.B, a.Lk, a.Hkv, a.D, 1, 128) || !make_map(&mv, a.v, a.B, a.Lk, a.Hkv, a.D, 1, 128) ||
         !make_map(&mg, a.dout, a.B, a.Lq, a.H, a.D, 1, 128) || !make_map(&mg64, a.dout, a.B, a.Lq, a.H, a.D, 1, 64))
         return fail(HSA_ERR_ARG, "hsa_dense_attn_bwd: the driver refused a tensor map");
-    BwdSplit sq{}, sk{};
-    sq.splits = dq_splits(a.B, a.Lq, a.Lk, a.H);
-    sk.splits = dkdv_splits(a.B, a.Lq, a.Lk, a.H, a.Hkv);
-    sq.wait_limit = sk.wait_limit = wait_limit_cycles();
-    sq.extra_tx = sk.extra_tx = wait_extra_tx();
-    const int64_t q_elems = (int64_t)a.B * a.Lq * a.H * a.D, k_elems = (int64_t)a.B * a.Lk * a.Hkv * a.D;
-    sq.part = (float *)workspace;
-    sk.part = (float *)((char *)workspace + (sq.splits > 1 ? up256((size_t)sq.splits * q_elems * sizeof(float)) : 0));
+    BwdSplit sq, sk;
+    bwd_splits(dq_splits(a.B, a.Lq, a.Lk, a.H), dkdv_splits(a.B, a.Lq, a.Lk, a.H, a.Hkv), a, workspace, sq, sk);
     const long long dq_blocks = (long long)a.B * a.H * ((a.Lq + 127) / 128) * sq.splits;
     const long long kv_blocks = (long long)a.B * a.Hkv * ((a.Lk + 127) / 128) * sk.splits;
     if (dq_blocks > 0x7fffffffLL || kv_blocks > 0x7fffffffLL) return fail(HSA_ERR_ARG, "hsa_dense_attn_bwd: too many tiles");
@@ -797,17 +762,7 @@ static int bwd_launch(const DenseArgs &a, void *workspace, cudaStream_t st) {
     if (int rc = launch_status("hsa_dense_attn_bwd(dk, dv)")) return rc;
     kdq<<<(unsigned)dq_blocks, kBwdThreads, smem_dq, st>>>(a, sq, mq, mk, mv, mg);
     if (int rc = launch_status("hsa_dense_attn_bwd(dq)")) return rc;
-    auto join = [&](const float *part, int splits, int64_t elems, const hsa_view &out, int rows, int heads, float scale) -> int {
-        dense_grad_join_kernel<T><<<(unsigned)((elems / 4 + 255) / 256), 256, 0, st>>>(part, splits, elems, out, rows, heads * a.D, elems, scale);
-        return launch_status("hsa_dense_attn_bwd(join)");
-    };
-    if (sq.splits > 1)
-        if (int rc = join(sq.part, sq.splits, q_elems, a.dq, a.Lq, a.H, a.scale)) return rc;
-    if (sk.splits > 1) {
-        if (int rc = join(sk.part, sk.splits, k_elems, a.dk, a.Lk, a.Hkv, a.scale)) return rc;
-        return join(sk.part + sk.splits * k_elems, sk.splits, k_elems, a.dv, a.Lk, a.Hkv, 1.f);
-    }
-    return 0;
+    return join_backward<T>(a, sq, sk, st);
 }
 
 // Whether the mask's tile states fit a block's table on both sides.

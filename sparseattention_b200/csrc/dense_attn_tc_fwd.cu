@@ -28,13 +28,6 @@ __device__ unsigned int g_dense_aborts = 0;
 // its registers go to the softmax (2 x 128 x 200 + 128 x 104 = 384 x 168, what the block is launched with).
 constexpr int kFwdThreads = 384;
 
-struct DenseSplit {
-    float *part_o, *part_ml;                     // [splits, B, Lq, H, D] and [splits, B, Lq, H, 2] when splits > 1
-    int splits;
-    unsigned int extra_tx;                       // test hook: bytes that the first copy is announced with and never brings
-    long long wait_limit;
-};
-
 template <int DP>
 struct FwdShape {
     static constexpr int kTile = 128 * DP * 2;                       // bytes of a tile of 128 rows
@@ -473,48 +466,12 @@ dense_fwd_tc5_kernel(const DenseArgs a, const DenseSplit sp, const __grid_consta
     if (threadIdx.x == 0 && *abort_flag) atomicAdd(&g_dense_aborts, 1u);
 }
 
-// Join the ranges of a query row: out = sum 2^(m_s - M) o_s / sum 2^(m_s - M) l_s.
-template <typename T>
-__global__ void __launch_bounds__(128) dense_join_kernel(const DenseArgs a, const DenseSplit sp) {
-    const int64_t rows = (int64_t)a.B * a.Lq * a.H, row = blockIdx.x * 4LL + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31;
-    if (row >= rows) return;
-    float M = -INFINITY;
-    for (int s = 0; s < sp.splits; ++s) M = fmaxf(M, sp.part_ml[2 * (s * rows + row)]);
-    const float ref = M == -INFINITY ? 0.f : M;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    float L = 0.f;
-    for (int s = 0; s < sp.splits; ++s) {
-        const int64_t at = s * rows + row;
-        const float w = exp2f(sp.part_ml[2 * at] - ref);
-        L = fmaf(w, sp.part_ml[2 * at + 1], L);
-        if (lane * 4 < a.D) {
-            const float4 o = *reinterpret_cast<const float4 *>(sp.part_o + at * a.D + lane * 4);
-            acc.x = fmaf(w, o.x, acc.x); acc.y = fmaf(w, o.y, acc.y); acc.z = fmaf(w, o.z, acc.z); acc.w = fmaf(w, o.w, acc.w);
-        }
-    }
-    const int h = (int)(row % a.H), i = (int)(row / a.H % a.Lq);
-    const int64_t b = row / a.H / a.Lq;
-    const bool none = L == 0.f;
-    const float inv = 1.f / L;
-    if (lane * 4 < a.D) {
-        uint2 v;
-        v.x = none ? pack2<T>(a.empty_value, a.empty_value) : pack2<T>(acc.x * inv, acc.y * inv);
-        v.y = none ? pack2<T>(a.empty_value, a.empty_value) : pack2<T>(acc.z * inv, acc.w * inv);
-        *reinterpret_cast<uint2 *>((T *)a.out.ptr + b * a.out.batch_stride + (int64_t)i * a.out.row_stride + (int64_t)h * a.D + lane * 4) = v;
-    }
-    if (a.lse != nullptr && lane == 0) a.lse[row] = none ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
-}
-
 // A block of queries costs its key tiles plus about four tiles' time of set-up and result, twice that when the result is partial.
-int dense_fwd_splits(int B, int Lq, int Lk, int H) {
+static int dense_fwd_splits(int B, int Lq, int Lk, int H) {
     return range_count((long long)B * H * ((Lq + 255) / 256), (Lk + 127) / 128, 4.0, 8.0);
 }
 
-size_t dense_fwd_tc_workspace(int B, int Lq, int Lk, int H, int D) {
-    const int s = dense_fwd_splits(B, Lq, Lk, H);
-    return s > 1 ? (size_t)s * B * Lq * H * (D + 2) * sizeof(float) : 0;
-}
+size_t dense_fwd_tc_workspace(int B, int Lq, int Lk, int H, int D) { return fwd_part_bytes(dense_fwd_splits(B, Lq, Lk, H), B, Lq, H, D); }
 
 static bool tc_view(const hsa_view &v, int B, int rows, int H, int D) { return view_vec_ok(v, 2) && map_ok(v, B, rows, H, D); }
 
@@ -543,25 +500,11 @@ static int fwd_launch(const DenseArgs &a, DenseSplit sp, cudaStream_t st) {
     if (e != cudaSuccess) return fail((int)e, "hsa_dense_attn_fwd: shared memory %d: %s", smem, cudaGetErrorString(e));
     kernel<<<(unsigned)blocks, kFwdThreads, smem, st>>>(a, sp, mq, mk, mv);
     if (int rc = launch_status("hsa_dense_attn_fwd")) return rc;
-    if (sp.splits == 1) return 0;
-    const long long rows = (long long)a.B * a.Lq * a.H;
-    dense_join_kernel<T><<<(unsigned)((rows + 3) / 4), 128, 0, st>>>(a, sp);
-    return launch_status("hsa_dense_attn_fwd(join)");
+    return sp.splits > 1 ? join_forward<T>(a, sp, st) : 0;
 }
 
-int dense_fwd_tc(const DenseArgs &a, void *workspace, size_t workspace_bytes, int dtype, cudaStream_t st) {
-    DenseSplit sp{};
-    sp.splits = dense_fwd_splits(a.B, a.Lq, a.Lk, a.H);
-    sp.wait_limit = wait_limit_cycles();
-    sp.extra_tx = wait_extra_tx();
-    if (sp.splits > 1) {
-        const size_t need = dense_fwd_tc_workspace(a.B, a.Lq, a.Lk, a.H, a.D);
-        if (workspace == nullptr || workspace_bytes < need)
-            return fail(HSA_ERR_WORKSPACE, "hsa_dense_attn_fwd: workspace of %zu bytes needed, %zu given", need, workspace_bytes);
-        if (reinterpret_cast<uintptr_t>(workspace) & 255u) return fail(HSA_ERR_ALIGN, "hsa_dense_attn_fwd: workspace must be 256-byte aligned");
-        sp.part_o = (float *)workspace;
-        sp.part_ml = sp.part_o + (size_t)sp.splits * a.B * a.Lq * a.H * a.D;
-    }
+int dense_fwd_tc(const DenseArgs &a, void *workspace, int dtype, cudaStream_t st) {
+    const DenseSplit sp = fwd_split(dense_fwd_splits(a.B, a.Lq, a.Lk, a.H), a, workspace);
     if (dtype == HSA_BF16)
         return a.D <= 64 ? fwd_launch<__nv_bfloat16, 64>(a, sp, st) : fwd_launch<__nv_bfloat16, 128>(a, sp, st);
     return a.D <= 64 ? fwd_launch<__half, 64>(a, sp, st) : fwd_launch<__half, 128>(a, sp, st);

@@ -8,6 +8,7 @@ Softmax statistics and sums are float32; the backward is deterministic (one writ
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 from ctypes import c_void_p
 from typing import NamedTuple, Optional, Tuple
@@ -88,6 +89,24 @@ def _check_inputs(q, k, v):
     return dev
 
 
+@functools.lru_cache(maxsize=1024)
+def _fwd_workspace(*sizes) -> int:
+    return int(_lib.load().hsa_dense_attn_fwd_workspace_bytes(*sizes[:-1]))          # the last one is the device
+
+
+@functools.lru_cache(maxsize=1024)
+def _bwd_workspace(*sizes) -> int:
+    return int(_lib.load().hsa_dense_attn_bwd_workspace_bytes(*sizes[:-1]))
+
+
+@functools.lru_cache(maxsize=1024)
+def _paged_plan(B, H, Hkv, D, page_size, max_pages, splits, device):
+    lib = _lib.load()
+    if splits is None:
+        splits = lib.hsa_paged_attn_choose_splits(B, H, Hkv, page_size, max_pages)
+    return splits, int(lib.hsa_paged_attn_workspace_bytes(B, H, D, splits))
+
+
 def _lengths32(lengths, B: int, top: int, dev, name: str):
     if lengths.dtype not in (torch.int32, torch.int64):
         raise _lib.HsaError(f"{name} must be int32 or int64")
@@ -125,7 +144,7 @@ def dense_attention_forward(q, k, v, key_lengths=None, packed_mask=None, scale: 
     out = torch.empty((B, Lq, H, D), dtype=q.dtype, device=dev)
     lse = torch.empty((B, Lq, H), dtype=torch.float32, device=dev) if need_lse else None
     dt = _lib.dtype_code(q)
-    need = lib.hsa_dense_attn_fwd_workspace_bytes(B, Lq, Lk, H, Hkv, D, dt, algo)
+    need = _fwd_workspace(B, Lq, Lk, H, Hkv, D, dt, algo, dev.index)
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     rs = H * D
     rc = lib.hsa_dense_attn_fwd(_view(q), _view(k), _view(v), _lib.HsaView(out.data_ptr(), Lq * rs, rs), _ptr(lse), _ptr(key_lengths),
@@ -149,7 +168,7 @@ def dense_attention_backward(q, k, v, out, lse, dout, key_lengths=None, packed_m
     dk = torch.empty((B, Lk, Hkv, D), dtype=q.dtype, device=dev)
     dv = torch.empty((B, Lk, Hkv, D), dtype=q.dtype, device=dev)
     dt = _lib.dtype_code(q)
-    need = lib.hsa_dense_attn_bwd_workspace_bytes(B, Lq, Lk, H, Hkv, D, dt, algo)
+    need = _bwd_workspace(B, Lq, Lk, H, Hkv, D, dt, algo, dev.index)
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
     rs, ks = H * D, Hkv * D
     view = _lib.HsaView
@@ -281,7 +300,7 @@ def paged_attention_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     assert page_table.dtype == torch.int32 and lengths.dtype == torch.int32, "page_table and lengths are int32"
     assert page_table.dim() == 2 and page_table.size(0) == B and lengths.shape == (B,), \
         f"page_table is [{B}, max_pages] and lengths [{B}]"
-    if not (_lib.inner_contiguous(k_pages) and _lib.inner_contiguous(v_pages)):
+    if not ((k_pages.is_contiguous() or _lib.inner_contiguous(k_pages)) and (v_pages.is_contiguous() or _lib.inner_contiguous(v_pages))):
         raise _lib.HsaError("a slot's [Hkv, D] block must be packed (the cache is not copied)")
     if scale is None:
         scale = D ** -0.5
@@ -294,18 +313,19 @@ def paged_attention_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     if max_pages == 0 or num_pages == 0 or page_size == 0:
         # no cache: every length has to be 0 (a table without room for a longer one gives NaN, as below)
         return out.copy_(torch.where(lengths.view(B, 1, 1) == 0, 0.0, math.nan).expand(B, H, D))
-    q = q.contiguous()
+    if not q.is_contiguous():
+        q = q.contiguous()
     if page_table.stride(1) != 1 and max_pages > 1:
         page_table = page_table.contiguous()
-    lengths = lengths.contiguous()
+    if not lengths.is_contiguous():
+        lengths = lengths.contiguous()
     with _lib.on_device(dev):
-        if splits is None:
-            splits = lib.hsa_paged_attn_choose_splits(B, H, Hkv, page_size, max_pages)
-        need = lib.hsa_paged_attn_workspace_bytes(B, H, D, splits)
+        splits, need = _paged_plan(B, H, Hkv, D, page_size, max_pages, splits, dev.index)
         ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
         rc = lib.hsa_paged_attn_decode(_lib.HsaView(q.data_ptr(), H * D, H * D), _lib.rows_view(k_pages), _lib.rows_view(v_pages),
                                        _lib.HsaView(out.data_ptr(), H * D, H * D), c_void_p(page_table.data_ptr()),
                                        page_table.stride(0), c_void_p(lengths.data_ptr()), _ptr(ws), need, B, H, Hkv, D,
                                        page_size, num_pages, max_pages, float(scale), dt, splits, algo, _lib.stream_ptr(dev))
-    _lib.check(rc, "hsa_paged_attn_decode")
+    if rc:
+        _lib.check(rc, "hsa_paged_attn_decode")
     return out

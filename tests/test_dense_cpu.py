@@ -78,8 +78,8 @@ def test_paged_workspace():
 
 def test_split_choice():
     lib = _lib.load()
-    assert lib.hsa_paged_attn_choose_splits(1, 8, 8, 16, 7) == 1          # 112 keys: one range
-    assert 1 < lib.hsa_paged_attn_choose_splits(1, 8, 8, 64, 2048) <= 128
+    assert lib.hsa_paged_attn_choose_splits(1, 8, 8, 16, 4) == 1          # 64 keys: one range
+    assert 1 < lib.hsa_paged_attn_choose_splits(1, 8, 8, 64, 2048) <= 148
     assert lib.hsa_paged_attn_choose_splits(4096, 8, 8, 64, 2048) == 1
     assert lib.hsa_paged_attn_choose_splits(0, 8, 8, 64, 2048) == 1
 
