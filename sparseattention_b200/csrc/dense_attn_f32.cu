@@ -6,8 +6,10 @@
 //
 // A warp owns 16 rows (queries; keys in the dk/dv kernel) and walks over tiles of the other side, which lie in shared memory as
 // float32.  Products run on the tensor cores in three passes: x = hi + lo with hi = x rounded to 11 bits (tf32) and lo the rest
-// rounded to 11 bits, a b ~ hi hi + hi lo + lo hi, off by at most about 3 * 2^-22 |a b|, summed in 32 bits.  That is what 32-bit
-// multiply-adds give, at twice their rate (2048 x 2048, 8 heads of 64, forward: SIMT_NOTE).
+// rounded to 11 bits, a b ~ hi hi + hi lo + lo hi, off by at most about 3 * 2^-22 |a b|, summed in 32 bits.  Bound by the rate of
+// these warp-level products, measured at about 130 multiply-adds per cycle and SM, three for one here.  (32-bit multiply-adds on
+// the same tiles did not come nearer to their own rate: forward 2048 x 2048, 8 heads of 64: 346 us here, 420 and 314 us with 8 x 4
+// and 4 x 4 of them per thread; forward and backward 2 x 1024 x 1024, 16 heads of 128: 2734 us against 3197 and 3594.)
 // Weights pass from the first product to the second through shared memory, inside a warp.  Rows are padded so that fragment reads
 // have no bank conflicts (two-way for the operands that are read along both axes).  One writer per output row, fixed order of
 // summation.  Keys behind a sequence's length, and keys that no query may look at, are stored as zeros: what lies there (NaN,
@@ -16,12 +18,14 @@
 
 namespace hsa {
 
-// Tile sizes by padded head dim: BT rows on either side, CS warps per row group (each with its share of the output columns)
+// Tile sizes by padded head dim: a block's own rows, the rows of a tile of the other side (32 where 64 would leave room for one block
+// per SM only: 4686 -> 2734 us at 2 x 1024 x 1024, 16 heads of 128, forward and backward), and warps per 16 own rows (each with its
+// share of the output columns)
 template <int DP> struct F32Shape {
-    static constexpr int kRows = DP <= 128 ? 64 : 32, kSplit = DP <= 128 ? 1 : 2;
+    static constexpr int kRows = DP <= 128 ? 64 : 32, kOther = DP <= 64 ? 64 : 32, kSplit = DP <= 128 ? 1 : 2;
     static constexpr int kThreads = kRows / 16 * kSplit * 32;
     static constexpr int kPitch = DP + 4;                    // floats between rows
-    static constexpr int kWeights = kRows + 4;
+    static constexpr int kWeights = kOther + 4;
 };
 
 __device__ __forceinline__ uint32_t to_tf32(float x) {
@@ -40,10 +44,16 @@ __device__ __forceinline__ void mma1688(float (&d)[4], uint32_t a0, uint32_t a1,
     asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void mma_split(float (&d)[4], const Split (&a)[4], const Split &b0, const Split &b1) {
-    mma1688(d, a[0].lo, a[1].lo, a[2].lo, a[3].lo, b0.hi, b1.hi);
-    mma1688(d, a[0].hi, a[1].hi, a[2].hi, a[3].hi, b0.lo, b1.lo);
-    mma1688(d, a[0].hi, a[1].hi, a[2].hi, a[3].hi, b0.hi, b1.hi);
+// d[n] += a b[n] for N tiles.  A pass runs over all tiles before the next one starts: back to back on one accumulator they would wait
+// for each other.
+template <int N, int NT>
+__device__ __forceinline__ void mma_split(float (&d)[NT][4], int first, const Split (&a)[4], const Split (&b)[N][2]) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) mma1688(d[first + n], a[0].lo, a[1].lo, a[2].lo, a[3].lo, b[n][0].hi, b[n][1].hi);
+#pragma unroll
+    for (int n = 0; n < N; ++n) mma1688(d[first + n], a[0].hi, a[1].hi, a[2].hi, a[3].hi, b[n][0].lo, b[n][1].lo);
+#pragma unroll
+    for (int n = 0; n < N; ++n) mma1688(d[first + n], a[0].hi, a[1].hi, a[2].hi, a[3].hi, b[n][0].hi, b[n][1].hi);
 }
 
 // rows row0 .. row0 + ROWS - 1 of a [rows, D] matrix as float32 into dst[ROWS][DP + 4]; rows >= limit, rows whose bit in `seen`
@@ -89,10 +99,16 @@ __device__ __forceinline__ void rows_dot(float (&s)[NT][4], const float *A, cons
     for (int d = 0; d < DP; d += 8) {
         const Split a[4] = {split(A[g * P + d + quad]), split(A[(g + 8) * P + d + quad]), split(A[g * P + d + quad + 4]),
                             split(A[(g + 8) * P + d + quad + 4])};
+        static_assert(NT % 4 == 0, "tiles come in fours");
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            const float *b = B + (8 * n + g) * P + d + quad;
-            mma_split(s[n], a, split(b[0]), split(b[4]));
+        for (int n = 0; n < NT; n += 4) {
+            Split b[4][2];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float *p = B + (8 * (n + j) + g) * P + d + quad;
+                b[j][0] = split(p[0]); b[j][1] = split(p[4]);
+            }
+            mma_split<4>(s, n, a, b);
         }
     }
 }
@@ -104,10 +120,16 @@ __device__ __forceinline__ void rows_acc(float (&o)[NT][4], const float *W, cons
     for (int k = 0; k < KT; k += 8) {
         const Split a[4] = {split(W[g * PW + k + quad]), split(W[(g + 8) * PW + k + quad]), split(W[g * PW + k + quad + 4]),
                             split(W[(g + 8) * PW + k + quad + 4])};
+        static_assert(NT % 4 == 0, "tiles come in fours");
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            const float *b = M + (k + quad) * P + 8 * n + g;
-            mma_split(o[n], a, split(b[0]), split(b[4 * P]));
+        for (int n = 0; n < NT; n += 4) {
+            Split b[4][2];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float *p = M + (k + quad) * P + 8 * (n + j) + g;
+                b[j][0] = split(p[0]); b[j][1] = split(p[4 * P]);
+            }
+            mma_split<4>(o, n, a, b);
         }
     }
 }
@@ -131,9 +153,9 @@ __device__ __forceinline__ bool mask_allows(const DenseMask &m, const uint32_t *
 template <typename T, int DP>
 __global__ void __launch_bounds__(F32Shape<DP>::kThreads) dense_fwd_f32_kernel(const DenseArgs a, const DenseSplit sp) {
     using S = F32Shape<DP>;
-    constexpr int BT = S::kRows, NT = BT / 8, NO = DP / S::kSplit / 8;
+    constexpr int BT = S::kRows, BO = S::kOther, NT = BO / 8, NO = DP / S::kSplit / 8;
     extern __shared__ __align__(16) float sm[];
-    float *Qs = sm, *Ks = Qs + BT * S::kPitch, *Vs = Ks + BT * S::kPitch, *Ps = Vs + BT * S::kPitch;
+    float *Qs = sm, *Ks = Qs + BT * S::kPitch, *Vs = Ks + BO * S::kPitch, *Ps = Vs + BO * S::kPitch;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, quad = lane & 3;
     const int wr = warp / S::kSplit, wc = warp % S::kSplit, col0 = wc * (DP / S::kSplit);
     const int qtiles = (a.Lq + BT - 1) / BT;
@@ -144,7 +166,7 @@ __global__ void __launch_bounds__(F32Shape<DP>::kThreads) dense_fwd_f32_kernel(c
     const T *Q = (const T *)a.q.ptr + b * a.q.batch_stride + (int64_t)h * a.D;
     const T *K = (const T *)a.k.ptr + b * a.k.batch_stride + (int64_t)hk * a.D;
     const T *V = (const T *)a.v.ptr + b * a.v.batch_stride + (int64_t)hk * a.D;
-    const int n = dense_keys(a, b), tiles = (n + BT - 1) / BT, per = (tiles + sp.splits - 1) / sp.splits;
+    const int n = dense_keys(a, b), tiles = (n + BO - 1) / BO, per = (tiles + sp.splits - 1) / sp.splits;
     const int64_t plane = (int64_t)b * a.mask.plane_b + (int64_t)h * a.mask.plane_h;
     const uint32_t *bits = a.mask.bits ? a.mask.bits + plane * a.mask.rows * a.mask.wk : nullptr;
     const uint32_t *seen = a.mask.bits ? a.mask.seen + plane * a.mask.wk : nullptr;
@@ -156,14 +178,14 @@ __global__ void __launch_bounds__(F32Shape<DP>::kThreads) dense_fwd_f32_kernel(c
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
     for (int t = range * per; t < min(tiles, (range + 1) * per); ++t) {
-        const int k0 = t * BT;
+        const int k0 = t * BO;
         if (bits != nullptr) {
             const int cell = a.mask.rows > 1 ? q0 / kDenseTile : 0;
             if (a.mask.tiles[(plane * a.mask.tq + cell) * a.mask.tk + k0 / kDenseTile] == 0) continue;
         }
         __syncthreads();                                   // everybody is done with the previous tile
-        load_rows<T, BT, DP, S::kThreads>(Ks, K, a.k.row_stride, k0, n, a.D, a.vec, seen);
-        load_rows<T, BT, DP, S::kThreads>(Vs, V, a.v.row_stride, k0, n, a.D, a.vec, seen);
+        load_rows<T, BO, DP, S::kThreads>(Ks, K, a.k.row_stride, k0, n, a.D, a.vec, seen);
+        load_rows<T, BO, DP, S::kThreads>(Vs, V, a.v.row_stride, k0, n, a.D, a.vec, seen);
         __syncthreads();
         float s[NT][4];
         rows_dot<NT, DP>(s, Qs + wr * 16 * S::kPitch, Ks, g, quad);
@@ -202,7 +224,7 @@ __global__ void __launch_bounds__(F32Shape<DP>::kThreads) dense_fwd_f32_kernel(c
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[i][e] *= corr[e >> 1];
         __syncwarp();
-        rows_acc<NO, BT, DP>(o, mine, Vs + col0, g, quad);
+        rows_acc<NO, BO, DP>(o, mine, Vs + col0, g, quad);
     }
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
@@ -236,9 +258,9 @@ __global__ void __launch_bounds__(F32Shape<DP>::kThreads) dense_fwd_f32_kernel(c
 template <typename T, int DP>
 __global__ void __launch_bounds__(F32Shape<DP>::kThreads) dense_dq_f32_kernel(const DenseArgs a, const BwdSplit sp) {
     using S = F32Shape<DP>;
-    constexpr int BT = S::kRows, NT = BT / 8, NO = DP / S::kSplit / 8;
+    constexpr int BT = S::kRows, BO = S::kOther, NT = BO / 8, NO = DP / S::kSplit / 8;
     extern __shared__ __align__(16) float sm[];
-    float *Qs = sm, *Gs = Qs + BT * S::kPitch, *Ks = Gs + BT * S::kPitch, *Vs = Ks + BT * S::kPitch, *Ds = Vs + BT * S::kPitch;
+    float *Qs = sm, *Gs = Qs + BT * S::kPitch, *Ks = Gs + BT * S::kPitch, *Vs = Ks + BO * S::kPitch, *Ds = Vs + BO * S::kPitch;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, quad = lane & 3;
     const int wr = warp / S::kSplit, wc = warp % S::kSplit, col0 = wc * (DP / S::kSplit);
     const int qtiles = (a.Lq + BT - 1) / BT;
@@ -250,7 +272,7 @@ __global__ void __launch_bounds__(F32Shape<DP>::kThreads) dense_dq_f32_kernel(co
     const T *G = (const T *)a.dout.ptr + b * a.dout.batch_stride + (int64_t)h * a.D;
     const T *K = (const T *)a.k.ptr + b * a.k.batch_stride + (int64_t)hk * a.D;
     const T *V = (const T *)a.v.ptr + b * a.v.batch_stride + (int64_t)hk * a.D;
-    const int n = dense_keys(a, b), tiles = (n + BT - 1) / BT, per = (tiles + sp.splits - 1) / sp.splits;
+    const int n = dense_keys(a, b), tiles = (n + BO - 1) / BO, per = (tiles + sp.splits - 1) / sp.splits;
     const int64_t plane = (int64_t)b * a.mask.plane_b + (int64_t)h * a.mask.plane_h;
     const uint32_t *bits = a.mask.bits ? a.mask.bits + plane * a.mask.rows * a.mask.wk : nullptr;
     const uint32_t *seen = a.mask.bits ? a.mask.seen + plane * a.mask.wk : nullptr;
@@ -269,14 +291,14 @@ __global__ void __launch_bounds__(F32Shape<DP>::kThreads) dense_dq_f32_kernel(co
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
     for (int t = range * per; t < min(tiles, (range + 1) * per); ++t) {
-        const int k0 = t * BT;
+        const int k0 = t * BO;
         if (bits != nullptr) {
             const int cell = a.mask.rows > 1 ? q0 / kDenseTile : 0;
             if (a.mask.tiles[(plane * a.mask.tq + cell) * a.mask.tk + k0 / kDenseTile] == 0) continue;
         }
         __syncthreads();
-        load_rows<T, BT, DP, S::kThreads>(Ks, K, a.k.row_stride, k0, n, a.D, a.vec, seen);
-        load_rows<T, BT, DP, S::kThreads>(Vs, V, a.v.row_stride, k0, n, a.D, a.vec, seen);
+        load_rows<T, BO, DP, S::kThreads>(Ks, K, a.k.row_stride, k0, n, a.D, a.vec, seen);
+        load_rows<T, BO, DP, S::kThreads>(Vs, V, a.v.row_stride, k0, n, a.D, a.vec, seen);
         __syncthreads();
         float s[NT][4], dp[NT][4];
         rows_dot<NT, DP>(s, Qs + wr * 16 * S::kPitch, Ks, g, quad);
@@ -297,7 +319,7 @@ __global__ void __launch_bounds__(F32Shape<DP>::kThreads) dense_dq_f32_kernel(co
                 *reinterpret_cast<float2 *>(mine + (g + 8 * r) * S::kWeights + 8 * i + 2 * quad) = make_float2(x[0], x[1]);
             }
         __syncwarp();
-        rows_acc<NO, BT, DP>(o, mine, Ks + col0, g, quad);
+        rows_acc<NO, BO, DP>(o, mine, Ks + col0, g, quad);
     }
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
@@ -317,12 +339,12 @@ __global__ void __launch_bounds__(F32Shape<DP>::kThreads) dense_dq_f32_kernel(co
 template <typename T, int DP>
 __global__ void __launch_bounds__(F32Shape<DP>::kThreads) dense_dkdv_f32_kernel(const DenseArgs a, const BwdSplit sp) {
     using S = F32Shape<DP>;
-    constexpr int BT = S::kRows, NT = BT / 8, NO = DP / S::kSplit / 8;
+    constexpr int BT = S::kRows, BO = S::kOther, NT = BO / 8, NO = DP / S::kSplit / 8;
     extern __shared__ __align__(16) float sm[];
-    float *Ks = sm, *Vs = Ks + BT * S::kPitch, *Qs = Vs + BT * S::kPitch, *Gs = Qs + BT * S::kPitch, *Ws = Gs + BT * S::kPitch;
+    float *Ks = sm, *Vs = Ks + BT * S::kPitch, *Qs = Vs + BT * S::kPitch, *Gs = Qs + BO * S::kPitch, *Ws = Gs + BO * S::kPitch;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, quad = lane & 3;
     const int wr = warp / S::kSplit, wc = warp % S::kSplit, col0 = wc * (DP / S::kSplit);
-    const int ktiles = (a.Lk + BT - 1) / BT, qtiles = (a.Lq + BT - 1) / BT;
+    const int ktiles = (a.Lk + BT - 1) / BT, qtiles = (a.Lq + BO - 1) / BO;
     int blk = blockIdx.x;
     const int k0 = blk % ktiles * BT; blk /= ktiles;
     const int hk = blk % a.Hkv; blk /= a.Hkv;
@@ -340,7 +362,7 @@ __global__ void __launch_bounds__(F32Shape<DP>::kThreads) dense_dkdv_f32_kernel(
     load_rows<T, BT, DP, S::kThreads>(Ks, K, a.k.row_stride, k0, n, a.D, a.vec, nullptr);
     load_rows<T, BT, DP, S::kThreads>(Vs, V, a.v.row_stride, k0, n, a.D, a.vec, nullptr);
     for (int u = range * per; u < min(units, (range + 1) * per); ++u) {
-        const int h = hk * a.group + u / qtiles, q0 = u % qtiles * BT;
+        const int h = hk * a.group + u / qtiles, q0 = u % qtiles * BO;
         const T *Q = (const T *)a.q.ptr + b * a.q.batch_stride + (int64_t)h * a.D;
         const T *G = (const T *)a.dout.ptr + b * a.dout.batch_stride + (int64_t)h * a.D;
         const int64_t plane = (int64_t)b * a.mask.plane_b + (int64_t)h * a.mask.plane_h;
@@ -350,8 +372,8 @@ __global__ void __launch_bounds__(F32Shape<DP>::kThreads) dense_dkdv_f32_kernel(
             if (a.mask.tiles[(plane * a.mask.tq + cell) * a.mask.tk + k0 / kDenseTile] == 0) continue;
         }
         __syncthreads();
-        load_rows<T, BT, DP, S::kThreads>(Qs, Q, a.q.row_stride, q0, a.Lq, a.D, a.vec, nullptr);
-        load_rows<T, BT, DP, S::kThreads>(Gs, G, a.dout.row_stride, q0, a.Lq, a.D, a.vec, nullptr);
+        load_rows<T, BO, DP, S::kThreads>(Qs, Q, a.q.row_stride, q0, a.Lq, a.D, a.vec, nullptr);
+        load_rows<T, BO, DP, S::kThreads>(Gs, G, a.dout.row_stride, q0, a.Lq, a.D, a.vec, nullptr);
         __syncthreads();
         float s[NT][4], dp[NT][4];                            // rows: keys, columns: queries
         rows_dot<NT, DP>(s, Ks + wr * 16 * S::kPitch, Qs, g, quad);
@@ -378,7 +400,7 @@ __global__ void __launch_bounds__(F32Shape<DP>::kThreads) dense_dkdv_f32_kernel(
             }
         }
         __syncwarp();
-        rows_acc<NO, BT, DP>(ov4, mine, Gs + col0, g, quad);
+        rows_acc<NO, BO, DP>(ov4, mine, Gs + col0, g, quad);
         __syncwarp();
 #pragma unroll
         for (int i = 0; i < NT; ++i)
@@ -386,7 +408,7 @@ __global__ void __launch_bounds__(F32Shape<DP>::kThreads) dense_dkdv_f32_kernel(
             for (int r = 0; r < 2; ++r)
                 *reinterpret_cast<float2 *>(mine + (g + 8 * r) * S::kWeights + 8 * i + 2 * quad) = make_float2(dp[i][2 * r], dp[i][2 * r + 1]);
         __syncwarp();
-        rows_acc<NO, BT, DP>(ok4, mine, Qs + col0, g, quad);
+        rows_acc<NO, BO, DP>(ok4, mine, Qs + col0, g, quad);
     }
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
@@ -414,15 +436,16 @@ __global__ void __launch_bounds__(F32Shape<DP>::kThreads) dense_dkdv_f32_kernel(
 // Partial rows are read and written in pieces of four, and only as aligned as the head dim makes them
 static bool f32_splittable(int D) { return D % 4 == 0; }
 static int f32_rows(int D) { return D <= 128 ? 64 : 32; }
+static int f32_other(int D) { return D <= 64 ? 64 : 32; }
 
-// A block costs its tiles plus about one tile's time of set-up, two as one of several ranges.
+// A block costs its tiles plus about one and a half tiles' time of set-up, three as one of several ranges.
 static int f32_fwd_splits(int B, int Lq, int Lk, int H, int D) {
     const int bt = f32_rows(D);
-    return f32_splittable(D) ? range_count((long long)B * H * ((Lq + bt - 1) / bt), (Lk + bt - 1) / bt, 1.0, 2.0) : 1;
+    return f32_splittable(D) ? range_count((long long)B * H * ((Lq + bt - 1) / bt), (Lk + f32_other(D) - 1) / f32_other(D), 1.5, 3.0) : 1;
 }
 static int f32_dkdv_splits(int B, int Lq, int Lk, int H, int Hkv, int D) {
     const int bt = f32_rows(D);
-    return f32_splittable(D) ? range_count((long long)B * Hkv * ((Lk + bt - 1) / bt), H / Hkv * ((Lq + bt - 1) / bt), 1.0, 2.0) : 1;
+    return f32_splittable(D) ? range_count((long long)B * Hkv * ((Lk + bt - 1) / bt), H / Hkv * ((Lq + f32_other(D) - 1) / f32_other(D)), 1.5, 3.0) : 1;
 }
 
 size_t dense_fwd_f32_workspace(int B, int Lq, int Lk, int H, int D) { return fwd_part_bytes(f32_fwd_splits(B, Lq, Lk, H, D), B, Lq, H, D); }
@@ -433,7 +456,7 @@ size_t dense_bwd_f32_workspace(int B, int Lq, int Lk, int H, int Hkv, int D) {
 template <typename T, int DP>
 static int f32_fwd(const DenseArgs &a, void *workspace, cudaStream_t st) {
     using S = F32Shape<DP>;
-    constexpr int smem = (3 * S::kRows * S::kPitch + S::kThreads / 32 * 16 * S::kWeights) * (int)sizeof(float);
+    constexpr int smem = ((S::kRows + 2 * S::kOther) * S::kPitch + S::kThreads / 32 * 16 * S::kWeights) * (int)sizeof(float);
     DenseSplit sp = fwd_split(f32_fwd_splits(a.B, a.Lq, a.Lk, a.H, a.D), a, workspace);
     const long long blocks = (long long)a.B * a.H * ((a.Lq + S::kRows - 1) / S::kRows) * sp.splits;
     if (blocks > 0x7fffffffLL) return fail(HSA_ERR_ARG, "hsa_dense_attn_fwd: too many tiles");
@@ -447,7 +470,7 @@ static int f32_fwd(const DenseArgs &a, void *workspace, cudaStream_t st) {
 template <typename T, int DP>
 static int f32_bwd(const DenseArgs &a, void *workspace, cudaStream_t st) {
     using S = F32Shape<DP>;
-    constexpr int smem = (4 * S::kRows * S::kPitch + S::kThreads / 32 * 16 * S::kWeights) * (int)sizeof(float);
+    constexpr int smem = (2 * (S::kRows + S::kOther) * S::kPitch + S::kThreads / 32 * 16 * S::kWeights) * (int)sizeof(float);
     BwdSplit sq, sk;
     bwd_splits(f32_fwd_splits(a.B, a.Lq, a.Lk, a.H, a.D), f32_dkdv_splits(a.B, a.Lq, a.Lk, a.H, a.Hkv, a.D), a, workspace, sq, sk);
     const long long q_blocks = (long long)a.B * a.H * ((a.Lq + S::kRows - 1) / S::kRows) * sq.splits;
