@@ -308,17 +308,19 @@ dense_dq_tc5_kernel(const DenseArgs a, const BwdSplit sp, const __grid_constant_
                     tmem_ld32(ts, r);
                     tmem_ld32(ts + 64, g);
                     tmem_ld_wait();
+                    auto gradients = [&](auto whole) {
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        const float2 e = unpair(fma2(pair_bits(r[2 * j], r[2 * j + 1]), c2, lse22));
-                        const uint64_t p = pair(fast_exp2(e.x), fast_exp2(e.y));
-                        float2 y = unpair(mul2(p, add2(pair_bits(g[2 * j], g[2 * j + 1]), delta2)));
-                        if (partial) {                       // not through p = 0: what a hidden row holds may be NaN
-                            if (!((keep >> (2 * j)) & 1u)) y.x = 0.f;
-                            if (!((keep >> (2 * j + 1)) & 1u)) y.y = 0.f;
+                        for (int j = 0; j < 16; ++j) {
+                            const float2 e = unpair(fma2(pair_bits(r[2 * j], r[2 * j + 1]), c2, lse22));
+                            float2 y = unpair(mul2(pair(fast_exp2(e.x), fast_exp2(e.y)), add2(pair_bits(g[2 * j], g[2 * j + 1]), delta2)));
+                            if (!decltype(whole)::value) {   // not through p = 0: what a hidden row holds may be NaN
+                                if (!((keep >> (2 * j)) & 1u)) y.x = 0.f;
+                                if (!((keep >> (2 * j + 1)) & 1u)) y.y = 0.f;
+                            }
+                            d[j] = pack2<T>(y.x, y.y);
                         }
-                        d[j] = pack2<T>(y.x, y.y);
-                    }
+                    };
+                    if (partial) gradients(std::false_type{}); else gradients(std::true_type{});
                     tmem_st16(ts, d);
                     tmem_st_wait();
                     fence_before_sync();
@@ -649,23 +651,26 @@ dense_dkdv_tc5_kernel(const DenseArgs a, const BwdSplit sp, const __grid_constan
                 tmem_ld32(ts, r);
                 tmem_ld32(ts + 64, g);
                 tmem_ld_wait();
+                auto gradients = [&](auto whole) {
 #pragma unroll
-                for (int j = 0; j < 16; j += 2) {
-                    const float4 lse = *reinterpret_cast<const float4 *>(st + 2 * j), dl = *reinterpret_cast<const float4 *>(st + 64 + 2 * j);
+                    for (int j = 0; j < 16; j += 2) {
+                        const float4 lse = *reinterpret_cast<const float4 *>(st + 2 * j), dl = *reinterpret_cast<const float4 *>(st + 64 + 2 * j);
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const int c = j + e;
-                        const float2 z = unpair(fma2(pair_bits(r[2 * c], r[2 * c + 1]), c2, e == 0 ? pair(lse.x, lse.y) : pair(lse.z, lse.w)));
-                        float2 p = make_float2(fast_exp2(z.x), fast_exp2(z.y));
-                        float2 y = unpair(mul2(pair(p.x, p.y), add2(pair_bits(g[2 * c], g[2 * c + 1]), e == 0 ? pair(dl.x, dl.y) : pair(dl.z, dl.w))));
-                        if (partial) {                           // not through p = 0: what a hidden row holds may be NaN
-                            if (!((keep >> (2 * c)) & 1u)) p.x = y.x = 0.f;
-                            if (!((keep >> (2 * c + 1)) & 1u)) p.y = y.y = 0.f;
+                        for (int e = 0; e < 2; ++e) {
+                            const int c = j + e;
+                            const float2 z = unpair(fma2(pair_bits(r[2 * c], r[2 * c + 1]), c2, e == 0 ? pair(lse.x, lse.y) : pair(lse.z, lse.w)));
+                            float2 p = make_float2(fast_exp2(z.x), fast_exp2(z.y));
+                            float2 y = unpair(mul2(pair(p.x, p.y), add2(pair_bits(g[2 * c], g[2 * c + 1]), e == 0 ? pair(dl.x, dl.y) : pair(dl.z, dl.w))));
+                            if (!decltype(whole)::value) {       // not through p = 0: what a hidden row holds may be NaN
+                                if (!((keep >> (2 * c)) & 1u)) p.x = y.x = 0.f;
+                                if (!((keep >> (2 * c + 1)) & 1u)) p.y = y.y = 0.f;
+                            }
+                            pk[c] = pack2<T>(p.x, p.y);
+                            dk[c] = pack2<T>(y.x, y.y);
                         }
-                        pk[c] = pack2<T>(p.x, p.y);
-                        dk[c] = pack2<T>(y.x, y.y);
                     }
-                }
+                };
+                if (partial) gradients(std::false_type{}); else gradients(std::true_type{});
                 tmem_st16(ts, pk);
                 tmem_st16(ts + 64, dk);
                 tmem_st_wait();
