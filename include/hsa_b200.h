@@ -408,7 +408,9 @@ int hsa_cross_entropy_bwd_inplace(void *logits, long long row_stride, const long
  *   A query without keys gives rows of `empty_value` and LSE = -inf.  What K and V hold behind a length, or in keys that no
  *   query of a mask's plane may look at, reaches no result (it may be NaN); keys that some queries see and others do not
  *   must be finite, as must Q and dOut in the backward.
- *   LSE, if not NULL, receives the log-sum-exp [B, Lq, H] float32 that the backward needs.
+ *   LSE, if not NULL, receives the log-sum-exp [B, Lq, H] float32 that the backward needs.  out_rest, if not NULL (16-bit types),
+ *   receives what rounding took from Out, in the same type, packed [B, Lq, H, D]: given to the backward it makes the row sums of
+ *   dOut * Out as exact as those of a 32-bit output.
  *   scale > 0.  D <= 256.  `algo`: 0 = automatic, 1 = 32-bit kernels (any type), 2 = tcgen05 kernels (bf16 / f16, D a multiple of
  *   8 up to 128, 16-byte aligned rows; HSA_ERR_ARG otherwise).  `workspace`: hsa_dense_attn_fwd_workspace_bytes(...) bytes (often 0; few
  *   queries over many keys are cut into ranges of keys that are joined afterwards), 256-byte aligned.
@@ -423,13 +425,13 @@ size_t hsa_dense_mask_bytes(int batches, int heads, int rows, int Lk);
 int hsa_dense_mask_pack(const void *mask, int64_t stride_b, int64_t stride_h, int64_t stride_q, int64_t stride_k, int batches,
                         int heads, int rows, int Lk, void *packed, size_t packed_bytes, void *stream);
 size_t hsa_dense_attn_fwd_workspace_bytes(int B, int Lq, int Lk, int H, int Hkv, int D, int dtype, int algo);
-int hsa_dense_attn_fwd(hsa_view Q, hsa_view K, hsa_view V, hsa_view Out, float *LSE, const int *key_lengths,
+int hsa_dense_attn_fwd(hsa_view Q, hsa_view K, hsa_view V, hsa_view Out, void *out_rest, float *LSE, const int *key_lengths,
                        const void *packed_mask, int mask_batches, int mask_heads, int mask_rows, void *workspace,
                        size_t workspace_bytes, int B, int Lq, int Lk, int H, int Hkv, int D, float scale, float empty_value,
                        int dtype, int algo, void *stream);
 size_t hsa_dense_attn_bwd_workspace_bytes(int B, int Lq, int Lk, int H, int Hkv, int D, int dtype, int algo);
-int hsa_dense_attn_bwd(hsa_view Q, hsa_view K, hsa_view V, hsa_view Out, const float *LSE, hsa_view dOut, hsa_view dQ,
-                       hsa_view dK, hsa_view dV, const int *key_lengths, const void *packed_mask, int mask_batches,
+int hsa_dense_attn_bwd(hsa_view Q, hsa_view K, hsa_view V, hsa_view Out, const void *out_rest, const float *LSE, hsa_view dOut,
+                       hsa_view dQ, hsa_view dK, hsa_view dV, const int *key_lengths, const void *packed_mask, int mask_batches,
                        int mask_heads, int mask_rows, void *workspace, size_t workspace_bytes, int B, int Lq, int Lk, int H,
                        int Hkv, int D, float scale, int dtype, int algo, void *stream);
 

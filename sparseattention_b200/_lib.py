@@ -95,10 +95,10 @@ SIGNATURES = {
     "hsa_dense_mask_bytes": (c_size_t, [c_int] * 4),
     "hsa_dense_mask_pack": (c_int, [c_void_p] + [c_int64] * 4 + [c_int] * 4 + [c_void_p, c_size_t, c_void_p]),
     "hsa_dense_attn_fwd_workspace_bytes": (c_size_t, [c_int] * 8),
-    "hsa_dense_attn_fwd": (c_int, [V, V, V, V, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_size_t]
+    "hsa_dense_attn_fwd": (c_int, [V, V, V, V, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_size_t]
                            + [c_int] * 6 + [c_float, c_float, c_int, c_int, c_void_p]),
     "hsa_dense_attn_bwd_workspace_bytes": (c_size_t, [c_int] * 8),
-    "hsa_dense_attn_bwd": (c_int, [V, V, V, V, c_void_p, V, V, V, V, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_size_t]
+    "hsa_dense_attn_bwd": (c_int, [V, V, V, V, c_void_p, c_void_p, V, V, V, V, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_size_t]
                            + [c_int] * 6 + [c_float, c_int, c_int, c_void_p]),
     "hsa_dense_attn_aborts": (c_int, [c_void_p]),
     "hsa_paged_attn_choose_splits": (c_int, [c_int] * 5),

@@ -75,7 +75,14 @@ __global__ void __launch_bounds__(256) dense_delta_kernel(const DenseArgs a, flo
     RowFrag<T, VEC, LPR, CPL> x, y;
     x.load((const T *)a.out.ptr + b * a.out.batch_stride + (int64_t)i * a.out.row_stride + (int64_t)h * a.D, g, a.D / VEC);
     y.load((const T *)a.dout.ptr + b * a.dout.batch_stride + (int64_t)i * a.dout.row_stride + (int64_t)h * a.D, g, a.D / VEC);
-    const float s = group_sum<LPR>(x.dot_partial(y));
+    float part = x.dot_partial(y);
+    if (a.out_lo != nullptr) {
+        // what rounding took from the output: without it a sum over few keys, whose differences are small, is off by more than
+        // the rest of the backward (2.9e-3 against 2.4e-3 in bfloat16)
+        x.load((const T *)a.out_lo + ((b * a.Lq + i) * a.H + h) * a.D, g, a.D / VEC);
+        part += x.dot_partial(y);
+    }
+    const float s = group_sum<LPR>(part);
     if (g == 0) {
         const float l = a.lse[(b * a.Lq + i) * a.H + h];
         const bool none = l == -INFINITY;
@@ -161,7 +168,7 @@ extern "C" size_t hsa_dense_attn_fwd_workspace_bytes(int B, int Lq, int Lk, int 
     return f32 > tc ? f32 : tc;
 }
 
-extern "C" int hsa_dense_attn_fwd(hsa_view Q, hsa_view K, hsa_view V, hsa_view Out, float *LSE, const int *key_lengths,
+extern "C" int hsa_dense_attn_fwd(hsa_view Q, hsa_view K, hsa_view V, hsa_view Out, void *out_rest, float *LSE, const int *key_lengths,
                                   const void *packed_mask, int mask_batches, int mask_heads, int mask_rows, void *workspace,
                                   size_t workspace_bytes, int B, int Lq, int Lk, int H, int Hkv, int D, float scale,
                                   float empty_value, int dtype, int algo, void *stream) {
@@ -171,7 +178,9 @@ extern "C" int hsa_dense_attn_fwd(hsa_view Q, hsa_view K, hsa_view V, hsa_view O
     DenseArgs a{};
     Q = dense_view(Q, B, Lq, H, D); Out = dense_view(Out, B, Lq, H, D);
     K = dense_view(K, B, Lk, Hkv, D); V = dense_view(V, B, Lk, Hkv, D);
-    a.q = Q; a.k = K; a.v = V; a.out = Out; a.lse = LSE;
+    HSA_CHECK_ARG(out_rest == nullptr || dtype != HSA_F32, "hsa_dense_attn_fwd: a float32 output has no rounding rest");
+    if (!aligned16(out_rest)) return fail(HSA_ERR_ALIGN, "hsa_dense_attn_fwd: the rounding rest must be 16-byte aligned");
+    a.q = Q; a.k = K; a.v = V; a.out = Out; a.out_lo = out_rest; a.lse = LSE;
     a.key_lengths = key_lengths;
     a.mask = dense_mask_view(packed_mask, mask_batches, mask_heads, mask_rows, Lk);
     a.B = B; a.Lq = Lq; a.Lk = Lk; a.H = H; a.Hkv = Hkv; a.D = D; a.group = H / Hkv;
@@ -201,7 +210,7 @@ extern "C" size_t hsa_dense_attn_bwd_workspace_bytes(int B, int Lq, int Lk, int 
     return bwd_stats_bytes(B, Lq, H) + (f32 > tc ? f32 : tc);
 }
 
-extern "C" int hsa_dense_attn_bwd(hsa_view Q, hsa_view K, hsa_view V, hsa_view Out, const float *LSE, hsa_view dOut, hsa_view dQ,
+extern "C" int hsa_dense_attn_bwd(hsa_view Q, hsa_view K, hsa_view V, hsa_view Out, const void *out_rest, const float *LSE, hsa_view dOut, hsa_view dQ,
                                   hsa_view dK, hsa_view dV, const int *key_lengths, const void *packed_mask, int mask_batches,
                                   int mask_heads, int mask_rows, void *workspace, size_t workspace_bytes, int B, int Lq, int Lk,
                                   int H, int Hkv, int D, float scale, int dtype, int algo, void *stream) {
@@ -215,7 +224,9 @@ extern "C" int hsa_dense_attn_bwd(hsa_view Q, hsa_view K, hsa_view V, hsa_view O
     DenseArgs a{};
     for (hsa_view *v : {&Q, &Out, &dOut, &dQ}) *v = dense_view(*v, B, Lq, H, D);
     for (hsa_view *v : {&K, &V, &dK, &dV}) *v = dense_view(*v, B, Lk, Hkv, D);
-    a.q = Q; a.k = K; a.v = V; a.out = Out; a.dout = dOut; a.dq = dQ; a.dk = dK; a.dv = dV;
+    HSA_CHECK_ARG(out_rest == nullptr || dtype != HSA_F32, "hsa_dense_attn_bwd: a float32 output has no rounding rest");
+    if (!aligned16(out_rest)) return fail(HSA_ERR_ALIGN, "hsa_dense_attn_bwd: the rounding rest must be 16-byte aligned");
+    a.q = Q; a.k = K; a.v = V; a.out = Out; a.out_lo = const_cast<void *>(out_rest); a.dout = dOut; a.dq = dQ; a.dk = dK; a.dv = dV;
     a.lse = const_cast<float *>(LSE);
     a.key_lengths = key_lengths;
     a.mask = dense_mask_view(packed_mask, mask_batches, mask_heads, mask_rows, Lk);

@@ -67,6 +67,7 @@ inline DenseMask dense_mask_view(const void *packed, int Bm, int Hm, int rows, i
 struct DenseArgs {
     hsa_view q, k, v, out, dout, dq, dk, dv;
     float *lse;                          // forward: [B, Lq, H] natural log-sum-exp, or null
+    void *out_lo;                        // [B, Lq, H, D] packed: what rounding took from the 16-bit output, in its type; or null
     const float *neg_lse2, *neg_delta;   // backward: [B, H, lq_pad] minus the log-sum-exp in base 2 (-inf: no key), minus the row sums of dout * out
     const int *key_lengths;              // [B] or null
     DenseMask mask;

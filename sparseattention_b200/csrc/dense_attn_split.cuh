@@ -66,6 +66,9 @@ inline void bwd_splits(int nq, int nk, const DenseArgs &a, void *workspace, BwdS
 }
 
 template <typename T>
+__device__ __forceinline__ float rounding_rest(float x) { return x - Traits<T>::to_f(Traits<T>::from_f(x)); }
+
+template <typename T>
 __device__ __forceinline__ void store4(T *p, float x, float y, float z, float w, bool vec) {
     if constexpr (sizeof(T) == 4) {
         if (vec) { *reinterpret_cast<float4 *>(p) = make_float4(x, y, z, w); return; }
@@ -101,6 +104,9 @@ __global__ void __launch_bounds__(128) dense_join_kernel(const DenseArgs a, cons
         const bool none = L == 0.f;
         const float inv = 1.f / L, e = a.empty_value;
         store4<T>(out + c, none ? e : acc.x * inv, none ? e : acc.y * inv, none ? e : acc.z * inv, none ? e : acc.w * inv, a.vec);
+        if (a.out_lo != nullptr)                                   // packed, and D a multiple of four
+            store4<T>((T *)a.out_lo + row * a.D + c, none ? 0.f : rounding_rest<T>(acc.x * inv), none ? 0.f : rounding_rest<T>(acc.y * inv),
+                      none ? 0.f : rounding_rest<T>(acc.z * inv), none ? 0.f : rounding_rest<T>(acc.w * inv), true);
         if (a.lse != nullptr && c == 0) a.lse[row] = none ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
     }
 }

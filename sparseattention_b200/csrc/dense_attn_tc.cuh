@@ -107,7 +107,8 @@ __device__ __forceinline__ void quad_pieces(uint4 (&p)[4], int quad) {
 }
 // A warp stores 32 consecutive columns of its 32 rows, as far as the head dim goes (a multiple of 8).  `row`: this lane's row,
 // `below`: rows of the tensor from this one on (may be <= 0).
-template <typename T>
+// REST: not the rounded values, but what rounding took from them.
+template <typename T, bool REST = false>
 __device__ __forceinline__ void store_rows32(T *row, int64_t row_stride, int below, int col, int D, const uint32_t (&v)[32], float scale) {
     const int quad = threadIdx.x & 3;
     uint4 p[4];
@@ -115,8 +116,10 @@ __device__ __forceinline__ void store_rows32(T *row, int64_t row_stride, int bel
     for (int j = 0; j < 4; ++j) {
         uint32_t o[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            o[e] = pack2<T>(__uint_as_float(v[8 * j + 2 * e]) * scale, __uint_as_float(v[8 * j + 2 * e + 1]) * scale);
+        for (int e = 0; e < 4; ++e) {
+            const float x = __uint_as_float(v[8 * j + 2 * e]) * scale, y = __uint_as_float(v[8 * j + 2 * e + 1]) * scale;
+            o[e] = REST ? pack2<T>(rounding_rest<T>(x), rounding_rest<T>(y)) : pack2<T>(x, y);
+        }
         p[j] = make_uint4(o[0], o[1], o[2], o[3]);
     }
     quad_pieces(p, quad);

@@ -423,6 +423,8 @@ dense_fwd_tc5_kernel(const DenseArgs a, const DenseSplit sp, const __grid_consta
                         store_rows32_f32(sp.part_o + at * a.D, (int64_t)a.H * a.D, a.Lq - qi, 32 * c, a.D, o);
                     } else {
                         store_rows32<T>(orow, a.out.row_stride, a.Lq - qi, 32 * c, a.D, o, inv);
+                        if (a.out_lo != nullptr)
+                            store_rows32<T, true>((T *)a.out_lo + at * a.D, (int64_t)a.H * a.D, a.Lq - qi, 32 * c, a.D, o, inv);
                     }
                 }
                 if (qi < a.Lq) {

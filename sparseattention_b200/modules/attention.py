@@ -52,6 +52,8 @@ class HierarchicalAttention(nn.Module):
     update_X_from_Y(x, y, mask=None)  the top-down pass used by forward.
     """
 
+    fused_attention = True          # attention without parents as one kernel where it applies; set False for the eager operations
+
     def __init__(self, dim: int, num_heads: int, dropout: float = 0.1, window_size: int = 16):
         super().__init__()
         self.dim = dim
@@ -66,7 +68,6 @@ class HierarchicalAttention(nn.Module):
             setattr(self, name, nn.Linear(dim, dim, bias=False))
         self.out_proj_x = nn.Linear(dim, dim)
         self.dropout = nn.Dropout(dropout)
-        self.fused_attention = True
 
         self.cached_tables = None
         self.cached_seq_len = -1

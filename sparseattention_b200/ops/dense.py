@@ -125,9 +125,17 @@ def dense_aborts() -> int:
     return int(count.value)
 
 
+_aborts_seen = {}
+
+
 def _debug_check(what: str) -> None:
-    if not torch.cuda.is_current_stream_capturing() and dense_aborts():
-        raise _lib.HsaError(f"{what}: a thread block gave up waiting; its rows hold NaN")
+    """With HSA_B200_DEBUG=1: synchronise and raise if a thread block of the call gave up waiting."""
+    if torch.cuda.is_current_stream_capturing():
+        return
+    dev, now = torch.cuda.current_device(), dense_aborts()
+    if now != _aborts_seen.get(dev, 0):
+        before, _aborts_seen[dev] = _aborts_seen.get(dev, 0), now
+        raise _lib.HsaError(f"{what}: {now - before} thread block(s) gave up waiting; their rows hold NaN")
 
 
 def _ptr(t: Optional[torch.Tensor]):
@@ -136,28 +144,31 @@ def _ptr(t: Optional[torch.Tensor]):
 
 def dense_attention_forward(q, k, v, key_lengths=None, packed_mask=None, scale: float = 1.0, empty_value: float = 0.0,
                             need_lse: bool = True, algo: int = _lib.ALGO_AUTO):
-    """Raw forward on checked inputs with the device current: returns (out, lse or None).  No autograd."""
+    """Raw forward on checked inputs with the device current: returns (out, rest, lse), the last two None unless need_lse.  `rest` is
+    what rounding took from a 16-bit output, for the backward's row sums.  No autograd."""
     lib = _lib.load()
     dev = q.device
     B, Lq, H, D = q.shape
     Lk, Hkv = k.shape[1:3]
     out = torch.empty((B, Lq, H, D), dtype=q.dtype, device=dev)
     lse = torch.empty((B, Lq, H), dtype=torch.float32, device=dev) if need_lse else None
+    rest = torch.empty((B, Lq, H, D), dtype=q.dtype, device=dev) if need_lse and q.dtype != torch.float32 else None
     dt = _lib.dtype_code(q)
     need = _fwd_workspace(B, Lq, Lk, H, Hkv, D, dt, algo, dev.index)
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     rs = H * D
-    rc = lib.hsa_dense_attn_fwd(_view(q), _view(k), _view(v), _lib.HsaView(out.data_ptr(), Lq * rs, rs), _ptr(lse), _ptr(key_lengths),
+    rc = lib.hsa_dense_attn_fwd(_view(q), _view(k), _view(v), _lib.HsaView(out.data_ptr(), Lq * rs, rs), _ptr(rest), _ptr(lse),
+                                _ptr(key_lengths),
                                 *_mask_args(packed_mask), _ptr(ws), need, B, Lq, Lk, H, Hkv, D, scale, empty_value, dt, algo,
                                 _lib.stream_ptr(dev))
     if rc:
         _lib.check(rc, "hsa_dense_attn_fwd")
     if _lib.DEBUG:
         _debug_check("hsa_dense_attn_fwd")
-    return out, lse
+    return out, rest, lse
 
 
-def dense_attention_backward(q, k, v, out, lse, dout, key_lengths=None, packed_mask=None, scale: float = 1.0,
+def dense_attention_backward(q, k, v, out, rest, lse, dout, key_lengths=None, packed_mask=None, scale: float = 1.0,
                              algo: int = _lib.ALGO_AUTO):
     """Raw backward with the device current: returns (dq, dk, dv)."""
     lib = _lib.load()
@@ -172,7 +183,7 @@ def dense_attention_backward(q, k, v, out, lse, dout, key_lengths=None, packed_m
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
     rs, ks = H * D, Hkv * D
     view = _lib.HsaView
-    rc = lib.hsa_dense_attn_bwd(_view(q), _view(k), _view(v), view(out.data_ptr(), Lq * rs, rs), _ptr(lse), _view(dout),
+    rc = lib.hsa_dense_attn_bwd(_view(q), _view(k), _view(v), view(out.data_ptr(), Lq * rs, rs), _ptr(rest), _ptr(lse), _view(dout),
                                 view(dq.data_ptr(), Lq * rs, rs), view(dk.data_ptr(), Lk * ks, ks), view(dv.data_ptr(), Lk * ks, ks),
                                 _ptr(key_lengths), *_mask_args(packed_mask), _ptr(ws), need, B, Lq, Lk, H, Hkv, D, scale,
                                 dt, algo, _lib.stream_ptr(dev))
@@ -206,22 +217,22 @@ class _CrossAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, key_lengths, packed_mask, scale, empty_value, algo):
         q, k, v = _rows(q), _rows(k), _rows(v)
-        out, lse = dense_attention_forward(q, k, v, key_lengths, packed_mask, scale, empty_value, True, algo)
+        out, rest, lse = dense_attention_forward(q, k, v, key_lengths, packed_mask, scale, empty_value, True, algo)
         if packed_mask is None:
-            ctx.save_for_backward(q, k, v, out, lse, key_lengths)
+            ctx.save_for_backward(q, k, v, out, rest, lse, key_lengths)
             ctx.meta = (None, scale, algo)
         else:
-            ctx.save_for_backward(q, k, v, out, lse, key_lengths, packed_mask.data)
+            ctx.save_for_backward(q, k, v, out, rest, lse, key_lengths, packed_mask.data)
             ctx.meta = (packed_mask.sizes, scale, algo)
         return out
 
     @staticmethod
     def backward(ctx, dout):
-        q, k, v, out, lse, key_lengths, *packed = ctx.saved_tensors
+        q, k, v, out, rest, lse, key_lengths, *packed = ctx.saved_tensors
         sizes, scale, algo = ctx.meta
         with _lib.on_device(q.device):
             dout = _rows(dout if dout.dtype == q.dtype else dout.to(q.dtype))
-            grads = dense_attention_backward(q, k, v, out, lse, dout, key_lengths, _Packed(packed[0], sizes) if packed else None,
+            grads = dense_attention_backward(q, k, v, out, rest, lse, dout, key_lengths, _Packed(packed[0], sizes) if packed else None,
                                              scale, algo)
         return (*_once(grads), None, None, None, None, None)
 
@@ -253,7 +264,9 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, key_lengt
     scale: positive; 1 / sqrt(D) if not given.
     A query that may look at no key gives a row of `empty_value` and passes no gradient on.  What k and v hold behind a
     length, or in keys that a mask hides from all queries, may be anything; everything else has to be finite.
-    Differentiable once with respect to q, k and v.
+    Differentiable once with respect to q, k and v.  In bfloat16 and float16 the weights and the gradients of the scores are
+    rounded to that type between the products (a gradient of a score beyond 65504 in float16 is infinite); sums are 32-bit.
+    A mask is packed into bits by every call; keys that only a length hides are cheaper given as key_lengths.
     """
     dev = _check_inputs(q, k, v)
     B, Lq, H, D = q.shape

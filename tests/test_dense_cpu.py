@@ -12,13 +12,13 @@ V = _lib.HsaView(0x1000, 0, 0)
 NULL = _lib.HsaView(0, 0, 0)
 
 
-def fwd(q=V, B=1, Lq=4, Lk=4, H=2, Hkv=2, D=64, scale=0.125, dtype=1, algo=0, mask=None, sizes=(0, 0, 0)):
-    return _lib.load().hsa_dense_attn_fwd(q, V, V, V, None, None, mask, *sizes, None, 0, B, Lq, Lk, H, Hkv, D, scale, 0.0, dtype,
+def fwd(q=V, B=1, Lq=4, Lk=4, H=2, Hkv=2, D=64, scale=0.125, dtype=1, algo=0, mask=None, sizes=(0, 0, 0), rest=None):
+    return _lib.load().hsa_dense_attn_fwd(q, V, V, V, rest, None, None, mask, *sizes, None, 0, B, Lq, Lk, H, Hkv, D, scale, 0.0, dtype,
                                           algo, None)
 
 
 def bwd(B=1, Lq=4, Lk=4, H=2, Hkv=2, D=64, scale=0.125, dtype=1, ws=P, nbytes=1 << 20):
-    return _lib.load().hsa_dense_attn_bwd(V, V, V, V, P, V, V, V, V, None, None, 0, 0, 0, ws, nbytes, B, Lq, Lk, H, Hkv, D, scale,
+    return _lib.load().hsa_dense_attn_bwd(V, V, V, V, None, P, V, V, V, V, None, None, 0, 0, 0, ws, nbytes, B, Lq, Lk, H, Hkv, D, scale,
                                           dtype, 0, None)
 
 
@@ -40,6 +40,7 @@ def test_attention_refuses_the_rest():
     assert fwd(q=NULL) == -1
     assert fwd(dtype=7) == -3 and bwd(dtype=-1) == -3
     assert fwd(algo=3) == -1
+    assert fwd(rest=P, dtype=0) == -1 and fwd(rest=ctypes.c_void_p(0x1008)) == -2
     assert fwd(mask=P, sizes=(2, 1, 1), B=3) == -1 and b"broadcast" in _lib.load().hsa_last_error()
     assert fwd(mask=P, sizes=(1, 1, 3), Lq=4) == -1
     assert bwd(ws=None) == -4 and bwd(nbytes=8) == -4

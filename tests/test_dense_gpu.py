@@ -375,12 +375,47 @@ def test_capture_and_replay_on_new_inputs_and_other_streams(shape):
         assert all(torch.equal(a, b) for a, b in zip(res, want))
 
 
+@pytest.mark.parametrize("shape,rows", [((1, 3, 98500, 2, 2, 64), 1), ((1, 50000, 10, 2, 1, 64), 50000)])
+def test_masks_beyond_the_tile_table(shape, rows):
+    """More 128 x 128 cells along one side than the tensor-core kernels keep per block: the 32-bit kernels take over."""
+    B, Lq, Lk, H, Hkv, D = shape
+    q, k, v, g = make(*shape, torch.bfloat16, seed=17)
+    mask = torch.rand(1, 1, rows, Lk, device="cuda") < 0.5
+    check(q, k, v, g, mask=mask)
+
+
+def test_offsets_past_32_bits():
+    """Keys and values of more than 2^31 elements, zeros but for the last rows: every zero row scores 0 and adds nothing."""
+    Lk, H, D, tail, Lq = 2_200_000, 8, 128, 300, 5
+    assert Lk * H * D > 2 ** 31
+    q, kt, vt, g = make(1, Lq, tail, H, H, D, torch.bfloat16, seed=18)
+    k = torch.zeros(1, Lk, H, D, dtype=torch.bfloat16, device="cuda")
+    v = torch.zeros(1, Lk, H, D, dtype=torch.bfloat16, device="cuda")
+    k[:, -tail:], v[:, -tail:] = kt * 3, vt
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    out = cross_attention(*leaves)
+    dq, dk, dv = torch.autograd.grad(out, leaves, g)
+    qd, kd, vd, gd = (heads_first(t, H) for t in (q, kt * 3, vt, g))
+    s = D ** -0.5 * qd @ kd.transpose(-1, -2)
+    top = s.amax(dim=-1, keepdim=True).clamp_min(0.0)
+    total = torch.exp(s - top).sum(dim=-1, keepdim=True) + (Lk - tail) * torch.exp(-top)
+    p = torch.exp(s - top) / total
+    o = p @ vd
+    ds = p * (gd @ vd.transpose(-1, -2) - (gd * o).sum(-1, keepdim=True))
+    flat = -torch.exp(-top) / total * (gd * o).sum(-1, keepdim=True)          # ds of a zero row
+    back = lambda t: t.permute(0, 2, 1, 3)                                      # noqa: E731
+    for name, got, want in (("out", out, back(o)), ("dv", dv[:, -tail:], back(p.transpose(-1, -2) @ gd)),
+                            ("dk", dk[:, -tail:], back(D ** -0.5 * ds.transpose(-1, -2) @ qd)), ("dq", dq, back(D ** -0.5 * ds @ kd)),
+                            ("dk of a zero row", dk[:, :2], back(D ** -0.5 * (flat * qd).sum(2, keepdim=True)).expand(1, 2, H, D))):
+        assert rel_err(got.detach().double(), want) < 2e-2, name
+
+
 def test_log_sum_exp():
     for dtype in (torch.float32, torch.bfloat16):
         q, k, v, _ = make(2, 70, 300, 4, 2, 64, dtype)
         lengths = torch.tensor([300, 0], dtype=torch.int32, device="cuda")
         want = Definition(q, k, v, by_length(lengths, 300))
-        _, lse = dense_attention_forward(q, k, v, lengths, None, 64 ** -0.5)
+        _, _, lse = dense_attention_forward(q, k, v, lengths, None, 64 ** -0.5)
         near(lse, want.lse, want.lse_tol, "lse")
 
 
@@ -658,24 +693,24 @@ def test_a_wait_that_runs_out_shows():
     limit, count themselves and leave NaN; afterwards everything is as before."""
     lib = _lib.load()
     q, k, v, g = make(2, 200, 300, 2, 2, 64, torch.bfloat16)
-    out, lse = dense_attention_forward(q, k, v, None, None, 0.125)
-    good = (out, *dense_attention_backward(q, k, v, out, lse, g, None, None, 0.125))
+    out, rest, lse = dense_attention_forward(q, k, v, None, None, 0.125)
+    good = (out, *dense_attention_backward(q, k, v, out, rest, lse, g, None, None, 0.125))
     torch.cuda.synchronize()
     before = dense_aborts()
     _lib.check(lib.hsa_debug_wait_test(20_000_000, 16), "hsa_debug_wait_test")
     try:
-        bad, bad_lse = dense_attention_forward(q, k, v, None, None, 0.125)
+        bad, _, bad_lse = dense_attention_forward(q, k, v, None, None, 0.125)
         torch.cuda.synchronize()
         mid = dense_aborts()
-        grads = dense_attention_backward(q, k, v, out, lse, g, None, None, 0.125)
+        grads = dense_attention_backward(q, k, v, out, rest, lse, g, None, None, 0.125)
         torch.cuda.synchronize()
     finally:
         _lib.check(lib.hsa_debug_wait_test(2_000_000_000, 0), "hsa_debug_wait_test")
     assert mid > before and dense_aborts() > mid
     assert bad.isnan().all() and bad_lse.isnan().all()
     assert all(t.isnan().all() for t in grads)
-    out, lse = dense_attention_forward(q, k, v, None, None, 0.125)
-    again = (out, *dense_attention_backward(q, k, v, out, lse, g, None, None, 0.125))
+    out, rest, lse = dense_attention_forward(q, k, v, None, None, 0.125)
+    again = (out, *dense_attention_backward(q, k, v, out, rest, lse, g, None, None, 0.125))
     assert all(torch.equal(a, b) for a, b in zip(good, again))
 
 
