@@ -189,8 +189,8 @@ extern "C" int hsa_dense_attn_fwd(hsa_view Q, hsa_view K, hsa_view V, hsa_view O
     const int es = dtype_size(dtype);
     a.vec = D % 4 == 0;
     for (const hsa_view &v : {Q, K, V, Out}) a.vec = a.vec && rows_in_fours(v, es);
-    // The tensor-core kernel wherever its layout rules allow it: it is ahead of the 32-bit kernel from the smallest call on
-    // (16 x 77, 8 heads of 64: both are bound by the launch) and 40 times as fast at 4096 x 4096.
+    // The tcgen05 kernel wherever its layout rules allow it: from the smallest call on it is not behind the 32-bit kernel (16 x 77,
+    // 8 heads of 64: both are bound by the launch), and at 4096 x 4096 it is 40 times as fast.
     const size_t need = hsa_dense_attn_fwd_workspace_bytes(B, Lq, Lk, H, Hkv, D, dtype, algo);
     if (need && (workspace == nullptr || workspace_bytes < need))
         return fail(HSA_ERR_WORKSPACE, "hsa_dense_attn_fwd: workspace of %zu bytes needed, %zu given", need, workspace_bytes);

@@ -56,8 +56,8 @@ __device__ __forceinline__ float2 exp2_poly(float2 x) {
 }
 
 // The value of lane 0, which is every lane's: tells the compiler that what depends on it is the same in the whole warp.  The
-// warps that issue products need that: with descriptors and loop state in uniform registers an issue takes ISSUE_NEW cycles,
-// with per-lane ones 69 (and a commit 100), which bound all three kernels.
+// warps that issue products need that: with descriptors and loop state in uniform registers an issue takes 10 cycles, with
+// per-lane ones 69 (and a commit 100), which bound all three kernels.
 __device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
 
 // Bit words of the keys [32 w, 32 w + 32) of a tile: those before `left` (keys of the sequence that remain)

@@ -10,8 +10,14 @@
 //   warps 0-3  and 4-7: the softmax of the first and of the second query tile, a thread per row
 // Tensor memory (512 columns): two half tiles of S for either query tile (64 columns each), O of both (DP each).  P replaces the
 // S it came from as 16-bit numbers, so it never passes through shared memory, and the other half tile's scores are computed
-// meanwhile.  (Scores in one piece of 128 columns, which had to wait for the product that consumes P, left a softmax warp
-// waiting a third of its time: 594 us where this takes FWD_US at 4096 x 4096, batch 4, 16 heads of 128.)
+// meanwhile.
+// Measured at 4096 x 4096, batch 4, 16 heads of 128, bf16: 459 to 464 us = 1.19 PFLOP/s, tensor pipe 66 % busy; what is left is the
+// softmax, two warps per scheduler that overlap each other only in part.  On the way there: scores in one piece of 128 columns,
+// which wait for the product that consumes P, 594 us; half tiles with products issued from per-lane registers slower still, from
+// uniform ones and by a warp per query tile 524 us; a quarter of the exponentials in multiply-adds 514 us; registers enough to
+// keep the softmax out of local memory (most of L1 is shared memory here, a spill goes to L2) 464 us.
+// Tried and slower: fetching the next scores before this half tile's weights are handed over (497), taking turns with the
+// exponentials (554), four softmax warps per 32 rows of which pairs exchange maxima (registers).
 // The output is rescaled only when a row's maximum has grown by more than 2^8 since the last time (the weights then lie below
 // 2^8, which changes nothing in their relative precision), so almost every tile leaves O alone.
 // Rounding: weights are rounded to the inputs' type for the second product (what the tensor cores take); their sum is taken
