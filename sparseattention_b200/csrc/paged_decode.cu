@@ -8,10 +8,13 @@
 // With one split the block writes the output itself.
 //
 // Measured, bf16: 2 x 131072 keys, 32 query heads on 4 key/value heads of 128, 537 MB: 88.6 us = 6.06 TB/s, 0.94 of the measured
-// copy bandwidth; 32 sequences of ragged length up to 4096, 16 heads of 128, 524 MB: 112 us = 0.72 of it (unequal shares).
+// copy bandwidth; 32 sequences of ragged length up to 4096, 16 heads of 128, 524 MB: 89.6 us = 0.90 of it (112 before the longest
+// sequences started first).
 //
 // A page number outside [0, num_pages), or a length outside [0, max_pages * page], is not followed: the sequence's output
 // is NaN.  Rows behind a sequence's length are not read.
+#include <climits>
+
 #include "dense_attn.cuh"
 #include "tc_common.cuh"
 
@@ -203,7 +206,26 @@ template <int DP> struct PagedShape {
     static constexpr int kSmem = kPagedWarps * kStages * kStage + 2 * kPagedWarps * 16 * 4;
 };
 
-template <typename T, int DP>
+// The batch entry that comes at place `at` when longer sequences come first (equal ones in their order).  All threads of a block call
+// it; B <= threads.
+__device__ __forceinline__ int by_length(const PagedArgs &a, int at) {
+    __shared__ int found;
+    __shared__ __align__(16) int lengths[kPagedWarps * 32];
+    const int i = threadIdx.x, mine = i < a.B ? __ldg(a.lengths + i) : INT_MIN;
+    lengths[i] = mine;
+    __syncthreads();
+    int rank = 0;
+    for (int j = 0; j < a.B; j += 4) {
+        const int4 x = *reinterpret_cast<const int4 *>(lengths + j);
+        rank += (x.x > mine || (x.x == mine && j < i)) + (x.y > mine || (x.y == mine && j + 1 < i)) +
+                (x.z > mine || (x.z == mine && j + 2 < i)) + (x.w > mine || (x.w == mine && j + 3 < i));
+    }
+    if (rank == at) found = i;
+    __syncthreads();
+    return found;
+}
+
+template <typename T, int DP, bool SORTED>
 __global__ void __launch_bounds__(kPagedWarps * 32) paged_decode_mma_kernel(const PagedArgs a) {
     using Shape = PagedShape<DP>;
     constexpr int ST = Shape::kStages, CPR = DP / 8, PIECES = 16 * CPR / 32;
@@ -211,7 +233,8 @@ __global__ void __launch_bounds__(kPagedWarps * 32) paged_decode_mma_kernel(cons
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
     const int chunks = (a.group + 15) / 16;
     const int split = blockIdx.x % a.splits, gc = blockIdx.x / a.splits % chunks;
-    const int hk = blockIdx.x / a.splits / chunks % a.Hkv, b = blockIdx.x / a.splits / chunks / a.Hkv;
+    const int hk = blockIdx.x / a.splits / chunks % a.Hkv, at = blockIdx.x / a.splits / chunks / a.Hkv;
+    const int b = SORTED ? by_length(a, at) : at;
     const int h0 = hk * a.group + gc * 16, heads = min(16, a.group - gc * 16);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quad = lane & 3, grow = lane >> 2;
     unsigned char *ring = smem + warp * ST * Shape::kStage;
@@ -423,20 +446,20 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const Paged
 }
 
 template <typename T>
-static int paged_mma(const PagedArgs &a, cudaStream_t st) {
+static int paged_mma(const PagedArgs &a, bool sorted, cudaStream_t st) {
     const long long blocks = (long long)a.B * a.Hkv * ((a.group + 15) / 16) * a.splits;
     if (blocks > 0x7fffffffLL) return fail(HSA_ERR_ARG, "hsa_paged_attn_decode: too many blocks");
-    auto go = [&]<int DP>() -> int {
-        constexpr auto kernel = paged_decode_mma_kernel<T, DP>;
+    auto go = [&]<int DP, bool SORTED>() -> int {
+        constexpr auto kernel = paged_decode_mma_kernel<T, DP, SORTED>;
         constexpr int smem = PagedShape<DP>::kSmem;
         const cudaError_t e = allow_smem<kernel>(smem);
         if (e != cudaSuccess) return fail((int)e, "hsa_paged_attn_decode: shared memory %d: %s", smem, cudaGetErrorString(e));
         kernel<<<(unsigned)blocks, kPagedWarps * 32, smem, st>>>(a);
         return launch_status("hsa_paged_attn_decode");
     };
-    if (a.D <= 64) return go.template operator()<64>();
-    if (a.D <= 128) return go.template operator()<128>();
-    return go.template operator()<256>();
+    if (a.D <= 64) return sorted ? go.template operator()<64, true>() : go.template operator()<64, false>();
+    if (a.D <= 128) return sorted ? go.template operator()<128, true>() : go.template operator()<128, false>();
+    return sorted ? go.template operator()<256, true>() : go.template operator()<256, false>();
 }
 
 template <typename T>
@@ -462,26 +485,43 @@ static int paged_simt(const PagedArgs &a, cudaStream_t st) {
 
 using namespace hsa;
 
+// Whether blocks start in the order of their sequences' lengths, the longest first: where more blocks are launched than run at
+// once, so that the last ones to start are short, and where sequences may be long enough to pay for every block's look at all
+// lengths (64 sequences of up to 2000 keys on 8 heads of 64: 50.1 us unsorted and 37.6 sorted when ragged, 70.0 and 72.0 when all
+// are full; 100 of up to 512 on 16 heads lose a tenth either way and stay unsorted).
+static bool paged_sorted(int B, int H, int Hkv, int page_size, int max_pages, int splits) {
+    const long long blocks = (long long)B * Hkv * ((H / Hkv + 15) / 16) * splits;
+    const long long room = (long long)max_pages * page_size;
+    return B > 1 && B <= kPagedWarps * 32 && blocks > 2LL * dense_sm_count() && room >= (long long)splits * (B > 64 ? 8 * B : 512);
+}
+
 // Ranges per sequence.  Two blocks fit an SM; a block costs its steps of 64 keys plus about two and a half steps' time, and the join
 // about one.  The count with the least (rounds of blocks) x (cost of a block): one full round where that fits (2 sequences of
 // 131072 keys on 8 key/value heads: 88.6 us in 37 ranges, 97.9 in 74, 143 in 16).  With more sequences than blocks fit at once,
-// where lengths may differ, a finer cut is taken if it costs no more than a twentieth (32 ragged sequences on 16 heads: 124 us in
-// one range, 112 in four).  The table's room stands in for the lengths, which are on the device.
+// where lengths may differ: the coarsest cut that costs no more than a tenth if the longest come first (32 sequences of up to 4096
+// keys on 16 heads: 88.6 us ragged and 184 full in one range, 110 and 188 in four), else the finest that costs no more than a
+// twentieth (the same unsorted: 121 us in one range, 112 in four).  The table's room stands in for the lengths, which are on the
+// device.
 extern "C" int hsa_paged_attn_choose_splits(int B, int H, int Hkv, int page_size, int max_pages) {
     if (B < 1 || H < 1 || Hkv < 1 || page_size < 1 || max_pages < 1) return 1;
     const long long units = (long long)B * Hkv * ((H / Hkv + 15) / 16), room = (long long)max_pages * page_size;
     const long long slots = 2LL * dense_sm_count(), steps = (room + 63) / 64;
-    const bool finer = units > slots && units < 8 * slots;
+    const bool sorted = paged_sorted(B, H, Hkv, page_size, max_pages, 1);
+    const bool finer = !sorted && units > slots && units < 8 * slots;
+    const int most = (int)(steps < 148 ? steps : 148);
+    auto cost = [&](int s) { return (double)((units * s + slots - 1) / slots) * ((double)((steps + s - 1) / s) + 2.5) + (s > 1 ? 1.0 : 0.0); };
     double best = 1e30;
     int best_s = 1;
-    for (int s = 1; s <= 148 && s <= steps; ++s) {
-        const double rounds = (double)((units * s + slots - 1) / slots);
-        const double t = rounds * ((double)((steps + s - 1) / s) + 2.5) + (s > 1 ? 1.0 : 0.0);
+    for (int s = 1; s <= most; ++s) {
+        const double t = cost(s);
         if (t < (finer ? 1.05 : 0.999) * best) {
             if (t < best) best = t;
             best_s = s;
         }
     }
+    if (sorted)
+        for (int s = 1; s < best_s; ++s)
+            if (cost(s) <= 1.1 * best) return s;
     return best_s;
 }
 
@@ -518,13 +558,14 @@ extern "C" int hsa_paged_attn_decode(hsa_view q, hsa_view k_pages, hsa_view v_pa
     a.page = page_size; a.page_shift = (page_size & (page_size - 1)) == 0 ? ilog2((unsigned)page_size) : -1;
     a.num_pages = num_pages; a.max_pages = max_pages; a.splits = splits;
     a.scale_log2 = scale * 1.4426950408889634f;
+    const bool sorted = paged_sorted(B, H, Hkv, page_size, max_pages, splits);
     // Whole 16-byte pieces everywhere: the tensor-core kernel
     const bool mma = algo != 1 && dtype != HSA_F32 && D % 8 == 0 && view_vec_ok(k_pages, 2) && view_vec_ok(v_pages, 2) &&
                      view_vec_ok(hsa_view{q.ptr, q.batch_stride, 0}, 2) && view_vec_ok(hsa_view{out.ptr, out.batch_stride, 0}, 2);
     HSA_CHECK_ARG(algo != 2 || mma, "hsa_paged_attn_decode: no tensor-core kernel for these inputs");
     cudaStream_t st = (cudaStream_t)stream;
     int rc;
-    if (mma) rc = dtype == HSA_BF16 ? paged_mma<__nv_bfloat16>(a, st) : paged_mma<__half>(a, st);
+    if (mma) rc = dtype == HSA_BF16 ? paged_mma<__nv_bfloat16>(a, sorted, st) : paged_mma<__half>(a, sorted, st);
     else rc = dispatch_dtype(dtype, [&]<typename T>() -> int { return paged_simt<T>(a, st); });
     if (rc != 0 || splits == 1) return rc;
     const long long rows = (long long)B * H;

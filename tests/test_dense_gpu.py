@@ -504,6 +504,28 @@ def test_paged_decode(case, dtype, algo, splits):
     check_paged(*make_cache(B, H, Hkv, D, page, lengths, dtype, seed=D), algo=algo, splits=splits)
 
 
+@pytest.mark.parametrize("case", [(40, 8, 8, 64, 16), (128, 6, 3, 128, 16), (129, 3, 3, 64, 16), (65, 5, 5, 200, 32)])
+@pytest.mark.parametrize("splits", [None, 1, 2])
+def test_paged_many_sequences_of_unequal_length(case, splits):
+    """More blocks than run at once, where the longest sequences may start first: each sequence gives what it gives alone, bit by
+    bit, whatever the others' lengths (equal ones, none, ones that the table cannot hold)."""
+    B, H, Hkv, D, page = case
+    lengths = [(7 * i * i) % 400 for i in range(B)]
+    lengths[1], lengths[-2] = 2100, 1500
+    lengths[2] = lengths[3] = lengths[-1] = 300
+    lengths[4] = lengths[5] = 0
+    q, kp, vp, table, n = make_cache(B, H, Hkv, D, page, lengths, torch.bfloat16, seed=B)
+    chosen = _lib.load().hsa_paged_attn_choose_splits(B, H, Hkv, page, table.size(1)) if splits is None else splits
+    got = check_paged(q, kp, vp, table, n, splits=splits)
+    for b in (0, 1, 2, 3, 4, B // 2, B - 2, B - 1):
+        assert torch.equal(paged_attention_decode(q[b:b + 1], kp, vp, table[b:b + 1], n[b:b + 1], splits=chosen)[0], got[b])
+    wild = n.clone()
+    wild[0], wild[7], wild[8] = -1, table.size(1) * page + 1, 2 ** 31 - 1
+    bad = paged_attention_decode(q, kp, vp, table, wild, splits=splits)
+    others = [b for b in range(B) if b not in (0, 7, 8)]
+    assert bad[[0, 7, 8]].isnan().all() and torch.equal(bad[others], got[others])
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_paged_bad_pages_and_lengths_show_as_nan(dtype):
     """What the table must not hold is not followed: the sequence's output is NaN and the others are as before."""
