@@ -201,7 +201,10 @@ __global__ void __launch_bounds__(kPagedWarps * 32) paged_decode_simt_kernel(con
 // swizzled by the row number, which keeps ldmatrix free of bank conflicts.  The running maximum is raised, and the sums
 // rescaled, only when a score exceeds it by 2^8.  Weights are rounded to the type for the second product; their sum is not.
 template <int DP> struct PagedShape {
-    static constexpr int kStages = DP == 64 ? 6 : 3;
+    // Three stages: at head dims up to 64 four blocks then share an SM, and one block's first loads pass under another's loop (six
+    // stages and two blocks, the same bytes in flight: 20 sequences of 8192 keys, 16 heads of 64, 166 us against 115; 100 of 512, 71
+    // against 45).  Two stages and three blocks at head dim 128: 92.9 us against 87.5 for 2 x 131072 keys.
+    static constexpr int kStages = 3;
     static constexpr int kStage = 2 * 16 * DP * 2;                               // 16 rows of K and of V
     static constexpr int kSmem = kPagedWarps * kStages * kStage + 2 * kPagedWarps * 16 * 4;
 };
@@ -495,7 +498,7 @@ static bool paged_sorted(int B, int H, int Hkv, int page_size, int max_pages, in
     return B > 1 && B <= kPagedWarps * 32 && blocks > 2LL * dense_sm_count() && room >= (long long)splits * (B > 64 ? 8 * B : 512);
 }
 
-// Ranges per sequence.  Two blocks fit an SM; a block costs its steps of 64 keys plus about two and a half steps' time, and the join
+// Ranges per sequence.  Two blocks fit an SM (four at small head dims, where the same counts came out near the best); a block costs its steps of 64 keys plus about two and a half steps' time, and the join
 // about one.  The count with the least (rounds of blocks) x (cost of a block): one full round where that fits (2 sequences of
 // 131072 keys on 8 key/value heads: 88.6 us in 37 ranges, 97.9 in 74, 143 in 16).  With more sequences than blocks fit at once,
 // where lengths may differ: the coarsest cut that costs no more than a tenth if the longest come first (32 sequences of up to 4096
