@@ -173,7 +173,7 @@ __device__ __forceinline__ int taken_over(uint32_t response) {
     return item;
 }
 
-// A short wait of its own, for a block that has given up and looks whether more items were handed to it
+// A wait of its own limit, for a block that has given up
 __device__ __forceinline__ bool mbar_wait_limited(uint32_t mb, uint32_t parity, long long limit) {
     const long long start = clock64();
     while (!tc5::mbar_try(mb, parity))
@@ -184,10 +184,37 @@ __device__ __forceinline__ bool mbar_wait_limited(uint32_t mb, uint32_t parity, 
 // Shared-memory side of it; barriers: info_full[2], info_empty[2], answer.
 struct ItemSlots {
     int item[2];
-    int pad[2];
+    int closed;                          // -1; in a block that has given up, how many items the copy warp has handed on
+    int pad;
     uint4 answer;
     uint8_t flags[2][kFlagTiles];
 };
 constexpr int kItemBars = 5;
+
+// In a block that has given up every item it holds must still be answered for, since a block number that was taken over runs
+// nowhere else.  The element-wise warps void the one they could not finish and those that the copy warp had handed on
+// already (`handed_on`, place k of the sequence); the copy warp hands on no more (`close_items`) and voids the one that is then
+// still on its way (`item_on_its_way`: in its hand, or in an answer that it waits for).
+constexpr long long kGiveUpCycles = 20000000;                    // each of these waits ends by itself in microseconds
+__device__ __forceinline__ bool handed_on(ItemSlots &items, uint32_t mb, int k) {
+    const volatile int *closed = &items.closed;
+    const long long start = clock64();
+    bool there;
+    while (!(there = tc5::mbar_try(mb, (k >> 1) & 1))) {
+        const int n = *closed;
+        if ((n >= 0 && k >= n) || clock64() - start > kGiveUpCycles) break;
+    }
+    return __all_sync(0xffffffffu, there);
+}
+__device__ __forceinline__ void close_items(ItemSlots &items, int count, int lane) {
+    __syncwarp();
+    if (lane == 0) *const_cast<volatile int *>(&items.closed) = count;
+    __syncwarp();
+}
+__device__ __forceinline__ int item_on_its_way(ItemSlots &items, bool asked, uint32_t answer, int k, int in_hand) {
+    if (!asked) return in_hand;
+    const bool there = __all_sync(0xffffffffu, mbar_wait_limited(answer, k & 1, kGiveUpCycles));
+    return there ? taken_over(smem_u32(&items.answer)) : -1;
+}
 
 }  // namespace hsa

@@ -93,6 +93,7 @@ dense_dq_tc5_kernel(const DenseArgs a, const BwdSplit sp, const __grid_constant_
         for (int s = 0; s < VS; ++s) { mbar_init(v_full(s), 1); mbar_init(v_empty(s), 1); }
         for (int x = 0; x < 2; ++x) { mbar_init(s_full(x), 1); mbar_init(d_full(x), 8); mbar_init(s_free(x), 1); mbar_init(info_full(x), 1); mbar_init(info_empty(x), 10); }
         *abort_flag = 0;
+        items.closed = -1;
         mbar_fence_init();
         prefetch_map(&map_q); prefetch_map(&map_k); prefetch_map(&map_v); prefetch_map(&map_g);
     }
@@ -102,6 +103,15 @@ dense_dq_tc5_kernel(const DenseArgs a, const BwdSplit sp, const __grid_constant_
     fence_after_sync();
     const uint32_t tmem = *tmem_slot;
     auto wait = [&](uint32_t bar, uint32_t parity) { return (bool)__all_sync(0xffffffffu, mbar_wait(bar, parity, sp.wait_limit, abort_flag)); };
+    // Gave up: a row of an item that will not be computed reads NaN
+    auto void_row = [&](const DqItem &it, int qi) {
+        if (qi >= a.Lq) return;
+        const float nan = __int_as_float(0x7fffffff);
+        if (sp.splits > 1)
+            for (int d = 0; d < a.D; ++d) sp.part[((((int64_t)it.split * a.B + it.b) * a.Lq + qi) * a.H + it.h) * a.D + d] = nan;
+        else
+            fill_row<T>((T *)a.dq.ptr + it.b * a.dq.batch_stride + (int64_t)qi * a.dq.row_stride + (int64_t)it.h * a.D, a.D, nan);
+    };
 
     if (warp == 8) {
         bool ok = true;
@@ -110,8 +120,9 @@ dense_dq_tc5_kernel(const DenseArgs a, const BwdSplit sp, const __grid_constant_
 #pragma unroll
             for (int p = 0; p < PLANES; ++p) tma_load_4d(smem_addr(dst + p * PLANE), map, p * 64, head, row, b, bar);
         };
-        int item = blockIdx.x;
-        for (int k = 0; ok; ++k) {
+        int item = blockIdx.x, k = 0, handed = 0;
+        bool asked = false;
+        for (; ok; ++k) {
             const int is = k & 1;
             if (!(ok = wait(info_empty(is), ((k >> 1) & 1) ^ 1))) break;
             if (item >= 0 && masked) {
@@ -122,10 +133,10 @@ dense_dq_tc5_kernel(const DenseArgs a, const BwdSplit sp, const __grid_constant_
             if (lane == 0) items.item[is] = item;
             __syncwarp();
             if (lane == 0) mbar_arrive(info_full(is));
+            ++handed;
             if (item < 0) break;
             // The next item is asked for when this one's last copies are due: an item taken over earlier would wait here while
             // other SMs run dry.
-            bool asked = false;
             auto ask = [&]() {
                 if (!asked && lane == 0) {
                     mbar_expect_tx(answer, 16);
@@ -169,8 +180,16 @@ dense_dq_tc5_kernel(const DenseArgs a, const BwdSplit sp, const __grid_constant_
             ask();
             if (!(ok = wait(answer, k & 1))) break;
             item = taken_over(smem_addr(&items.answer));
+            asked = false;
         }
         if (!ok) {
+            close_items(items, handed, lane);
+            const int lost = item_on_its_way(items, asked, answer, k, handed > k ? -1 : item);
+            if (lost >= 0) {
+                const DqItem it(a, sp.splits, lost);
+                for (int row = lane; row < 128; row += 32) void_row(it, it.q0 + row);
+            }
+            // let copies already issued land before the block goes
             const long long start = clock64();
             while (clock64() - start < 200000) {}
         }
@@ -357,21 +376,15 @@ dense_dq_tc5_kernel(const DenseArgs a, const BwdSplit sp, const __grid_constant_
             __syncwarp();
             if (lane == 0) mbar_arrive(info_empty(is));
         }
-        if (!ok) {
-            // gave up: this item, and any that the block has already taken over, read NaN
+        if (!ok) {                                           // gave up: this item, and any handed on already
             for (;; ++k) {
                 if (item < 0) {
-                    if (!__all_sync(0xffffffffu, mbar_wait_limited(info_full(k & 1), (k >> 1) & 1, 400000))) break;
+                    if (!handed_on(items, info_full(k & 1), k)) break;
                     item = items.item[k & 1];
                     if (item < 0) break;
                 }
                 const DqItem it(a, sp.splits, item);
-                const float nan = __int_as_float(0x7fffffff);
-                const int qi = it.q0 + row;
-                if (qi < a.Lq && sp.splits > 1)
-                    for (int d = 0; d < a.D; ++d) sp.part[((((int64_t)it.split * a.B + it.b) * a.Lq + qi) * a.H + it.h) * a.D + d] = nan;
-                else if (qi < a.Lq)
-                    fill_row<T>((T *)a.dq.ptr + it.b * a.dq.batch_stride + (int64_t)qi * a.dq.row_stride + (int64_t)it.h * a.D, a.D, nan);
+                void_row(it, it.q0 + row);
                 item = -1;
             }
         }
@@ -449,6 +462,7 @@ dense_dkdv_tc5_kernel(const DenseArgs a, const BwdSplit sp, const __grid_constan
         for (int x = 0; x < 2; ++x) { mbar_init(s_full(x), 1); mbar_init(d_full(x), 8); mbar_init(s_free(x), 1); mbar_init(info_full(x), 1); mbar_init(info_empty(x), 10); }
         for (int s = 0; s < ST; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
         *abort_flag = 0;
+        items.closed = -1;
         mbar_fence_init();
         prefetch_map(&map_q); prefetch_map(&map_k); prefetch_map(&map_v); prefetch_map(&map_g);
     }
@@ -458,6 +472,19 @@ dense_dkdv_tc5_kernel(const DenseArgs a, const BwdSplit sp, const __grid_constan
     fence_after_sync();
     const uint32_t tmem = *tmem_slot;
     auto wait = [&](uint32_t bar, uint32_t parity) { return (bool)__all_sync(0xffffffffu, mbar_wait(bar, parity, sp.wait_limit, abort_flag)); };
+    auto part_row = [&](const DkvItem &it, int x, int key) {
+        return sp.part + (((((int64_t)(x == 0 ? sp.splits : 0) + it.split) * a.B + it.b) * a.Lk + key) * a.Hkv + it.hk) * a.D;
+    };
+    // Gave up: a row (x = 0: of dv, 1: of dk) of an item that will not be computed reads NaN
+    auto void_row = [&](const DkvItem &it, int x, int key) {
+        if (key >= a.Lk) return;
+        const float nan = __int_as_float(0x7fffffff);
+        const hsa_view &g = x == 0 ? a.dv : a.dk;
+        if (sp.splits > 1)
+            for (int d = 0; d < a.D; ++d) part_row(it, x, key)[d] = nan;
+        else
+            fill_row<T>((T *)g.ptr + it.b * g.batch_stride + (int64_t)key * g.row_stride + (int64_t)it.hk * a.D, a.D, nan);
+    };
     auto plane_of = [&](int b, int h) { return (int64_t)b * a.mask.plane_b + (int64_t)h * a.mask.plane_h; };
     auto flag_of = [&](int is, int u) { return items.flags[is][u / qtiles * cells + (a.mask.rows > 1 ? (u % qtiles) >> 1 : 0)]; };
     auto next_unit = [&](int is, int u, int total) {
@@ -468,8 +495,9 @@ dense_dkdv_tc5_kernel(const DenseArgs a, const BwdSplit sp, const __grid_constan
     if (warp == 8) {
         bool ok = true;
         int s = 0; uint32_t ph = 0, kc = 0;
-        int item = blockIdx.x;
-        for (int k = 0; ok; ++k) {
+        int item = blockIdx.x, k = 0, handed = 0;
+        bool asked = false;
+        for (; ok; ++k) {
             const int is = k & 1;
             if (!(ok = wait(info_empty(is), ((k >> 1) & 1) ^ 1))) break;
             if (item >= 0 && masked) {
@@ -481,10 +509,10 @@ dense_dkdv_tc5_kernel(const DenseArgs a, const BwdSplit sp, const __grid_constan
             if (lane == 0) items.item[is] = item;
             __syncwarp();
             if (lane == 0) mbar_arrive(info_full(is));
+            ++handed;
             if (item < 0) break;
             // The next item is asked for when this one's last copies are due: an item taken over earlier would wait here while
             // other SMs run dry.
-            bool asked = false;
             auto ask = [&]() {
                 if (!asked && lane == 0) {
                     mbar_expect_tx(answer, 16);
@@ -530,8 +558,19 @@ dense_dkdv_tc5_kernel(const DenseArgs a, const BwdSplit sp, const __grid_constan
             ask();
             if (!(ok = wait(answer, k & 1))) break;
             item = taken_over(smem_addr(&items.answer));
+            asked = false;
         }
         if (!ok) {
+            close_items(items, handed, lane);
+            const int lost = item_on_its_way(items, asked, answer, k, handed > k ? -1 : item);
+            if (lost >= 0) {
+                const DkvItem it(a, sp.splits, lost, qtiles);
+                for (int row = lane; row < 128; row += 32) {
+                    void_row(it, 0, it.k0 + row);
+                    void_row(it, 1, it.k0 + row);
+                }
+            }
+            // let copies already issued land before the block goes
             const long long start = clock64();
             while (clock64() - start < 200000) {}
         }
@@ -618,9 +657,6 @@ dense_dkdv_tc5_kernel(const DenseArgs a, const BwdSplit sp, const __grid_constan
         const int x = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane;      // warpgroup x: queries [32 x, 32 x + 32) of a tile
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
         const uint64_t c2 = pair(a.scale_log2, a.scale_log2);
-        auto part_row = [&](const DkvItem &it, int key) {
-            return sp.part + (((((int64_t)(x == 0 ? sp.splits : 0) + it.split) * a.B + it.b) * a.Lk + key) * a.Hkv + it.hk) * a.D;
-        };
         bool ok = true;
         uint32_t i = 0, kc = 0;                              // tiles, and items that had any
         int s = 0, k = 0, item = -1; uint32_t ph = 0;
@@ -701,7 +737,7 @@ dense_dkdv_tc5_kernel(const DenseArgs a, const BwdSplit sp, const __grid_constan
                     for (int j = 0; j < 32; ++j) o[j] = 0u;
                 }
                 if (sp.splits > 1)
-                    store_rows32_f32(part_row(it, key), (int64_t)a.Hkv * a.D, a.Lk - key, 32 * c, a.D, o);
+                    store_rows32_f32(part_row(it, x, key), (int64_t)a.Hkv * a.D, a.Lk - key, 32 * c, a.D, o);
                 else
                     store_rows32<T>(out, g.row_stride, a.Lk - key, 32 * c, a.D, o, x == 0 ? 1.f : a.scale);
             }
@@ -709,22 +745,15 @@ dense_dkdv_tc5_kernel(const DenseArgs a, const BwdSplit sp, const __grid_constan
             __syncwarp();
             if (lane == 0) mbar_arrive(info_empty(is));
         }
-        if (!ok) {
-            // gave up: this item, and any that the block has already taken over, read NaN
-            const hsa_view &g = x == 0 ? a.dv : a.dk;
+        if (!ok) {                                           // gave up: this item, and any handed on already
             for (;; ++k) {
                 if (item < 0) {
-                    if (!__all_sync(0xffffffffu, mbar_wait_limited(info_full(k & 1), (k >> 1) & 1, 400000))) break;
+                    if (!handed_on(items, info_full(k & 1), k)) break;
                     item = items.item[k & 1];
                     if (item < 0) break;
                 }
                 const DkvItem it(a, sp.splits, item, qtiles);
-                const float nan = __int_as_float(0x7fffffff);
-                const int key = it.k0 + row;
-                if (key < a.Lk && sp.splits > 1)
-                    for (int d = 0; d < a.D; ++d) part_row(it, key)[d] = nan;
-                else if (key < a.Lk)
-                    fill_row<T>((T *)g.ptr + it.b * g.batch_stride + (int64_t)key * g.row_stride + (int64_t)it.hk * a.D, a.D, nan);
+                void_row(it, x, it.k0 + row);
                 item = -1;
             }
         }

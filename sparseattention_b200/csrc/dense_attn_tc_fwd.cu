@@ -103,6 +103,7 @@ dense_fwd_tc5_kernel(const DenseArgs a, const DenseSplit sp, const __grid_consta
         for (int s = 0; s < SLOTS; ++s) { mbar_init(kv_full(s), 1); mbar_init(kv_empty(s), 2); }
         mbar_init(answer, 1);
         *abort_flag = 0;
+        items.closed = -1;
         mbar_fence_init();
         prefetch_map(&map_q); prefetch_map(&map_k); prefetch_map(&map_v);
     }
@@ -113,6 +114,16 @@ dense_fwd_tc5_kernel(const DenseArgs a, const DenseSplit sp, const __grid_consta
     const uint32_t tmem = *tmem_slot;
     // a whole warp waits, and goes on or gives up as one
     auto wait = [&](uint32_t bar, uint32_t parity) { return (bool)__all_sync(0xffffffffu, mbar_wait(bar, parity, sp.wait_limit, abort_flag)); };
+    // Gave up: a row of an item that will not be computed reads NaN
+    auto void_row = [&](const FwdItem &it, int qi) {
+        if (qi >= a.Lq) return;
+        const float nan = __int_as_float(0x7fffffff);
+        const int64_t at = (((int64_t)it.split * a.B + it.b) * a.Lq + qi) * a.H + it.h;
+        if (sp.splits > 1) { *reinterpret_cast<float2 *>(sp.part_ml + 2 * at) = make_float2(0.f, nan); return; }
+        fill_row<T>((T *)a.out.ptr + it.b * a.out.batch_stride + (int64_t)qi * a.out.row_stride + (int64_t)it.h * a.D, a.D, nan);
+        if (a.out_lo != nullptr) fill_row<T>((T *)a.out_lo + at * a.D, a.D, nan);
+        if (a.lse != nullptr) a.lse[at] = nan;
+    };
 
     if (warp == 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 104;\n");
@@ -130,8 +141,9 @@ dense_fwd_tc5_kernel(const DenseArgs a, const DenseSplit sp, const __grid_consta
             __syncwarp();
             if (++slot == SLOTS) { slot = 0; ph ^= 1; }
         };
-        int item = blockIdx.x;
-        for (int k = 0; ok; ++k) {
+        int item = blockIdx.x, k = 0, handed = 0;
+        bool asked = false;
+        for (; ok; ++k) {
             const int is = k & 1;
             if (!(ok = wait(info_empty(is), ((k >> 1) & 1) ^ 1))) break;
             if (item >= 0 && masked) {
@@ -149,10 +161,10 @@ dense_fwd_tc5_kernel(const DenseArgs a, const DenseSplit sp, const __grid_consta
             if (lane == 0) items.item[is] = item;
             __syncwarp();
             if (lane == 0) mbar_arrive(info_full(is));
+            ++handed;
             if (item < 0) break;
             // The next item is asked for when this one's last copies are due: an item taken over earlier would wait here while
             // other SMs run dry.
-            bool asked = false;
             auto ask = [&]() {
                 if (!asked && lane == 0) {
                     mbar_expect_tx(answer, 16);
@@ -187,8 +199,16 @@ dense_fwd_tc5_kernel(const DenseArgs a, const DenseSplit sp, const __grid_consta
             ask();
             if (!(ok = wait(answer, k & 1))) break;
             item = taken_over(smem_addr(&items.answer));
+            asked = false;
         }
-        if (!ok) {                                       // let copies already issued land before the block goes
+        if (!ok) {
+            close_items(items, handed, lane);
+            const int lost = item_on_its_way(items, asked, answer, k, handed > k ? -1 : item);
+            if (lost >= 0) {
+                const FwdItem it(a, sp.splits, lost);
+                for (int row = lane; row < 128 * it.nw; row += 32) void_row(it, it.q0 + row);
+            }
+            // let copies already issued land before the block goes
             const long long start = clock64();
             while (clock64() - start < 200000) {}
         }
@@ -446,23 +466,15 @@ dense_fwd_tc5_kernel(const DenseArgs a, const DenseSplit sp, const __grid_consta
             __syncwarp();
             if (lane == 0) mbar_arrive(info_empty(is));
         }
-        if (!ok) {
-            // gave up: this item, and any that the block has already taken over, read NaN
-            const float nan = __int_as_float(0x7fffffff);
+        if (!ok) {                                           // gave up: this item, and any handed on already
             for (;; ++k) {
                 if (item < 0) {
-                    if (!__all_sync(0xffffffffu, mbar_wait_limited(info_full(k & 1), (k >> 1) & 1, 400000))) break;
+                    if (!handed_on(items, info_full(k & 1), k)) break;
                     item = items.item[k & 1];
                     if (item < 0) break;
                 }
                 const FwdItem it(a, sp.splits, item);
-                const int qi = it.q0 + 128 * w + row;
-                if (qi < a.Lq) {
-                    const int64_t at = (((int64_t)it.split * a.B + it.b) * a.Lq + qi) * a.H + it.h;
-                    if (sp.splits > 1) *reinterpret_cast<float2 *>(sp.part_ml + 2 * at) = make_float2(0.f, nan);
-                    else fill_row<T>((T *)a.out.ptr + it.b * a.out.batch_stride + (int64_t)qi * a.out.row_stride + (int64_t)it.h * a.D, a.D, nan);
-                    if (sp.splits == 1 && a.lse != nullptr) a.lse[at] = nan;
-                }
+                if (w < it.nw) void_row(it, it.q0 + 128 * w + row);
                 item = -1;
             }
         }
