@@ -19,7 +19,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from ..ops.dense import cross_attention
+from ..ops.dense import cross_attention, transforms_active
 from ..ops.functional import build_parent_nodes, hierarchical_attention
 from ..ops.topology import build_tree_topology, generate_span_input_Y  # noqa: F401  (re-exported like the reference)
 
@@ -47,7 +47,9 @@ class HierarchicalAttention(nn.Module):
         Otherwise (no parents, or key rows of another length: an encoder's states, a memory) plain multi-head
         attention of `query` over `key` / `value`; `mask == 0` hides an entry.  On CUDA in bfloat16 or float16, with no
         dropout active and no weights asked for, that runs as one kernel (ops.dense.cross_attention) without the
-        [B, H, L_Q, L_K] matrix; set `fused_attention = False` for the eager operations (differentiable twice).
+        [B, H, L_Q, L_K] matrix; set `fused_attention = False` for the eager operations (differentiable twice).  While torch
+        traces, compiles or transforms the module, watches its operations or carries forward-mode tangents, it runs the eager
+        operations.
     cross_update_Y(x, y_in)  bottom-up refresh of the parents from x.
     update_X_from_Y(x, y, mask=None)  the top-down pass used by forward.
     """
@@ -148,7 +150,9 @@ class HierarchicalAttention(nn.Module):
     def _dense_mask(self, q, k, v, mask):
         """(whether the dense kernel takes these inputs, the mask in its form)."""
         B, L_Q, H, Dh = q.shape
-        if not (self.fused_attention and q.is_cuda and q.dtype in (torch.bfloat16, torch.float16) and k.shape == v.shape
+        if not self.fused_attention or transforms_active() or not type(q) is type(k) is type(v) is torch.Tensor:
+            return False, None
+        if not (q.is_cuda and q.dtype in (torch.bfloat16, torch.float16) and k.shape == v.shape
                 and k.dtype == v.dtype == q.dtype and Dh % 8 == 0 and Dh <= 128 and k.size(1) > 0):
             return False, None
         if self.training and self.dropout.p > 0.0:

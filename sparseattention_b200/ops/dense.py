@@ -14,8 +14,40 @@ from ctypes import c_void_p
 from typing import NamedTuple, Optional, Tuple
 
 import torch
+from torch._compile import _disable_dynamo
+from torch.autograd import forward_ad
 
 from .. import _lib
+
+
+# The kernels write through raw pointers: of a call, a tracer or a transform would see the allocation of the result and nothing that
+# fills it, and a forward-mode tangent would end there.
+_INFRA_MODES = (torch._C._TorchDispatchModeKey.PROXY, torch._C._TorchDispatchModeKey.FAKE, torch._C._TorchDispatchModeKey.FUNCTIONAL)
+
+
+def transforms_active() -> bool:
+    """Whether torch is tracing, compiling, transforming or watching operations, or computes forward-mode derivatives."""
+    return (torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() > 0 or torch._C._get_tracing_state() is not None
+            or forward_ad._current_level >= 0 or torch._C._functorch.peek_interpreter_stack() is not None)
+
+
+def _refuse_transforms(who: str, *tensors: Optional[torch.Tensor]) -> None:
+    if not transforms_active():
+        return
+    if torch._C._get_tracing_state() is not None or any(torch._C._get_dispatch_mode(m) is not None for m in _INFRA_MODES):
+        raise _lib.HsaError(f"{who} cannot be traced: the graph would hold the allocation of its result and not the kernel")
+    for t in tensors:
+        if t is None:
+            continue
+        if torch._C._functorch.is_functorch_wrapped_tensor(t) or torch._is_functional_tensor(t):
+            raise _lib.HsaError(f"{who} has no rule for torch.func transforms")
+        if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+            raise _lib.HsaError(f"{who} has no forward-mode derivative; its inputs must not carry tangents")
+
+
+@_disable_dynamo
+def _outside_the_graph(op, *args):
+    return op(*args)
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
@@ -267,7 +299,15 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, key_lengt
     Differentiable once with respect to q, k and v.  In bfloat16 and float16 the weights and the gradients of the scores are
     rounded to that type between the products (a gradient of a score beyond 65504 in float16 is infinite); sums are 32-bit.
     A mask is packed into bits by every call; keys that only a length hides are cheaper given as key_lengths.
+    torch.compile breaks its graph here; tracing, torch.func transforms and forward-mode tangents are refused.
     """
+    if torch.compiler.is_compiling():
+        return _outside_the_graph(_cross_attention, q, k, v, key_lengths, mask, scale, empty_value, algo)
+    return _cross_attention(q, k, v, key_lengths, mask, scale, empty_value, algo)
+
+
+def _cross_attention(q, k, v, key_lengths, mask, scale, empty_value, algo):
+    _refuse_transforms("cross_attention", q, k, v, key_lengths, mask)
     dev = _check_inputs(q, k, v)
     B, Lq, H, D = q.shape
     Lk = k.size(1)
@@ -298,7 +338,15 @@ def paged_attention_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     Returns [B, H, D] of q's type; zeros for a length of 0.  A page number outside the pages that the length reaches, or a length the
     table cannot hold, makes that sequence's output NaN; table entries behind the length are not read.
     splits: ranges a sequence's keys are cut into (None: chosen from the sizes).  No autograd.
+    torch.compile breaks its graph here; tracing, torch.func transforms and forward-mode tangents are refused.
     """
+    if torch.compiler.is_compiling():
+        return _outside_the_graph(_paged_attention_decode, q, k_pages, v_pages, page_table, lengths, scale, splits, algo)
+    return _paged_attention_decode(q, k_pages, v_pages, page_table, lengths, scale, splits, algo)
+
+
+def _paged_attention_decode(q, k_pages, v_pages, page_table, lengths, scale, splits, algo):
+    _refuse_transforms("paged_attention_decode", q, k_pages, v_pages, page_table, lengths)
     lib = _lib.load()
     dev = _lib.require_cuda(q, k_pages, v_pages, page_table, lengths)
     dt = _lib.dtype_code(q)

@@ -1,0 +1,91 @@
+"""HierarchicalAttention over another sequence: what its elementary operations could do, it can do where a kernel stands in for them."""
+import pytest
+import torch
+from torch.autograd import forward_ad
+from torch.utils.flop_counter import FlopCounterMode
+
+from sparseattention_b200 import HierarchicalAttention
+from sparseattention_b200.ops import cross_attention
+from tests.conftest import rel_err
+
+pytestmark = pytest.mark.gpu
+
+
+def layer_and_rows(dtype=torch.bfloat16, d=128, H=2, dropout=0.1, seed=3, **kind):
+    torch.manual_seed(seed)
+    layer = kind.get("cls", HierarchicalAttention)(d, H, dropout=dropout).cuda().to(dtype).eval()
+    q, m = (torch.randn(2, n, d, device="cuda").to(dtype) for n in (9, 13))
+    return layer, q, m
+
+
+def eager(layer, *args, **kw):
+    layer.fused_attention = False
+    try:
+        return layer(*args, **kw)
+    finally:
+        del layer.fused_attention
+
+
+def test_traced_module_follows_its_inputs():
+    layer, q, m = layer_and_rows()
+    mask = torch.rand(9, 13, device="cuda") < 0.7
+    mask[:, 0] = True
+    with torch.no_grad():
+        traced = torch.jit.trace(layer, example_kwarg_inputs={"query": q, "key": m, "value": m.clone(), "mask": mask})
+        q2, m2, mask2 = q * 0.5 + 1, m.flip(1), mask.flip(1) | (torch.arange(13, device="cuda") == 0)
+        assert torch.equal(traced(query=q2, key=m2, value=m2, mask=mask2), eager(layer, q2, m2, m2, mask=mask2))
+
+
+def test_module_in_one_compiled_graph():
+    layer, q, m = layer_and_rows()
+    torch._dynamo.reset()
+    compiled = torch.compile(lambda q, m: layer(q, m, m), backend="eager", fullgraph=True)
+    with torch.no_grad():
+        assert torch.equal(compiled(q, m), eager(layer, q, m, m))
+    torch._dynamo.reset()
+
+
+def test_compiled_caller_of_the_operator():
+    q, k = torch.randn(2, 9, 2, 64, device="cuda").bfloat16(), torch.randn(2, 13, 2, 64, device="cuda").bfloat16()
+    torch._dynamo.reset()
+    compiled = torch.compile(lambda q, k: cross_attention(q * 2, k, k) + 1, backend="eager")
+    assert torch.equal(compiled(q, k), cross_attention(q * 2, k, k) + 1)
+    leaf = q.clone().requires_grad_(True)
+    (got,) = torch.autograd.grad(compiled(leaf, k).float().square().sum(), leaf)
+    (want,) = torch.autograd.grad((cross_attention(leaf * 2, k, k) + 1).float().square().sum(), leaf)
+    assert torch.equal(got, want)
+    torch._dynamo.reset()
+
+
+@pytest.mark.parametrize("frozen", [True, False])
+def test_forward_mode_tangents_pass_through_the_module(frozen):
+    layer, q, m = layer_and_rows()
+    layer.requires_grad_(not frozen)
+    dq = torch.randn_like(q)
+    want = torch.func.jvp(lambda q: eager(layer, q, m, m), (q,), (dq,))[1]
+    with forward_ad.dual_level():
+        got = forward_ad.unpack_dual(layer(forward_ad.make_dual(q, dq), m, m)).tangent
+    assert got is not None and torch.equal(got, want)
+    assert torch.equal(torch.func.jvp(lambda q: layer(q, m, m), (q,), (dq,))[1], want)
+
+
+def test_module_under_vmap_and_per_sample_gradients():
+    layer, q, m = layer_and_rows()
+    many = torch.stack([q, q.flip(1), -q])
+    got = torch.vmap(lambda q: layer(q, m, m))(many)
+    for i in range(3):
+        assert rel_err(got[i].detach().float(), eager(layer, many[i], m, m).detach().float()) < 2e-2
+    grads = torch.func.grad(lambda q: layer(q, m, m).float().square().sum())(q)
+    leaf = q.clone().requires_grad_(True)
+    (want,) = torch.autograd.grad(eager(layer, leaf, m, m).float().square().sum(), leaf)
+    assert torch.equal(grads, want)
+
+
+def test_watched_operations_are_the_elementary_ones():
+    layer, q, m = layer_and_rows()
+    counts = []
+    for call in (layer, lambda *a: eager(layer, *a)):
+        with FlopCounterMode(display=False) as counter, torch.no_grad():
+            call(q, m, m)
+        counts.append(counter.get_total_flops())
+    assert counts[0] == counts[1]
