@@ -155,7 +155,8 @@ class HierarchicalAttention(nn.Module):
         if not (q.is_cuda and q.dtype in (torch.bfloat16, torch.float16) and k.shape == v.shape
                 and k.dtype == v.dtype == q.dtype and Dh % 8 == 0 and Dh <= 128 and k.size(1) > 0):
             return False, None
-        if self.training and self.dropout.p > 0.0:
+        # a module of another kind in its place, or a dropout kept active in evaluation, goes through the weights
+        if type(self.dropout) is not nn.Dropout or (self.dropout.training and self.dropout.p > 0.0):
             return False, None
         if mask is None:
             return True, None

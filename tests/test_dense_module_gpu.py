@@ -89,3 +89,28 @@ def test_watched_operations_are_the_elementary_ones():
             call(q, m, m)
         counts.append(counter.get_total_flops())
     assert counts[0] == counts[1]
+
+
+class Doubled(torch.nn.Module):
+    def forward(self, weights):
+        return weights * 2
+
+
+@pytest.mark.parametrize("kind", ["kept active", "identity", "other", "probability"])
+def test_the_dropout_that_is_there_decides(kind):
+    """Dropout sampled in evaluation, no dropout at all, another module in its place."""
+    layer, q, m = layer_and_rows()
+    if kind == "kept active":
+        layer.dropout.train()
+    elif kind == "identity":
+        layer.dropout = torch.nn.Identity()
+        layer.train()
+    elif kind == "other":
+        layer.dropout = Doubled()
+    else:
+        layer.dropout.p = 0.9
+        layer.dropout.train()
+    torch.manual_seed(11)
+    got = layer(q, m, m)
+    torch.manual_seed(11)
+    assert torch.equal(got, eager(layer, q, m, m))
