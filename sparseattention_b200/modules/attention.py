@@ -156,7 +156,13 @@ class HierarchicalAttention(nn.Module):
                 and k.dtype == v.dtype == q.dtype and Dh % 8 == 0 and Dh <= 128 and k.size(1) > 0):
             return False, None
         # a module of another kind in its place, or a dropout kept active in evaluation, goes through the weights
-        if type(self.dropout) is not nn.Dropout or (self.dropout.training and self.dropout.p > 0.0):
+        drop = self.dropout
+        if type(drop) is not nn.Dropout or (drop.training and drop.p > 0.0):
+            return False, None
+        # so do hooks that change what passes through it, and an attention of a subclass or of this object
+        if drop._forward_pre_hooks or drop._backward_hooks or drop._backward_pre_hooks:
+            return False, None
+        if getattr(self._standard_attention, "__func__", None) is not HierarchicalAttention._standard_attention:
             return False, None
         if mask is None:
             return True, None

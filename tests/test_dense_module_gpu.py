@@ -114,3 +114,25 @@ def test_the_dropout_that_is_there_decides(kind):
     got = layer(q, m, m)
     torch.manual_seed(11)
     assert torch.equal(got, eager(layer, q, m, m))
+
+
+class Sharper(HierarchicalAttention):
+    def _standard_attention(self, Q, K, V, mask):
+        return super()._standard_attention(2 * Q, K, V, mask)
+
+
+@pytest.mark.parametrize("kind", ["subclass", "object", "pre-hook", "backward hook"])
+def test_what_replaces_or_enters_the_elementary_operations_is_called(kind):
+    layer, q, m = layer_and_rows(cls=Sharper if kind == "subclass" else HierarchicalAttention)
+    seen = []
+    if kind == "object":
+        inner = layer._standard_attention
+        layer._standard_attention = lambda Q, K, V, mask: inner(Q, K, -V, mask)
+    elif kind == "pre-hook":
+        layer.dropout.register_forward_pre_hook(lambda mod, args: (args[0] * 3,))
+    elif kind == "backward hook":
+        layer.dropout.register_full_backward_hook(lambda *a: seen.append(1))
+    got, want = layer(q, m, m), eager(layer, q, m, m)
+    assert torch.equal(got, want)
+    got.float().sum().backward()
+    assert kind != "backward hook" or seen
