@@ -19,7 +19,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from ..ops.dense import cross_attention, transforms_active
+from ..ops.dense import transforms_active, twice_differentiable_attention
 from ..ops.functional import build_parent_nodes, hierarchical_attention
 from ..ops.topology import build_tree_topology, generate_span_input_Y  # noqa: F401  (re-exported like the reference)
 
@@ -47,9 +47,9 @@ class HierarchicalAttention(nn.Module):
         Otherwise (no parents, or key rows of another length: an encoder's states, a memory) plain multi-head
         attention of `query` over `key` / `value`; `mask == 0` hides an entry.  On CUDA in bfloat16 or float16, with no
         dropout active and no weights asked for, that runs as one kernel (ops.dense.cross_attention) without the
-        [B, H, L_Q, L_K] matrix; set `fused_attention = False` for the eager operations (differentiable twice).  While torch
-        traces, compiles or transforms the module, watches its operations or carries forward-mode tangents, it runs the eager
-        operations.
+        [B, H, L_Q, L_K] matrix, gradients included unless they are taken with create_graph.  While torch traces, compiles or
+        transforms the module, watches its operations or carries forward-mode tangents, it runs the eager operations;
+        set `fused_attention = False` to have them always (a forward hook on `dropout` is only called there).
     cross_update_Y(x, y_in)  bottom-up refresh of the parents from x.
     update_X_from_Y(x, y, mask=None)  the top-down pass used by forward.
     """
@@ -184,7 +184,7 @@ class HierarchicalAttention(nn.Module):
         q, k, v = split(query, self.Wq_x), split(key, self.Wk_x), split(value, self.Wv_x)
         fused, allowed = (False, None) if return_attention else self._dense_mask(q, k, v, mask)
         if fused:                                        # a row that the mask leaves empty is NaN, as a softmax over nothing is
-            return self.out_proj_x(cross_attention(q, k, v, mask=allowed, empty_value=math.nan).reshape(B, L_Q, D))
+            return self.out_proj_x(twice_differentiable_attention(q, k, v, allowed).reshape(B, L_Q, D))
         ctx, weights = self._standard_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), mask)
         output = self.out_proj_x(ctx.transpose(1, 2).reshape(B, L_Q, D))
         return (output, weights) if return_attention else output

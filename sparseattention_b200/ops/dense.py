@@ -245,28 +245,51 @@ def _once(grads):
     return _Once.apply(*(t.requires_grad_(True) for t in grads))
 
 
+def _unpack_mask(packed: _Packed, Lk: int) -> torch.Tensor:
+    """The truth values [batches, heads, rows, Lk] of a packed mask (its first array: bit k of a row's words = key k)."""
+    words = (Lk + 127) // 128 * 4
+    count = math.prod(packed.sizes) * words
+    bits = packed.data[:4 * count].view(torch.int32).view(*packed.sizes, words, 1) >> torch.arange(32, device=packed.data.device, dtype=torch.int32)
+    return (bits & 1).bool().flatten(3)[..., :Lk]
+
+
+def _elementary_gradients(q, k, v, dout, packed: Optional[_Packed], scale: float):
+    """(dq, dk, dv) in torch operations, which can be differentiated again.  Heads are not shared, no lengths, no rows to fill."""
+    q, k, v, dout = (t.transpose(1, 2) for t in (q, k, v, dout))
+    s = (q @ k.transpose(-1, -2)) * scale
+    if packed is not None:
+        s = s.masked_fill(~_unpack_mask(packed, k.size(2)), -math.inf)
+    p = s.softmax(dim=-1)
+    dp = dout @ v.transpose(-1, -2)
+    ds = p * (dp - (dp * p).sum(dim=-1, keepdim=True)) * scale
+    return tuple(t.transpose(1, 2) for t in (ds @ k, ds.transpose(-1, -2) @ q, p.transpose(-1, -2) @ dout))
+
+
 class _CrossAttention(torch.autograd.Function):
+    """twice: gradients of gradients are wanted where the engine records them (create_graph); otherwise they are refused."""
+
     @staticmethod
-    def forward(ctx, q, k, v, key_lengths, packed_mask, scale, empty_value, algo):
-        q, k, v = _rows(q), _rows(k), _rows(v)
+    def forward(ctx, q, k, v, key_lengths, packed_mask, scale, empty_value, algo, twice):
         out, rest, lse = dense_attention_forward(q, k, v, key_lengths, packed_mask, scale, empty_value, True, algo)
         if packed_mask is None:
             ctx.save_for_backward(q, k, v, out, rest, lse, key_lengths)
-            ctx.meta = (None, scale, algo)
+            ctx.meta = (None, scale, algo, twice)
         else:
             ctx.save_for_backward(q, k, v, out, rest, lse, key_lengths, packed_mask.data)
-            ctx.meta = (packed_mask.sizes, scale, algo)
+            ctx.meta = (packed_mask.sizes, scale, algo, twice)
         return out
 
     @staticmethod
     def backward(ctx, dout):
         q, k, v, out, rest, lse, key_lengths, *packed = ctx.saved_tensors
-        sizes, scale, algo = ctx.meta
+        sizes, scale, algo, twice = ctx.meta
+        packed = _Packed(packed[0], sizes) if packed else None
+        if twice and torch.is_grad_enabled():
+            return (*_elementary_gradients(q, k, v, dout, packed, scale), None, None, None, None, None, None)
         with _lib.on_device(q.device):
             dout = _rows(dout if dout.dtype == q.dtype else dout.to(q.dtype))
-            grads = dense_attention_backward(q, k, v, out, rest, lse, dout, key_lengths, _Packed(packed[0], sizes) if packed else None,
-                                             scale, algo)
-        return (*_once(grads), None, None, None, None, None)
+            grads = dense_attention_backward(q, k, v, out, rest, lse, dout, key_lengths, packed, scale, algo)
+        return (*_once(grads), None, None, None, None, None, None)
 
 
 class _NoRows(torch.autograd.Function):
@@ -306,7 +329,13 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, key_lengt
     return _cross_attention(q, k, v, key_lengths, mask, scale, empty_value, algo)
 
 
-def _cross_attention(q, k, v, key_lengths, mask, scale, empty_value, algo):
+def twice_differentiable_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """cross_attention for HierarchicalAttention: as many key/value heads as query heads, rows that see nothing are NaN, and gradients
+    taken with create_graph come from elementary operations (with the [B, H, Lq, Lk] weights), to be differentiated again."""
+    return _cross_attention(q, k, v, None, mask, None, math.nan, _lib.ALGO_AUTO, True)
+
+
+def _cross_attention(q, k, v, key_lengths, mask, scale, empty_value, algo, twice=False):
     _refuse_transforms("cross_attention", q, k, v, key_lengths, mask)
     dev = _check_inputs(q, k, v)
     B, Lq, H, D = q.shape
@@ -323,7 +352,7 @@ def _cross_attention(q, k, v, key_lengths, mask, scale, empty_value, algo):
     with _lib.on_device(dev):
         packed = None if mask is None else _pack_mask(mask, dev, Lk)
         if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-            return _CrossAttention.apply(q, k, v, key_lengths, packed, scale, float(empty_value), algo)
+            return _CrossAttention.apply(_rows(q), _rows(k), _rows(v), key_lengths, packed, scale, float(empty_value), algo, twice)
         return dense_attention_forward(_rows(q), _rows(k), _rows(v), key_lengths, packed, scale, float(empty_value), False, algo)[0]
 
 

@@ -136,3 +136,39 @@ def test_what_replaces_or_enters_the_elementary_operations_is_called(kind):
     assert torch.equal(got, want)
     got.float().sum().backward()
     assert kind != "backward hook" or seen
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("masked", [False, True])
+def test_gradients_of_gradients(dtype, masked):
+    """A penalty on the gradient of the queries, as the elementary operations give it: against the same weights in 32 bits within twice
+    2e-2, what the suite grants a 16-bit layer for one pass, of which this makes two.  The elementary operations have to hold that too.
+    The second pass's numbers are about 1e-9 here, and float16 has none between 0 and 2^-24: in that type an entry may be off by that
+    step on top, and a weight's gradient by as much for every row it sums, times the largest input."""
+    layer, q, m = layer_and_rows(dtype)
+    exact = HierarchicalAttention(128, 2).cuda().eval()
+    exact.load_state_dict({n: t.float() for n, t in layer.state_dict().items()})
+    mask = None
+    if masked:
+        mask = torch.rand(2, 1, 9, 13, device="cuda") < 0.6
+        mask[..., 0] = True
+    names = [n for n, _ in layer.named_parameters() if n[:2] in ("Wq", "Wk", "Wv") and n.split(".")[0].endswith("_x")]
+
+    def penalty(layer, q, m, mask, run):
+        ql, ml = q.clone().requires_grad_(True), m.clone().requires_grad_(True)
+        out = run(layer, ql, ml, ml, mask=mask)
+        if mask is not None:
+            mask.zero_()                                       # what the caller does with a mask afterwards changes nothing
+        (dq,) = torch.autograd.grad(out.float().square().mean(), ql, create_graph=True)
+        params = dict(layer.named_parameters())
+        return [dq] + list(torch.autograd.grad(dq.float().square().sum(), [ml] + [params[n] for n in names]))
+
+    copy = lambda: None if mask is None else mask.clone()                                                    # noqa: E731
+    want = penalty(exact, q.float(), m.float(), copy(), lambda layer, *a, **k: layer(*a, **k))
+    for run in (lambda layer, *a, **k: layer(*a, **k), eager):
+        for i, (got, ref) in enumerate(zip(penalty(layer, q, m, copy(), run), want)):
+            step = 0.0 if dtype == torch.bfloat16 else 2.0 ** -24 * (1.0 if i < 2 else 2 * 13 * float(torch.cat([q, m], 1).abs().max()))
+            assert got.isfinite().all()
+            diff = (got.detach().float() - ref.detach()).abs()
+            assert float(diff.max()) <= 4e-2 * float(ref.abs().max()) + step, i
+            assert float(diff.mean()) <= 4e-2 * float(ref.abs().mean()) + step, i
