@@ -474,7 +474,7 @@ dense_fwd_tc5_kernel(const DenseArgs a, const DenseSplit sp, const __grid_consta
                     if (item < 0) break;
                 }
                 const FwdItem it(a, sp.splits, item);
-                if (w < it.nw) void_row(it, it.q0 + 128 * w + row);
+                void_row(it, it.q0 + 128 * w + row);
                 item = -1;
             }
         }
