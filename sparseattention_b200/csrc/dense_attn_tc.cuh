@@ -35,24 +35,32 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
 }
 __device__ __forceinline__ uint64_t pair_bits(uint32_t lo, uint32_t hi) { return pair(__uint_as_float(lo), __uint_as_float(hi)); }
 
+// The largest of three; NaN if one of them is
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;\n" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
 // 2^x for both numbers of a pair without the special-function unit, x <= 8 (below -126: 2^-126).  x = n + f with n the nearest
-// whole number (the addition of 1.5 * 2^23 + 127 leaves n + 127, the exponent of 2^n, in the low bits), |f| <= 1/2, 2^f by the
-// degree-5 polynomial of least greatest relative error on that interval (found by exchange; 7.5e-8), times 2^n.  Off by at most
-// 2^-22 in 32-bit arithmetic, as the special-function unit is.  NaN stays NaN: the polynomial's value is one, and the factor that
-// its bits become (minus infinity) keeps it, where n added to the exponent made the largest finite number of it.
+// whole number (the addition of 1.5 * 2^23 leaves it in the low bits), |f| <= 1/2, 2^f by the degree-5 polynomial of least
+// greatest relative error on that interval (found by exchange; 7.5e-8), and n goes into the exponent.  Off by at most 2^-22 in
+// 32-bit arithmetic, as the special-function unit is.  NaN does not stay NaN (n added to its bits makes a finite number of them):
+// callers take care of it.
 __device__ __forceinline__ float2 exp2_poly(float2 x) {
-    asm("max.NaN.f32 %0, %0, 0fC2FC0000;\n" : "+f"(x.x));
-    asm("max.NaN.f32 %0, %0, 0fC2FC0000;\n" : "+f"(x.y));
+    x.x = fmaxf(x.x, -126.f);
+    x.y = fmaxf(x.y, -126.f);
     const uint64_t x2 = pair(x.x, x.y);
-    const uint64_t r = add2(x2, pair(12583039.f, 12583039.f));
-    const uint64_t f = fma2(add2(r, pair(-12583039.f, -12583039.f)), pair(-1.f, -1.f), x2);
+    const uint64_t r = add2(x2, pair(12582912.f, 12582912.f));
+    const uint64_t f = fma2(add2(r, pair(-12582912.f, -12582912.f)), pair(-1.f, -1.f), x2);
     uint64_t p = fma2(pair(0.00132764725f, 0.00132764725f), f, pair(0.00967554096f, 0.00967554096f));
     p = fma2(p, f, pair(0.0555071309f, 0.0555071309f));
     p = fma2(p, f, pair(0.240221202f, 0.240221202f));
     p = fma2(p, f, pair(0.693146944f, 0.693146944f));
     p = fma2(p, f, pair(1.00000012f, 1.00000012f));
-    const float2 n = unpair(r);
-    return unpair(mul2(p, pair_bits(__float_as_uint(n.x) << 23, __float_as_uint(n.y) << 23)));
+    const float2 y = unpair(p), n = unpair(r);
+    return make_float2(__uint_as_float(__float_as_uint(y.x) + (__float_as_uint(n.x) << 23)),
+                       __uint_as_float(__float_as_uint(y.y) + (__float_as_uint(n.y) << 23)));
 }
 
 // The value of lane 0, which is every lane's: tells the compiler that what depends on it is the same in the whole warp.  The

@@ -374,8 +374,9 @@ dense_fwd_tc5_kernel(const DenseArgs a, const DenseSplit sp, const __grid_consta
                         }
                         float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                        for (int j = 0; j < 64; ++j) tops[j & 3] = fmaxf(tops[j & 3], __uint_as_float(r[j >> 5][j & 31]));
-                        const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * a.scale_log2;
+                        for (int j = 0; j < 64; j += 2)
+                            tops[j >> 1 & 3] = max3_nan(tops[j >> 1 & 3], __uint_as_float(r[j >> 5][j & 31]), __uint_as_float(r[j >> 5][(j + 1) & 31]));
+                        const float top = max3_nan(max3_nan(tops[0], tops[1], tops[2]), tops[3], tops[3]) * a.scale_log2;
                         const bool grow = top > m + 8.f;             // also the first finite maximum (m = -inf)
                         if (__any_sync(0xffffffffu, grow)) {
                             const float m_new = grow ? top : m;
@@ -396,7 +397,8 @@ dense_fwd_tc5_kernel(const DenseArgs a, const DenseSplit sp, const __grid_consta
                             }
                             m = m_new;
                         }
-                        const float ref = m == -INFINITY ? 0.f : m;
+                        // a NaN score, or one of plus infinity, makes NaN of all weights of its row here, and so of its sum and result
+                        const float ref = !(top < INFINITY) ? NAN : m == -INFINITY ? 0.f : m;
                         const uint64_t c2 = pair(a.scale_log2, a.scale_log2), ref2 = pair(-ref, -ref);
                         uint64_t sum[2] = {0, 0};                    // two pairs of zeros
                         uint32_t pk[32];
