@@ -539,7 +539,8 @@ namespace hsa { cudaError_t dense_bwd_aborts(unsigned int *count); }
 extern "C" int hsa_dense_attn_aborts(unsigned int *count) {
     if (count == nullptr) return hsa::fail(HSA_ERR_ARG, "hsa_dense_attn_aborts: null pointer");
     unsigned int bwd = 0;
-    cudaError_t e = cudaMemcpyFromSymbol(count, hsa::g_dense_aborts, sizeof(unsigned int));
+    cudaError_t e = cudaDeviceSynchronize();                 // the copy alone does not wait for streams that do not wait for the default one
+    if (e == cudaSuccess) e = cudaMemcpyFromSymbol(count, hsa::g_dense_aborts, sizeof(unsigned int));
     if (e == cudaSuccess) e = hsa::dense_bwd_aborts(&bwd);
     if (e == cudaSuccess) *count += bwd;
     return e == cudaSuccess ? 0 : hsa::fail((int)e, "hsa_dense_attn_aborts: %s", cudaGetErrorString(e));

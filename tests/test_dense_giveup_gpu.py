@@ -10,6 +10,7 @@ import pytest
 import torch
 
 from sparseattention_b200 import _lib
+from sparseattention_b200.ops import dense
 from sparseattention_b200.ops.dense import dense_aborts
 
 pytestmark = pytest.mark.gpu
@@ -102,3 +103,30 @@ def test_no_row_is_left_unwritten(case, dtype):
     again = call.forward()
     assert all(torch.equal(a, b) for a, b in zip(again, good))
     assert all(torch.equal(a, b) for a, b in zip(call.backward(*good), good_grads))
+
+
+def test_the_count_waits_for_calls_on_other_streams(monkeypatch):
+    """Read right after a call on a stream of its own, the count has that call's blocks, and the debug check blames it and no later one."""
+    call = Call(4, 300, 200, 8, 8, 64, torch.bfloat16)
+    good = call.forward()
+    good_grads = call.backward(*good)
+    args = (call.q, call.k, call.v)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    monkeypatch.setattr(_lib, "DEBUG", True)
+    with torch.cuda.stream(side):
+        monkeypatch.setattr(dense, "_aborts_seen", {torch.cuda.current_device(): dense_aborts()})
+        before = dense_aborts()
+        _lib.check(_lib.load().hsa_debug_wait_test(20_000_000, 16), "hsa_debug_wait_test")
+        try:
+            with pytest.raises(_lib.HsaError, match="fwd"):
+                dense.dense_attention_forward(*args, scale=64 ** -0.5)
+            with pytest.raises(_lib.HsaError, match="bwd"):
+                dense.dense_attention_backward(*args, *good, call.g, scale=64 ** -0.5)
+        finally:
+            _lib.check(_lib.load().hsa_debug_wait_test(2_000_000_000, 0), "hsa_debug_wait_test")
+        assert dense_aborts() > before
+        healthy = dense.dense_attention_forward(*args, scale=64 ** -0.5)
+        grads = dense.dense_attention_backward(*args, *good, call.g, scale=64 ** -0.5)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip((*healthy, *grads), (*good, *good_grads)))
