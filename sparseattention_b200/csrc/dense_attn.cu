@@ -61,16 +61,11 @@ dense_mask_pack_kernel(const uint8_t *__restrict__ mask, int64_t sb, int64_t sh,
 // -sum_d dout * out and minus the row's log-sum-exp in base 2 (the kernels add both), padded with rows that give weight zero.  A
 // query without keys gets -inf and 0 whatever its output row holds.
 template <typename T, int VEC, int LPR, int CPL>
-__global__ void __launch_bounds__(256) dense_delta_kernel(const DenseArgs a, float *__restrict__ neg_lse2, float *__restrict__ neg_delta) {
-    const long long row = (long long)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
-    const int g = threadIdx.x % LPR;
-    const int h = (int)(row % a.H), i = (int)(row / a.H % a.lq_pad);
-    const long long b = row / a.H / a.lq_pad;
-    if (b >= a.B) return;
+__device__ __forceinline__ float delta_row(const DenseArgs &a, int64_t b, int i, int h, int g, float *neg_lse2, float *neg_delta, float shift) {
     const int64_t at = (b * a.H + h) * a.lq_pad + i;
     if (i >= a.Lq) {
         if (g == 0) { neg_lse2[at] = -INFINITY; neg_delta[at] = 0.f; }
-        return;
+        return 0.f;
     }
     RowFrag<T, VEC, LPR, CPL> x, y;
     x.load((const T *)a.out.ptr + b * a.out.batch_stride + (int64_t)i * a.out.row_stride + (int64_t)h * a.D, g, a.D / VEC);
@@ -86,8 +81,72 @@ __global__ void __launch_bounds__(256) dense_delta_kernel(const DenseArgs a, flo
     if (g == 0) {
         const float l = a.lse[(b * a.Lq + i) * a.H + h];
         const bool none = l == -INFINITY;
-        neg_lse2[at] = none ? -INFINITY : l * -1.4426950408889634f;
+        neg_lse2[at] = none ? -INFINITY : l * -1.4426950408889634f + shift;
         neg_delta[at] = none ? 0.f : -s;
+    }
+    return y.dot_partial(y);                              // this lane's part of dout's squared length
+}
+template <typename T, int VEC, int LPR, int CPL>
+__global__ void __launch_bounds__(256) dense_delta_kernel(const DenseArgs a, float *__restrict__ neg_lse2, float *__restrict__ neg_delta) {
+    const long long row = (long long)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
+    const int h = (int)(row % a.H), i = (int)(row / a.H % a.lq_pad);
+    const long long b = row / a.H / a.lq_pad;
+    if (b >= a.B) return;
+    delta_row<T, VEC, LPR, CPL>(a, b, i, h, threadIdx.x % LPR, neg_lse2, neg_delta, 0.f);
+}
+
+// The same for float16 on the tensor cores, with the squared lengths of dout's rows and the largest of those and of V's rows per (batch
+// entry, key/value head): a block takes a stretch of the query rows of all heads of a group, or of V's rows (those that may be looked
+// at: the others may hold anything).
+constexpr int kStretch = 4;                               // times 256 / LPR rows
+template <int VEC, int LPR, int CPL>
+__global__ void __launch_bounds__(256)
+dense_delta_f16_kernel(const DenseArgs a, float *__restrict__ neg_lse2, float *__restrict__ neg_delta, float *__restrict__ dout_sq,
+                       unsigned int *__restrict__ top_sq, int q_blocks, int v_blocks) {
+    using T = __half;
+    constexpr int RPB = 256 / LPR;
+    const int g = threadIdx.x % LPR, unit = threadIdx.x / LPR;
+    const int at = blockIdx.x % (q_blocks + v_blocks);
+    const int bh = blockIdx.x / (q_blocks + v_blocks), hk = bh % a.Hkv;
+    const int64_t b = bh / a.Hkv;
+    const bool values = at >= q_blocks;
+    float top = 0.f;
+    if (!values) {
+        const int rows = a.group * a.lq_pad;
+        for (int s = 0; s < kStretch; ++s) {
+            const int r = (at * kStretch + s) * RPB + unit, h = hk * a.group + r / a.lq_pad, i = r % a.lq_pad;
+            if (r >= rows) break;
+            const float sq = group_sum<LPR>(delta_row<T, VEC, LPR, CPL>(a, b, i, h, g, neg_lse2, neg_delta, (float)kWeightShift));
+            if (g == 0) dout_sq[(b * a.H + h) * a.lq_pad + i] = sq;
+            top = sq > top || sq != sq ? sq : top;
+        }
+    } else {
+        const int n = dense_keys(a, (int)b);
+        for (int s = 0; s < kStretch; ++s) {
+            const int j = ((at - q_blocks) * kStretch + s) * RPB + unit;
+            if (j >= n) break;
+            bool seen = a.mask.bits == nullptr;
+            for (int h = hk * a.group; !seen && h < (hk + 1) * a.group; ++h) {
+                const int64_t plane = b * a.mask.plane_b + (int64_t)h * a.mask.plane_h;
+                seen = (a.mask.seen[plane * a.mask.wk + (j >> 5)] >> (j & 31)) & 1u;
+            }
+            if (!seen) continue;
+            RowFrag<T, VEC, LPR, CPL> x;
+            x.load((const T *)a.v.ptr + b * a.v.batch_stride + (int64_t)j * a.v.row_stride + (int64_t)hk * a.D, g, a.D / VEC);
+            const float sq = group_sum<LPR>(x.dot_partial(x));
+            top = sq > top || sq != sq ? sq : top;
+        }
+    }
+    __shared__ unsigned int warp_top[8];
+    // bit patterns of numbers that are not negative are in the numbers' order, NaN last
+    const unsigned int bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top) & 0x7fffffffu);
+    if ((threadIdx.x & 31) == 0) warp_top[threadIdx.x >> 5] = bits;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        unsigned int all = warp_top[0];
+#pragma unroll
+        for (int w = 1; w < 8; ++w) all = max(all, warp_top[w]);
+        if (all != 0) atomicMax(top_sq + 2 * bh + values, all);
     }
 }
 
@@ -102,6 +161,20 @@ static int dense_delta(const DenseArgs &a, float *neg_lse2, float *neg_delta, in
         });
         return ok ? rc : fail(HSA_ERR_ARG, "hsa_dense_attn_bwd: head dim %d not supported", a.D);
     });
+}
+static int dense_delta_f16(const DenseArgs &a, float *neg_lse2, float *neg_delta, float *dout_sq, unsigned int *top_sq, bool vec, cudaStream_t st) {
+    const cudaError_t e = cudaMemsetAsync(top_sq, 0, (size_t)2 * a.B * a.Hkv * sizeof(unsigned int), st);
+    if (e != cudaSuccess) return fail((int)e, "hsa_dense_attn_bwd: %s", cudaGetErrorString(e));
+    int rc = 0;
+    const bool ok = dispatch_row_shape<__half>(a.D, vec, [&]<typename T, int VEC, int LPR, int CPL>() {
+        constexpr int per = kStretch * (256 / LPR);
+        const long long q_blocks = ((long long)a.group * a.lq_pad + per - 1) / per, v_blocks = (a.Lk + per - 1) / per;
+        const long long blocks = (q_blocks + v_blocks) * a.B * a.Hkv;
+        if (blocks > 0x7fffffffLL || (long long)a.group * a.lq_pad > 0x7fffffffLL) { rc = fail(HSA_ERR_ARG, "hsa_dense_attn_bwd: too many rows"); return; }
+        dense_delta_f16_kernel<VEC, LPR, CPL><<<(unsigned)blocks, 256, 0, st>>>(a, neg_lse2, neg_delta, dout_sq, top_sq, (int)q_blocks, (int)v_blocks);
+        rc = launch_status("hsa_dense_attn_bwd(row sums)");
+    });
+    return ok ? rc : fail(HSA_ERR_ARG, "hsa_dense_attn_bwd: head dim %d not supported", a.D);
 }
 
 static bool rows_in_fours(const hsa_view &v, int esize) {
@@ -200,14 +273,18 @@ extern "C" int hsa_dense_attn_fwd(hsa_view Q, hsa_view K, hsa_view V, hsa_view O
     return dense_fwd_f32(a, workspace, dtype, (cudaStream_t)stream);
 }
 
-// Row sums and log-sum-exps of the padded rows, then what the tensor-core kernels keep of partial gradients
-static size_t bwd_stats_bytes(int B, int Lq, int H) { return (size_t)2 * B * H * ((Lq + 127) / 128 * 128) * sizeof(float); }
+// Row sums and log-sum-exps of the padded rows, in float16 with what the shift of score gradients follows from, then what the kernels
+// keep of partial gradients
+static size_t bwd_stats_bytes(int B, int Lq, int H, int Hkv, bool f16) {
+    const size_t row = (size_t)B * H * ((Lq + 127) / 128 * 128) * sizeof(float);
+    return f16 ? 3 * row + ((size_t)2 * B * Hkv * sizeof(unsigned int) + 255) / 256 * 256 : 2 * row;
+}
 
 extern "C" size_t hsa_dense_attn_bwd_workspace_bytes(int B, int Lq, int Lk, int H, int Hkv, int D, int dtype, int algo) {
     if (B < 1 || Lq < 1 || Lk < 1 || H < 1 || Hkv < 1 || H % Hkv != 0 || D < 1) return 0;
     const size_t f32 = algo != 2 ? dense_bwd_f32_workspace(B, Lq, Lk, H, Hkv, D) : 0;
     const size_t tc = tc_shape(D, dtype, algo) ? dense_bwd_tc_workspace(B, Lq, Lk, H, Hkv, D) : 0;
-    return bwd_stats_bytes(B, Lq, H) + (f32 > tc ? f32 : tc);
+    return bwd_stats_bytes(B, Lq, H, Hkv, dtype == HSA_F16 && tc_shape(D, dtype, algo)) + (f32 > tc ? f32 : tc);
 }
 
 extern "C" int hsa_dense_attn_bwd(hsa_view Q, hsa_view K, hsa_view V, hsa_view Out, const void *out_rest, const float *LSE, hsa_view dOut, hsa_view dQ,
@@ -241,7 +318,15 @@ extern "C" int hsa_dense_attn_bwd(hsa_view Q, hsa_view K, hsa_view V, hsa_view O
     const bool tc = algo != 1 && dense_tc_ok(a, dtype, true) && dense_bwd_tables_ok(a);
     HSA_CHECK_ARG(algo != 2 || tc, "hsa_dense_attn_bwd: no tensor-core kernel for these inputs");
     cudaStream_t st = (cudaStream_t)stream;
-    if (int rc = dense_delta(a, neg_lse2, neg_delta, dtype, D % (16 / es) == 0 && view_vec_ok(Out, es) && view_vec_ok(dOut, es), st)) return rc;
-    void *rest = (char *)workspace + bwd_stats_bytes(B, Lq, H);
+    const bool f16 = dtype == HSA_F16 && tc_shape(D, dtype, algo), vec = D % (16 / es) == 0 && view_vec_ok(Out, es) && view_vec_ok(dOut, es);
+    if (f16 && tc) {
+        float *dout_sq = neg_delta + (size_t)B * H * a.lq_pad;
+        unsigned int *top_sq = (unsigned int *)(dout_sq + (size_t)B * H * a.lq_pad);
+        a.dout_sq = dout_sq; a.top_sq = top_sq;
+        if (int rc = dense_delta_f16(a, neg_lse2, neg_delta, dout_sq, top_sq, vec, st)) return rc;
+    } else if (int rc = dense_delta(a, neg_lse2, neg_delta, dtype, vec, st)) {
+        return rc;
+    }
+    void *rest = (char *)workspace + bwd_stats_bytes(B, Lq, H, Hkv, f16);
     return tc ? dense_bwd_tc(a, rest, dtype, st) : dense_bwd_f32(a, rest, dtype, st);
 }

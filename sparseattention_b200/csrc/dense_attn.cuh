@@ -69,6 +69,10 @@ struct DenseArgs {
     float *lse;                          // forward: [B, Lq, H] natural log-sum-exp, or null
     void *out_lo;                        // [B, Lq, H, D] packed: what rounding took from the 16-bit output, in its type; or null
     const float *neg_lse2, *neg_delta;   // backward: [B, H, lq_pad] minus the log-sum-exp in base 2 (-inf: no key), minus the row sums of dout * out
+    // backward on the tensor cores in f16 (kWeightShift is then part of neg_lse2): squared lengths of dout's rows [B, H, lq_pad], and the
+    // largest of them and of V's rows [B, Hkv, 2] as bit patterns
+    const float *dout_sq;
+    const unsigned int *top_sq;
     const int *key_lengths;              // [B] or null
     DenseMask mask;
     int B, Lq, Lk, H, Hkv, D, group;     // group = H / Hkv
@@ -77,6 +81,21 @@ struct DenseArgs {
     float empty_value;                   // what the output row of a query without keys holds
     bool vec;                            // rows may be read four elements at a time
 };
+
+// float16 holds nothing between 0 and 2^-24, and full precision from 2^-14 only: weights near 1 / Lk, and score gradients, which are
+// those times differences of the size of dout, would lose bits as operands or vanish while the sums over them do not.  So the
+// backward's products take weights times 2^15 (at most 2^15: the weights do not pass 1), and score gradients times the power of two
+// that a bound on them allows: |ds| <= |do.(v - out)| <= 2 |do| max |v|, as the output is a mean of rows of V.  What is multiplied
+// by it stays below 2^15; the results are multiplied by the inverse, exactly.  (8192 keys, output gradients of 1e-3: dq off by
+// 5.7e-3 of its size without this; 5.2e-4 is what rounding the result alone leaves.)  It costs a read of V's rows next to the row sums
+// and a clearing of the tops: 4 to 8 us of 180 for 3 x 515 x 1027, 12 on 4 heads of 128, forward and backward.
+constexpr int kWeightShift = 15;
+__device__ __forceinline__ float grad_shift(float dout_sq, unsigned int v_sq_bits) {
+    const float bound = 2.f * sqrtf(dout_sq) * sqrtf(__uint_as_float(v_sq_bits));
+    return bound > 0.f && bound < INFINITY ? (float)(14 - ilogbf(bound)) : 0.f;
+}
+// 2^e for whole e between -126 and 127
+__device__ __forceinline__ float pow2(float e) { return __int_as_float(((int)e + 127) << 23); }
 
 // Raise a kernel's shared-memory limit, once per device
 template <auto Kernel>

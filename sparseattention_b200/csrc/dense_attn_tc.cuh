@@ -136,6 +136,10 @@ __device__ __forceinline__ void store_rows32(T *row, int64_t row_stride, int bel
     for (int t = 0; t < 4; ++t)
         if (t - quad < below) *reinterpret_cast<uint4 *>(row + (t - quad) * row_stride + col + 8 * quad) = p[t];
 }
+__device__ __forceinline__ void scale_all(uint32_t (&v)[32], float by) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * by);
+}
 // The same for 32-bit rows.
 __device__ __forceinline__ void store_rows32_f32(float *row, int64_t row_stride, int below, int col, int D, const uint32_t (&v)[32]) {
     const int quad = threadIdx.x & 3;

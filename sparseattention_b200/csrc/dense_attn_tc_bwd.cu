@@ -18,7 +18,8 @@
 // thirds of the tensor cores').  On the way there: a warpgroup per buffer instead of both on one 738 us and 128 columns in one buffer 436 us;
 // products issued from uniform registers 492 and 427 us; scores and gradients issued by a warp each 445 and 350 us; output rows
 // through quad transposes 430 and 341 us.
-// Rounding: p and ds are rounded to the inputs' type once, as operands; all sums are 32-bit.
+// Rounding: p and ds are rounded to the inputs' type once, as operands; all sums are 32-bit.  In float16 both are moved into the middle
+// of the type's range first (grad_shift): p by 2^15, ds by a power of two per query row for dq, per key/value head for dk.
 #include "dense_attn_tc.cuh"
 
 namespace hsa {
@@ -308,7 +309,12 @@ dense_dq_tc5_kernel(const DenseArgs a, const BwdSplit sp, const __grid_constant_
             const DqItem it(a, sp.splits, item);
             const int qi = it.q0 + row;
             const int64_t at = ((int64_t)it.b * a.H + it.h) * a.lq_pad + qi;
-            const float neg_lse2 = a.neg_lse2[at], neg_delta = a.neg_delta[at];
+            float neg_lse2 = a.neg_lse2[at], neg_delta = a.neg_delta[at], unshift = 1.f;
+            if constexpr (!BF) {
+                const float e = grad_shift(a.dout_sq[at], a.top_sq[2 * (it.b * a.Hkv + it.hk) + 1]);
+                neg_lse2 += e - (float)kWeightShift;
+                unshift = pow2(-e);
+            }
             const uint64_t c2 = pair(a.scale_log2, a.scale_log2), lse22 = pair(neg_lse2, neg_lse2), delta2 = pair(neg_delta, neg_delta);
             const uint32_t *bits = masked ? a.mask.bits + (it.plane * a.mask.rows + (a.mask.rows > 1 ? min(qi, a.Lq - 1) : 0)) * a.mask.wk : nullptr;
             bool any = false;
@@ -366,11 +372,13 @@ dense_dq_tc5_kernel(const DenseArgs a, const BwdSplit sp, const __grid_constant_
 #pragma unroll
                     for (int j = 0; j < 32; ++j) o[j] = 0u;
                 }
-                if (sp.splits > 1)
+                if (sp.splits > 1) {
+                    if constexpr (!BF) scale_all(o, unshift);
                     store_rows32_f32(sp.part + ((((int64_t)it.split * a.B + it.b) * a.Lq + qi) * a.H + it.h) * a.D, (int64_t)a.H * a.D, a.Lq - qi,
                                      32 * c, a.D, o);
-                else
-                    store_rows32<T>(out, a.dq.row_stride, a.Lq - qi, 32 * c, a.D, o, a.scale);
+                } else {
+                    store_rows32<T>(out, a.dq.row_stride, a.Lq - qi, 32 * c, a.D, o, a.scale * unshift);
+                }
             }
             fence_before_sync();                             // the accumulator may be written again
             __syncwarp();
@@ -670,6 +678,13 @@ dense_dkdv_tc5_kernel(const DenseArgs a, const BwdSplit sp, const __grid_constan
             const int key = it.k0 + row;
             const bool tail = it.n - it.k0 < 128;
             bool any = false;
+            float ds_shift = 0.f;
+            if constexpr (!BF) {
+                const unsigned int *tops = a.top_sq + 2 * (it.b * a.Hkv + it.hk);
+                ds_shift = grad_shift(__uint_as_float(tops[0]), tops[1]);
+            }
+            const float ds_factor = pow2(ds_shift - (float)kWeightShift), unshift = BF ? 1.f : pow2(x == 0 ? -(float)kWeightShift : -ds_shift);
+            const uint64_t ds_factor2 = pair(ds_factor, ds_factor);
             for (int u = next_unit(is, it.u0, it.u1); u < it.u1; u = next_unit(is, u + 1, it.u1)) {
                 uint32_t keep = 0xffffffffu;
                 bool partial = tail;
@@ -704,6 +719,7 @@ dense_dkdv_tc5_kernel(const DenseArgs a, const BwdSplit sp, const __grid_constan
                                 if (!((keep >> (2 * c)) & 1u)) p.x = y.x = 0.f;
                                 if (!((keep >> (2 * c + 1)) & 1u)) p.y = y.y = 0.f;
                             }
+                            if constexpr (!BF) y = unpair(mul2(pair(y.x, y.y), ds_factor2));
                             pk[c] = pack2<T>(p.x, p.y);
                             dk[c] = pack2<T>(y.x, y.y);
                         }
@@ -736,10 +752,12 @@ dense_dkdv_tc5_kernel(const DenseArgs a, const BwdSplit sp, const __grid_constan
 #pragma unroll
                     for (int j = 0; j < 32; ++j) o[j] = 0u;
                 }
-                if (sp.splits > 1)
+                if (sp.splits > 1) {
+                    if constexpr (!BF) scale_all(o, unshift);
                     store_rows32_f32(part_row(it, x, key), (int64_t)a.Hkv * a.D, a.Lk - key, 32 * c, a.D, o);
-                else
-                    store_rows32<T>(out, g.row_stride, a.Lk - key, 32 * c, a.D, o, x == 0 ? 1.f : a.scale);
+                } else {
+                    store_rows32<T>(out, g.row_stride, a.Lk - key, 32 * c, a.D, o, (x == 0 ? 1.f : a.scale) * unshift);
+                }
             }
             fence_before_sync();
             __syncwarp();

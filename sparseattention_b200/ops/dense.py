@@ -320,7 +320,7 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, key_lengt
     A query that may look at no key gives a row of `empty_value` and passes no gradient on.  What k and v hold behind a
     length, or in keys that a mask hides from all queries, may be anything; everything else has to be finite.
     Differentiable once with respect to q, k and v.  In bfloat16 and float16 the weights and the gradients of the scores are
-    rounded to that type between the products (a gradient of a score beyond 65504 in float16 is infinite); sums are 32-bit.
+    rounded to that type between the products (in float16's backward moved into the middle of its range first); sums are 32-bit.
     A mask is packed into bits by every call; keys that only a length hides are cheaper given as key_lengths.
     torch.compile breaks its graph here; tracing, torch.func transforms and forward-mode tangents are refused.
     """

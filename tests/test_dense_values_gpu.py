@@ -8,6 +8,7 @@ import math
 import pytest
 import torch
 
+from sparseattention_b200.ops import cross_attention
 from sparseattention_b200.ops.dense import dense_attention_forward
 
 pytestmark = pytest.mark.gpu
@@ -55,3 +56,107 @@ def test_infinite_scores(algo):
             assert lse[0, rest, 0].isfinite().all()
             if sign > 0:
                 assert out[0, 17].isnan().all() and not lse[0, 17].isfinite().any(), key
+
+
+def definition(q, k, v, g, allowed=None):
+    """(out, dq, dk, dv, ds) in 64 bits; allowed [B, H or 1, Lq or 1, Lk]."""
+    B, Lq, H, D = q.shape
+    Lk, Hkv = k.shape[1:3]
+    heads = lambda t: t.double().permute(0, 2, 1, 3).repeat_interleave(H // t.size(2), dim=1)                # noqa: E731
+    qd, kd, vd, gd = (heads(t) for t in (q, k, v, g))
+    s = D ** -0.5 * qd @ kd.transpose(-1, -2)
+    if allowed is not None:
+        s = s.masked_fill(~allowed, -math.inf)
+        vd = torch.where(allowed.expand(B, H, Lq, Lk).any(2).unsqueeze(-1), vd, 0.0)
+    p = torch.softmax(s, -1).nan_to_num(nan=0.0)
+    out = p @ vd
+    ds = p * (gd @ vd.transpose(-1, -2) - (gd * out).sum(-1, keepdim=True))
+    group = lambda t: t.view(B, Hkv, H // Hkv, Lk, D).sum(2).permute(0, 2, 1, 3)                             # noqa: E731
+    back = lambda t: t.permute(0, 2, 1, 3)                                                                   # noqa: E731
+    return (back(out), back(D ** -0.5 * ds @ kd), group(D ** -0.5 * ds.transpose(-1, -2) @ qd), group(p.transpose(-1, -2) @ gd), ds)
+
+
+def run_training(q, k, v, g, algo=2, **kw):
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+    return torch.autograd.grad(cross_attention(*leaves, algo=algo, **kw), leaves, g)
+
+
+def as_good_as_rounded(got, want, what):
+    """Off in norm by no more than rounding the exact result costs, plus twice half a step: weights and score gradients are rounded
+    once each, relative to their own size, and errors of independent signs add up as the terms themselves do."""
+    u = 2.0 ** -11
+    floor = float((want.half().double() - want).norm() / want.norm())
+    err = float((got.double() - want).norm() / want.norm())
+    assert err <= floor + 2 * u, f"{what}: {err:.3g}, the result's own rounding {floor:.3g}"
+
+
+@pytest.mark.parametrize("case", [(1, 64, 8192, 2, 1, 64, 1e-3), (1, 64, 32768, 2, 2, 64, 1e-2), (1, 64, 32768, 1, 1, 64, 1e-3),
+                                  (2, 200, 5000, 4, 2, 128, 1e-3), (1, 6000, 40, 2, 1, 64, 1e-4), (2, 300, 2000, 2, 2, 72, 1e-3)])
+def test_float16_gradients_of_long_rows(case):
+    """Weights of about 1 / Lk and small output gradients: as float16 their score gradients are below 2^-14, or below 2^-24."""
+    *(B, Lq, Lk, H, Hkv, D), size = case
+    q, k, v = (normal(B, n, h, D, dtype=torch.float16, seed=n + h) for n, h in ((Lq, H), (Lk, Hkv), (Lk + 1, Hkv)))
+    v = v[:, :Lk].contiguous()
+    g = (normal(B, Lq, H, D, dtype=torch.float32, seed=5) * size).half()
+    _, *want, _ = definition(q, k, v, g)
+    for name, a, b in zip(("dq", "dk", "dv"), run_training(q, k, v, g), want):
+        as_good_as_rounded(a, b, name)
+
+
+def test_float16_score_gradients_beyond_the_type():
+    q, k, v, g = (normal(2, n, 2, 64, dtype=torch.float32, seed=i) for i, n in enumerate((8, 3, 3, 8)))
+    q, k, v, g = (q * 0.05).half(), (k * 0.05).half(), (v * 3).half(), (g * 12000).half()
+    _, *want, ds = definition(q, k, v, g)
+    assert float(ds.abs().max()) > 65504 and all(float(t.abs().max()) < 65504 for t in want)
+    for name, a, b in zip(("dq", "dk", "dv"), run_training(q, k, v, g), want):
+        as_good_as_rounded(a, b, name)
+
+
+def test_float16_gradients_of_unequal_size():
+    """Rows, heads and batch entries whose output gradients differ by powers of ten, and none at all."""
+    B, Lq, Lk, H, Hkv, D = 3, 150, 3000, 4, 2, 64
+    q, k, v = (normal(B, n, h, D, dtype=torch.float16, seed=n) for n, h in ((Lq, H), (Lk, Hkv), (Lk, Hkv)))
+    g = normal(B, Lq, H, D, dtype=torch.float32, seed=6)
+    g[0] *= 1e-3
+    g[1, :, 2:] *= 1e-2
+    g[1, ::2] *= 0.05
+    g[2] = 0
+    g = g.half()
+    dq, dk, dv = run_training(q, k, v, g)
+    _, wq, wk, wv, _ = definition(q, k, v, g)
+    assert not dq[2].any() and not dk[2].any() and not dv[2].any()
+    as_good_as_rounded(dq[0], wq[0], "dq of small gradients")
+    for part in (slice(0, None, 2), slice(1, None, 2)):
+        for heads in (slice(0, 2), slice(2, 4)):
+            as_good_as_rounded(dq[1, part, heads], wq[1, part, heads], "dq of some rows")
+    for name, a, b in (("dk", dk, wk), ("dv", dv, wv)):
+        for at in ((0, slice(None), 0), (0, slice(None), 1), (1, slice(None), 0), (1, slice(None), 1)):
+            as_good_as_rounded(a[at], b[at], name)
+
+
+@pytest.mark.parametrize("D", [64, 72, 128])
+@pytest.mark.parametrize("kind", ["lengths", "keys", "heads"])
+def test_float16_hidden_rows_have_no_say(D, kind):
+    """What lies in rows of V that nobody looks at (NaN, infinities, the largest numbers) changes no bit of a gradient."""
+    B, Lq, Lk, H, Hkv = 2, 140, 700, 4, 2
+    q, k, v, g = (normal(B, n, h, D, dtype=torch.float16, seed=n + h) for n, h in ((Lq, H), (Lk, Hkv), (Lk + 2, Hkv), (Lq + 1, H)))
+    v, g = v[:, :Lk].contiguous(), g[:, :Lq].contiguous()
+    kw = {}
+    if kind == "lengths":
+        kw["key_lengths"] = torch.tensor([531, 0], dtype=torch.int32, device="cuda")
+        hidden = torch.arange(Lk, device="cuda") >= kw["key_lengths"].view(-1, 1)
+        hidden = hidden.view(B, Lk, 1).expand(B, Lk, Hkv)
+        allowed = ~hidden[..., 0].view(B, 1, 1, Lk)
+    else:
+        mask = torch.rand(B, H if kind == "heads" else 1, 1, Lk, device="cuda") < 0.4
+        kw["mask"] = allowed = mask
+        hidden = ~mask.expand(B, H, 1, Lk).view(B, Hkv, H // Hkv, Lk).any(2).transpose(1, 2)
+    want = run_training(q, k, v, g, **kw)
+    for value in (math.nan, math.inf, 65504.0):
+        bad = v.clone()
+        bad[hidden] = value
+        assert all(torch.equal(a, b) for a, b in zip(run_training(q, k, bad, g, **kw), want))
+    if kind != "lengths":
+        _, *exact, _ = definition(q, k, v, g, allowed)
+        for name, a, b in zip(("dq", "dk", "dv"), want, exact):
+            as_good_as_rounded(a, b, name)
