@@ -9,7 +9,8 @@ import pytest
 import torch
 
 from sparseattention_b200.ops import cross_attention
-from sparseattention_b200.ops.dense import dense_attention_forward
+from sparseattention_b200.ops.dense import dense_attention_backward, dense_attention_forward
+from tests.test_dense_gpu import SHAPES, check, make
 
 pytestmark = pytest.mark.gpu
 
@@ -160,3 +161,64 @@ def test_float16_hidden_rows_have_no_say(D, kind):
         _, *exact, _ = definition(q, k, v, g, allowed)
         for name, a, b in zip(("dq", "dk", "dv"), want, exact):
             as_good_as_rounded(a, b, name)
+
+
+@pytest.mark.parametrize("shape", [s for s in SHAPES if s[5] % 8 == 0 and s[5] <= 128])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_tensor_core_kernels_by_name(shape, dtype):
+    check(*make(*shape, dtype, seed=sum(shape)), algo=2)
+
+
+# one key, few, a tail, whole tiles, and few rows over many keys (ranges that are joined)
+RESTS = [(1, 5, 1, 2, 1, 64), (2, 40, 3, 2, 2, 64), (2, 130, 300, 4, 2, 128), (1, 300, 513, 2, 2, 72), (1, 40, 6000, 2, 1, 64),
+         (1, 3, 20000, 2, 2, 128)]
+
+
+@pytest.mark.parametrize("shape", RESTS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("algo", [1, 2])
+def test_what_rounding_took_is_kept(shape, dtype, algo):
+    """Queries of zeros weigh all keys alike, in numbers that every kernel holds exactly: output and rest together are the mean of the
+    values up to the 32-bit sum (2 sqrt(n) + 8 half steps w of the magnitudes, 2^-21 for the exponentials of zero and the division)
+    and the rest's own rounding, u of u |out|, or half of float16's smallest step."""
+    B, Lq, Lk, H, Hkv, D = shape
+    u, w, tiny = torch.finfo(dtype).eps / 2, 2.0 ** -24, 2.0 ** -25 if dtype == torch.float16 else 0.0
+    q, _, v, _ = make(*shape, dtype, seed=Lk)
+    k = make(*shape, dtype, seed=Lk + 1)[1]
+    lengths = torch.tensor([Lk, Lk // 2][:B], dtype=torch.int32, device="cuda")
+    out, rest, lse = dense_attention_forward(torch.zeros_like(q), k, v, lengths, scale=0.125, algo=algo)
+    for b, n in enumerate(lengths.tolist()):
+        vd = v[b, :n].double().repeat_interleave(H // Hkv, dim=1)                                            # [n, H, D]
+        want, size = vd.mean(0), vd.abs().mean(0)
+        total = out[b].double() + rest[b].double()
+        tol = u * u * want.abs() + ((2 * math.sqrt(n) + 8) * w + 2.0 ** -21) * size + tiny
+        assert ((total - want).abs() <= tol).all()
+        assert (rest[b].double().abs() <= u * out[b].double().abs() * (1 + 2 * u) + tiny).all()
+        assert ((lse[b].double() - math.log(n)).abs() <= (math.log(n) + 4) * 2.0 ** -22).all()
+
+
+@pytest.mark.parametrize("keys", [2, 3])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("algo", [1, 2])
+def test_the_rest_carries_gradients_over_few_keys(keys, dtype, algo):
+    """Values that differ by a step or two of their type, under equal weights: the gradients of the scores are differences of numbers
+    that agree in their leading bits, and the output's rounding alone is as large as they are."""
+    B, Lq, H, D, scale = 2, 70, 2, 64, 0.125
+    u, w = torch.finfo(dtype).eps / 2, 2.0 ** -24
+    tiny = 2.0 ** -25 if dtype == torch.float16 else 0.0
+    q, k, v, g = make(B, Lq, keys, H, H, D, dtype, seed=keys)
+    q = torch.zeros_like(q)
+    steps = torch.randint(-2, 3, v.shape, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda")
+    v = (v[:, :1].double() * (1 + 2 * u * steps)).to(dtype)
+    out, rest, lse = dense_attention_forward(q, k, v, scale=scale, algo=algo)
+    _, want, _, _, _ = definition(q, k * (scale * D ** 0.5), v, g)
+    kd, vd, gd = (t.double().permute(0, 2, 1, 3) for t in (k, v, g))
+    dp = gd @ vd.transpose(-1, -2)
+    size = gd.abs() @ vd.abs().transpose(-1, -2)                                   # sums of magnitudes of dp, and of the row sum
+    ds = (dp - dp.mean(-1, keepdim=True)) / keys
+    e_ds = u * ds.abs() + (2 * (D + 2) * w + u * u + 2.0 ** -20) * (size + size.mean(-1, keepdim=True)) / keys + tiny
+    tol = (scale * (e_ds @ kd.abs() + (keys + 2) * w * (ds.abs() @ kd.abs()))).permute(0, 2, 1, 3) + u * want.abs() + tiny
+    dq = dense_attention_backward(q, k, v, out, rest, lse, g, scale=scale, algo=algo)[0].double()
+    assert ((dq - want).abs() <= tol).all()
+    without = dense_attention_backward(q, k, v, out, None, lse, g, scale=scale, algo=algo)[0].double()
+    assert float(((without - want).abs() / tol).max()) > 4.0
