@@ -125,10 +125,6 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map
     asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];\n"
                  ::"r"(dst), "l"(map), "r"(x), "r"(h), "r"(row), "r"(b), "r"(mb) : "memory");
 }
-__device__ __forceinline__ void tma_store_4d(const CUtensorMap *map, uint32_t src, int x, int h, int row, int b) {
-    asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4, %5}], [%1];\n"
-                 ::"l"(map), "r"(src), "r"(x), "r"(h), "r"(row), "r"(b) : "memory");
-}
 // Shared-memory writes made by this thread become visible to the copy engine and the tensor cores.
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory"); }
 
