@@ -42,7 +42,7 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
     return d;
 }
 
-// 2^x for both numbers of a pair without the special-function unit, x <= 8 (below -126: 2^-126).  x = n + f with n the nearest
+// 2^x for both numbers of a pair without the special-function unit, x <= 15 (below -126: 2^-126).  x = n + f with n the nearest
 // whole number (the addition of 1.5 * 2^23 leaves it in the low bits), |f| <= 1/2, 2^f by the degree-5 polynomial of least
 // greatest relative error on that interval (found by exchange; 7.5e-8), and n goes into the exponent.  Off by at most 2^-22 in
 // 32-bit arithmetic, as the special-function unit is.  NaN does not stay NaN (n added to its bits makes a finite number of them):

@@ -21,7 +21,9 @@
 // The output is rescaled only when a row's maximum has grown by more than 2^8 since the last time (the weights then lie below
 // 2^8, which changes nothing in their relative precision), so almost every tile leaves O alone.
 // Rounding: weights are rounded to the inputs' type for the second product (what the tensor cores take); their sum is taken
-// from the unrounded 32-bit values, and the division by it comes last, in 32 bits.
+// from the unrounded 32-bit values, and the division by it comes last, in 32 bits.  In float16 all weights of a row are 2^7 times as
+// large: the largest then still fits (2^15), and what a weight loses below the type's smallest step is 2^-32 of the row's largest
+// instead of 2^-25, which many small weights next to a large one would show (100000 keys 17.6 below one: all of their part).
 // Keys behind a sequence's length and keys that no query may look at: the scores are replaced, and their V rows are zeroed in
 // shared memory, so that NaN there cannot come back as 0 * NaN.
 #include "dense_attn_tc.cuh"
@@ -71,6 +73,7 @@ dense_fwd_tc5_kernel(const DenseArgs a, const DenseSplit sp, const __grid_consta
     constexpr bool BF = std::is_same<T, __nv_bfloat16>::value;
     constexpr uint32_t IDESC_S = instr_desc(128, 64, BF, false, false), IDESC_O = instr_desc(128, DP, BF, false, true);
     constexpr uint32_t COL_S = 0, COL_O = 256;
+    constexpr float SHIFT = BF ? 0.f : 7.f;                          // weights are taken times 2^SHIFT
 
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char *smem = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
@@ -398,7 +401,7 @@ dense_fwd_tc5_kernel(const DenseArgs a, const DenseSplit sp, const __grid_consta
                             m = m_new;
                         }
                         // a NaN score, or one of plus infinity, makes NaN of all weights of its row here, and so of its sum and result
-                        const float ref = !(top < INFINITY) ? NAN : m == -INFINITY ? 0.f : m;
+                        const float ref = !(top < INFINITY) ? NAN : m == -INFINITY ? 0.f : m - SHIFT;
                         const uint64_t c2 = pair(a.scale_log2, a.scale_log2), ref2 = pair(-ref, -ref);
                         uint64_t sum[2] = {0, 0};                    // two pairs of zeros
                         uint32_t pk[32];
@@ -456,8 +459,8 @@ dense_fwd_tc5_kernel(const DenseArgs a, const DenseSplit sp, const __grid_consta
                     }
                 }
                 if (qi < a.Lq) {
-                    if (sp.splits > 1) *reinterpret_cast<float2 *>(sp.part_ml + 2 * at) = make_float2(m, l);
-                    if (sp.splits == 1 && a.lse != nullptr) a.lse[at] = none ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+                    if (sp.splits > 1) *reinterpret_cast<float2 *>(sp.part_ml + 2 * at) = make_float2(m - SHIFT, l);
+                    if (sp.splits == 1 && a.lse != nullptr) a.lse[at] = none ? -INFINITY : (m - SHIFT + log2f(l)) * 0.6931471805599453f;
                 }
                 if (sp.splits == 1 && a.empty_value != 0.f) {        // other lanes wrote the row's zeros: they come first
                     __syncwarp();

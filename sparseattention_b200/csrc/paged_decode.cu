@@ -199,7 +199,8 @@ __global__ void __launch_bounds__(kPagedWarps * 32) paged_decode_simt_kernel(con
 // m16n8k16 products whose 16 rows are the query heads that share the key head (rows behind them are zeros).  Half-empty tiles
 // cost nothing here: a 4 KB step of K takes 16 products, far less than HBM needs to deliver it.  Rows are 16-byte pieces
 // swizzled by the row number, which keeps ldmatrix free of bank conflicts.  The running maximum is raised, and the sums
-// rescaled, only when a score exceeds it by 2^8.  Weights are rounded to the type for the second product; their sum is not.
+// rescaled, only when a score exceeds it by 2^8.  Weights are rounded to the type for the second product; their sum is not.  In
+// float16 they are 2^7 times as large, so that many small ones next to a large one keep their bits (they stay below 2^15).
 template <int DP> struct PagedShape {
     // Three stages: at head dims up to 64 four blocks then share an SM, and one block's first loads pass under another's loop (six
     // stages and two blocks, the same bytes in flight: 20 sequences of 8192 keys, 16 heads of 64, 166 us against 115; 100 of 512, 71
@@ -231,6 +232,7 @@ __device__ __forceinline__ int by_length(const PagedArgs &a, int at) {
 template <typename T, int DP, bool SORTED>
 __global__ void __launch_bounds__(kPagedWarps * 32) paged_decode_mma_kernel(const PagedArgs a) {
     using Shape = PagedShape<DP>;
+    constexpr float SHIFT = std::is_same<T, __half>::value ? 7.f : 0.f;
     constexpr int ST = Shape::kStages, CPR = DP / 8, PIECES = 16 * CPR / 32;
     extern __shared__ __align__(128) unsigned char smem[];
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
@@ -343,7 +345,7 @@ __global__ void __launch_bounds__(kPagedWarps * 32) paged_decode_mma_kernel(cons
                 for (int i = 0; i < DP / 8; ++i) { o[i][2 * r] *= corr; o[i][2 * r + 1] *= corr; }
             }
         }
-        const float ref[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
+        const float ref[2] = {m[0] == -INFINITY ? 0.f : m[0] - SHIFT, m[1] == -INFINITY ? 0.f : m[1] - SHIFT};
 #pragma unroll
         for (int n = 0; n < 2; ++n)
 #pragma unroll

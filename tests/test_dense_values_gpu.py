@@ -8,7 +8,7 @@ import math
 import pytest
 import torch
 
-from sparseattention_b200.ops import cross_attention
+from sparseattention_b200.ops import cross_attention, paged_attention_decode
 from sparseattention_b200.ops.dense import dense_attention_backward, dense_attention_forward
 from tests.test_dense_gpu import SHAPES, check, make
 
@@ -222,3 +222,29 @@ def test_the_rest_carries_gradients_over_few_keys(keys, dtype, algo):
     assert ((dq - want).abs() <= tol).all()
     without = dense_attention_backward(q, k, v, out, None, lse, g, scale=scale, algo=algo)[0].double()
     assert float(((without - want).abs() / tol).max()) > 4.0
+
+
+@pytest.mark.parametrize("kind", ["rows", "ranges", "paged", "paged ranges"])
+@pytest.mark.parametrize("algo", [1, 2])
+def test_float16_keeps_many_small_weights_next_to_a_large_one(kind, algo):
+    """One key with score 0 and the value 0, and 100000 others 17.6 below it with the value 1: each weighs 2^-25.4 of the first, less
+    than float16 holds, all of them 2.3e-3.  A weight may be off by 2^-32 of the largest; the result is rounded once."""
+    n, sink, u = 100001, 130, 2.0 ** -11
+    rows = 300 if kind == "rows" else 3
+    heads = 80 if kind == "rows" else 2
+    q = torch.zeros(1, rows, heads, 64, dtype=torch.float16, device="cuda")
+    q[..., 0] = 1
+    k = torch.zeros(1, n, 1, 64, dtype=torch.float16, device="cuda")
+    k[..., 0] = -17.59375
+    v = torch.ones_like(k)
+    k[:, sink, :, 0], v[:, sink] = 0, 0
+    small = (n - 1) * math.exp(-17.59375)
+    want = small / (1 + small)
+    if kind.startswith("paged"):
+        pages = -(-n // 64)
+        kp, vp = (torch.cat([t[0], t[0, :pages * 64 - n]]).view(pages, 64, 1, 64) for t in (k, v))
+        out = paged_attention_decode(q[:, 0], kp, vp, torch.arange(pages, dtype=torch.int32, device="cuda").view(1, -1),
+                                     torch.tensor([n], dtype=torch.int32, device="cuda"), scale=1.0, algo=algo, splits=1 if kind == "paged" else 40)
+    else:
+        out = cross_attention(q, k, v, scale=1.0, algo=algo)
+    assert float((out.double() - want).abs().max()) <= n * 2.0 ** -32 + want * (u + 2.0 ** -15)
