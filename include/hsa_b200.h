@@ -418,7 +418,8 @@ int hsa_cross_entropy_bwd_inplace(void *logits, long long row_stride, const long
  *   [batches, heads, rows, Lk] with batches 1 or B, heads 1 or H, rows 1 or Lq; `packed` receives
  *   hsa_dense_mask_bytes(...) bytes, 256-byte aligned.
  * Backward: dQ, dK, dV of the inputs' shapes, every row written (zeros where nothing arrives), float32 accumulation, one
- *   writer per row: deterministic.  dK and dV of a shared head are summed over its query heads.  `workspace`:
+ *   writer per row: deterministic.  dK and dV of a shared head are summed over its query heads.  A null dQ.ptr, or null dK.ptr
+ *   and dV.ptr, leave that side out and its kernel with it.  `workspace`:
  *   hsa_dense_attn_bwd_workspace_bytes(...) bytes, 256-byte aligned.
  */
 size_t hsa_dense_mask_bytes(int batches, int heads, int rows, int Lk);

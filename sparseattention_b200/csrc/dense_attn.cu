@@ -291,7 +291,8 @@ extern "C" int hsa_dense_attn_bwd(hsa_view Q, hsa_view K, hsa_view V, hsa_view O
                                   hsa_view dK, hsa_view dV, const int *key_lengths, const void *packed_mask, int mask_batches,
                                   int mask_heads, int mask_rows, void *workspace, size_t workspace_bytes, int B, int Lq, int Lk,
                                   int H, int Hkv, int D, float scale, int dtype, int algo, void *stream) {
-    HSA_CHECK_ARG(Q.ptr && K.ptr && V.ptr && Out.ptr && LSE && dOut.ptr && dQ.ptr && dK.ptr && dV.ptr, "hsa_dense_attn_bwd: null pointer");
+    HSA_CHECK_ARG(Q.ptr && K.ptr && V.ptr && Out.ptr && LSE && dOut.ptr && (dQ.ptr || dK.ptr), "hsa_dense_attn_bwd: null pointer");
+    HSA_CHECK_ARG((dK.ptr == nullptr) == (dV.ptr == nullptr), "hsa_dense_attn_bwd: dK and dV are wanted together or not at all");
     if (int rc = check_shape("hsa_dense_attn_bwd", B, Lq, Lk, H, Hkv, D, scale, dtype, algo)) return rc;
     if (int rc = check_mask("hsa_dense_attn_bwd", packed_mask, mask_batches, mask_heads, mask_rows, B, H, Lq)) return rc;
     const size_t need = hsa_dense_attn_bwd_workspace_bytes(B, Lq, Lk, H, Hkv, D, dtype, algo);
@@ -314,7 +315,7 @@ extern "C" int hsa_dense_attn_bwd(hsa_view Q, hsa_view K, hsa_view V, hsa_view O
     a.neg_lse2 = neg_lse2; a.neg_delta = neg_delta;
     const int es = dtype_size(dtype);
     a.vec = D % 4 == 0;
-    for (const hsa_view &v : {Q, K, V, dOut, dQ, dK, dV}) a.vec = a.vec && rows_in_fours(v, es);
+    for (const hsa_view &v : {Q, K, V, dOut, dQ, dK, dV}) a.vec = a.vec && (v.ptr == nullptr || rows_in_fours(v, es));
     const bool tc = algo != 1 && dense_tc_ok(a, dtype, true) && dense_bwd_tables_ok(a);
     HSA_CHECK_ARG(algo != 2 || tc, "hsa_dense_attn_bwd: no tensor-core kernel for these inputs");
     cudaStream_t st = (cudaStream_t)stream;

@@ -488,10 +488,14 @@ static int f32_bwd(const DenseArgs &a, void *workspace, cudaStream_t st) {
     cudaError_t e = allow_smem<dense_dq_f32_kernel<T, DP>>(smem);
     if (e == cudaSuccess) e = allow_smem<dense_dkdv_f32_kernel<T, DP>>(smem);
     if (e != cudaSuccess) return fail((int)e, "hsa_dense_attn_bwd: shared memory %d: %s", smem, cudaGetErrorString(e));
-    dense_dkdv_f32_kernel<T, DP><<<(unsigned)k_blocks, S::kThreads, smem, st>>>(a, sk);
-    if (int rc = launch_status("hsa_dense_attn_bwd(dk, dv)")) return rc;
-    dense_dq_f32_kernel<T, DP><<<(unsigned)q_blocks, S::kThreads, smem, st>>>(a, sq);
-    if (int rc = launch_status("hsa_dense_attn_bwd(dq)")) return rc;
+    if (a.dk.ptr != nullptr) {
+        dense_dkdv_f32_kernel<T, DP><<<(unsigned)k_blocks, S::kThreads, smem, st>>>(a, sk);
+        if (int rc = launch_status("hsa_dense_attn_bwd(dk, dv)")) return rc;
+    }
+    if (a.dq.ptr != nullptr) {
+        dense_dq_f32_kernel<T, DP><<<(unsigned)q_blocks, S::kThreads, smem, st>>>(a, sq);
+        if (int rc = launch_status("hsa_dense_attn_bwd(dq)")) return rc;
+    }
     return join_backward<T>(a, sq, sk, st);
 }
 

@@ -144,9 +144,9 @@ int join_backward(const DenseArgs &a, const BwdSplit &sq, const BwdSplit &sk, cu
         return launch_status("hsa_dense_attn_bwd(join)");
     };
     const int64_t q_elems = (int64_t)a.B * a.Lq * a.H * a.D, k_elems = (int64_t)a.B * a.Lk * a.Hkv * a.D;
-    if (sq.splits > 1)
+    if (sq.splits > 1 && a.dq.ptr != nullptr)
         if (int rc = join(sq.part, sq.splits, q_elems, a.dq, a.Lq, a.H, a.scale)) return rc;
-    if (sk.splits > 1) {
+    if (sk.splits > 1 && a.dk.ptr != nullptr) {
         if (int rc = join(sk.part, sk.splits, k_elems, a.dk, a.Lk, a.Hkv, a.scale)) return rc;
         return join(sk.part + sk.splits * k_elems, sk.splits, k_elems, a.dv, a.Lk, a.Hkv, 1.f);
     }

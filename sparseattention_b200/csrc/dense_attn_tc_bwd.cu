@@ -813,10 +813,14 @@ static int bwd_launch(const DenseArgs &a, void *workspace, cudaStream_t st) {
     cudaError_t e = allow_smem<kdq>(smem_dq);
     if (e == cudaSuccess) e = allow_smem<kkv>(smem_kv);
     if (e != cudaSuccess) return fail((int)e, "hsa_dense_attn_bwd: shared memory %d / %d: %s", smem_dq, smem_kv, cudaGetErrorString(e));
-    kkv<<<(unsigned)kv_blocks, kBwdThreads, smem_kv, st>>>(a, sk, mq64, mk, mv, mg64);
-    if (int rc = launch_status("hsa_dense_attn_bwd(dk, dv)")) return rc;
-    kdq<<<(unsigned)dq_blocks, kBwdThreads, smem_dq, st>>>(a, sq, mq, mk, mv, mg);
-    if (int rc = launch_status("hsa_dense_attn_bwd(dq)")) return rc;
+    if (a.dk.ptr != nullptr) {
+        kkv<<<(unsigned)kv_blocks, kBwdThreads, smem_kv, st>>>(a, sk, mq64, mk, mv, mg64);
+        if (int rc = launch_status("hsa_dense_attn_bwd(dk, dv)")) return rc;
+    }
+    if (a.dq.ptr != nullptr) {
+        kdq<<<(unsigned)dq_blocks, kBwdThreads, smem_dq, st>>>(a, sq, mq, mk, mv, mg);
+        if (int rc = launch_status("hsa_dense_attn_bwd(dq)")) return rc;
+    }
     return join_backward<T>(a, sq, sk, st);
 }
 

@@ -507,8 +507,8 @@ bool dense_tc_ok(const DenseArgs &a, int dtype, bool backward) {
     if (a.mask.bits != nullptr && a.mask.tk > kFlagTiles) return false;
     if (!tc_view(a.q, a.B, a.Lq, a.H, a.D) || !tc_view(a.k, a.B, a.Lk, a.Hkv, a.D) || !tc_view(a.v, a.B, a.Lk, a.Hkv, a.D)) return false;
     if (!backward) return tc_view(a.out, a.B, a.Lq, a.H, a.D);
-    return tc_view(a.dout, a.B, a.Lq, a.H, a.D) && tc_view(a.dq, a.B, a.Lq, a.H, a.D) && tc_view(a.dk, a.B, a.Lk, a.Hkv, a.D) &&
-           tc_view(a.dv, a.B, a.Lk, a.Hkv, a.D);
+    return tc_view(a.dout, a.B, a.Lq, a.H, a.D) && (a.dq.ptr == nullptr || tc_view(a.dq, a.B, a.Lq, a.H, a.D)) &&
+           (a.dk.ptr == nullptr || (tc_view(a.dk, a.B, a.Lk, a.Hkv, a.D) && tc_view(a.dv, a.B, a.Lk, a.Hkv, a.D)));
 }
 
 template <typename T, int DP>

@@ -200,23 +200,26 @@ def dense_attention_forward(q, k, v, key_lengths=None, packed_mask=None, scale: 
     return out, rest, lse
 
 
+_NO_VIEW = _lib.HsaView(None, 0, 0)
+
+
 def dense_attention_backward(q, k, v, out, rest, lse, dout, key_lengths=None, packed_mask=None, scale: float = 1.0,
-                             algo: int = _lib.ALGO_AUTO):
-    """Raw backward with the device current: returns (dq, dk, dv)."""
+                             algo: int = _lib.ALGO_AUTO, need_q: bool = True, need_kv: bool = True):
+    """Raw backward with the device current: returns (dq, dk, dv), None for a side that is not asked for (one at least is)."""
     lib = _lib.load()
     dev = q.device
     B, Lq, H, D = q.shape
     Lk, Hkv = k.shape[1:3]
-    dq = torch.empty((B, Lq, H, D), dtype=q.dtype, device=dev)
-    dk = torch.empty((B, Lk, Hkv, D), dtype=q.dtype, device=dev)
-    dv = torch.empty((B, Lk, Hkv, D), dtype=q.dtype, device=dev)
+    dq = torch.empty((B, Lq, H, D), dtype=q.dtype, device=dev) if need_q else None
+    dk = torch.empty((B, Lk, Hkv, D), dtype=q.dtype, device=dev) if need_kv else None
+    dv = torch.empty((B, Lk, Hkv, D), dtype=q.dtype, device=dev) if need_kv else None
     dt = _lib.dtype_code(q)
     need = _bwd_workspace(B, Lq, Lk, H, Hkv, D, dt, algo, dev.index)
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
     rs, ks = H * D, Hkv * D
     view = _lib.HsaView
     rc = lib.hsa_dense_attn_bwd(_view(q), _view(k), _view(v), view(out.data_ptr(), Lq * rs, rs), _ptr(rest), _ptr(lse), _view(dout),
-                                view(dq.data_ptr(), Lq * rs, rs), view(dk.data_ptr(), Lk * ks, ks), view(dv.data_ptr(), Lk * ks, ks),
+                                *(_NO_VIEW if t is None else view(t.data_ptr(), n * row, row) for t, n, row in ((dq, Lq, rs), (dk, Lk, ks), (dv, Lk, ks))),
                                 _ptr(key_lengths), *_mask_args(packed_mask), _ptr(ws), need, B, Lq, Lk, H, Hkv, D, scale,
                                 dt, algo, _lib.stream_ptr(dev))
     if rc:
@@ -242,7 +245,8 @@ def _once(grads):
     # gradient mode is on inside a backward only when its result is to be differentiated (create_graph)
     if not torch.is_grad_enabled():
         return grads
-    return _Once.apply(*(t.requires_grad_(True) for t in grads))
+    there = iter(_Once.apply(*(t.requires_grad_(True) for t in grads if t is not None)))
+    return tuple(None if t is None else next(there) for t in grads)
 
 
 def _unpack_mask(packed: _Packed, Lk: int) -> torch.Tensor:
@@ -288,7 +292,8 @@ class _CrossAttention(torch.autograd.Function):
             return (*_elementary_gradients(q, k, v, dout, packed, scale), None, None, None, None, None, None)
         with _lib.on_device(q.device):
             dout = _rows(dout if dout.dtype == q.dtype else dout.to(q.dtype))
-            grads = dense_attention_backward(q, k, v, out, rest, lse, dout, key_lengths, packed, scale, algo)
+            grads = dense_attention_backward(q, k, v, out, rest, lse, dout, key_lengths, packed, scale, algo, ctx.needs_input_grad[0],
+                                             ctx.needs_input_grad[1] or ctx.needs_input_grad[2])
         return (*_once(grads), None, None, None, None, None, None)
 
 
@@ -302,7 +307,7 @@ class _NoRows(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dout):
-        return (*_once(tuple(torch.zeros_like(t) for t in ctx.saved_tensors)), None)
+        return (*_once(tuple(torch.zeros_like(t) if need else None for t, need in zip(ctx.saved_tensors, ctx.needs_input_grad))), None)
 
 
 def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, key_lengths: Optional[torch.Tensor] = None,

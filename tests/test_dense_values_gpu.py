@@ -248,3 +248,24 @@ def test_float16_keeps_many_small_weights_next_to_a_large_one(kind, algo):
     else:
         out = cross_attention(q, k, v, scale=1.0, algo=algo)
     assert float((out.double() - want).abs().max()) <= n * 2.0 ** -32 + want * (u + 2.0 ** -15)
+
+
+@pytest.mark.parametrize("case", [(2, 150, 300, 4, 2, 64, torch.bfloat16), (1, 20, 5000, 2, 1, 128, torch.float16), (1, 5000, 70, 2, 2, 64, torch.bfloat16),
+                                  (2, 40, 90, 2, 1, 40, torch.float32), (1, 10, 4000, 2, 2, 32, torch.float32), (2, 3, 0, 2, 2, 64, torch.float32)])
+def test_gradients_that_nobody_asked_for_are_not_computed(case):
+    """Each subset of the inputs gets the bits that it gets with all of them, and the entry takes null pointers for a side left out."""
+    *shape, dtype = case
+    q, k, v, g = make(*shape, dtype, seed=8)
+    want = run_training(q, k, v, g, algo=0)
+    for subset in ((0,), (1,), (2,), (1, 2), (0, 2)):
+        leaves = [t.detach().requires_grad_(i in subset) for i, t in enumerate((q, k, v))]
+        with torch.autograd.graph.save_on_cpu():                 # and what is saved may be stored elsewhere meanwhile
+            out = cross_attention(*leaves)
+        made = torch.autograd.grad(out, [leaves[i] for i in subset], g)
+        assert all(torch.equal(a, want[i]) for a, i in zip(made, subset))
+    if shape[2]:
+        out, rest, lse = dense_attention_forward(q, k, v, scale=shape[-1] ** -0.5)
+        dq, dk, dv = dense_attention_backward(q, k, v, out, rest, lse, g, scale=shape[-1] ** -0.5, need_kv=False)
+        assert dk is None and dv is None and torch.equal(dq, want[0])
+        dq, dk, dv = dense_attention_backward(q, k, v, out, rest, lse, g, scale=shape[-1] ** -0.5, need_q=False)
+        assert dq is None and torch.equal(dk, want[1]) and torch.equal(dv, want[2])
