@@ -19,7 +19,7 @@
 // products issued from uniform registers 492 and 427 us; scores and gradients issued by a warp each 445 and 350 us; output rows
 // through quad transposes 430 and 341 us.
 // Rounding: p and ds are rounded to the inputs' type once, as operands; all sums are 32-bit.  In float16 both are moved into the middle
-// of the type's range first (grad_shift): p by 2^15, ds by a power of two per query row for dq, per key/value head for dk.
+// of the type's range first (grad_shift): p by 2^13, ds by a power of two per query row for dq, per key/value head for dk.
 #include "dense_attn_tc.cuh"
 
 namespace hsa {
@@ -345,7 +345,7 @@ dense_dq_tc5_kernel(const DenseArgs a, const BwdSplit sp, const __grid_constant_
                                 if (!((keep >> (2 * j)) & 1u)) y.x = 0.f;
                                 if (!((keep >> (2 * j + 1)) & 1u)) y.y = 0.f;
                             }
-                            d[j] = pack2<T>(y.x, y.y);
+                            d[j] = pack2_finite<T>(y.x, y.y);
                         }
                     };
                     if (partial) gradients(std::false_type{}); else gradients(std::true_type{});
@@ -720,8 +720,8 @@ dense_dkdv_tc5_kernel(const DenseArgs a, const BwdSplit sp, const __grid_constan
                                 if (!((keep >> (2 * c + 1)) & 1u)) p.y = y.y = 0.f;
                             }
                             if constexpr (!BF) y = unpair(mul2(pair(y.x, y.y), ds_factor2));
-                            pk[c] = pack2<T>(p.x, p.y);
-                            dk[c] = pack2<T>(y.x, y.y);
+                            pk[c] = pack2_finite<T>(p.x, p.y);
+                            dk[c] = pack2_finite<T>(y.x, y.y);
                         }
                     }
                 };

@@ -413,7 +413,7 @@ dense_fwd_tc5_kernel(const DenseArgs a, const DenseSplit sp, const __grid_consta
                                 if (decltype(mixed)::value && j % 3 == 0) p = exp2_poly(e);
                                 else p = make_float2(fast_exp2(e.x), fast_exp2(e.y));
                                 sum[j & 1] = add2(sum[j & 1], pair(p.x, p.y));
-                                pk[j] = pack2<T>(p.x, p.y);
+                                pk[j] = pack2_finite<T>(p.x, p.y);
                             }
                         };
                         // A third of the exponentials goes to the multiply-add units: with fewer the special-function unit, with

@@ -353,7 +353,7 @@ __global__ void __launch_bounds__(kPagedWarps * 32) paged_decode_mma_kernel(cons
                 s[n][e] = fast_exp2(s[n][e] - ref[e >> 1]);
                 l[e >> 1] += s[n][e];
             }
-        const uint32_t p[4] = {pack2<T>(s[0][0], s[0][1]), pack2<T>(s[0][2], s[0][3]), pack2<T>(s[1][0], s[1][1]), pack2<T>(s[1][2], s[1][3])};
+        const uint32_t p[4] = {pack2_finite<T>(s[0][0], s[0][1]), pack2_finite<T>(s[0][2], s[0][3]), pack2_finite<T>(s[1][0], s[1][1]), pack2_finite<T>(s[1][2], s[1][3])};
 #pragma unroll
         for (int d = 0; d < DP / 16; ++d) {
             uint32_t f[4];

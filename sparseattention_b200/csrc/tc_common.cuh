@@ -59,6 +59,18 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
         return *reinterpret_cast<uint32_t *>(&v);
     }
 }
+// The same for operands moved up in float16's range: what passes its largest number by a rounding (of a score beyond 2^20, say) becomes
+// that number instead of infinity, which a product would turn into NaN.
+template <typename T>
+__device__ __forceinline__ uint32_t pack2_finite(float lo, float hi) {
+    if constexpr (std::is_same<T, __half>::value) {
+        uint32_t r;
+        asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;\n" : "=r"(r) : "f"(hi), "f"(lo));
+        return r;
+    } else {
+        return pack2<T>(lo, hi);
+    }
+}
 
 // ---- tile-local tree storage ------------------------------------------------------------------
 // In-tile nodes of levels 1..5 are stored level after level; causal tiles keep only even nodes.

@@ -269,3 +269,21 @@ def test_gradients_that_nobody_asked_for_are_not_computed(case):
         assert dk is None and dv is None and torch.equal(dq, want[0])
         dq, dk, dv = dense_attention_backward(q, k, v, out, rest, lse, g, scale=shape[-1] ** -0.5, need_q=False)
         assert dq is None and torch.equal(dk, want[1]) and torch.equal(dv, want[2])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("size", [120.0, 1000.0, 4096.0])
+def test_scores_so_large_that_their_rounding_shows(size, dtype):
+    """Every score 1.2e5, 8e6, 1.3e8: the 32-bit log-sum-exp is then off by a part of 1, or by tens (its tolerance says by how much),
+    and a weight recomputed from it passes 1.  Results stay finite, and the forward stays the mean of the values."""
+    q, k, v, g = make(1, 130, 300, 1, 1, 64, dtype, seed=14)
+    q, k = torch.full_like(q, size), torch.full_like(k, size)
+    out, *grads = check(q, k, v, g, algo=2)
+    assert all(t.isfinite().all() for t in grads)
+    mean = v[0, :, 0].double().mean(0)
+    u = torch.finfo(dtype).eps / 2
+    assert ((out[0, :, 0].double() - mean).abs() <= u * mean.abs() + (u + 2.0 ** -15) * v[0, :, 0].double().abs().mean(0)).all()
+    page = torch.arange(19, dtype=torch.int32, device="cuda").view(1, -1)
+    kp, vp = (torch.cat([t[0], t[0, :4]]).view(19, 16, 1, 64) for t in (k, v))
+    got = paged_attention_decode(q[:, 0], kp, vp, page, torch.tensor([300], dtype=torch.int32, device="cuda"), algo=2)
+    assert ((got[0, 0].double() - mean).abs() <= u * mean.abs() + (u + 2.0 ** -15) * v[0, :, 0].double().abs().mean(0)).all()
