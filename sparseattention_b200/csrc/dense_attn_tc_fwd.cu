@@ -35,6 +35,7 @@ __device__ unsigned int g_dense_aborts = 0;
 // Softmax of two query tiles, copies, a warp of products for either tile, and an idle warp that completes the last warpgroup:
 // its registers go to the softmax (2 x 128 x 200 + 128 x 104 = 384 x 168, what the block is launched with).
 constexpr int kFwdThreads = 384;
+constexpr float kLargeScore = 1048576.f;         // in base 2
 
 template <int DP>
 struct FwdShape {
@@ -379,11 +380,12 @@ dense_fwd_tc5_kernel(const DenseArgs a, const DenseSplit sp, const __grid_consta
 #pragma unroll
                         for (int j = 0; j < 64; j += 2)
                             tops[j >> 1 & 3] = max3_nan(tops[j >> 1 & 3], __uint_as_float(r[j >> 5][j & 31]), __uint_as_float(r[j >> 5][(j + 1) & 31]));
-                        const float top = max3_nan(max3_nan(tops[0], tops[1], tops[2]), tops[3], tops[3]) * a.scale_log2;
-                        const bool grow = top > m + 8.f;             // also the first finite maximum (m = -inf)
-                        if (__any_sync(0xffffffffu, grow)) {
+                        const float top = max3_nan(max3_nan(tops[0], tops[1], tops[2]), tops[3], tops[3]);
+                        float ref = m * a.scale_log2;
+                        const bool grow = top * a.scale_log2 > ref + 8.f;       // also the first finite maximum (m = -inf)
+                        if (__any_sync(0xffffffffu, grow || (fabsf(ref) > kLargeScore && m != -INFINITY))) {
                             const float m_new = grow ? top : m;
-                            const float corr = grow ? fast_exp2(m - m_new) : 1.f;
+                            const float corr = grow ? fast_exp2((m - m_new) * a.scale_log2) : 1.f;
                             if (any) {
                                 if (!(ok = wait(o_full(w), (sc - 1) & 1))) break;      // these scores follow the product before that one
                                 fence_after_sync();
@@ -399,9 +401,19 @@ dense_fwd_tc5_kernel(const DenseArgs a, const DenseSplit sp, const __grid_consta
                                 l *= corr;
                             }
                             m = m_new;
+                            ref = m * a.scale_log2;
+                            // c s - c m, one rounding of c m apart, is off by that rounding: a common factor of the row's weights, but
+                            // beyond 2^24 one that leaves their range.  Such rows take the difference first.
+                            const bool large = fabsf(ref) > kLargeScore && m != -INFINITY;
+                            if (__any_sync(0xffffffffu, large)) {
+                                const float base = large ? m : 0.f;
+#pragma unroll
+                                for (int j = 0; j < 64; ++j) r[j >> 5][j & 31] = __float_as_uint(__uint_as_float(r[j >> 5][j & 31]) - base);
+                                if (large) ref = 0.f;
+                            }
                         }
                         // a NaN score, or one of plus infinity, makes NaN of all weights of its row here, and so of its sum and result
-                        const float ref = !(top < INFINITY) ? NAN : m == -INFINITY ? 0.f : m - SHIFT;
+                        ref = !(top < INFINITY) ? NAN : ref == -INFINITY ? 0.f : ref - SHIFT;
                         const uint64_t c2 = pair(a.scale_log2, a.scale_log2), ref2 = pair(-ref, -ref);
                         uint64_t sum[2] = {0, 0};                    // two pairs of zeros
                         uint32_t pk[32];
@@ -459,8 +471,8 @@ dense_fwd_tc5_kernel(const DenseArgs a, const DenseSplit sp, const __grid_consta
                     }
                 }
                 if (qi < a.Lq) {
-                    if (sp.splits > 1) *reinterpret_cast<float2 *>(sp.part_ml + 2 * at) = make_float2(m - SHIFT, l);
-                    if (sp.splits == 1 && a.lse != nullptr) a.lse[at] = none ? -INFINITY : (m - SHIFT + log2f(l)) * 0.6931471805599453f;
+                    if (sp.splits > 1) *reinterpret_cast<float2 *>(sp.part_ml + 2 * at) = make_float2(m * a.scale_log2 - SHIFT, l);
+                    if (sp.splits == 1 && a.lse != nullptr) a.lse[at] = none ? -INFINITY : (m * a.scale_log2 - SHIFT + log2f(l)) * 0.6931471805599453f;
                 }
                 if (sp.splits == 1 && a.empty_value != 0.f) {        // other lanes wrote the row's zeros: they come first
                     __syncwarp();

@@ -272,9 +272,9 @@ def test_gradients_that_nobody_asked_for_are_not_computed(case):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
-@pytest.mark.parametrize("size", [120.0, 1000.0, 4096.0])
+@pytest.mark.parametrize("size", [120.0, 1000.0, 4096.0, 30000.0])
 def test_scores_so_large_that_their_rounding_shows(size, dtype):
-    """Every score 1.2e5, 8e6, 1.3e8: the 32-bit log-sum-exp is then off by a part of 1, or by tens (its tolerance says by how much),
+    """Every score 1.2e5, 8e6, 1.3e8, 7e9: the 32-bit log-sum-exp is then off by a part of 1, or by tens (its tolerance says by how much),
     and a weight recomputed from it passes 1.  Results stay finite, and the forward stays the mean of the values."""
     q, k, v, g = make(1, 130, 300, 1, 1, 64, dtype, seed=14)
     q, k = torch.full_like(q, size), torch.full_like(k, size)
@@ -287,3 +287,24 @@ def test_scores_so_large_that_their_rounding_shows(size, dtype):
     kp, vp = (torch.cat([t[0], t[0, :4]]).view(19, 16, 1, 64) for t in (k, v))
     got = paged_attention_decode(q[:, 0], kp, vp, page, torch.tensor([300], dtype=torch.int32, device="cuda"), algo=2)
     assert ((got[0, 0].double() - mean).abs() <= u * mean.abs() + (u + 2.0 ** -15) * v[0, :, 0].double().abs().mean(0)).all()
+
+
+@pytest.mark.parametrize("algo", [1, 2])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_large_scores_of_either_sign_choose_the_largest(dtype, algo):
+    """Scores from -7e9 to 7e9 in steps that no rounding closes: the result is the one value, row by row, wherever its key lies."""
+    Lq, Lk = 140, 330
+    q, _, v, _ = make(1, Lq, Lk, 1, 1, 64, dtype, seed=4)
+    order = torch.randperm(Lk, generator=torch.Generator(device="cuda").manual_seed(2), device="cuda")
+    k = torch.zeros_like(v)
+    k[0, :, 0, 0] = ((order.double() + 1) * 64 - 10624).to(dtype)                       # at least 64 apart in float16, 0 to 128 in bfloat16
+    q = torch.zeros_like(q)
+    q[0, :, 0, 0] = torch.linspace(-30000, 30000, Lq, device="cuda").to(dtype)
+    out, _, lse = dense_attention_forward(q, k, v, scale=8.0, algo=algo)
+    s = 8 * q[0, :, 0, 0].double().view(-1, 1) * k[0, :, 0, 0].double()
+    p = torch.softmax(s, -1)
+    want = p @ v[0, :, 0].double()
+    u = torch.finfo(dtype).eps / 2
+    assert ((out[0, :, 0].double() - want).abs() <= (u + 2.0 ** -15) * (p @ v[0, :, 0].double().abs()) + u * want.abs()).all()
+    top = s.amax(-1) + torch.log(torch.exp(s - s.amax(-1, keepdim=True)).sum(-1))
+    assert ((lse[0, :, 0].double() - top).abs() <= (top.abs() + 4) * 2.0 ** -22).all()
