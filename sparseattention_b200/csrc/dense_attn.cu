@@ -95,47 +95,61 @@ __global__ void __launch_bounds__(256) dense_delta_kernel(const DenseArgs a, flo
     delta_row<T, VEC, LPR, CPL>(a, b, i, h, threadIdx.x % LPR, neg_lse2, neg_delta, 0.f);
 }
 
-// The same for float16 on the tensor cores, with the squared lengths of dout's rows and the largest of those and of V's rows per (batch
-// entry, key/value head): a block takes a stretch of the query rows of all heads of a group, or of V's rows (those that may be looked
-// at: the others may hold anything).
-constexpr int kStretch = 4;                               // times 256 / LPR rows
+// The same for float16 on the tensor cores, with the squared lengths of dout's rows, the largest of those per (batch entry, key/value
+// head), and a bound on those of V's rows: D times the square of the largest entry.  A block takes a stretch of the query rows of all
+// heads of a group, or of V's rows (those that may be looked at: the others may hold anything).  V's part is bound by HBM, so a thread
+// asks for eight pieces before it looks at one, and takes entries instead of lengths of rows, whose sums would stand between the loads.
+constexpr int kStretch = 4;                               // times 256 / LPR query rows
+constexpr int kValueRows = 128;
 template <int VEC, int LPR, int CPL>
 __global__ void __launch_bounds__(256)
 dense_delta_f16_kernel(const DenseArgs a, float *__restrict__ neg_lse2, float *__restrict__ neg_delta, float *__restrict__ dout_sq,
                        unsigned int *__restrict__ top_sq, int q_blocks, int v_blocks) {
     using T = __half;
     constexpr int RPB = 256 / LPR;
-    const int g = threadIdx.x % LPR, unit = threadIdx.x / LPR;
     const int at = blockIdx.x % (q_blocks + v_blocks);
     const int bh = blockIdx.x / (q_blocks + v_blocks), hk = bh % a.Hkv;
     const int64_t b = bh / a.Hkv;
-    const bool values = at >= q_blocks;
+    const bool values = at < v_blocks;
     float top = 0.f;
     if (!values) {
-        const int rows = a.group * a.lq_pad;
+        const int g = threadIdx.x % LPR, unit = threadIdx.x / LPR, rows = a.group * a.lq_pad;
         for (int s = 0; s < kStretch; ++s) {
-            const int r = (at * kStretch + s) * RPB + unit, h = hk * a.group + r / a.lq_pad, i = r % a.lq_pad;
+            const int r = ((at - v_blocks) * kStretch + s) * RPB + unit, h = hk * a.group + r / a.lq_pad, i = r % a.lq_pad;
             if (r >= rows) break;
             const float sq = group_sum<LPR>(delta_row<T, VEC, LPR, CPL>(a, b, i, h, g, neg_lse2, neg_delta, (float)kWeightShift));
             if (g == 0) dout_sq[(b * a.H + h) * a.lq_pad + i] = sq;
             top = sq > top || sq != sq ? sq : top;
         }
     } else {
-        const int n = dense_keys(a, (int)b);
-        for (int s = 0; s < kStretch; ++s) {
-            const int j = ((at - q_blocks) * kStretch + s) * RPB + unit;
-            if (j >= n) break;
-            bool seen = a.mask.bits == nullptr;
-            for (int h = hk * a.group; !seen && h < (hk + 1) * a.group; ++h) {
-                const int64_t plane = b * a.mask.plane_b + (int64_t)h * a.mask.plane_h;
-                seen = (a.mask.seen[plane * a.mask.wk + (j >> 5)] >> (j & 31)) & 1u;
+        const int n = dense_keys(a, (int)b), chunks = a.D / 8, j0 = at * kValueRows, pieces = min(kValueRows, n - j0) * chunks;
+        const T *V = (const T *)a.v.ptr + b * a.v.batch_stride + (int64_t)j0 * a.v.row_stride + (int64_t)hk * a.D;
+        __half2 most = __float2half2_rn(0.f);
+        for (int first = threadIdx.x; first < pieces; first += 8 * 256) {
+            uint4 x[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const int idx = first + u * 256, r = idx / chunks;
+                bool take = idx < pieces;
+                if (take && a.mask.bits != nullptr) {
+                    take = false;
+                    for (int h = hk * a.group; !take && h < (hk + 1) * a.group; ++h) {
+                        const int64_t plane = b * a.mask.plane_b + (int64_t)h * a.mask.plane_h;
+                        take = (a.mask.seen[plane * a.mask.wk + ((j0 + r) >> 5)] >> ((j0 + r) & 31)) & 1u;
+                    }
+                }
+                x[u] = take ? __ldg(reinterpret_cast<const uint4 *>(V + (int64_t)r * a.v.row_stride + (idx - r * chunks) * 8)) : make_uint4(0, 0, 0, 0);
             }
-            if (!seen) continue;
-            RowFrag<T, VEC, LPR, CPL> x;
-            x.load((const T *)a.v.ptr + b * a.v.batch_stride + (int64_t)j * a.v.row_stride + (int64_t)hk * a.D, g, a.D / VEC);
-            const float sq = group_sum<LPR>(x.dot_partial(x));
-            top = sq > top || sq != sq ? sq : top;
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t w = e == 0 ? x[u].x : e == 1 ? x[u].y : e == 2 ? x[u].z : x[u].w;
+                    most = __hmax2(most, __habs2(*reinterpret_cast<const __half2 *>(&w)));
+                }
         }
+        const float m = fmaxf(__low2float(most), __high2float(most));
+        top = (float)a.D * m * m;
     }
     __shared__ unsigned int warp_top[8];
     // bit patterns of numbers that are not negative are in the numbers' order, NaN last
@@ -168,7 +182,7 @@ static int dense_delta_f16(const DenseArgs &a, float *neg_lse2, float *neg_delta
     int rc = 0;
     const bool ok = dispatch_row_shape<__half>(a.D, vec, [&]<typename T, int VEC, int LPR, int CPL>() {
         constexpr int per = kStretch * (256 / LPR);
-        const long long q_blocks = ((long long)a.group * a.lq_pad + per - 1) / per, v_blocks = (a.Lk + per - 1) / per;
+        const long long q_blocks = ((long long)a.group * a.lq_pad + per - 1) / per, v_blocks = (a.Lk + kValueRows - 1) / kValueRows;
         const long long blocks = (q_blocks + v_blocks) * a.B * a.Hkv;
         if (blocks > 0x7fffffffLL || (long long)a.group * a.lq_pad > 0x7fffffffLL) { rc = fail(HSA_ERR_ARG, "hsa_dense_attn_bwd: too many rows"); return; }
         dense_delta_f16_kernel<VEC, LPR, CPL><<<(unsigned)blocks, 256, 0, st>>>(a, neg_lse2, neg_delta, dout_sq, top_sq, (int)q_blocks, (int)v_blocks);
