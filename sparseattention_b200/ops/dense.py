@@ -23,18 +23,18 @@ from .. import _lib
 # The kernels write through raw pointers: of a call, a tracer or a transform would see the allocation of the result and nothing that
 # fills it, and a forward-mode tangent would end there.
 _INFRA_MODES = (torch._C._TorchDispatchModeKey.PROXY, torch._C._TorchDispatchModeKey.FAKE, torch._C._TorchDispatchModeKey.FUNCTIONAL)
+_modes, _tracing, _transform = torch._C._len_torch_dispatch_stack, torch._C._is_tracing, torch._C._functorch.peek_interpreter_stack
 
 
 def transforms_active() -> bool:
     """Whether torch is tracing, compiling, transforming or watching operations, or computes forward-mode derivatives."""
-    return (torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() > 0 or torch._C._get_tracing_state() is not None
-            or forward_ad._current_level >= 0 or torch._C._functorch.peek_interpreter_stack() is not None)
+    return torch.compiler.is_compiling() or _modes() > 0 or _tracing() or forward_ad._current_level >= 0 or _transform() is not None
 
 
 def _refuse_transforms(who: str, *tensors: Optional[torch.Tensor]) -> None:
-    if not transforms_active():
+    if not (_modes() > 0 or _tracing() or forward_ad._current_level >= 0 or _transform() is not None):
         return
-    if torch._C._get_tracing_state() is not None or any(torch._C._get_dispatch_mode(m) is not None for m in _INFRA_MODES):
+    if _tracing() or any(torch._C._get_dispatch_mode(m) is not None for m in _INFRA_MODES):
         raise _lib.HsaError(f"{who} cannot be traced: the graph would hold the allocation of its result and not the kernel")
     for t in tensors:
         if t is None:
