@@ -308,3 +308,31 @@ def test_large_scores_of_either_sign_choose_the_largest(dtype, algo):
     assert ((out[0, :, 0].double() - want).abs() <= (u + 2.0 ** -15) * (p @ v[0, :, 0].double().abs()) + u * want.abs()).all()
     top = s.amax(-1) + torch.log(torch.exp(s - s.amax(-1, keepdim=True)).sum(-1))
     assert ((lse[0, :, 0].double() - top).abs() <= (top.abs() + 4) * 2.0 ** -22).all()
+
+
+def test_float16_training_captured_and_replayed():
+    """The powers of two follow each replay's own inputs, up and down, and two graphs do not disturb each other."""
+    shapes = [(2, 140, 300, 4, 2, 64), (1, 20, 5000, 2, 2, 128)]
+    static, graphs = [], []
+    for shape in shapes:
+        static.append([t.clone() for t in make(*shape, torch.float16, seed=3)])
+        run_training(*static[-1], algo=0)
+    torch.cuda.synchronize()
+    for tensors in static:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            res = run_training(*tensors, algo=0)
+        graphs.append((graph, res))
+    for seed, size in ((5, 1e-3), (6, 4.0), (7, 1e-4), (8, 0.0)):
+        for tensors, shape in zip(static, shapes):
+            for t, new in zip(tensors, make(*shape, torch.float16, seed=seed)):
+                t.copy_(new)
+            tensors[3].mul_(size)
+        for graph, _ in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for tensors, (_, res) in zip(static, graphs):
+            assert all(torch.equal(a, b) for a, b in zip(res, run_training(*tensors, algo=0)))
+            _, *want, _ = definition(*tensors)
+            for name, a, b in zip(("dq", "dk", "dv"), res, want):
+                assert not a.any() if size == 0 else as_good_as_rounded(a, b, name) is None
