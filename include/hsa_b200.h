@@ -412,7 +412,8 @@ int hsa_cross_entropy_bwd_inplace(void *logits, long long row_stride, const long
  *   receives what rounding took from Out, in the same type, packed [B, Lq, H, D]: given to the backward it makes the row sums of
  *   dOut * Out as exact as those of a 32-bit output.
  *   scale > 0.  D <= 256.  `algo`: 0 = automatic, 1 = 32-bit kernels (any type), 2 = tcgen05 kernels (bf16 / f16, D a multiple of
- *   8 up to 128, 16-byte aligned rows; HSA_ERR_ARG otherwise).  `workspace`: hsa_dense_attn_fwd_workspace_bytes(...) bytes (often 0; few
+ *   8 up to 128, 16-byte aligned rows, and with a mask Lk <= 98304 and, in the backward with a row per query,
+ *   H / Hkv * ceil(Lq / 128) <= 768; HSA_ERR_ARG otherwise, where 0 takes the far slower 32-bit kernels).  `workspace`: hsa_dense_attn_fwd_workspace_bytes(...) bytes (often 0; few
  *   queries over many keys are cut into ranges of keys that are joined afterwards), 256-byte aligned.
  * Masks come packed (hsa_dense_mask_pack): `mask` points to bytes (0 = may not look), four strides in bytes, of a tensor
  *   [batches, heads, rows, Lk] with batches 1 or B, heads 1 or H, rows 1 or Lq; `packed` receives

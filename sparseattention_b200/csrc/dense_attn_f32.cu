@@ -7,9 +7,10 @@
 // A warp owns 16 rows (queries; keys in the dk/dv kernel) and walks over tiles of the other side, which lie in shared memory as
 // float32.  Products run on the tensor cores in three passes: x = hi + lo with hi = x rounded to 11 bits (tf32) and lo the rest
 // rounded to 11 bits, a b ~ hi hi + hi lo + lo hi, off by at most about 3 * 2^-22 |a b|, summed in 32 bits.  Bound by the rate of
-// these warp-level products, measured at about 130 multiply-adds per cycle and SM, three for one here.  (32-bit multiply-adds on
-// the same tiles did not come nearer to their own rate: forward 2048 x 2048, 8 heads of 64: 346 us here, 420 and 314 us with 8 x 4
-// and 4 x 4 of them per thread; forward and backward 2 x 1024 x 1024, 16 heads of 128: 2734 us against 3197 and 3594.)
+// these warp-level products, measured at about 130 multiply-adds per cycle and SM, three for one here, and by the additions between them
+// (mma_split): forward 2048 x 2048, 8 heads of 64: 399 us; forward and backward 2 x 1024 x 1024, 16 heads of 128: 3350 us.  That is no
+// faster than 32-bit multiply-adds on the same tiles were: 420 and 314 us, and 3197 and 3594 us, with 8 x 4 and 4 x 4 of them per
+// thread, either of which wins one of the two.  (With all sums left to the tensor cores, which cut off, it was 346 and 2734 us.)
 // Weights pass from the first product to the second through shared memory, inside a warp.  Rows are padded so that fragment reads
 // have no bank conflicts (two-way for the operands that are read along both axes).  One writer per output row, fixed order of
 // summation.  Keys behind a sequence's length, and keys that no query may look at, are stored as zeros: what lies there (NaN,
@@ -19,7 +20,7 @@
 namespace hsa {
 
 // Tile sizes by padded head dim: a block's own rows, the rows of a tile of the other side (32 where 64 would leave room for one block
-// per SM only: 4686 -> 2734 us at 2 x 1024 x 1024, 16 heads of 128, forward and backward), and warps per 16 own rows (each with its
+// per SM only: 4686 -> 2734 us at 2 x 1024 x 1024, 16 heads of 128, forward and backward, with all sums in the tensor cores), and warps per 16 own rows (each with its
 // share of the output columns)
 template <int DP> struct F32Shape {
     static constexpr int kRows = DP <= 128 ? 64 : 32, kOther = DP <= 64 ? 64 : 32, kSplit = DP <= 128 ? 1 : 2;

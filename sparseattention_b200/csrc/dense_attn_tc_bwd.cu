@@ -19,7 +19,8 @@
 // products issued from uniform registers 492 and 427 us; scores and gradients issued by a warp each 445 and 350 us; output rows
 // through quad transposes 430 and 341 us.
 // Rounding: p and ds are rounded to the inputs' type once, as operands; all sums are 32-bit.  In float16 both are moved into the middle
-// of the type's range first (grad_shift): p by 2^13, ds by a power of two per query row for dq, per key/value head for dk.
+// of the type's range first (grad_shift): p by 2^13, ds by a power of two per query row for dq, per key/value head for dk.  Weights
+// come back from the saved log-sum-exp, whose 32 bits hold a score of 1e5 to 1e-2: beyond that gradients follow its rounding.
 #include "dense_attn_tc.cuh"
 
 namespace hsa {

@@ -492,21 +492,24 @@ using namespace hsa;
 
 // Whether blocks start in the order of their sequences' lengths, the longest first: where more blocks are launched than run at
 // once, so that the last ones to start are short, and where sequences may be long enough to pay for every block's look at all
-// lengths (64 sequences of up to 2000 keys on 8 heads of 64: 50.1 us unsorted and 37.6 sorted when ragged, 70.0 and 72.0 when all
-// are full; 100 of up to 512 on 16 heads lose a tenth either way and stay unsorted).
+// lengths (64 sequences of up to 2000 keys on 8 heads of 64 in one range: 41.2 us unsorted and 38.3 sorted when ragged, 50.7 and 51.7
+// when all are full; 100 of up to 512 on 16 heads would go from 32.2 to 33.6 and from 44.8 to 47.8, and stay unsorted).
 static bool paged_sorted(int B, int H, int Hkv, int page_size, int max_pages, int splits) {
     const long long blocks = (long long)B * Hkv * ((H / Hkv + 15) / 16) * splits;
     const long long room = (long long)max_pages * page_size;
     return B > 1 && B <= kPagedWarps * 32 && blocks > 2LL * dense_sm_count() && room >= (long long)splits * (B > 64 ? 8 * B : 512);
 }
 
-// Ranges per sequence.  Two blocks fit an SM (four at small head dims, where the same counts came out near the best); a block costs its steps of 64 keys plus about two and a half steps' time, and the join
-// about one.  The count with the least (rounds of blocks) x (cost of a block): one full round where that fits (2 sequences of
-// 131072 keys on 8 key/value heads: 88.6 us in 37 ranges, 97.9 in 74, 143 in 16).  With more sequences than blocks fit at once,
-// where lengths may differ: the coarsest cut that costs no more than a tenth if the longest come first (32 sequences of up to 4096
-// keys on 16 heads: 88.6 us ragged and 184 full in one range, 110 and 188 in four), else the finest that costs no more than a
-// twentieth (the same unsorted: 121 us in one range, 112 in four).  The table's room stands in for the lengths, which are on the
-// device.
+// Ranges per sequence.  Two blocks fit an SM at head dims from 72 to 128; a block costs its steps of 64 keys plus about two and a
+// half steps' time, and the join about one.  The count with the least (rounds of blocks) x (cost of a block): one full round where
+// that fits (2 sequences of 131072 keys on 4 key/value heads of 128: 88.7 us in 37 ranges, 96.6 in 74, 144 in 16).  With more sequences
+// than blocks fit at once, where lengths may differ: the coarsest cut that costs no more than a tenth if the longest come first (32
+// sequences of up to 4096 keys on 16 heads of 128: 89.2 us ragged and 186 full in one range, 110 and 188 in four), else the finest
+// that costs no more than a twentieth (the same unsorted: 121 us ragged in one range, 112 in four).  The table's room stands in for
+// the lengths, which are on the device.
+// The head dim has no part in it, though four blocks fit an SM up to 64 and one above 128: at 64 the count is the best or near it for
+// some sizes (20 sequences of up to 8192 keys on 16 heads: three ranges, 57.1 us ragged and 115 full; 100 of 512: one, 44.8) and far
+// from it for others (16 of up to 4096 on 16 heads: 54.5 and 60.2 us in its one range, 29.3 and 51.4 in four).
 extern "C" int hsa_paged_attn_choose_splits(int B, int H, int Hkv, int page_size, int max_pages) {
     if (B < 1 || H < 1 || Hkv < 1 || page_size < 1 || max_pages < 1) return 1;
     const long long units = (long long)B * Hkv * ((H / Hkv + 15) / 16), room = (long long)max_pages * page_size;

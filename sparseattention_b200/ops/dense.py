@@ -326,7 +326,10 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, key_lengt
     length, or in keys that a mask hides from all queries, may be anything; everything else has to be finite.
     Differentiable once with respect to q, k and v.  In bfloat16 and float16 the weights and the gradients of the scores are
     rounded to that type between the products (in float16's backward moved into the middle of its range first); sums are 32-bit.
-    A mask is packed into bits by every call; keys that only a length hides are cheaper given as key_lengths.
+    A mask is packed into bits by every call; keys that only a length hides are cheaper given as key_lengths.  With a mask of more
+        than 98304 keys, or in the backward one with a row per query where H // Hkv * ceil(Lq / 128) > 768 (say 8 query heads per
+        key/value head from 12289 queries on), bfloat16 and float16 run the 32-bit kernels too, at a small part of the speed;
+        algo=2 refuses there instead.
     torch.compile breaks its graph here; tracing, torch.func transforms and forward-mode tangents are refused.
     """
     if torch.compiler.is_compiling():
