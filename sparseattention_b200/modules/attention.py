@@ -153,7 +153,7 @@ class HierarchicalAttention(nn.Module):
         if not self.fused_attention or transforms_active() or not type(q) is type(k) is type(v) is torch.Tensor:
             return False, None
         if not (q.is_cuda and q.dtype in (torch.bfloat16, torch.float16) and k.shape == v.shape
-                and k.dtype == v.dtype == q.dtype and Dh % 8 == 0 and Dh <= 128 and k.size(1) > 0):
+                and k.dtype == v.dtype == q.dtype and Dh % 8 == 0 and Dh <= 128 and q.numel() > 0 and k.size(1) > 0):
             return False, None
         # a module of another kind in its place, or a dropout kept active in evaluation, goes through the weights
         drop = self.dropout

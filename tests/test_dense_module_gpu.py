@@ -172,3 +172,15 @@ def test_gradients_of_gradients(dtype, masked):
             diff = (got.detach().float() - ref.detach()).abs()
             assert float(diff.max()) <= 4e-2 * float(ref.abs().max()) + step, i
             assert float(diff.mean()) <= 4e-2 * float(ref.abs().mean()) + step, i
+
+
+@pytest.mark.parametrize("rows", [(0, 9), (2, 0)])
+def test_nothing_to_attend_with(rows):
+    """No batch or no query: shapes, and gradients of gradients, are those of the elementary operations."""
+    layer, q, m = layer_and_rows()
+    q, m = q[:rows[0], :rows[1]].clone().requires_grad_(True), m[:rows[0]].clone()
+    out = layer(q, m, m)
+    assert out.shape == q.shape
+    (grad,) = torch.autograd.grad(out.float().sum(), q, create_graph=True)
+    (again,) = torch.autograd.grad(grad.float().sum() + (q.float() ** 2).sum(), q)
+    assert again.shape == q.shape
