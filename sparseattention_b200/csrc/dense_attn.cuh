@@ -84,16 +84,17 @@ struct DenseArgs {
 
 // float16 holds nothing between 0 and 2^-24, and full precision from 2^-14 only: weights near 1 / Lk, and score gradients, which are
 // those times differences of the size of dout, would lose bits as operands or vanish while the sums over them do not.  So the
-// backward's products take weights times 2^13 (the weights do not pass 1, but for the rounding of a large log-sum-exp), and score gradients times the power of two
-// that a bound on them allows: |ds| <= |do.(v - out)| <= 2 |do| max |v|, as the output is a mean of rows of V.  What is multiplied
-// by it stays below 2^14; the results are multiplied by the inverse, exactly.  (8192 keys, output gradients of 1e-3: dq off by
-// 5.7e-3 of its size without this; 5.2e-4 is what rounding the result alone leaves.)  It costs a read of V next to the row sums and
-// a clearing of the tops: backward of 3 x 515 x 1027, 12 on 4 heads of 128, 98.6 us against 91.7; 2 x 4096 x 4096, 16 heads of 128, 799
-// against 792; most where few queries look at many keys, 2 x 33 x 30011, 16 heads of 128, 343 against 294.
+// backward's products take weights times 2^13 (the weights do not pass 1, but for the rounding of a large log-sum-exp), and score
+// gradients times the power of two that a bound on them allows: ds_j = p_j sum_k p_k do.(v_j - v_k), so |ds_j| <= p_j (1 - p_j) 2 |do|
+// max |v| <= |do| max |v| / 2.  What is multiplied by it does not pass 2^16 (and saturates there); the results are multiplied by the
+// inverse, exactly.  (8192 keys, output gradients of 1e-3: dq off by 5.7e-3 of its size without this; 5.2e-4 is what rounding the
+// result alone leaves.)  It costs a read of V next to the row sums and a clearing of the tops: backward of 3 x 515 x 1027, 12 on 4
+// heads of 128, 98.6 us against 91.7; 2 x 4096 x 4096, 16 heads of 128, 799 against 792; most where few queries look at many keys, 2 x 33 x
+// 30011, 16 heads of 128, 343 against 294.
 constexpr int kWeightShift = 13;
 __device__ __forceinline__ float grad_shift(float dout_sq, unsigned int v_sq_bits) {
-    const float bound = 2.f * sqrtf(dout_sq) * sqrtf(__uint_as_float(v_sq_bits));
-    return bound > 0.f && bound < INFINITY ? (float)(13 - ilogbf(bound)) : 0.f;
+    const float bound = 0.5f * sqrtf(dout_sq) * sqrtf(__uint_as_float(v_sq_bits));
+    return bound > 0.f && bound < INFINITY ? (float)(15 - ilogbf(bound)) : 0.f;
 }
 // 2^e for whole e between -126 and 127
 __device__ __forceinline__ float pow2(float e) { return __int_as_float(((int)e + 127) << 23); }

@@ -336,3 +336,11 @@ def test_float16_training_captured_and_replayed():
             _, *want, _ = definition(*tensors)
             for name, a, b in zip(("dq", "dk", "dv"), res, want):
                 assert not a.any() if size == 0 else as_good_as_rounded(a, b, name) is None
+
+
+def test_float16_small_gradients_next_to_large_ones():
+    """Output gradients of 30 over sharp weights: entries of dk range from 20 down to what float16 does not hold, and none may be off by
+    more than the rounding of a score gradient as it is, half of 2^-24, would make it."""
+    for shape, scale in (((1, 4, 89, 1, 1, 128), 0.3), ((2, 1, 973, 2, 2, 96), 96 ** -0.5)):
+        q, k, v, g = make(*shape, torch.float16, seed=3, sharp=3.0)
+        check(q, k, v, (g.float() * 30).half(), scale=scale, algo=2)
