@@ -11,7 +11,7 @@
 // Tensor memory (512 columns): two half tiles of S for either query tile (64 columns each), O of both (DP each).  P replaces the
 // S it came from as 16-bit numbers, so it never passes through shared memory, and the other half tile's scores are computed
 // meanwhile.
-// Measured at 4096 x 4096, batch 4, 16 heads of 128, bf16: 459 to 464 us = 1.19 PFLOP/s, tensor pipe 66 % busy; what is left is the
+// Measured at 4096 x 4096, batch 4, 16 heads of 128, bf16: 459 to 464 us = 1.19 PFLOP/s, tensor pipe 65 % busy; what is left is the
 // softmax, two warps per scheduler that overlap each other only in part (459 with the treatment of NaN and large scores).  On the way there: scores in one piece of 128 columns,
 // which wait for the product that consumes P, 594 us; half tiles with products issued from per-lane registers slower still, from
 // uniform ones and by a warp per query tile 524 us; a quarter of the exponentials in multiply-adds 514 us; registers enough to
